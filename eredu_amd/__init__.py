@@ -18,8 +18,11 @@ host-side mirror of the reference's operator API:
 * :mod:`eredu_amd.gguf_file` -- GGUF container reader/writer and the
   streaming load into the device-side convert.
 * :mod:`eredu_amd.decode` -- the Llama decode step around the projections.
+* :mod:`eredu_amd.paged` -- ``PagedKVCache``: the paged 8-bit key/value cache of
+  many sequences, its attention and its pages.
 """
 from ._native import EreduError
+from .paged import PagedKVCache, rope_table
 from .quantization import (
     DEFAULT_BITS,
     DEFAULT_GROUP_SIZE,
@@ -42,6 +45,7 @@ __all__ = [
     "EreduError",
     "DEFAULT_BITS",
     "DEFAULT_GROUP_SIZE",
+    "PagedKVCache",
     "QuantizationMode",
     "QuantizedEmbedding",
     "QuantizedLinear",
@@ -55,4 +59,5 @@ __all__ = [
     "quantized_packed_dimension",
     "quantize",
     "quantize_with_mode",
+    "rope_table",
 ]

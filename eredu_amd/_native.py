@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in ``include/eredu_hip.h``.
+"""ctypes binding of the C ABI in ``include/eredu_hip.h`` and ``include/eredu_kv.h``.
 
 The shared library is built in-tree by ``eredu_amd.build``.  There is no
 fallback: if the library is missing, loading fails with an error that says so.
@@ -71,6 +71,29 @@ SIGNATURES["eq_quantized_matmul_swiglu"] = (
     [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, ctypes.c_char_p, _i32, _i32, ctypes.POINTER(ActivationPrologue),
      _vp], _i32)
 
+
+class KvCache(ctypes.Structure):
+    """eq_kv_cache of include/eredu_kv.h."""
+
+    _fields_ = [(n, _vp) for n in ("k_codes", "v_codes", "k_scales", "v_scales", "tables", "lengths", "refs", "missing")] + [
+        (n, _i64) for n in ("layers", "pages", "sequences", "width")] + [
+        (n, _i32) for n in ("kv_heads", "page_tokens", "head_dim")]
+
+
+# the entry points of include/eredu_kv.h
+KV_SIGNATURES = {}
+_kv = ctypes.POINTER(KvCache)
+KV_SIGNATURES["eq_kv_append"] = ([_kv, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp], _i32)
+KV_SIGNATURES["eq_kv_attention"] = ([_vp, _vp, _i64, _i32, _kv, _i64, _vp, _i64, _vp, _i64, ctypes.c_float, _b, _i64, _vp,
+                                  _i64, _i32, _vp, _i64, _vp], _i32)
+KV_SIGNATURES["eq_kv_attention_scratch"] = ([_kv, _i32, _i64, _i64, _b], _i64)
+KV_SIGNATURES["eq_kv_read"] = ([_vp, _vp, _kv, _i64, _vp, _i64, _vp, _i64, _i32, _vp], _i32)
+KV_SIGNATURES["eq_kv_extend"] = ([_kv, _vp, _i64, _vp, _i64, _vp, _i64, _vp], _i32)
+KV_SIGNATURES["eq_kv_fork"] = ([_kv, _vp, _vp, _i64, _vp, _i64, _vp], _i32)
+KV_SIGNATURES["eq_kv_free"] = ([_kv, _vp, _i64, _vp], _i32)
+KV_SIGNATURES["eq_kv_compact"] = ([_kv, _vp, _i64, _vp], _i32)
+KV_SIGNATURES["eq_kv_pages_scratch"] = ([_kv, _i64], _i64)
+
 _lib = None
 _lock = threading.Lock()
 
@@ -94,7 +117,7 @@ def lib() -> ctypes.CDLL:
                     f"HIP kernel library not found at {path}; build it with `python -m eredu_amd.build`"
                 )
             L = ctypes.CDLL(path)
-            for name, (args, res) in SIGNATURES.items():
+            for name, (args, res) in {**SIGNATURES, **KV_SIGNATURES}.items():
                 fn = getattr(L, name)
                 fn.argtypes = args
                 fn.restype = res
