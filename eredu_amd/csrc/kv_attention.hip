@@ -50,46 +50,81 @@ struct Rows {
     int base;                      // scale byte that o is relative to
 };
 
-// The query row at x (null: no row) turned by rot (null: not), as digits of
-// its largest magnitude; s2 = scale * log2 e.
-template <typename T, int D>
-__device__ __forceinline__ void kv_query(const uint16_t* x, const float* rot, float s2, i32x4* hi, i32x4* lo, float& f) {
-    constexpr int KS = D / 64;
+// A query row's values and angles as this lane has them on the way: dimensions
+// 64 ks + 16 g .. of the row, and the angles of the pairs that they are in (the other
+// of a pair is the lane's own 64-group ks + D / 128, or lane group g + 2's where D = 64).
+template <int D>
+struct RawQuery {
+    static constexpr int KS = D / 64, AS = D >= 128 ? D / 128 : 1;
+    uint4 x[KS][2];
+    float4 cs[AS][4], sn[AS][4];
+};
+template <int D>
+__device__ __forceinline__ void kv_query_load(const uint16_t* x, const float* rot, RawQuery<D>& q) {
     const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int ks = 0; ks < D / 64; ks++) {
+        const uint4* p = reinterpret_cast<const uint4*>(x + 64 * ks + 16 * g);
+        q.x[ks][0] = p[0], q.x[ks][1] = p[1];
+    }
+    if (!rot) return;
+#pragma unroll
+    for (int i = 0; i < RawQuery<D>::AS; i++) {
+        const float4* p = reinterpret_cast<const float4*>(rot + (D >= 128 ? 64 * i + 16 * g : 16 * (g & 1)));
+#pragma unroll
+        for (int j = 0; j < 4; j++) q.cs[i][j] = p[j], q.sn[i][j] = p[D / 8 + j];
+    }
+}
+
+// The row turned (where it has angles), as digits of its largest magnitude;
+// s2 = scale * log2 e.  sees: whether there is a row that sees anything.
+template <typename T, int D>
+__device__ __forceinline__ void kv_query(const RawQuery<D>& q, bool sees, bool turn, float s2, i32x4* hi, i32x4* lo, float& f) {
+    constexpr int KS = D / 64;
     float v[KS][16];
     uint32_t most = 0;
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++) {
-        const int d0 = 64 * ks + 16 * g;
-        if (x) {
-            kv_load8<T>(x + d0, v[ks]);
-            kv_load8<T>(x + d0 + 8, v[ks] + 8);
-            if (rot) {
-                float p[16];
-                const bool first = d0 < D / 2;
-                const int pd = first ? d0 + D / 2 : d0 - D / 2;
-                const float* cs = rot + (first ? d0 : pd);
-                kv_load8<T>(x + pd, p);
-                kv_load8<T>(x + pd + 8, p + 8);
+    for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float a = v[ks][i] * cs[i], b = p[i] * cs[D / 2 + i];
-                    v[ks][i] = first ? a - b : a + b;
-                }
+        for (int i = 0; i < 2; i++) {
+            const uint32_t w[4] = {q.x[ks][i].x, q.x[ks][i].y, q.x[ks][i].z, q.x[ks][i].w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                v[ks][8 * i + 2 * j] = sees ? kv_to_f32<T>(w[j] & 0xffffu) : 0.f;
+                v[ks][8 * i + 2 * j + 1] = sees ? kv_to_f32<T>(w[j] >> 16) : 0.f;
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; i++) v[ks][i] = 0.f;
         }
+    if (turn) {  // (the same for the whole wave)
+        if constexpr (D >= 128) {
+#pragma unroll
+            for (int i = 0; i < KS / 2; i++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const float cs = (&q.cs[i][j >> 2].x)[j & 3], sn = (&q.sn[i][j >> 2].x)[j & 3];
+                    const float a = v[i][j], b = v[i + KS / 2][j];
+                    v[i][j] = sees ? a * cs - b * sn : 0.f;
+                    v[i + KS / 2][j] = sees ? b * cs + a * sn : 0.f;
+                }
+        } else {
+            const bool first = (threadIdx.x & 63) < 32;
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const float cs = (&q.cs[0][j >> 2].x)[j & 3], sn = (&q.sn[0][j >> 2].x)[j & 3];
+                const float a = v[0][j], b = __shfl_xor(a, 32), x = a * cs, y = b * sn;
+                v[0][j] = sees ? (first ? x - y : x + y) : 0.f;
+            }
+        }
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
 #pragma unroll
         for (int i = 0; i < 16; i++) most = max(most, __float_as_uint(v[ks][i]) & 0x7fffffffu);
-    }
     most = max(most, uint32_t(__shfl_xor(int(most), 16)));
     most = max(most, uint32_t(__shfl_xor(int(most), 32)));
     const bool fine = most > 0u && most < 0x7f800000u;
-    const int e = fine ? __builtin_amdgcn_frexp_expf(__uint_as_float(most)) : 0;
-    const float mant = fine ? __builtin_amdgcn_frexp_mantf(__uint_as_float(most)) : 1.f;
-    const float inv = 32512.f / mant;
+    const float one = fine ? __uint_as_float(most) : 1.f;
+    const int e = __builtin_amdgcn_frexp_expf(one);
+    const float mant = __builtin_amdgcn_frexp_mantf(one), inv = 32512.f / mant;
     f = fine ? __builtin_amdgcn_ldexpf(mant * (s2 / 32512.f), e) : (most ? __uint_as_float(0x7fc00000u) : 0.f);
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) {
@@ -98,23 +133,21 @@ __device__ __forceinline__ void kv_query(const uint16_t* x, const float* rot, fl
             uint32_t h = 0, l = 0;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int q = fine ? int(rintf(__builtin_amdgcn_ldexpf(v[ks][4 * w + i], -e) * inv)) : 0;
-                const int top = (q + 128) >> 8;
+                const int x = int(rintf(__builtin_amdgcn_ldexpf(v[ks][4 * w + i], -e) * inv));
+                const int top = (x + 128) >> 8;
                 h |= uint32_t(top & 0xff) << (8 * i);
-                l |= uint32_t((q - 256 * top) & 0xff) << (8 * i);
+                l |= uint32_t((x - 256 * top) & 0xff) << (8 * i);
             }
-            hi[ks][w] = int(h), lo[ks][w] = int(l);
+            hi[ks][w] = fine ? int(h) : 0, lo[ks][w] = fine ? int(l) : 0;
         }
     }
 }
 
-// 64 tokens: k(t, ks) and v(dt) give this lane's operands, kb and vb are its
-// group's scale bytes, j0 its first token; dead: its page is missing.  EDGE: some row does not
-// see some of the tokens.
-template <bool EDGE, int D, int NR, typename KF, typename VF>
-__device__ __forceinline__ void kv_tile(Rows<D, NR>& R, KF k, VF v, int kb, int vb, int j0, bool dead) {
-    constexpr int KS = D / 64, DT = D / 16;
-    i32x4 s[NR][4];
+// The integer scores of 64 tokens: s[r][t][i] is row r's with token 4 t + i of
+// this lane group's 16; k(t, ks) gives the operands.
+template <int D, int NR, typename KF>
+__device__ __forceinline__ void kv_scores(const Rows<D, NR>& R, KF k, i32x4 (&s)[NR][4]) {
+    constexpr int KS = D / 64;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
         i32x4 a[KS];
@@ -131,6 +164,15 @@ __device__ __forceinline__ void kv_tile(Rows<D, NR>& R, KF k, VF v, int kb, int 
             s[r][t] = acc;
         }
     }
+}
+
+// The softmax of those scores and their values: v(dt) gives the operands, kb and
+// vb are this lane group's scale bytes, j0 its first token; dead: its page is missing.
+// edge (the same for the wave): some row does not see some of the tokens; their
+// scores are set below all others for the maximum, their exponents to -inf.
+template <int D, int NR, typename VF>
+__device__ __forceinline__ void kv_values(Rows<D, NR>& R, i32x4 (&s)[NR][4], VF v, int kb, int vb, int j0, bool dead, bool edge) {
+    constexpr int DT = D / 16;
     const bool nan = kb == 255 || vb == 255;
     const float kf = nan ? __uint_as_float(0x7fc00000u) : e8m0_to_f32(uint32_t(kb));
     const int ev = nan || dead ? 0 : vb;
@@ -138,20 +180,24 @@ __device__ __forceinline__ void kv_tile(Rows<D, NR>& R, KF k, VF v, int kb, int 
     int first[NR], seen[NR];
     bool need = ev > R.base;
 #pragma unroll
-    for (int r = 0; r < NR; r++) {
-        f[r] = R.f[r] * kf;
-        if constexpr (EDGE) {
+    for (int r = 0; r < NR; r++) first[r] = 0, seen[r] = 16;
+    if (edge) {
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
             first[r] = dead ? 16 : max(R.from[r] - j0, 0);
             seen[r] = max(min(R.until[r] - j0, 16) - first[r], 0);
 #pragma unroll
             for (int n = 0; n < 16; n++)
                 if (unsigned(n - first[r]) >= unsigned(seen[r])) s[r][n >> 2][n & 3] = INT32_MIN;
         }
+    }
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        f[r] = R.f[r] * kf;
         int mx = s[r][0][0];
 #pragma unroll
         for (int n = 1; n < 16; n++) mx = max(mx, s[r][n >> 2][n & 3]);
-        top[r] = float(mx) * f[r];
-        if constexpr (EDGE) top[r] = seen[r] > 0 ? top[r] : -INFINITY;
+        top[r] = seen[r] > 0 ? float(mx) * f[r] : -INFINITY;
         need |= top[r] > R.m[r] + kMaxSlack;
     }
     if (__any(need)) {
@@ -171,29 +217,40 @@ __device__ __forceinline__ void kv_tile(Rows<D, NR>& R, KF k, VF v, int kb, int 
             for (int dt = 0; dt < DT; dt++) R.o[r][dt] *= al * down;
         }
     }
-    h16x8 p[NR][2];
+    f32x4 x[NR][4];
 #pragma unroll
     for (int r = 0; r < NR; r++) {
         const float shift = kProbBias - R.m[r];
+#pragma unroll
+        for (int n = 0; n < 16; n++) x[r][n >> 2][n & 3] = fmaf(float(s[r][n >> 2][n & 3]), f[r], shift);
+    }
+    if (edge) {
+#pragma unroll
+        for (int r = 0; r < NR; r++)
+#pragma unroll
+            for (int n = 0; n < 16; n++)
+                if (unsigned(n - first[r]) >= unsigned(seen[r])) x[r][n >> 2][n & 3] = -INFINITY;
+    }
+    h16x8 p[NR][2];
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
         float sum = 0.f;
 #pragma unroll
-        for (int n = 0; n < 16; n += 4) {
-            f32x4 e;
+        for (int t = 0; t < 4; t++) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                e[i] = __builtin_amdgcn_exp2f(fmaf(float(s[r][n >> 2][i]), f[r], shift));
-                if constexpr (EDGE) e[i] = unsigned(n + i - first[r]) < unsigned(seen[r]) ? e[i] : 0.f;
-                sum += e[i];
+                x[r][t][i] = __builtin_amdgcn_exp2f(x[r][t][i]);
+                sum += x[r][t][i];
             }
-            const h16x4 h = __builtin_convertvector(e, h16x4);
+            const h16x4 h = __builtin_convertvector(x[r][t], h16x4);
 #pragma unroll
-            for (int i = 0; i < 4; i++) p[r][n >> 3][(n & 4) + i] = h[i];
+            for (int i = 0; i < 4; i++) p[r][t >> 1][(t & 1) * 4 + i] = h[i];
         }
         R.l[r] += sum;
     }
     // 2^(15 + ev - base) in f16, subnormal below 2^-14
-    const int x = 30 + ev - R.base;
-    const uint16_t bits = uint16_t(x >= 1 ? x << 10 : (x >= -9 ? 1 << (9 + x) : 0));
+    const int ex = 30 + ev - R.base;
+    const uint16_t bits = uint16_t(ex >= 1 ? ex << 10 : (ex >= -9 ? 1 << (9 + ex) : 0));
     const _Float16 sc = __builtin_bit_cast(_Float16, bits);
     const h16x2 sc2 = {sc, sc}, off2 = sc2 * h16x2{_Float16(-1.125f), _Float16(-1.125f)};
 #pragma unroll
@@ -213,6 +270,8 @@ __device__ __forceinline__ void kv_tile(Rows<D, NR>& R, KF k, VF v, int kb, int 
 #pragma unroll
             for (int r = 0; r < NR; r++) R.o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p[r][u], R.o[r][dt], 0, 0, 0);
         }
+        // (values converted further ahead only take registers)
+        if (dt % 2 == 1) __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -224,10 +283,12 @@ struct AttnCall {
     KvBatch b;
     const float* rope;
     float s2;      // scale * log2 e
-    int heads, group, tiles, splits, window;  // window 0: none
+    int heads, tiles, splits, window;  // window 0: none
+    unsigned group;
     bool causal;
-    float* part;   // [row][head][split][D], normalised; null: one split
-    float* lse;    // [row][head][split]
+    int groups;    // kv_stream_kernel's workgroups
+    float* part;   // kv_block_kernel: [row][head][split][D], normalised; null: one split.  kv_stream_kernel: [slot][row][D]
+    float* lse;    // [row][head][split], or [slot][row]
 };
 
 // The 64-token tiles that query tokens [i0, i1] of an entry see, and their
@@ -256,7 +317,7 @@ __device__ __forceinline__ int kv_share(const AttnCall& A, const TileRange& t) {
 // Where a launch's workgroup works: the KV head varies fastest, so that one
 // head's codes stay in one XCD's L2 where there are 8 of them.
 struct Place {
-    int kvh, split;
+    int kvh, split;  // split: of kv_block_kernel
     KvEntry e;
     int first;  // row of the entry's rows * group that the tile begins with
 };
@@ -270,26 +331,42 @@ __device__ __forceinline__ bool kv_place(const AttnCall& A, Place& P) {
     // the last tiles first: in causal prompts they have the most to do
     if (!kv_locate(A.b, A.tiles - 1 - id % per / A.c.kv_heads, [&](int n) { return (n * group + BM - 1) / BM; }, entry, place))
         return false;
-    P.e = kv_entry(A.c, A.b, entry);
+    const KvEntry e = kv_entry(A.c, A.b, entry);
+    P.e = KvEntry{__builtin_amdgcn_readfirstlane(e.seq), __builtin_amdgcn_readfirstlane(e.start),
+                  __builtin_amdgcn_readfirstlane(e.count), __builtin_amdgcn_readfirstlane(e.length)};
     P.first = place * BM;
     return true;
 }
 
-// This lane's rows of the wave's tile, first .. first + 16 NR - 1.
-template <typename T, int D, int NR>
-__device__ __forceinline__ void kv_begin(const AttnCall& A, const Place& P, int first, Rows<D, NR>& R) {
+// This lane's rows of the wave's tile, first .. first + 16 NR - 1: what they
+// see and the loads of their queries (of the entry's first row where there is none, in bounds
+// and not used), then the rest.
+template <int D, int NR>
+struct RowLoads {
+    RawQuery<D> q[NR];
+    bool sees[NR];
+};
+template <int D, int NR>
+__device__ __forceinline__ void kv_begin_loads(const AttnCall& A, const Place& P, int first, Rows<D, NR>& R, RowLoads<D, NR>& W) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int r = 0; r < NR; r++) {
-        const int row = first + 16 * r + (lane & 15), i = row / A.group;
-        const bool live = i < P.e.count;
-        const int pos = P.e.length - P.e.count + i;
-        R.from[r] = live ? kv_from(A, P.e, i) : 0;
-        R.until[r] = live ? kv_until(A, P.e, i) : 0;
-        const bool sees = live && R.from[r] < R.until[r];
-        const uint16_t* x = A.q + int64_t(P.e.start + i) * A.q_stride + int64_t(P.kvh * A.group + row % A.group) * D;
-        kv_query<T, D>(sees ? x : nullptr, sees && A.rope && pos >= 0 ? A.rope + int64_t(pos) * D : nullptr, A.s2,
-                       R.hi[r], R.lo[r], R.f[r]);
+        const unsigned row = first + 16 * r + (lane & 15);
+        const int i = row / A.group, ii = i < P.e.count ? i : 0;
+        const int pos = P.e.length - P.e.count + ii;
+        R.from[r] = i < P.e.count ? kv_from(A, P.e, i) : 0;
+        R.until[r] = i < P.e.count ? kv_until(A, P.e, i) : 0;
+        W.sees[r] = R.from[r] < R.until[r];
+        const uint16_t* x = A.q + int64_t(P.e.start + ii) * A.q_stride + int64_t(P.kvh * A.group + (row - i * A.group)) * D;
+        // (a position that has pages is inside the table of angles; any other is not used)
+        kv_query_load<D>(x, A.rope ? A.rope + int64_t(kv_clamp(pos, 0, (A.c.width << A.c.log2_page) - 1)) * D : nullptr, W.q[r]);
+    }
+}
+template <typename T, int D, int NR>
+__device__ __forceinline__ void kv_begin(const AttnCall& A, Rows<D, NR>& R, const RowLoads<D, NR>& W) {
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        kv_query<T, D>(W.q[r], W.sees[r], A.rope != nullptr, A.s2, R.hi[r], R.lo[r], R.f[r]);
         R.m[r] = -INFINITY;
         R.l[r] = 0.f;
 #pragma unroll
@@ -298,139 +375,379 @@ __device__ __forceinline__ void kv_begin(const AttnCall& A, const Place& P, int 
     R.base = 0;
 }
 
-// 4 dimensions of one row: the output, or its part of one split.
+// 4 dimensions of one row of the output, or of its part of one split.
 template <typename T, int D>
 __device__ __forceinline__ void kv_store4(const AttnCall& A, const Place& P, int row, int d, f32x4 o) {
-    const int i = row / A.group, h = P.kvh * A.group + row % A.group;
+    const int i = unsigned(row) / A.group, h = P.kvh * A.group + unsigned(row) % A.group;
     const int64_t at = int64_t(P.e.start + i) * A.heads + h;
-    if (A.part) {
-        *reinterpret_cast<f32x4*>(A.part + (at * A.splits + P.split) * D + d) = o;
-    } else {
-        uint16_t w[4];
+    uint16_t w[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) w[j] = to_storage<T>(o[j]);
-        *reinterpret_cast<uint2*>(A.out + at * D + d) = make_uint2(w[0] | uint32_t(w[1]) << 16, w[2] | uint32_t(w[3]) << 16);
-    }
+    for (int j = 0; j < 4; j++) w[j] = to_storage<T>(o[j]);
+    *reinterpret_cast<uint2*>(A.out + at * D + d) = make_uint2(w[0] | uint32_t(w[1]) << 16, w[2] | uint32_t(w[3]) << 16);
+}
+template <int D>
+__device__ __forceinline__ void kv_store_part4(const AttnCall& A, const Place& P, int row, int d, f32x4 o) {
+    const int i = unsigned(row) / A.group, h = P.kvh * A.group + unsigned(row) % A.group;
+    const int64_t at = int64_t(P.e.start + i) * A.heads + h;
+    *reinterpret_cast<f32x4*>(A.part + (at * A.splits + P.split) * D + d) = o;
 }
 __device__ __forceinline__ void kv_store_lse(const AttnCall& A, const Place& P, int row, float lse) {
-    const int i = row / A.group, h = P.kvh * A.group + row % A.group;
+    const int i = unsigned(row) / A.group, h = P.kvh * A.group + unsigned(row) % A.group;
     A.lse[(int64_t(P.e.start + i) * A.heads + h) * A.splits + P.split] = lse;
 }
 
 // --------------------------------------------------- few rows: a stream of tokens
 //
-// 16 rows a workgroup, whose 4 waves take the split's tiles in turn, each
-// with a softmax of its own, joined at the end.  Operands go from memory to
-// registers as the matrix cores take them, the next tile's under way while one is computed.
+// 16 rows at a time, each wave by itself.  Operands go from memory to registers as
+// the matrix cores take them.
+//
+// The work is the list of all tiles: of all entries, their blocks of 16 rows,
+// KV heads and 64-token tiles, in that order.  Each of the launch's waves takes
+// an equal run of it, whatever the sequences' lengths, and works off the units
+// (a block of rows and a KV head) in it one by one.  A unit that lies in one run
+// is written out; of the others a run has its first and its last, at most, and
+// these go to two slots of the wave, to be joined by kv_stream_join_kernel.
 
+constexpr int kStreamRows = 16;
+
+// An entry's tiles: [begin, end) are those that any of its rows sees, `tiles`
+// their number, at least 1 (rows that see nothing are written too), and `all`
+// that of all its units together.  (A plan bounds their sum below 2^31.)
+struct Units {
+    int begin, end, tiles, all;
+};
+__device__ __forceinline__ Units kv_units(const AttnCall& A, const KvEntry& e) {
+    Units u = {0, 0, 0, 0};
+    if (e.count > 0) {
+        const TileRange t = kv_tiles(A, e, 0, e.count - 1);
+        u.begin = t.begin, u.end = t.end;
+        u.tiles = max(t.end - t.begin, 1);
+        u.all = (e.count * A.group + kStreamRows - 1) / kStreamRows * A.c.kv_heads * u.tiles;
+    }
+    return u;
+}
+
+// The list of tiles, as a wave knows it.  Up to 64 entries: a lane has one and
+// the tiles before it, and the rest is exchanges between lanes.  More: thread t
+// goes through the entries t * per .. (t + 1) * per - 1 and LDS has what the
+// other waves need, up to 256 entries themselves.
+struct TileListLds {
+    KvEntry entries[256];
+    int sums[4], found[4], found_entry[4];
+};
+struct TileList {
+    TileListLds& lds;
+    KvEntry mine;
+    int before, own, all;  // tiles before this lane's (thread's) entries, of them, and of all
+
+    __device__ __forceinline__ TileList(const AttnCall& A, TileListLds& L) : lds(L) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        mine = KvEntry{-1, 0, 0, 0};
+        own = 0;
+        if (A.b.n <= 64) {
+            if (lane < A.b.n) {
+                mine = kv_entry(A.c, A.b, lane);
+                own = kv_units(A, mine).all;
+            }
+        } else {
+            const int per = (A.b.n + 255) / 256;
+            for (int i = threadIdx.x * per; i < min(A.b.n, int(threadIdx.x + 1) * per); i++) {
+                const KvEntry e = kv_entry(A.c, A.b, i);
+                if (per == 1) L.entries[i] = e;
+                own += kv_units(A, e).all;
+            }
+        }
+        int upto = own;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int t = __shfl_up(upto, o);
+            if (lane >= o) upto += t;
+        }
+        before = upto - own;
+        all = __builtin_amdgcn_readlane(upto, 63);
+        if (A.b.n <= 64) return;
+        if (lane == 63) L.sums[wave] = upto;
+        if (threadIdx.x < 4) L.found[threadIdx.x] = L.found_entry[threadIdx.x] = 0;
+        __syncthreads();
+        all = 0;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            if (w < wave) before += L.sums[w];
+            all += L.sums[w];
+        }
+    }
+    // entry i, the same for all lanes of the wave
+    __device__ __forceinline__ KvEntry entry(const AttnCall& A, int i) const {
+        if (A.b.n <= 64)
+            return KvEntry{__builtin_amdgcn_readlane(mine.seq, i), __builtin_amdgcn_readlane(mine.start, i),
+                           __builtin_amdgcn_readlane(mine.count, i), __builtin_amdgcn_readlane(mine.length, i)};
+        const KvEntry e = A.b.n <= 256 ? lds.entries[i] : kv_entry(A.c, A.b, i);
+        return KvEntry{__builtin_amdgcn_readfirstlane(e.seq), __builtin_amdgcn_readfirstlane(e.start),
+                       __builtin_amdgcn_readfirstlane(e.count), __builtin_amdgcn_readfirstlane(e.length)};
+    }
+    // tiles before entry i (all threads of the workgroup call this)
+    __device__ __forceinline__ int tiles_before(const AttnCall& A, int i) {
+        if (A.b.n <= 64) return __builtin_amdgcn_readlane(before, i);
+        const int per = (A.b.n + 255) / 256;
+        if (i / per == int(threadIdx.x)) {
+            int at = before;
+            for (int k = threadIdx.x * per; k < i; k++) at += kv_units(A, per == 1 ? lds.entries[k] : kv_entry(A.c, A.b, k)).all;
+            lds.found[0] = at;
+        }
+        __syncthreads();
+        return __builtin_amdgcn_readfirstlane(lds.found[0]);
+    }
+    // the entry of tile first + wave * step, and the tiles before it (all threads of the workgroup call this)
+    __device__ __forceinline__ int find(const AttnCall& A, int first, int step, int& base) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pos = first + wave * step;
+        if (A.b.n <= 64) {
+            const uint64_t at = __ballot(before <= pos && pos < before + own);
+            const int i = at ? __ffsll((unsigned long long)at) - 1 : 0;
+            base = __builtin_amdgcn_readlane(before, i);
+            return i;
+        }
+        const int per = (A.b.n + 255) / 256;
+        int at = before;
+        for (int i = threadIdx.x * per; i < min(A.b.n, int(threadIdx.x + 1) * per); i++) {
+            const int n = per == 1 ? own : kv_units(A, kv_entry(A.c, A.b, i)).all;
+#pragma unroll
+            for (int w = 0; w < 4; w++)
+                if (at <= first + w * step && first + w * step < at + n) lds.found[w] = at, lds.found_entry[w] = i;
+            at += n;
+        }
+        __syncthreads();
+        base = __builtin_amdgcn_readfirstlane(lds.found[wave]);
+        return __builtin_amdgcn_readfirstlane(lds.found_entry[wave]);
+    }
+};
+__device__ __forceinline__ int kv_run(const AttnCall& A, int all) { return max(1, int(unsigned(all + 4 * A.groups - 1) / unsigned(4 * A.groups))); }
+
+// (Keys and values have one set of registers each: the next tile's keys are
+// requested when the scores are done, its values when the values are, so 2 or
+// 3 waves fit a SIMD and cover each other's waits.)
 template <int D>
 struct Tile {
     i32x4 k[4][D / 64], v[D / 16];
-    int kb, vb;
-    bool dead;
 };
 
 template <int D>
-__device__ __forceinline__ void kv_fetch(const AttnCall& A, const Place& P, int tile, int ida, int idg, Tile<D>& t) {
+__device__ __forceinline__ void kv_fetch_keys(const AttnCall& A, const Place& P, int tile, int id, Tile<D>& t) {
     const int lane = threadIdx.x & 63, g = lane >> 4, a = (lane & 15) >> 2, T = 1 << A.c.log2_page;
-    t.dead = idg < 0;
-    const int64_t pa = int64_t(max(ida, 0)) * A.c.kv_heads + P.kvh, pg = int64_t(max(idg, 0)) * A.c.kv_heads + P.kvh;
-    t.kb = A.c.ks[pg];
-    t.vb = A.c.vs[pg];
-    const int8_t* k = A.c.k + (pa * T + ((tile * 64 + 16 * a) & (T - 1)) + (lane & 3)) * D + 16 * g;
-    const int8_t* v = A.c.v + (pg * D + (lane & 15)) * T + ((tile * 64 + 16 * g) & (T - 1));
+    const int8_t* k = A.c.k + ((int64_t(max(id, 0)) * A.c.kv_heads + P.kvh) * T + ((tile * 64 + 16 * a) & (T - 1)) + (lane & 3)) * D + 16 * g;
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int ks = 0; ks < D / 64; ks++) t.k[i][ks] = *reinterpret_cast<const i32x4*>(k + 4 * i * D + 64 * ks);
+}
+template <int D>
+__device__ __forceinline__ void kv_fetch_values(const AttnCall& A, const Place& P, int tile, int id, Tile<D>& t) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, T = 1 << A.c.log2_page;
+    const int8_t* v = A.c.v + ((int64_t(max(id, 0)) * A.c.kv_heads + P.kvh) * D + (lane & 15)) * T + ((tile * 64 + 16 * g) & (T - 1));
 #pragma unroll
-    for (int dt = 0; dt < D / 16; dt++) t.v[dt] = *reinterpret_cast<const i32x4*>(v + 16 * dt * T);
+    for (int dt = 0; dt < D / 16; dt++, v += 16 * T) t.v[dt] = *reinterpret_cast<const i32x4*>(v);
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void kv_stream_kernel(const AttnCall A) {
-    constexpr int NR = 1, BM = 16, DC = D < 128 ? D : 128;
-    __shared__ float os[4][16][DC + 4];
-    __shared__ float ms[4][16], ls[4][16];
-    __shared__ int bs[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_stream_kernel(const AttnCall A) {
+    constexpr int NR = 1, BM = kStreamRows;
+    __shared__ TileListLds lds;
+    const int lane = threadIdx.x & 63, g = lane >> 4, a = (lane & 15) >> 2;
+    TileList list(A, lds);
+    const int run = kv_run(A, list.all), wid = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (blockIdx.x * 4 * int64_t(run) >= list.all) return;
+    int base, entry = list.find(A, blockIdx.x * 4 * run, run, base);
+    const int start = int(min(int64_t(wid) * run, int64_t(list.all))), stop = min(start + run, list.all);
+    if (start >= stop) return;
+    int pos = start;
     Place P;
-    if (!kv_place<BM>(A, P)) return;
-    const int rows = min(BM, P.e.count * A.group - P.first);
-    const TileRange all = kv_tiles(A, P.e, P.first / A.group, (P.first + rows - 1) / A.group);
-    const int share = kv_share(A, all), begin = all.begin + P.split * share, end = min(all.end, begin + share);
-    if (P.split > 0 && begin >= end) return;
-    Rows<D, NR> R;
-    kv_begin<T, D, NR>(A, P, P.first, R);
-    // tiles [clear_from, clear_until) are seen whole by every row there is
-    const int clear_from = (kv_from(A, P.e, (P.first + rows - 1) / A.group) + 63) >> 6, clear_until = max(kv_until(A, P.e, P.first / A.group), 0) >> 6;
-
-    auto page = [&](int tile, int block) { return kv_page(A.c, P.e.seq, (tile * 64 + 16 * block) >> A.c.log2_page); };
-    const int a = (lane & 15) >> 2;
-    int tile = begin + wave;
-    if (tile < end) {
-        Tile<D> cur, nxt;
-        kv_fetch<D>(A, P, tile, page(tile, a), page(tile, g), cur);
-        int ida = page(tile + 4, a), idg = page(tile + 4, g);
-        auto step = [&](Tile<D>& now, Tile<D>& next) __attribute__((always_inline)) {
-            const bool more = tile + 4 < end;
-            if (more) {
-                kv_fetch<D>(A, P, tile + 4, ida, idg, next);
-                ida = page(tile + 8, a), idg = page(tile + 8, g);
-            }
-            auto k = [&](int t, int ks) __attribute__((always_inline)) { return now.k[t][ks]; };
-            auto v = [&](int dt) __attribute__((always_inline)) { return now.v[dt]; };
-            if (tile >= clear_from && tile < clear_until && !__any(now.dead))
-                kv_tile<false, D, NR>(R, k, v, now.kb, now.vb, tile * 64 + 16 * g, false);
-            else
-                kv_tile<true, D, NR>(R, k, v, now.kb, now.vb, tile * 64 + 16 * g, now.dead);
-            tile += 4;
-            return more;
+    P.split = 0;
+    auto enter = [&]() __attribute__((always_inline)) {
+        P.e = list.entry(A, entry);
+        return kv_units(A, P.e);
+    };
+    Units U = enter();
+    while (true) {
+        const int local = pos - base, unit = unsigned(local) / unsigned(U.tiles), tile0 = local - unit * U.tiles;
+        const int tiles = min(U.tiles - tile0, stop - pos);
+        const int block = unsigned(unit) / unsigned(A.c.kv_heads);
+        P.kvh = unit - block * A.c.kv_heads;
+        P.first = block * BM;
+        const int rows = min(BM, P.e.count * A.group - P.first), end = min(U.begin + tile0 + tiles, U.end);
+        // tiles [clear_from, clear_until) are seen whole by every row there is
+        const int clear_from = (kv_from(A, P.e, unsigned(P.first + rows - 1) / A.group) + 63) >> 6,
+                  clear_until = max(kv_until(A, P.e, unsigned(P.first) / A.group), 0) >> 6;
+        auto page = [&](int tile, int block) { return kv_page(A.c, P.e.seq, (tile * 64 + 16 * block) >> A.c.log2_page); };
+        auto scales = [&](int id, int& x, int& y) __attribute__((always_inline)) {
+            const int64_t at = int64_t(max(id, 0)) * A.c.kv_heads + P.kvh;
+            x = A.c.ks[at], y = A.c.vs[at];
         };
-        while (step(cur, nxt) && step(nxt, cur)) {
+        Rows<D, NR> R;
+        RowLoads<D, NR> W;
+        kv_begin_loads<D, NR>(A, P, P.first, R, W);
+        __builtin_amdgcn_sched_barrier(0);
+        int tile = U.begin + tile0, ida = -1, idg = -1, idd = -1, kb = 0, vb = 0;
+        Tile<D> t;
+        // (a unit without tiles, of rows that see nothing, reads page 0 and uses none of it)
+        ida = page(tile, a), idg = idd = page(tile, g);
+        kv_fetch_keys<D>(A, P, tile, ida, t);
+        scales(idg, kb, vb);
+        __builtin_amdgcn_sched_barrier(0);
+        kv_begin<T, D, NR>(A, R, W);  // (while the first keys are under way)
+        __builtin_amdgcn_sched_barrier(0);
+        kv_fetch_values<D>(A, P, tile, idg, t);
+        ida = page(tile + 1, a), idg = page(tile + 1, g);
+        for (; tile < end; tile++) {
+            const bool more = tile + 1 < end;
+            i32x4 s[NR][4];
+            kv_scores<D, NR>(R, [&](int i, int ks) __attribute__((always_inline)) { return t.k[i][ks]; }, s);
+            int kbn = 0, vbn = 0, ida2 = -1, idg2 = -1;
+            if (more) {
+                kv_fetch_keys<D>(A, P, tile + 1, ida, t);
+                scales(idg, kbn, vbn);
+                ida2 = page(tile + 2, a), idg2 = page(tile + 2, g);
+            }
+            auto v = [&](int dt) __attribute__((always_inline)) { return t.v[dt]; };
+            const bool dead = idd < 0;
+            kv_values<D, NR>(R, s, v, kb, vb, tile * 64 + 16 * g, dead, tile < clear_from || tile >= clear_until || __any(dead));
+            if (more) kv_fetch_values<D>(A, P, tile + 1, idg, t);
+            idd = idg, kb = kbn, vb = vbn, ida = ida2, idg = idg2;
         }
-    }
-    // join the four waves' states
-    float l = R.l[0];
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if (lane < 16) ms[wave][lane] = R.m[0], ls[wave][lane] = l;
-    if (lane == 0) bs[wave] = R.base;
-#pragma unroll
-    for (int d0 = 0; d0 < D; d0 += DC) {
-        if (d0) __syncthreads();
-#pragma unroll
-        for (int dt = 0; dt < DC / 16; dt++)
-            *reinterpret_cast<f32x4*>(&os[wave][lane & 15][16 * dt + 4 * g]) = R.o[0][d0 / 16 + dt];
-        __syncthreads();
-        const int row = tid >> 4;
+        // a unit of several runs goes to a slot
+        const bool part = tiles < U.tiles;
+        const int slot = 2 * wid + (pos == start ? 0 : 1), row = lane & 15;
+        float l = R.l[0];
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
         if (row < rows) {
-            float m = -INFINITY, sum = 0.f, w[4];
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            if (part && g == 0) A.lse[slot * BM + row] = l == 0.f ? -INFINITY : R.m[0] + __builtin_amdgcn_logf(l);
 #pragma unroll
-            for (int i = 0; i < 4; i++) m = fmaxf(m, ms[i][row]);
+            for (int dt = 0; dt < D / 16; dt++) {
+                f32x4 o;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float up = ms[i][row] == m ? 1.f : __builtin_amdgcn_exp2f(ms[i][row] - m);
-                sum += ls[i][row] * up;
-                w[i] = up;
-            }
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-            for (int i = 0; i < 4; i++) w[i] *= inv;
-            if (A.part && d0 == 0 && (tid & 15) == 0)
-                kv_store_lse(A, P, P.first + row, sum == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(sum));
-            for (int d = 4 * (tid & 15); d < DC; d += 64) {
-                f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(&os[i][row][d]);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) o[j] += __builtin_amdgcn_ldexpf(x[j] * w[i], bs[i] - 132);
-                }
-                kv_store4<T, D>(A, P, P.first + row, d0 + d, o);
+                for (int j = 0; j < 4; j++) o[j] = __builtin_amdgcn_ldexpf(R.o[0][dt][j] * inv, R.base - 132);
+                if (part) *reinterpret_cast<f32x4*>(A.part + (int64_t(slot) * BM + row) * D + 16 * dt + 4 * g) = o;
+                else kv_store4<T, D>(A, P, P.first + row, 16 * dt + 4 * g, o);
             }
         }
+        pos += tiles;
+        if (pos >= stop) return;
+        while (pos - base >= U.all) {  // on to the next entry that has rows
+            base += U.all;
+            if (++entry >= A.b.n) return;
+            U = enter();
+        }
     }
+}
+
+// 4 lanes' worth of one state: (m, sum, o) in every lane of a set of D / 4
+// lanes, joined over the sets of W waves (state of set 0 on return; only the
+// threads t < D / 4 go on).
+template <int D, int W>
+struct Joiner {
+    static constexpr int LANES = D / 4, SETS = 64 * W / LANES;
+    f32x4 os[W == 1 ? 1 : SETS][LANES];
+    float ms[4], sums[W == 1 ? 1 : SETS];
+
+    __device__ __forceinline__ bool join(int t, float m, float& sum, f32x4& o) {
+        const int set = t / LANES;
+        float top = m;
+#pragma unroll
+        for (int w = LANES; w < 64; w <<= 1) top = fmaxf(top, __shfl_xor(top, w));
+        if constexpr (W > 1) {
+            if ((t & 63) == 0) ms[t >> 6] = top;
+            __syncthreads();
+            top = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
+        }
+        const float al = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+        sum *= al;
+        o *= al;
+        if constexpr (W > 1) {
+            os[set][t % LANES] = o;
+            if (t % LANES == 0) sums[set] = sum;
+            __syncthreads();
+            if (t >= LANES) return false;
+            sum = sums[0];
+            o = os[0][t];
+#pragma unroll
+            for (int s = 1; s < SETS; s++) {
+                sum += sums[s];
+                o += os[s][t];
+            }
+            return true;
+        } else {
+#pragma unroll
+            for (int w = LANES; w < 64; w <<= 1) {
+                sum += __shfl_xor(sum, w);
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[i] += __shfl_xor(o[i], w);
+            }
+            return t < LANES;
+        }
+    }
+};
+
+// 4 states (exponents e, -inf: nothing; parts x) into a running one.
+__device__ __forceinline__ void kv_merge4(const float (&e)[4], const f32x4 (&x)[4], float& m, float& sum, f32x4& o) {
+    const float mn = fmaxf(m, fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])));
+    const float al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    sum *= al;
+    o *= al;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (e[j] == -INFINITY) continue;
+        const float w = __builtin_amdgcn_exp2f(e[j] - mn);  // (NaN for a NaN)
+        sum += w;
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = fmaf(w, x[j][i], o[i]);
+    }
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void kv_out4(const AttnCall& A, int64_t at, int t, float sum, f32x4 o) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    uint16_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = to_storage<T>(o[i] * inv);
+    *reinterpret_cast<uint2*>(A.out + at * D + 4 * t) = make_uint2(w[0] | uint32_t(w[1]) << 16, w[2] | uint32_t(w[3]) << 16);
+}
+
+// The units that lie in several runs of kv_stream_kernel: a workgroup for each row
+// (of the rows that entries cover) and query head.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv_stream_join_kernel(const AttnCall A) {
+    __shared__ Joiner<D, 4> J;
+    __shared__ TileListLds lds;
+    const int t = threadIdx.x, h = blockIdx.y, u = blockIdx.x;
+    int entry, i;
+    if (!kv_locate(A.b, u, [](int n) { return n; }, entry, i)) return;
+    TileList list(A, lds);
+    const int run = kv_run(A, list.all), base = list.tiles_before(A, entry);
+    const KvEntry e = list.entry(A, entry);
+    const Units U = kv_units(A, e);
+    const int row = i * A.group + unsigned(h) % A.group;
+    const int S = base + (row / kStreamRows * A.c.kv_heads + int(unsigned(h) / A.group)) * U.tiles;
+    const int w0 = unsigned(S) / unsigned(run), w1 = unsigned(S + U.tiles - 1) / unsigned(run);
+    if (w0 == w1) return;  // written out
+    constexpr int LANES = D / 4, SETS = 256 / LANES;
+    const int set = t / LANES;
+    float m = -INFINITY, sum = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int b = w0; b <= w1; b += 4 * SETS) {
+        f32x4 x[4];
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int w = b + j * SETS + set;
+            const bool is = w <= w1;
+            const int64_t slot = int64_t(2 * (is ? w : w0) + (w == w0 && S != w0 * run ? 1 : 0)) * kStreamRows + row % kStreamRows;
+            f[j] = is ? A.lse[slot] : -INFINITY;
+            x[j] = is ? reinterpret_cast<const f32x4*>(A.part + slot * D)[t % LANES] : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        kv_merge4(f, x, m, sum, o);
+    }
+    if (J.join(t, m, sum, o)) kv_out4<T, D>(A, int64_t(e.start + i) * A.heads + h, t, sum, o);
 }
 
 // ------------------------------------------ many rows: blocks of rows over shared tiles
@@ -457,7 +774,7 @@ template <int D>
 __device__ __forceinline__ void kv_stage(const AttnCall& A, const Place& P, int tile, int idg, int idv, lds_char* kbuf,
                                          lds_char* vbuf) {
     constexpr int KP = D / 16;  // 16-byte pieces of a key
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, T = 1 << A.c.log2_page;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), T = 1 << A.c.log2_page;
 #pragma unroll
     for (int j = 0; j < D / 64; j++) {
         const int p = (j * 4 + wave) * 64 + lane, token = p / KP, c = (p % KP) ^ kv_key_swap<D>(token);
@@ -478,23 +795,30 @@ __device__ __forceinline__ void kv_stage(const AttnCall& A, const Place& P, int 
 }
 
 template <typename T, int D, int NR>
-__global__ __launch_bounds__(256) void kv_block_kernel(const AttnCall A) {
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_block_kernel(const AttnCall A) {
     constexpr int BM = 64 * NR;
     __shared__ __attribute__((aligned(16))) char k0[64 * D], k1[64 * D], v0[64 * D], v1[64 * D];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     Place P;
     if (!kv_place<BM>(A, P)) return;
     const int rows = min(BM, P.e.count * A.group - P.first);
-    const TileRange all = kv_tiles(A, P.e, P.first / A.group, (P.first + rows - 1) / A.group);
+    const TileRange all = kv_tiles(A, P.e, unsigned(P.first) / A.group, unsigned(P.first + rows - 1) / A.group);
     const int share = kv_share(A, all), begin = all.begin + P.split * share, end = min(all.end, begin + share);
-    if (P.split > 0 && begin >= end) return;
+    if (A.part && begin >= end) {
+        if (int(threadIdx.x) < rows) kv_store_lse(A, P, P.first + threadIdx.x, -INFINITY);
+        return;
+    }
     // this wave's rows, the tiles that any of them sees and those that all see whole
     const int first = P.first + 16 * NR * wave, mine = min(16 * NR, rows - 16 * NR * wave);
     Rows<D, NR> R;
-    kv_begin<T, D, NR>(A, P, first, R);
+    {
+        RowLoads<D, NR> W;
+        kv_begin_loads<D, NR>(A, P, first, R, W);
+        kv_begin<T, D, NR>(A, R, W);
+    }
     int see_from = 0, see_until = 0, clear_from = 0, clear_until = 0;
     if (mine > 0) {
-        const int i0 = first / A.group, i1 = (first + mine - 1) / A.group;
+        const int i0 = unsigned(first) / A.group, i1 = unsigned(first + mine - 1) / A.group;
         const TileRange t = kv_tiles(A, P.e, i0, i1);
         see_from = t.begin, see_until = t.end;
         clear_from = (kv_from(A, P.e, i1) + 63) >> 6, clear_until = max(kv_until(A, P.e, i0), 0) >> 6;
@@ -533,10 +857,9 @@ __global__ __launch_bounds__(256) void kv_block_kernel(const AttnCall A) {
                     const int d = 16 * dt + (lane & 15);
                     return *reinterpret_cast<const i32x4*>(vc + d * 64 + 16 * (g ^ kv_value_swap(d)));
                 };
-                if (tile >= clear_from && tile < clear_until && !__any(dead))
-                    kv_tile<false, D, NR>(R, k, v, kb, vb, tile * 64 + 16 * g, false);
-                else
-                    kv_tile<true, D, NR>(R, k, v, kb, vb, tile * 64 + 16 * g, dead);
+                i32x4 s[NR][4];
+                kv_scores<D, NR>(R, k, s);
+                kv_values<D, NR>(R, s, v, kb, vb, tile * 64 + 16 * g, dead, tile < clear_from || tile >= clear_until || __any(dead));
             }
             tile++;
             return more;
@@ -558,47 +881,49 @@ __global__ __launch_bounds__(256) void kv_block_kernel(const AttnCall A) {
             f32x4 o;
 #pragma unroll
             for (int j = 0; j < 4; j++) o[j] = __builtin_amdgcn_ldexpf(R.o[r][dt][j] * inv, R.base - 132);
-            kv_store4<T, D>(A, P, first + row, 16 * dt + 4 * g, o);
+            if (A.part) kv_store_part4<D>(A, P, first + row, 16 * dt + 4 * g, o);
+            else kv_store4<T, D>(A, P, first + row, 16 * dt + 4 * g, o);
         }
     }
 }
 
-// One wave for each row and head: its splits' parts, weighed by their sums.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void kv_join_kernel(const AttnCall A, int bm) {
-    const int lane = threadIdx.x & 63, u = blockIdx.x * 4 + (threadIdx.x >> 6), h = u % A.heads;
-    int entry, i;
-    if (u / A.heads >= A.b.total || !kv_locate(A.b, u / A.heads, [](int n) { return n; }, entry, i)) return;
-    const KvEntry e = kv_entry(A.c, A.b, entry);
-    const int row = i * A.group + h % A.group, first = row / bm * bm, rows = min(bm, e.count * A.group - first);
-    const TileRange t = kv_tiles(A, e, first / A.group, (first + rows - 1) / A.group);
-    const int share = kv_share(A, t), parts = (t.end - t.begin + share - 1) / share;
-    const int64_t at = int64_t(e.start + i) * A.heads + h;
-    constexpr int V = D / 64;
-    float m = -INFINITY, sum = 0.f, o[V] = {};
-    for (int s0 = 0; s0 < parts; s0 += 64) {
-        const float mine = s0 + lane < parts ? A.lse[at * A.splits + s0 + lane] : -INFINITY;
-        float top = mine;
-#pragma unroll
-        for (int w = 32; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
-        const float mn = fmaxf(m, top), al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-        m = mn;
-        float w = s0 + lane < parts ? (mine == mn ? 1.f : __builtin_amdgcn_exp2f(mine - mn)) : 0.f;
-        if (mine == -INFINITY) w = 0.f;
-        sum = sum * al + wave_sum(w);
-#pragma unroll
-        for (int j = 0; j < V; j++) o[j] *= al;
-        const int n = min(64, parts - s0);
-        for (int s = 0; s < n; s++) {
-            const float ws = __shfl(w, s);
-            const float* p = A.part + (at * A.splits + s0 + s) * D + lane * V;
-#pragma unroll
-            for (int j = 0; j < V; j++) o[j] = fmaf(ws, p[j], o[j]);
-        }
+// The splits of one row and head, weighed by their sums; a split that had
+// nothing to do has lse = -inf and its part is not used.  W waves (1, or 4 where
+// there are many splits); D / 4 lanes take one split's part, and the parts are
+// requested with the sums, before any weight is known, 4 splits ahead.
+template <typename T, int D, int W>
+__global__ __launch_bounds__(256) void kv_join_kernel(const AttnCall A) {
+    __shared__ Joiner<D, W> J;
+    constexpr int LANES = D / 4, SETS = 64 * W / LANES;
+    const int t = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+    // (grid: rows by heads, or by 4 heads)
+    const int h = W == 1 ? blockIdx.y * 4 + (threadIdx.x >> 6) : blockIdx.y;
+    int64_t row = blockIdx.x;
+    if (h >= A.heads) return;
+    if (A.b.cu) {  // which row of the call that is
+        int entry, i, start, count;
+        if (!kv_locate(A.b, int(row), [](int n) { return n; }, entry, i)) return;
+        kv_rows(A.b, entry, start, count);
+        row = start + i;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t at = row * A.heads + h;
+    const float* lse = A.lse + at * A.splits;
+    const f32x4* part = reinterpret_cast<const f32x4*>(A.part + at * A.splits * D) + t % LANES;
+    const int set = t / LANES;
+    float m = -INFINITY, sum = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < A.splits; s0 += 4 * SETS) {
+        f32x4 x[4];
+        float e[4];
 #pragma unroll
-    for (int j = 0; j < V; j++) A.out[at * D + lane * V + j] = to_storage<T>(o[j] * inv);
+        for (int j = 0; j < 4; j++) {
+            const int s = s0 + j * SETS + set;
+            e[j] = s < A.splits ? lse[s] : -INFINITY;
+            x[j] = s < A.splits ? part[int64_t(s) * LANES] : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        kv_merge4(e, x, m, sum, o);
+    }
+    if (J.join(t, m, sum, o)) kv_out4<T, D>(A, at, t, sum, o);
 }
 
 bool attention_sizes_ok(const char* who, const eq_kv_cache* c, int n_heads, int64_t n, int64_t total) {
@@ -618,19 +943,34 @@ bool attention_sizes_ok(const char* who, const eq_kv_cache* c, int n_heads, int6
 struct Plan {
     int rows;    // of a workgroup: 16 (stream), 64 or 128 (block)
     int64_t tiles;
-    int splits;
+    int splits;  // of a block's tokens
+    int groups;  // workgroups of a stream
     size_t part_bytes, lse_bytes;
 };
 Plan plan_attention(const eq_kv_cache* c, int n_heads, int64_t n, int64_t total, bool ragged) {
     Plan p;
     const int64_t group = n_heads / c->kv_heads, rows = n ? total * group / n : 0;  // of a sequence and KV head, on average
-    p.rows = rows <= 48 ? 16 : (rows <= 64 || c->head_dim > 128 ? 64 : 128);
-    p.tiles = ragged ? total * group / p.rows + n : n * ((total / (n ? n : 1) * group + p.rows - 1) / p.rows);
-    const int64_t groups = p.tiles * c->kv_heads, cap = (c->width * c->page_tokens + 63) / 64;
-    int64_t splits = groups ? (2 * device_cu_count() + groups - 1) / groups : 1;
+    const int64_t cap = (c->width * c->page_tokens + 63) / 64;
+    auto blocks = [&](int bm) {
+        return ragged ? total * group / bm + n : n * ((total / (n ? n : 1) * group + bm - 1) / bm);
+    };
+    const int64_t most = blocks(kStreamRows) * c->kv_heads;  // units of a stream (over 2^31 tiles are not listed)
+    p.rows = rows <= 48 && most < INT32_MAX / cap ? kStreamRows : (rows <= 64 || c->head_dim > 128 ? 64 : 128);
+    p.tiles = blocks(p.rows);
+    const int64_t units = p.tiles * c->kv_heads;
+    if (p.rows == kStreamRows) {
+        const int64_t runs = (units * cap + 3) / 4;  // at least a tile for each of 4 waves
+        p.splits = 1;
+        p.groups = int(runs < 2 * device_cu_count() ? runs : 2 * device_cu_count());
+        p.part_bytes = size_t(p.groups) * 8 * kStreamRows * c->head_dim * 4;
+        p.lse_bytes = (size_t(p.groups) * 8 * kStreamRows * 4 + 255) & ~size_t(255);
+        return p;
+    }
+    int64_t splits = units ? (2 * device_cu_count() + units - 1) / units : 1;
     if (splits > (cap + 3) / 4) splits = (cap + 3) / 4;
     if (splits > 1024) splits = 1024;
     p.splits = splits < 1 ? 1 : int(splits);
+    p.groups = 0;
     p.part_bytes = p.splits > 1 ? size_t(total) * n_heads * p.splits * c->head_dim * 4 : 0;
     p.lse_bytes = p.splits > 1 ? (size_t(total) * n_heads * p.splits * 4 + 255) & ~size_t(255) : 0;
     return p;
@@ -679,14 +1019,14 @@ extern "C" int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n
     }
     const Plan plan = plan_attention(cache, n_heads, n, total, cu != nullptr);
     const int64_t blocks = plan.tiles * cache->kv_heads * plan.splits;
-    if (blocks >= (1 << 24)) {  // a grid of under 2^32 threads
+    if (blocks >= (1 << 24) || total >= (1 << 24)) {  // grids of under 2^32 threads a side
         set_error("eq_kv_attention: too many rows");
         return 1;
     }
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     AttnCall A;
     A.part = A.lse = nullptr;
-    if (plan.splits > 1) {
+    if (plan.part_bytes) {
         const size_t need = plan.part_bytes + plan.lse_bytes;
         if (scratch && (scratch_bytes < 0 || size_t(scratch_bytes) < need || !aligned(scratch, 256))) {
             set_error("eq_kv_attention: needs " + std::to_string(need) + " bytes of 256-byte aligned scratch");
@@ -712,16 +1052,22 @@ extern "C" int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n
     A.group = n_heads / cache->kv_heads;
     A.tiles = int(plan.tiles);
     A.splits = plan.splits;
+    A.groups = plan.groups;
     A.window = int(window < kKvMaxLength ? window : kKvMaxLength);
     A.causal = causal;
-    const dim3 grid{unsigned(blocks)}, join(unsigned((total * n_heads + 3) / 4));
+    const dim3 grid{unsigned(blocks)};
     auto go = [&](auto t, auto d) {
         typedef decltype(t) T;
         constexpr int DIM = decltype(d)::value;
-        if (plan.rows == 16) kv_stream_kernel<T, DIM><<<grid, dim3(256), 0, st>>>(A);
-        else if (plan.rows == 64) kv_block_kernel<T, DIM, 1><<<grid, dim3(256), 0, st>>>(A);
+        if (plan.rows == kStreamRows) {
+            kv_stream_kernel<T, DIM><<<dim3(unsigned(plan.groups)), dim3(256), 0, st>>>(A);
+            kv_stream_join_kernel<T, DIM><<<dim3(unsigned(total), unsigned(n_heads)), dim3(256), 0, st>>>(A);
+            return;
+        }
+        if (plan.rows == 64) kv_block_kernel<T, DIM, 1><<<grid, dim3(256), 0, st>>>(A);
         else if constexpr (DIM <= 128) kv_block_kernel<T, DIM, 2><<<grid, dim3(256), 0, st>>>(A);
-        if (plan.splits > 1) kv_join_kernel<T, DIM><<<join, dim3(256), 0, st>>>(A, plan.rows);
+        if (plan.splits > 16) kv_join_kernel<T, DIM, 4><<<dim3(unsigned(total), unsigned(n_heads)), dim3(256), 0, st>>>(A);
+        else if (plan.splits > 1) kv_join_kernel<T, DIM, 1><<<dim3(unsigned(total), unsigned((n_heads + 3) / 4)), dim3(256), 0, st>>>(A);
     };
     auto with_d = [&](auto t) {
         if (D == 64) go(t, std::integral_constant<int, 64>{});

@@ -100,7 +100,7 @@ __device__ __forceinline__ bool kv_locate(const KvBatch& b, int u, F units, int&
 }
 
 __device__ __forceinline__ int kv_page(const KvView& c, int seq, int index) {
-    if (unsigned(index) >= unsigned(c.width)) return -1;
+    if (seq < 0 || unsigned(index) >= unsigned(c.width)) return -1;
     const int id = c.tables[int64_t(seq) * c.width + index];
     return unsigned(id) < unsigned(c.pages) ? id : -1;
 }

@@ -50,10 +50,19 @@ def rope_table(freqs, positions: int, device=None) -> torch.Tensor:
     return t.to(torch.device("cuda") if device is None else device)
 
 
-def _ids(t: torch.Tensor, what: str, device: torch.device) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.device != device or t.dim() != 1:
-        raise EreduError(f"{what} must be a one-dimensional int32 tensor on {device}")
+def _ids(t: torch.Tensor, what: str, index: int) -> torch.Tensor:
+    if t.dtype is not torch.int32 or t.get_device() != index or t.dim() != 1:
+        raise EreduError(f"{what} must be a one-dimensional int32 tensor on cuda:{index}")
     return t if t.is_contiguous() else t.contiguous()
+
+
+# Whether the current stream is being captured (a method of torch.cuda without its wrapper).
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+# Scratch of an eager call up to this size comes from the library's workspace of
+# the stream, which saves a call its allocation (about 3 us); more comes from torch and
+# goes back to it.
+_OWN_SCRATCH = 64 << 20
 
 
 class PagedKVCache:
@@ -112,16 +121,17 @@ class PagedKVCache:
         self.missing = torch.zeros((1,), dtype=torch.int32, device=k_codes.device)
         self.n_layers, self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = L, P, H, T, D
         self.max_seqs, self.max_pages_per_seq = S, W
+        self._scale = D ** -0.5
         self.device = k_codes.device
         c = _native.KvCache(*(t.data_ptr() for t in (k_codes, v_codes, k_scales, v_scales, tables, lengths, refs,
                                                      self.missing)), L, P, S, W, H, T, D)
-        self._c, self._ref = c, ctypes.byref(c)
+        self._c, self._ref, self._index = c, ctypes.byref(c), k_codes.get_device()
 
     # ------------------------------------------------------------ operands
 
     def _here(self) -> int:
         """The current stream, once the current device is the cache's."""
-        if (_get_device() if _get_device is not None else torch.cuda.current_device()) != self.device.index:
+        if (_get_device() if _get_device is not None else torch.cuda.current_device()) != self._index:
             raise EreduError(f"the cache lives on {self.device}: make that the current device")
         return _stream()
 
@@ -129,7 +139,7 @@ class PagedKVCache:
         """[rows, heads, dim] (or [rows, heads * dim]) with heads and dimensions
         contiguous; rows may lie at any stride of a multiple of 8, as parts of a
         fused projection do."""
-        if t.device != self.device:
+        if t.get_device() != self._index:
             raise EreduError(f"{what} must live on {self.device}")
         if t.dtype not in _HALVES:
             raise EreduError(f"{what} must be bfloat16 or float16, got {t.dtype}")
@@ -138,18 +148,20 @@ class PagedKVCache:
             t = t.unflatten(1, (-1, D))
         if t.dim() != 3 or t.shape[2] != D:
             raise EreduError(f"{what} must be [rows, heads, {D}], got {tuple(t.shape)}")
+        if t.is_contiguous() and t.data_ptr() % 16 == 0:
+            return t
         if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != D) or t.stride(0) % 8 or \
                 t.stride(0) < t.shape[1] * D or t.data_ptr() % 16:
             t = t.clone(memory_format=torch.contiguous_format)
         return t
 
     def _batch(self, seqs: torch.Tensor, cu: Optional[torch.Tensor], total: int) -> Tuple[torch.Tensor, int, Optional[torch.Tensor]]:
-        seqs = _ids(seqs, "seqs", self.device)
-        n = seqs.numel()
+        seqs = _ids(seqs, "seqs", self._index)
+        n = seqs.shape[0]
         if cu is not None:
-            cu = _ids(cu, "cu", self.device)
-            if cu.numel() != n + 1:
-                raise EreduError(f"cu must hold {n + 1} offsets for {n} sequences, got {cu.numel()}")
+            cu = _ids(cu, "cu", self._index)
+            if cu.shape[0] != n + 1:
+                raise EreduError(f"cu must hold {n + 1} offsets for {n} sequences, got {cu.shape[0]}")
         elif total % n if n else total:
             raise EreduError(f"{total} rows do not divide evenly among {n} sequences: pass cu")
         return seqs, n, cu
@@ -157,17 +169,21 @@ class PagedKVCache:
     def _rope(self, rope: Optional[torch.Tensor]) -> Tuple[Optional[int], int]:
         if rope is None:
             return None, 0
-        if rope.dtype != torch.float32 or rope.dim() != 2 or rope.shape[1] != self.head_dim or \
-                not rope.is_contiguous() or rope.device != self.device:
+        if rope.dtype is not torch.float32 or rope.dim() != 2 or rope.shape[1] != self.head_dim or \
+                not rope.is_contiguous() or rope.get_device() != self._index:
             raise EreduError(f"rope must be a contiguous float32 tensor [positions, {self.head_dim}] on {self.device}")
         return rope.data_ptr(), rope.shape[0]
 
-    def _scratch(self, need: int) -> Optional[torch.Tensor]:
-        # From torch's allocator, in stream order (a captured graph's own pool
-        # under capture), so calls and graphs on several streams share nothing.
+    def _scratch(self, need: int) -> Tuple[Optional[int], int, Optional[torch.Tensor]]:
+        """Scratch of a call: the library's workspace of the stream (None), or, under
+        capture and where it is large, torch's memory, in stream order and a captured
+        graph's own, so that graphs share nothing."""
         if need < 0:
             check(1)
-        return torch.empty((need,), dtype=torch.uint8, device=self.device) if need else None
+        if need <= _OWN_SCRATCH and not _capturing():
+            return None, 0, None
+        t = torch.empty((need,), dtype=torch.uint8, device=self.device)
+        return t.data_ptr(), need, t
 
     # ------------------------------------------------------------ tokens
 
@@ -181,8 +197,8 @@ class PagedKVCache:
             raise EreduError(f"k and v must both be [rows, {self.n_kv_heads}, {self.head_dim}] of one dtype")
         seqs, n, cu = self._batch(seqs, cu, k.shape[0])
         rp, rn = self._rope(rope)
-        check(_native.lib().eq_kv_append(self._ref, int(layer), k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0),
-                                         seqs.data_ptr(), n, cu.data_ptr() if cu is not None else None, k.shape[0], rp,
+        check(_native.lib().eq_kv_append(self._ref, layer, k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0),
+                                         seqs.data_ptr(), n, None if cu is None else cu.data_ptr(), k.shape[0], rp,
                                          rn, _DTYPE_CODE[k.dtype], self._here()))
 
     def attention(self, layer: int, q: torch.Tensor, seqs: torch.Tensor, cu: Optional[torch.Tensor] = None,
@@ -200,15 +216,15 @@ class PagedKVCache:
         rp, rn = self._rope(rope)
         if out is None:
             out = torch.empty((rows, heads, D), dtype=q.dtype, device=self.device)
-        elif out.dtype != q.dtype or out.numel() != q.numel() or not out.is_contiguous() or out.device != self.device:
+        elif out.dtype != q.dtype or out.numel() != q.numel() or not out.is_contiguous() or out.get_device() != self._index:
             raise EreduError(f"out must be a contiguous {q.dtype} tensor of {q.numel()} values on {self.device}")
         L, st = _native.lib(), self._here()
-        ws = self._scratch(L.eq_kv_attention_scratch(self._ref, heads, n, rows, cu is not None))
-        check(L.eq_kv_attention(out.data_ptr(), q.data_ptr(), q.stride(0), heads, self._ref, int(layer),
-                                seqs.data_ptr(), n, cu.data_ptr() if cu is not None else None, rows,
-                                D ** -0.5 if scale is None else float(scale), bool(causal), int(window), rp, rn,
-                                _DTYPE_CODE[q.dtype], ws.data_ptr() if ws is not None else None,
-                                ws.numel() if ws is not None else 0, st))
+        wp = wn = ws = None
+        if rows * heads > 8192 or _capturing():  # (fewer rows take a few MB of the library's workspace)
+            wp, wn, ws = self._scratch(L.eq_kv_attention_scratch(self._ref, heads, n, rows, cu is not None))
+        check(L.eq_kv_attention(out.data_ptr(), q.data_ptr(), q.stride(0), heads, self._ref, layer, seqs.data_ptr(), n,
+                                None if cu is None else cu.data_ptr(), rows, self._scale if scale is None else scale,
+                                causal, window, rp, rn, _DTYPE_CODE[q.dtype], wp, wn or 0, st))
         return out
 
     def read(self, layer: int, seqs: torch.Tensor, tokens: Union[int, torch.Tensor], total: Optional[int] = None,
@@ -224,8 +240,8 @@ class PagedKVCache:
             raise EreduError("read needs a number of tokens that is not negative, and float32, float16 or bfloat16")
         seqs, n, cu = self._batch(seqs, cu, rows)
         k, v = (torch.empty((rows, self.n_kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2))
-        check(_native.lib().eq_kv_read(k.data_ptr(), v.data_ptr(), self._ref, int(layer), seqs.data_ptr(), n,
-                                       cu.data_ptr() if cu is not None else None, rows, _DTYPE_CODE[dtype],
+        check(_native.lib().eq_kv_read(k.data_ptr(), v.data_ptr(), self._ref, layer, seqs.data_ptr(), n,
+                                       None if cu is None else cu.data_ptr(), rows, _DTYPE_CODE[dtype],
                                        self._here()))
         return k, v
 
@@ -239,30 +255,30 @@ class PagedKVCache:
         cu = tokens if isinstance(tokens, torch.Tensor) else None
         seqs, n, cu = self._batch(seqs, cu, 0)
         L, st = _native.lib(), self._here()
-        ws = self._scratch(L.eq_kv_pages_scratch(self._ref, n))
-        check(L.eq_kv_extend(self._ref, seqs.data_ptr(), n, cu.data_ptr() if cu is not None else None,
-                             0 if cu is not None else int(tokens), ws.data_ptr(), ws.numel(), st))
+        wp, wn, ws = self._scratch(L.eq_kv_pages_scratch(self._ref, n))
+        check(L.eq_kv_extend(self._ref, seqs.data_ptr(), n, None if cu is None else cu.data_ptr(),
+                             0 if cu is not None else tokens, wp, wn, st))
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Sequence dst[i] becomes a copy of src[i], sharing its pages; all pairs from
         the state before the call, so beams can be permuted (C ABI: eq_kv_fork)."""
-        src, dst = _ids(src, "src", self.device), _ids(dst, "dst", self.device)
+        src, dst = _ids(src, "src", self._index), _ids(dst, "dst", self._index)
         if src.numel() != dst.numel():
             raise EreduError(f"src and dst must be of one length, got {src.numel()} and {dst.numel()}")
         L, st = _native.lib(), self._here()
-        ws = self._scratch(L.eq_kv_pages_scratch(self._ref, src.numel()))
-        check(L.eq_kv_fork(self._ref, src.data_ptr(), dst.data_ptr(), src.numel(), ws.data_ptr(), ws.numel(), st))
+        wp, wn, ws = self._scratch(L.eq_kv_pages_scratch(self._ref, src.numel()))
+        check(L.eq_kv_fork(self._ref, src.data_ptr(), dst.data_ptr(), src.numel(), wp, wn, st))
 
     def free(self, seqs: torch.Tensor) -> None:
         """Empties the sequences and gives up their pages (C ABI: eq_kv_free)."""
-        seqs = _ids(seqs, "seqs", self.device)
+        seqs = _ids(seqs, "seqs", self._index)
         check(_native.lib().eq_kv_free(self._ref, seqs.data_ptr(), seqs.numel(), self._here()))
 
     def compact(self) -> None:
         """Moves the pages in use to the lowest indices (C ABI: eq_kv_compact)."""
         L, st = _native.lib(), self._here()
-        ws = self._scratch(L.eq_kv_pages_scratch(self._ref, 0))
-        check(L.eq_kv_compact(self._ref, ws.data_ptr(), ws.numel(), st))
+        wp, wn, ws = self._scratch(L.eq_kv_pages_scratch(self._ref, 0))
+        check(L.eq_kv_compact(self._ref, wp, wn, st))
 
     def free_pages(self) -> int:
         """Pages that no sequence holds (waits for the GPU)."""
