@@ -166,19 +166,20 @@ __device__ __forceinline__ void kv_scores(const Rows<D, NR>& R, KF k, i32x4 (&s)
     }
 }
 
-// The softmax of those scores and their values: v(dt) gives the operands, kb and
-// vb are this lane group's scale bytes, j0 its first token; dead: its page is missing.
-// edge (the same for the wave): some row does not see some of the tokens; their
-// scores are set below all others for the maximum, their exponents to -inf.
-template <int D, int NR, typename VF>
-__device__ __forceinline__ void kv_values(Rows<D, NR>& R, i32x4 (&s)[NR][4], VF v, int kb, int vb, int j0, bool dead, bool edge) {
+// The softmax of those scores: the probabilities p, their sums, and the
+// states so far brought to the tile's maximum (if that moves) and base.  kb is
+// this lane group's key scale byte, nan: it or the value's is 255; j0 its first
+// token; dead: its page is missing; base: the largest value scale byte so far,
+// this tile's included.  edge (the same for the wave): some row does not see some of the
+// tokens; their scores are set below all others for the maximum, their exponents to -inf.
+template <int D, int NR>
+__device__ __forceinline__ void kv_softmax(Rows<D, NR>& R, i32x4 (&s)[NR][4], int kb, bool nan, int j0, bool dead, bool edge,
+                                           int base, h16x8 (&p)[NR][2]) {
     constexpr int DT = D / 16;
-    const bool nan = kb == 255 || vb == 255;
     const float kf = nan ? __uint_as_float(0x7fc00000u) : e8m0_to_f32(uint32_t(kb));
-    const int ev = nan || dead ? 0 : vb;
     float f[NR], top[NR];
     int first[NR], seen[NR];
-    bool need = ev > R.base;
+    bool need = base > R.base;
 #pragma unroll
     for (int r = 0; r < NR; r++) first[r] = 0, seen[r] = 16;
     if (edge) {
@@ -201,9 +202,6 @@ __device__ __forceinline__ void kv_values(Rows<D, NR>& R, i32x4 (&s)[NR][4], VF 
         need |= top[r] > R.m[r] + kMaxSlack;
     }
     if (__any(need)) {
-        const int up = max(max(__builtin_amdgcn_readlane(ev, 0), __builtin_amdgcn_readlane(ev, 16)),
-                           max(__builtin_amdgcn_readlane(ev, 32), __builtin_amdgcn_readlane(ev, 48)));
-        const int base = max(R.base, up);
         const float down = __builtin_amdgcn_ldexpf(1.f, R.base - base);
         R.base = base;
 #pragma unroll
@@ -231,7 +229,6 @@ __device__ __forceinline__ void kv_values(Rows<D, NR>& R, i32x4 (&s)[NR][4], VF 
             for (int n = 0; n < 16; n++)
                 if (unsigned(n - first[r]) >= unsigned(seen[r])) x[r][n >> 2][n & 3] = -INFINITY;
     }
-    h16x8 p[NR][2];
 #pragma unroll
     for (int r = 0; r < NR; r++) {
         float sum = 0.f;
@@ -248,31 +245,52 @@ __device__ __forceinline__ void kv_values(Rows<D, NR>& R, i32x4 (&s)[NR][4], VF 
         }
         R.l[r] += sum;
     }
-    // 2^(15 + ev - base) in f16, subnormal below 2^-14
-    const int ex = 30 + ev - R.base;
-    const uint16_t bits = uint16_t(ex >= 1 ? ex << 10 : (ex >= -9 ? 1 << (9 + ex) : 0));
-    const _Float16 sc = __builtin_bit_cast(_Float16, bits);
-    const h16x2 sc2 = {sc, sc}, off2 = sc2 * h16x2{_Float16(-1.125f), _Float16(-1.125f)};
+}
+
+// What a page's codes become f16 by: 1 + (c + 128) / 1024 times `mul`, plus `add`,
+// is c * 2^(5 + vb - base); subnormal below 2^-29 of base, and 0 at last.
+struct Convert {
+    h16x2 mul, add;
+    __device__ __forceinline__ Convert(int vb, int base) {
+        const int ex = 30 + vb - base;
+        const uint16_t bits = uint16_t(ex >= 1 ? ex << 10 : (ex >= -9 ? 1 << (9 + ex) : 0));
+        const _Float16 m = __builtin_bit_cast(_Float16, bits);
+        mul = h16x2{m, m};
+        add = mul * h16x2{_Float16(-1.125f), _Float16(-1.125f)};
+    }
+    // 8 codes
+    __device__ __forceinline__ h16x8 operator()(uint32_t w0, uint32_t w1) const {
+        h16x8 a;
+        const uint32_t w[2] = {w0 ^ 0x80808080u, w1 ^ 0x80808080u};  // code + 128
 #pragma unroll
-    for (int dt = 0; dt < DT; dt++) {
-        const i32x4 w = v(dt);
+        for (int i = 0; i < 2; i++) {
+            const h16x2 x0 = __builtin_bit_cast(h16x2, __builtin_amdgcn_perm(0x3c3c3c3cu, w[i], 0x04010400u));
+            const h16x2 x1 = __builtin_bit_cast(h16x2, __builtin_amdgcn_perm(0x3c3c3c3cu, w[i], 0x04030402u));
+            const h16x2 y0 = __builtin_elementwise_fma(x0, mul, add), y1 = __builtin_elementwise_fma(x1, mul, add);
+            a[4 * i] = y0[0], a[4 * i + 1] = y0[1], a[4 * i + 2] = y1[0], a[4 * i + 3] = y1[1];
+        }
+        return a;
+    }
+};
+
+// v(dt, u): this lane's 8 values of dimension 16 dt + lane % 16, tokens 8 u .. of its group's 16.
+template <int D, int NR, typename VF>
+__device__ __forceinline__ void kv_values(Rows<D, NR>& R, const h16x8 (&p)[NR][2], VF v) {
+#pragma unroll
+    for (int dt = 0; dt < D / 16; dt++) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            h16x8 a;
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const uint32_t c = uint32_t(w[2 * u + i]) ^ 0x80808080u;  // code + 128
-                const h16x2 x0 = __builtin_bit_cast(h16x2, __builtin_amdgcn_perm(0x3c3c3c3cu, c, 0x04010400u));
-                const h16x2 x1 = __builtin_bit_cast(h16x2, __builtin_amdgcn_perm(0x3c3c3c3cu, c, 0x04030402u));
-                const h16x2 y0 = __builtin_elementwise_fma(x0, sc2, off2), y1 = __builtin_elementwise_fma(x1, sc2, off2);
-                a[4 * i] = y0[0], a[4 * i + 1] = y0[1], a[4 * i + 2] = y1[0], a[4 * i + 3] = y1[1];
-            }
+            const h16x8 a = v(dt, u);
 #pragma unroll
             for (int r = 0; r < NR; r++) R.o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p[r][u], R.o[r][dt], 0, 0, 0);
         }
-        // (values converted further ahead only take registers)
-        if (dt % 2 == 1) __builtin_amdgcn_sched_barrier(0);
     }
+}
+
+// The largest of four lane groups' values, in a scalar register.
+__device__ __forceinline__ int kv_group_max(int v) {
+    return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+               max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
 
 struct AttnCall {
@@ -606,9 +624,15 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_stream_kernel(const 
                 scales(idg, kbn, vbn);
                 ida2 = page(tile + 2, a), idg2 = page(tile + 2, g);
             }
-            auto v = [&](int dt) __attribute__((always_inline)) { return t.v[dt]; };
             const bool dead = idd < 0;
-            kv_values<D, NR>(R, s, v, kb, vb, tile * 64 + 16 * g, dead, tile < clear_from || tile >= clear_until || __any(dead));
+            const int ev = vb == 255 || dead ? 0 : vb, top = max(R.base, kv_group_max(ev));
+            h16x8 p[NR][2];
+            kv_softmax<D, NR>(R, s, kb, kb == 255 || vb == 255, tile * 64 + 16 * g, dead,
+                              tile < clear_from || tile >= clear_until || __any(dead), top, p);
+            const Convert to(ev, top);
+            kv_values<D, NR>(R, p, [&](int dt, int u) __attribute__((always_inline)) {
+                return to(uint32_t(t.v[dt][2 * u]), uint32_t(t.v[dt][2 * u + 1]));
+            });
             if (more) kv_fetch_values<D>(A, P, tile + 1, idg, t);
             idd = idg, kb = kbn, vb = vbn, ida = ida2, idg = idg2;
         }
@@ -753,55 +777,51 @@ __global__ __launch_bounds__(256) void kv_stream_join_kernel(const AttnCall A) {
 // ------------------------------------------ many rows: blocks of rows over shared tiles
 //
 // 64 * NR rows a workgroup, 16 * NR for each of its 4 waves, all over the same
-// tokens: a tile's 64 keys and values go from memory straight to LDS once for the
-// workgroup, one tile ahead, and each wave takes its operands from there.
-// 16-byte pieces of a row are swapped by an exclusive or with bits of the row, so
-// that the 8 lanes of a read lie in different banks: keys (row = token 16 a + 4 t + b,
-// read for all a and b at once) by b and a's low bit, values (row = dimension) by its
-// next bits.
+// tokens.  A tile's keys go from memory straight to LDS, its values through
+// registers, where they become f16 once for the workgroup (a wave converting them for
+// itself had 3/8 of its vector instructions for that), one tile ahead, and
+// each wave takes its operands from there.  16-byte pieces of a row are swapped by
+// an exclusive or with bits of the row, so that the 8 lanes of a read lie in
+// different banks: keys (row = token 16 a + 4 t + b, read for all a and b at once) by b
+// and a's low bit, values (row = dimension, 8 pieces of 8 tokens) by its low bits.
 template <int D>
 __device__ __forceinline__ int kv_key_swap(int token) {
     return D >= 128 ? (token & 3) | (token >> 2 & 4) : (token >> 1 & 1) | (token >> 3 & 2);
 }
-__device__ __forceinline__ int kv_value_swap(int d) { return d >> 1 & 3; }
 
 typedef __attribute__((address_space(3))) char lds_char;
 
-// A wave's share of a tile: 64 lanes' pieces land side by side, so the swap is
-// in the addresses they come from.  idg: this lane group's page, idv: that of the
-// lane's value pieces.
+// A wave's share of a tile's keys: 64 lanes' pieces land side by side, so the swap
+// is in the addresses they come from, which are a page's (a scalar: a wave's 1024 / D
+// tokens lie in one block of 16) and the lane's in it, the same for every tile.
 template <int D>
-__device__ __forceinline__ void kv_stage(const AttnCall& A, const Place& P, int tile, int idg, int idv, lds_char* kbuf,
-                                         lds_char* vbuf) {
+__device__ __forceinline__ int kv_key_offset(int j, int T) {
     constexpr int KP = D / 16;  // 16-byte pieces of a key
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), T = 1 << A.c.log2_page;
+    const int p = (j * 4 + int(threadIdx.x >> 6)) * 64 + (threadIdx.x & 63), token = p / KP;
+    return (token & (T - 1)) * D + 16 * ((p % KP) ^ kv_key_swap<D>(token));
+}
+template <int D>
+__device__ __forceinline__ void kv_stage_keys(const AttnCall& A, const Place& P, int tile, int idg, const int (&ofs)[D / 64],
+                                              lds_char* buf) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), T = 1 << A.c.log2_page;
 #pragma unroll
     for (int j = 0; j < D / 64; j++) {
-        const int p = (j * 4 + wave) * 64 + lane, token = p / KP, c = (p % KP) ^ kv_key_swap<D>(token);
-        const int block = __builtin_amdgcn_readfirstlane(token >> 4);  // (a wave's 1024 / D tokens lie in one block)
-        const int id = __builtin_amdgcn_readlane(idg, 16 * block);
-        const int8_t* src = A.c.k + ((int64_t(max(id, 0)) * A.c.kv_heads + P.kvh) * T + ((tile * 64 + token) & (T - 1))) * D + 16 * c;
-        __builtin_amdgcn_global_load_lds(
-            const_cast<int8_t*>(src), (__attribute__((address_space(3))) void*)(kbuf + (j * 4 + wave) * 1024), 16, 0, 0);
-    }
-    const int g = (lane & 3) ^ kv_value_swap(lane >> 2);
-    const int8_t* src0 = A.c.v + (int64_t(max(idv, 0)) * A.c.kv_heads + P.kvh) * D * T + ((tile * 64 + 16 * g) & (T - 1));
-#pragma unroll
-    for (int j = 0; j < D / 64; j++) {
-        const int d = (j * 4 + wave) * 16 + (lane >> 2);
-        __builtin_amdgcn_global_load_lds(
-            const_cast<int8_t*>(src0 + d * T), (__attribute__((address_space(3))) void*)(vbuf + (j * 4 + wave) * 1024), 16, 0, 0);
+        const int id = __builtin_amdgcn_readlane(idg, (j * 4 + wave) * 64 / D * 16);  // of token block (j * 4 + wave) * 64 / D
+        const int8_t* page = A.c.k + ((int64_t(max(id, 0)) * A.c.kv_heads + P.kvh) * T + (tile * 64 & (T - 1))) * D;
+        __builtin_amdgcn_global_load_lds(const_cast<int8_t*>(page) + unsigned(ofs[j]),
+                                         (__attribute__((address_space(3))) void*)(buf + (j * 4 + wave) * 1024), 16, 0, 0);
     }
 }
 
 template <typename T, int D, int NR>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_block_kernel(const AttnCall A) {
     constexpr int BM = 64 * NR;
-    __shared__ __attribute__((aligned(16))) char k0[64 * D], k1[64 * D], v0[64 * D], v1[64 * D];
+    __shared__ __attribute__((aligned(16))) char k0[64 * D], k1[64 * D];
+    __shared__ __attribute__((aligned(16))) h16x8 v0[8 * D], v1[8 * D];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     Place P;
     if (!kv_place<BM>(A, P)) return;
-    const int rows = min(BM, P.e.count * A.group - P.first);
+    const int rows = min(BM, P.e.count * int(A.group) - P.first);
     const TileRange all = kv_tiles(A, P.e, unsigned(P.first) / A.group, unsigned(P.first + rows - 1) / A.group);
     const int share = kv_share(A, all), begin = all.begin + P.split * share, end = min(all.end, begin + share);
     if (A.part && begin >= end) {
@@ -823,44 +843,62 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_block_kernel(const A
         see_from = t.begin, see_until = t.end;
         clear_from = (kv_from(A, P.e, i1) + 63) >> 6, clear_until = max(kv_until(A, P.e, i0), 0) >> 6;
     }
-    const int gv = (lane & 3) ^ kv_value_swap(lane >> 2);
+    const int page_tokens = 1 << A.c.log2_page;
+    int ofs[D / 64];
+#pragma unroll
+    for (int j = 0; j < D / 64; j++) ofs[j] = kv_key_offset<D>(j, page_tokens);
+    // of the values, this thread's pieces are the 16 tokens 16 gv .. of dimensions tid / 4 + 64 j
+    const int gv = lane & 3, dv = threadIdx.x >> 2;
     auto page = [&](int tile, int block) { return kv_page(A.c, P.e.seq, (tile * 64 + 16 * block) >> A.c.log2_page); };
     if (begin < end) {
-        int idg = page(begin, g), idv = page(begin, gv);
-        int kb, vb, kbn, vbn, idn = idg;
-        auto scales = [&](int id, int& x, int& y) __attribute__((always_inline)) {
-            const int64_t at = int64_t(max(id, 0)) * A.c.kv_heads + P.kvh;
-            x = A.c.ks[at], y = A.c.vs[at];
+        int tile = begin, base = 0, base_next = 0;
+        int idg = page(tile, g), idv = page(tile, gv), idn, kb, vb, kbn, vbn, vbv;
+        uint4 raw[D / 64];
+        // requests tile `t` (pages idg, idv): its scales, values and keys
+        auto request = [&](int t, char* kbuf) __attribute__((always_inline)) {
+            const int64_t at = int64_t(max(idg, 0)) * A.c.kv_heads + P.kvh, av = int64_t(max(idv, 0)) * A.c.kv_heads + P.kvh;
+            kbn = A.c.ks[at], vbn = A.c.vs[at], vbv = A.c.vs[av];
+            vbv = idv < 0 || vbv == 255 ? 0 : vbv;
+            const int8_t* src = A.c.v + (av * D + dv) * page_tokens + ((t * 64 + 16 * gv) & (page_tokens - 1));
+#pragma unroll
+            for (int j = 0; j < D / 64; j++) raw[j] = *reinterpret_cast<const uint4*>(src + 64 * j * page_tokens);
+            kv_stage_keys<D>(A, P, t, idg, ofs, (lds_char*)kbuf);
+            idn = idg;
+            if (t + 1 < end) idg = page(t + 1, g), idv = page(t + 1, gv);
         };
-        scales(idg, kbn, vbn);
-        kv_stage<D>(A, P, begin, idg, idv, (lds_char*)k0, (lds_char*)v0);
-        int tile = begin;
-        if (tile + 1 < end) idg = page(tile + 1, g), idv = page(tile + 1, gv);
-        auto step = [&](const char* kc, const char* vc, char* kn, char* vn) __attribute__((always_inline)) {
-            __syncthreads();  // this tile is there, and the other buffers are read
-            const bool dead = idn < 0;
-            kb = kbn, vb = vbn;
-            const bool more = tile + 1 < end;
-            if (more) {
-                scales(idg, kbn, vbn);
-                idn = idg;
-                const int sg = idg, sv = idv;
-                if (tile + 2 < end) idg = page(tile + 2, g), idv = page(tile + 2, gv);
-                kv_stage<D>(A, P, tile + 1, sg, sv, (lds_char*)kn, (lds_char*)vn);
+        // its values as f16
+        auto convert = [&](h16x8* vbuf) __attribute__((always_inline)) {
+            base_next = max(base, kv_group_max(idn < 0 || vbn == 255 ? 0 : vbn));
+            const Convert to(vbv, base_next);
+#pragma unroll
+            for (int j = 0; j < D / 64; j++) {
+                const int d = dv + 64 * j;
+                vbuf[8 * d + ((2 * gv) ^ (d & 7))] = to(raw[j].x, raw[j].y);
+                vbuf[8 * d + ((2 * gv + 1) ^ (d & 7))] = to(raw[j].z, raw[j].w);
             }
+        };
+        request(tile, k0);
+        convert(v0);
+        auto step = [&](const char* kc, const h16x8* vc, char* kn, h16x8* vn) __attribute__((always_inline)) {
+            __syncthreads();  // this tile is there, and the other buffers are read
+            const bool dead = idn < 0, more = tile + 1 < end;
+            kb = kbn, vb = vbn, base = base_next;
+            if (more) request(tile + 1, kn);
             if (tile >= see_from && tile < see_until) {
-                auto k = [&](int t, int ks) __attribute__((always_inline)) {
+                i32x4 s[NR][4];
+                kv_scores<D, NR>(R, [&](int t, int ks) __attribute__((always_inline)) {
                     const int token = 4 * (lane & 12) + 4 * t + (lane & 3);
                     return *reinterpret_cast<const i32x4*>(kc + token * D + 16 * ((4 * ks + g) ^ kv_key_swap<D>(token)));
-                };
-                auto v = [&](int dt) __attribute__((always_inline)) {
+                }, s);
+                h16x8 p[NR][2];
+                kv_softmax<D, NR>(R, s, kb, kb == 255 || vb == 255, tile * 64 + 16 * g, dead,
+                                  tile < clear_from || tile >= clear_until || __any(dead), base, p);
+                kv_values<D, NR>(R, p, [&](int dt, int u) __attribute__((always_inline)) {
                     const int d = 16 * dt + (lane & 15);
-                    return *reinterpret_cast<const i32x4*>(vc + d * 64 + 16 * (g ^ kv_value_swap(d)));
-                };
-                i32x4 s[NR][4];
-                kv_scores<D, NR>(R, k, s);
-                kv_values<D, NR>(R, s, v, kb, vb, tile * 64 + 16 * g, dead, tile < clear_from || tile >= clear_until || __any(dead));
+                    return vc[8 * d + ((2 * g + u) ^ (d & 7))];
+                });
             }
+            if (more) convert(vn);
             tile++;
             return more;
         };
