@@ -155,13 +155,12 @@ __device__ __forceinline__ void kv_scores(const Rows<D, NR>& R, KF k, i32x4 (&s)
         for (int ks = 0; ks < KS; ks++) a[ks] = k(t, ks);
 #pragma unroll
         for (int r = 0; r < NR; r++) {
-            i32x4 acc = {0, 0, 0, 0};
+            i32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[ks], R.hi[r][ks], acc, 0, 0, 0);
-            acc = acc << 8;
+            for (int ks = 0; ks < KS; ks++) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[ks], R.hi[r][ks], hi, 0, 0, 0);
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[ks], R.lo[r][ks], acc, 0, 0, 0);
-            s[r][t] = acc;
+            for (int ks = 0; ks < KS; ks++) lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[ks], R.lo[r][ks], lo, 0, 0, 0);
+            s[r][t] = (hi << 8) + lo;
         }
     }
 }
@@ -594,37 +593,44 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_stream_kernel(const 
         // tiles [clear_from, clear_until) are seen whole by every row there is
         const int clear_from = (kv_from(A, P.e, unsigned(P.first + rows - 1) / A.group) + 63) >> 6,
                   clear_until = max(kv_until(A, P.e, unsigned(P.first) / A.group), 0) >> 6;
-        auto page = [&](int tile, int block) { return kv_page(A.c, P.e.seq, (tile * 64 + 16 * block) >> A.c.log2_page); };
+        // (table entries and scale bytes are looked at a tile after they are requested, so
+        // that nothing waits for them)
+        const int seq = max(P.e.seq, 0);
+        auto table = [&](int tile, int block) __attribute__((always_inline)) {
+            return kv_page_entry(A.c, seq, (tile * 64 + 16 * block) >> A.c.log2_page);
+        };
         auto scales = [&](int id, int& x, int& y) __attribute__((always_inline)) {
             const int64_t at = int64_t(max(id, 0)) * A.c.kv_heads + P.kvh;
             x = A.c.ks[at], y = A.c.vs[at];
         };
         Rows<D, NR> R;
         RowLoads<D, NR> W;
+        int tile = U.begin + tile0, kb, vb;
+        int ea = table(tile, a), eg = table(tile, g);
         kv_begin_loads<D, NR>(A, P, P.first, R, W);
         __builtin_amdgcn_sched_barrier(0);
-        int tile = U.begin + tile0, ida = -1, idg = -1, idd = -1, kb = 0, vb = 0;
+        // (a unit without tiles, of rows that see nothing, reads some page and uses none of it)
         Tile<D> t;
-        // (a unit without tiles, of rows that see nothing, reads page 0 and uses none of it)
-        ida = page(tile, a), idg = idd = page(tile, g);
-        kv_fetch_keys<D>(A, P, tile, ida, t);
+        int idg = kv_page_of(A.c, eg);
+        kv_fetch_keys<D>(A, P, tile, kv_page_of(A.c, ea), t);
         scales(idg, kb, vb);
+        ea = table(tile + 1, a), eg = table(tile + 1, g);
         __builtin_amdgcn_sched_barrier(0);
         kv_begin<T, D, NR>(A, R, W);  // (while the first keys are under way)
         __builtin_amdgcn_sched_barrier(0);
         kv_fetch_values<D>(A, P, tile, idg, t);
-        ida = page(tile + 1, a), idg = page(tile + 1, g);
         for (; tile < end; tile++) {
             const bool more = tile + 1 < end;
             i32x4 s[NR][4];
             kv_scores<D, NR>(R, [&](int i, int ks) __attribute__((always_inline)) { return t.k[i][ks]; }, s);
-            int kbn = 0, vbn = 0, ida2 = -1, idg2 = -1;
+            int kbn = 0, vbn = 0, idn = -1;
             if (more) {
-                kv_fetch_keys<D>(A, P, tile + 1, ida, t);
-                scales(idg, kbn, vbn);
-                ida2 = page(tile + 2, a), idg2 = page(tile + 2, g);
+                idn = kv_page_of(A.c, eg);
+                kv_fetch_keys<D>(A, P, tile + 1, kv_page_of(A.c, ea), t);
+                scales(idn, kbn, vbn);
+                ea = table(tile + 2, a), eg = table(tile + 2, g);
             }
-            const bool dead = idd < 0;
+            const bool dead = idg < 0;
             const int ev = vb == 255 || dead ? 0 : vb, top = max(R.base, kv_group_max(ev));
             h16x8 p[NR][2];
             kv_softmax<D, NR>(R, s, kb, kb == 255 || vb == 255, tile * 64 + 16 * g, dead,
@@ -633,8 +639,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_stream_kernel(const 
             kv_values<D, NR>(R, p, [&](int dt, int u) __attribute__((always_inline)) {
                 return to(uint32_t(t.v[dt][2 * u]), uint32_t(t.v[dt][2 * u + 1]));
             });
-            if (more) kv_fetch_values<D>(A, P, tile + 1, idg, t);
-            idd = idg, kb = kbn, vb = vbn, ida = ida2, idg = idg2;
+            if (more) kv_fetch_values<D>(A, P, tile + 1, idn, t);
+            idg = idn, kb = kbn, vb = vbn;
         }
         // a unit of several runs goes to a slot
         const bool part = tiles < U.tiles;
@@ -781,13 +787,17 @@ __global__ __launch_bounds__(256) void kv_stream_join_kernel(const AttnCall A) {
 // registers, where they become f16 once for the workgroup (a wave converting them for
 // itself had 3/8 of its vector instructions for that), one tile ahead, and
 // each wave takes its operands from there.  16-byte pieces of a row are swapped by
-// an exclusive or with bits of the row, so that the 8 lanes of a read lie in
-// different banks: keys (row = token 16 a + 4 t + b, read for all a and b at once) by b
-// and a's low bit, values (row = dimension, 8 pieces of 8 tokens) by its low bits.
+// an exclusive or with bits of the row, so that the lanes that a read or a write takes
+// together (16 of them, of two lane groups) lie in different banks: a key's (row =
+// token 16 a + 4 t + b, read for all a and b at once) by bits of a and b, a value's
+// (row = dimension, pieces 4 u + g of the 8 tokens 16 g + 8 u ..) by its low bits.
 template <int D>
 __device__ __forceinline__ int kv_key_swap(int token) {
-    return D >= 128 ? (token & 3) | (token >> 2 & 4) : (token >> 1 & 1) | (token >> 3 & 2);
+    if (D == 64) return -(token >> 4) & 3;
+    if (D == 128) return (token & 3) | (token >> 2 & 4);
+    return (token & 3) | (token >> 2 & 12);
 }
+__device__ __forceinline__ int kv_value_swap(int d) { return (d & 1) | (d >> 1 & 2) | (d << 1 & 4); }
 
 typedef __attribute__((address_space(3))) char lds_char;
 
@@ -849,32 +859,36 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_block_kernel(const A
     for (int j = 0; j < D / 64; j++) ofs[j] = kv_key_offset<D>(j, page_tokens);
     // of the values, this thread's pieces are the 16 tokens 16 gv .. of dimensions tid / 4 + 64 j
     const int gv = lane & 3, dv = threadIdx.x >> 2;
-    auto page = [&](int tile, int block) { return kv_page(A.c, P.e.seq, (tile * 64 + 16 * block) >> A.c.log2_page); };
+    // (table entries and scale bytes are looked at a step after they are requested, so that nothing
+    // waits for them; begin < end: there is a sequence)
+    auto table = [&](int tile, int block) __attribute__((always_inline)) {
+        return kv_page_entry(A.c, P.e.seq, (tile * 64 + 16 * block) >> A.c.log2_page);
+    };
     if (begin < end) {
         int tile = begin, base = 0, base_next = 0;
-        int idg = page(tile, g), idv = page(tile, gv), idn, kb, vb, kbn, vbn, vbv;
+        int eg = table(tile, g), ev = table(tile, gv), idn, idv, kb, vb, kbn, vbn, vbv;
         uint4 raw[D / 64];
-        // requests tile `t` (pages idg, idv): its scales, values and keys
+        // requests tile `t` (table entries eg, ev): its scales, values and keys
         auto request = [&](int t, char* kbuf) __attribute__((always_inline)) {
-            const int64_t at = int64_t(max(idg, 0)) * A.c.kv_heads + P.kvh, av = int64_t(max(idv, 0)) * A.c.kv_heads + P.kvh;
+            idn = kv_page_of(A.c, eg), idv = kv_page_of(A.c, ev);
+            const int64_t at = int64_t(max(idn, 0)) * A.c.kv_heads + P.kvh, av = int64_t(max(idv, 0)) * A.c.kv_heads + P.kvh;
+            const int next = min(t + 1, end - 1);
+            eg = table(next, g), ev = table(next, gv);
             kbn = A.c.ks[at], vbn = A.c.vs[at], vbv = A.c.vs[av];
-            vbv = idv < 0 || vbv == 255 ? 0 : vbv;
             const int8_t* src = A.c.v + (av * D + dv) * page_tokens + ((t * 64 + 16 * gv) & (page_tokens - 1));
 #pragma unroll
             for (int j = 0; j < D / 64; j++) raw[j] = *reinterpret_cast<const uint4*>(src + 64 * j * page_tokens);
-            kv_stage_keys<D>(A, P, t, idg, ofs, (lds_char*)kbuf);
-            idn = idg;
-            if (t + 1 < end) idg = page(t + 1, g), idv = page(t + 1, gv);
+            kv_stage_keys<D>(A, P, t, idn, ofs, (lds_char*)kbuf);
         };
         // its values as f16
         auto convert = [&](h16x8* vbuf) __attribute__((always_inline)) {
             base_next = max(base, kv_group_max(idn < 0 || vbn == 255 ? 0 : vbn));
-            const Convert to(vbv, base_next);
+            const Convert to(idv < 0 || vbv == 255 ? 0 : vbv, base_next);
 #pragma unroll
             for (int j = 0; j < D / 64; j++) {
                 const int d = dv + 64 * j;
-                vbuf[8 * d + ((2 * gv) ^ (d & 7))] = to(raw[j].x, raw[j].y);
-                vbuf[8 * d + ((2 * gv + 1) ^ (d & 7))] = to(raw[j].z, raw[j].w);
+                vbuf[8 * d + (gv ^ kv_value_swap(d))] = to(raw[j].x, raw[j].y);
+                vbuf[8 * d + ((4 + gv) ^ kv_value_swap(d))] = to(raw[j].z, raw[j].w);
             }
         };
         request(tile, k0);
@@ -895,7 +909,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_block_kernel(const A
                                   tile < clear_from || tile >= clear_until || __any(dead), base, p);
                 kv_values<D, NR>(R, p, [&](int dt, int u) __attribute__((always_inline)) {
                     const int d = 16 * dt + (lane & 15);
-                    return vc[8 * d + ((2 * g + u) ^ (d & 7))];
+                    return vc[8 * d + ((4 * u + g) ^ kv_value_swap(d))];
                 });
             }
             if (more) convert(vn);
@@ -994,6 +1008,7 @@ Plan plan_attention(const eq_kv_cache* c, int n_heads, int64_t n, int64_t total,
     };
     const int64_t most = blocks(kStreamRows) * c->kv_heads;  // units of a stream (over 2^31 tiles are not listed)
     p.rows = rows <= 48 && most < INT32_MAX / cap ? kStreamRows : (rows <= 64 || c->head_dim > 128 ? 64 : 128);
+    if (const char* e=getenv("KVR")) if (p.rows==128) p.rows=atoi(e);
     p.tiles = blocks(p.rows);
     const int64_t units = p.tiles * c->kv_heads;
     if (p.rows == kStreamRows) {

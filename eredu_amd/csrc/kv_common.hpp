@@ -105,6 +105,14 @@ __device__ __forceinline__ int kv_page(const KvView& c, int seq, int index) {
     return unsigned(id) < unsigned(c.pages) ? id : -1;
 }
 
+// The same in two halves, so that nothing waits for the entry before it is
+// used: the table entry of a page index of a sequence (index >= 0; behind the table: its
+// last entry, whose tokens there are not), and the page it names.
+__device__ __forceinline__ int kv_page_entry(const KvView& c, int seq, int index) {
+    return c.tables[int64_t(seq) * c.width + min(index, c.width - 1)];
+}
+__device__ __forceinline__ int kv_page_of(const KvView& c, int entry) { return unsigned(entry) < unsigned(c.pages) ? entry : -1; }
+
 template <typename T> __device__ __forceinline__ float kv_to_f32(uint32_t bits);
 template <> __device__ __forceinline__ float kv_to_f32<BF16T>(uint32_t b) { return bf16_bits_to_f32(b); }
 template <> __device__ __forceinline__ float kv_to_f32<F16T>(uint32_t b) { return f16_bits_to_f32(b); }
