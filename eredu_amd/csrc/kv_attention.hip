@@ -677,7 +677,7 @@ template <int D, int W>
 struct Joiner {
     static constexpr int LANES = D / 4, SETS = 64 * W / LANES;
     f32x4 os[W == 1 ? 1 : SETS][LANES];
-    float ms[4], sums[W == 1 ? 1 : SETS];
+    float ms[W], sums[W == 1 ? 1 : SETS];
 
     __device__ __forceinline__ bool join(int t, float m, float& sum, f32x4& o) {
         const int set = t / LANES;
@@ -687,7 +687,8 @@ struct Joiner {
         if constexpr (W > 1) {
             if ((t & 63) == 0) ms[t >> 6] = top;
             __syncthreads();
-            top = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
+#pragma unroll
+            for (int w = 0; w < W; w++) top = fmaxf(top, ms[w]);
         }
         const float al = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
         sum *= al;
@@ -744,10 +745,11 @@ __device__ __forceinline__ void kv_out4(const AttnCall& A, int64_t at, int t, fl
 }
 
 // The units that lie in several runs of kv_stream_kernel: a workgroup for each row
-// (of the rows that entries cover) and query head.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void kv_stream_join_kernel(const AttnCall A) {
-    __shared__ Joiner<D, 4> J;
+// (of the rows that entries cover) and query head, of 4 waves, or of 16 where there are
+// few (at most 64 entries, which TileList keeps within a wave): then a unit has many parts.
+template <typename T, int D, int W>
+__global__ __launch_bounds__(64 * W) void kv_stream_join_kernel(const AttnCall A) {
+    __shared__ Joiner<D, W> J;
     __shared__ TileListLds lds;
     const int t = threadIdx.x, h = blockIdx.y, u = blockIdx.x;
     int entry, i;
@@ -760,7 +762,7 @@ __global__ __launch_bounds__(256) void kv_stream_join_kernel(const AttnCall A) {
     const int S = base + (row / kStreamRows * A.c.kv_heads + int(unsigned(h) / A.group)) * U.tiles;
     const int w0 = unsigned(S) / unsigned(run), w1 = unsigned(S + U.tiles - 1) / unsigned(run);
     if (w0 == w1) return;  // written out
-    constexpr int LANES = D / 4, SETS = 256 / LANES;
+    constexpr int LANES = D / 4, SETS = 64 * W / LANES;
     const int set = t / LANES;
     float m = -INFINITY, sum = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -799,34 +801,33 @@ __device__ __forceinline__ int kv_key_swap(int token) {
 }
 __device__ __forceinline__ int kv_value_swap(int d) { return (d & 1) | (d >> 1 & 2) | (d << 1 & 4); }
 
-typedef __attribute__((address_space(3))) char lds_char;
-
-// A wave's share of a tile's keys: 64 lanes' pieces land side by side, so the swap
-// is in the addresses they come from, which are a page's (a scalar: a wave's 1024 / D
-// tokens lie in one block of 16) and the lane's in it, the same for every tile.
+// A wave's share of a tile's keys, pieces (j * 4 + wave) * 64 + lane of it: from a page
+// (a scalar: a wave's 1024 / D tokens lie in one block of 16) and an offset in it that is
+// the same for every tile.
 template <int D>
 __device__ __forceinline__ int kv_key_offset(int j, int T) {
     constexpr int KP = D / 16;  // 16-byte pieces of a key
     const int p = (j * 4 + int(threadIdx.x >> 6)) * 64 + (threadIdx.x & 63), token = p / KP;
-    return (token & (T - 1)) * D + 16 * ((p % KP) ^ kv_key_swap<D>(token));
+    return (token & (T - 1)) * D + 16 * (p % KP);
 }
 template <int D>
-__device__ __forceinline__ void kv_stage_keys(const AttnCall& A, const Place& P, int tile, int idg, const int (&ofs)[D / 64],
-                                              lds_char* buf) {
+__device__ __forceinline__ int kv_key_place(int j) {
+    constexpr int KP = D / 16;
+    const int p = (j * 4 + int(threadIdx.x >> 6)) * 64 + (threadIdx.x & 63), token = p / KP;
+    return token * KP + ((p % KP) ^ kv_key_swap<D>(token));
+}
+// Where piece (j * 4 + wave) * 64 of a tile's keys lies, in page `id` of those of this lane's group.
+template <int D>
+__device__ __forceinline__ const int8_t* kv_key_page(const AttnCall& A, const Place& P, int tile, int idg, int j) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), T = 1 << A.c.log2_page;
-#pragma unroll
-    for (int j = 0; j < D / 64; j++) {
-        const int id = __builtin_amdgcn_readlane(idg, (j * 4 + wave) * 64 / D * 16);  // of token block (j * 4 + wave) * 64 / D
-        const int8_t* page = A.c.k + ((int64_t(max(id, 0)) * A.c.kv_heads + P.kvh) * T + (tile * 64 & (T - 1))) * D;
-        __builtin_amdgcn_global_load_lds(const_cast<int8_t*>(page) + unsigned(ofs[j]),
-                                         (__attribute__((address_space(3))) void*)(buf + (j * 4 + wave) * 1024), 16, 0, 0);
-    }
+    const int id = __builtin_amdgcn_readlane(idg, (j * 4 + wave) * 64 / D * 16);  // of token block (j * 4 + wave) * 64 / D
+    return A.c.k + ((int64_t(max(id, 0)) * A.c.kv_heads + P.kvh) * T + (tile * 64 & (T - 1))) * D;
 }
 
 template <typename T, int D, int NR>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_block_kernel(const AttnCall A) {
     constexpr int BM = 64 * NR;
-    __shared__ __attribute__((aligned(16))) char k0[64 * D], k1[64 * D];
+    __shared__ i32x4 k0[4 * D], k1[4 * D];
     __shared__ __attribute__((aligned(16))) h16x8 v0[8 * D], v1[8 * D];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     Place P;
@@ -867,9 +868,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_block_kernel(const A
     if (begin < end) {
         int tile = begin, base = 0, base_next = 0;
         int eg = table(tile, g), ev = table(tile, gv), idn, idv, kb, vb, kbn, vbn, vbv;
-        uint4 raw[D / 64];
+        i32x4 raw[D / 64], rawk[D / 64];
         // requests tile `t` (table entries eg, ev): its scales, values and keys
-        auto request = [&](int t, char* kbuf) __attribute__((always_inline)) {
+        auto request = [&](int t) __attribute__((always_inline)) {
             idn = kv_page_of(A.c, eg), idv = kv_page_of(A.c, ev);
             const int64_t at = int64_t(max(idn, 0)) * A.c.kv_heads + P.kvh, av = int64_t(max(idv, 0)) * A.c.kv_heads + P.kvh;
             const int next = min(t + 1, end - 1);
@@ -877,32 +878,36 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_block_kernel(const A
             kbn = A.c.ks[at], vbn = A.c.vs[at], vbv = A.c.vs[av];
             const int8_t* src = A.c.v + (av * D + dv) * page_tokens + ((t * 64 + 16 * gv) & (page_tokens - 1));
 #pragma unroll
-            for (int j = 0; j < D / 64; j++) raw[j] = *reinterpret_cast<const uint4*>(src + 64 * j * page_tokens);
-            kv_stage_keys<D>(A, P, t, idn, ofs, (lds_char*)kbuf);
+            for (int j = 0; j < D / 64; j++) raw[j] = *reinterpret_cast<const i32x4*>(src + 64 * j * page_tokens);
+#pragma unroll
+            for (int j = 0; j < D / 64; j++)
+                rawk[j] = *reinterpret_cast<const i32x4*>(kv_key_page<D>(A, P, t, idn, j) + unsigned(ofs[j]));
         };
         // its values as f16
-        auto convert = [&](h16x8* vbuf) __attribute__((always_inline)) {
+        auto convert = [&](i32x4* kbuf, h16x8* vbuf) __attribute__((always_inline)) {
             base_next = max(base, kv_group_max(idn < 0 || vbn == 255 ? 0 : vbn));
+#pragma unroll
+            for (int j = 0; j < D / 64; j++) kbuf[kv_key_place<D>(j)] = rawk[j];
             const Convert to(idv < 0 || vbv == 255 ? 0 : vbv, base_next);
 #pragma unroll
             for (int j = 0; j < D / 64; j++) {
                 const int d = dv + 64 * j;
-                vbuf[8 * d + (gv ^ kv_value_swap(d))] = to(raw[j].x, raw[j].y);
-                vbuf[8 * d + ((4 + gv) ^ kv_value_swap(d))] = to(raw[j].z, raw[j].w);
+                vbuf[8 * d + (gv ^ kv_value_swap(d))] = to(uint32_t(raw[j][0]), uint32_t(raw[j][1]));
+                vbuf[8 * d + ((4 + gv) ^ kv_value_swap(d))] = to(uint32_t(raw[j][2]), uint32_t(raw[j][3]));
             }
         };
-        request(tile, k0);
-        convert(v0);
-        auto step = [&](const char* kc, const h16x8* vc, char* kn, h16x8* vn) __attribute__((always_inline)) {
+        request(tile);
+        convert(k0, v0);
+        auto step = [&](const i32x4* kc, const h16x8* vc, i32x4* kn, h16x8* vn) __attribute__((always_inline)) {
             __syncthreads();  // this tile is there, and the other buffers are read
             const bool dead = idn < 0, more = tile + 1 < end;
             kb = kbn, vb = vbn, base = base_next;
-            if (more) request(tile + 1, kn);
+            if (more) request(tile + 1);
             if (tile >= see_from && tile < see_until) {
                 i32x4 s[NR][4];
                 kv_scores<D, NR>(R, [&](int t, int ks) __attribute__((always_inline)) {
                     const int token = 4 * (lane & 12) + 4 * t + (lane & 3);
-                    return *reinterpret_cast<const i32x4*>(kc + token * D + 16 * ((4 * ks + g) ^ kv_key_swap<D>(token)));
+                    return kc[token * (D / 16) + ((4 * ks + g) ^ kv_key_swap<D>(token))];
                 }, s);
                 h16x8 p[NR][2];
                 kv_softmax<D, NR>(R, s, kb, kb == 255 || vb == 255, tile * 64 + 16 * g, dead,
@@ -912,7 +917,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_block_kernel(const A
                     return vc[8 * d + ((4 * u + g) ^ kv_value_swap(d))];
                 });
             }
-            if (more) convert(vn);
+            if (more) convert(kn, vn);
             tile++;
             return more;
         };
@@ -997,6 +1002,7 @@ struct Plan {
     int64_t tiles;
     int splits;  // of a block's tokens
     int groups;  // workgroups of a stream
+    bool wide_join;
     size_t part_bytes, lse_bytes;
 };
 Plan plan_attention(const eq_kv_cache* c, int n_heads, int64_t n, int64_t total, bool ragged) {
@@ -1015,6 +1021,8 @@ Plan plan_attention(const eq_kv_cache* c, int n_heads, int64_t n, int64_t total,
         const int64_t runs = (units * cap + 3) / 4;  // at least a tile for each of 4 waves
         p.splits = 1;
         p.groups = int(runs < 2 * device_cu_count() ? runs : 2 * device_cu_count());
+        // 256 parts take 16 waves 2.7 us instead of 4 waves 6 us, 17 parts 4.7 instead of 3.9
+        p.wide_join = n <= 64 && total * n_heads <= 2 * device_cu_count() && cap > 64;
         p.part_bytes = size_t(p.groups) * 8 * kStreamRows * c->head_dim * 4;
         p.lse_bytes = (size_t(p.groups) * 8 * kStreamRows * 4 + 255) & ~size_t(255);
         return p;
@@ -1114,7 +1122,9 @@ extern "C" int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n
         constexpr int DIM = decltype(d)::value;
         if (plan.rows == kStreamRows) {
             kv_stream_kernel<T, DIM><<<dim3(unsigned(plan.groups)), dim3(256), 0, st>>>(A);
-            kv_stream_join_kernel<T, DIM><<<dim3(unsigned(total), unsigned(n_heads)), dim3(256), 0, st>>>(A);
+            const dim3 rows{unsigned(total), unsigned(n_heads)};
+            if (plan.wide_join) kv_stream_join_kernel<T, DIM, 16><<<rows, dim3(1024), 0, st>>>(A);
+            else kv_stream_join_kernel<T, DIM, 4><<<rows, dim3(256), 0, st>>>(A);
             return;
         }
         if (plan.rows == 64) kv_block_kernel<T, DIM, 1><<<grid, dim3(256), 0, st>>>(A);

@@ -138,27 +138,69 @@ __device__ __forceinline__ KvSpan kv_span(const KvView& c, const KvEntry& e, int
     return s;
 }
 
-// 8 values at dimension d0 < D / 2 of a row and the 8 that they pair with,
-// turned by the row's angles where there are any.
-template <typename T>
-__device__ __forceinline__ void kv_pairs(const uint16_t* x, int d0, int D, const float* rot, float* a, float* b) {
-    kv_load8<T>(x + d0, a);
-    kv_load8<T>(x + d0 + D / 2, b);
-    if (rot) {
+// 8 values at dimension d0 < D / 2 of a row and the 8 that they pair with, as
+// loaded with the angles of theirs, and turned.
+struct KvPairs {
+    uint4 a, b;
+    float4 cs[2], sn[2];
+
+    __device__ __forceinline__ void load(const uint16_t* x, int d0, int D, const float* rot) {
+        a = *reinterpret_cast<const uint4*>(x + d0);
+        b = *reinterpret_cast<const uint4*>(x + d0 + D / 2);
+        if (!rot) return;
+        const float4* p = reinterpret_cast<const float4*>(rot + d0);
+        cs[0] = p[0], cs[1] = p[1], sn[0] = p[D / 8], sn[1] = p[D / 8 + 1];
+    }
+    template <typename T>
+    __device__ __forceinline__ void values(bool turn, float (&f)[16]) const {
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const float cs = rot[d0 + i], sn = rot[D / 2 + d0 + i];
-            const float u = a[i] * cs - b[i] * sn;
-            b[i] = b[i] * cs + a[i] * sn;
-            a[i] = u;
+            f[2 * i] = kv_to_f32<T>(w[i] & 0xffffu);
+            f[2 * i + 1] = kv_to_f32<T>(w[i] >> 16);
+        }
+        if (!turn) return;
+        const float c[8] = {cs[0].x, cs[0].y, cs[0].z, cs[0].w, cs[1].x, cs[1].y, cs[1].z, cs[1].w};
+        const float n[8] = {sn[0].x, sn[0].y, sn[0].z, sn[0].w, sn[1].x, sn[1].y, sn[1].z, sn[1].w};
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float u = f[i] * c[i] - f[8 + i] * n[i];
+            f[8 + i] = f[8 + i] * c[i] + f[i] * n[i];
+            f[i] = u;
         }
     }
+};
+
+__device__ __forceinline__ uint32_t kv_most(const float (&f)[16]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i++) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+    return m;
+}
+
+// 4 rows of 4 bytes <-> 4 columns.
+__device__ __forceinline__ void kv_turn4(const uint32_t r0, const uint32_t r1, const uint32_t r2, const uint32_t r3, uint32_t (&c)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(r1, r0, 0x05010400u), b = __builtin_amdgcn_perm(r1, r0, 0x07030602u);
+    const uint32_t d = __builtin_amdgcn_perm(r3, r2, 0x05010400u), e = __builtin_amdgcn_perm(r3, r2, 0x07030602u);
+    c[0] = __builtin_amdgcn_perm(d, a, 0x05040100u), c[1] = __builtin_amdgcn_perm(d, a, 0x07060302u);
+    c[2] = __builtin_amdgcn_perm(e, b, 0x05040100u), c[3] = __builtin_amdgcn_perm(e, b, 0x07060302u);
+}
+
+// The bytes of a word of 4 places, from place t on, that lie in [from, until).
+__device__ __forceinline__ uint32_t kv_places(int t, int from, int until) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) m |= t + i >= from && t + i < until ? 0xffu << (8 * i) : 0u;
+    return m;
 }
 
 // Grid (page units, kv_heads, keys | values), 256 threads: one page of one
-// head.  Two passes over the page's new rows, the largest magnitude and then the codes
-// (the second reads them from L2); values go through LDS to be written along
-// the tokens, 16 of a dimension at once.
+// head.  The page's new rows are read for their largest magnitude and, where
+// that is one round of 2 pieces a thread (64 tokens of 128 dimensions), stay in registers for
+// their codes; else they are read again, from L2.  Values turn in LDS, by 4 x 4
+// bytes, to be written along the tokens, 16 of a dimension at once.
+constexpr int kAppendItems = 2;
+
 template <typename T>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvView c, KvBatch b, const uint16_t* __restrict__ k,
                                                         const uint16_t* __restrict__ v, int64_t k_stride,
@@ -171,47 +213,61 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvView c, KvBatch b, con
     if (!kv_locate(b, blockIdx.x, [&](int n) { return kv_spanned(n, log2_page); }, entry, place)) return;
     const KvEntry e = kv_entry(c, b, entry);
     if (e.seq < 0) return;
-    bool later = false;  // another entry names this sequence
-    for (int j = entry + 1 + tid; j < b.n; j += 256) later |= b.seqs[j] == e.seq;
-    if (__syncthreads_or(later)) return;
     const KvSpan s = kv_span(c, e, place);
-    if (s.page < 0) return;
-
+    const int groups = D / 16, items = max(s.until - s.from, 0) * groups;
     const uint16_t* x = (values ? v + int64_t(s.row) * v_stride : k + int64_t(s.row) * k_stride) + int64_t(head) * D;
     const int64_t stride = values ? v_stride : k_stride;
-    const float* rot = rope && !values ? rope + int64_t(s.position) * D : nullptr;
-    const int groups = D / 16, items = (s.until - s.from) * groups;
-    uint32_t most = 0;
-    for (int it = tid; it < items; it += 256) {
-        const int t = it / groups, d0 = it % groups * 8;
-        float f[16];
-        kv_pairs<T>(x + int64_t(t) * stride, d0, D, rot ? rot + int64_t(t) * D : nullptr, f, f + 8);
+    // (the rows are read whether or not the page is there: they are rows of this call; the angles only
+    // of positions that have a page)
+    const float* rot = rope && !values && s.page >= 0 ? rope + int64_t(s.position) * D : nullptr;
+    KvPairs raw[kAppendItems];
 #pragma unroll
-        for (int i = 0; i < 16; i++) most = max(most, __float_as_uint(f[i]) & 0x7fffffffu);
+    for (int j = 0; j < kAppendItems; j++) {
+        const int it = tid + 256 * j, t = it / groups;
+        if (it < items) raw[j].load(x + int64_t(t) * stride, it % groups * 8, D, rot ? rot + int64_t(t) * D : nullptr);
+    }
+    bool later = false;  // another entry names this sequence
+    for (int j = entry + 1 + tid; j < b.n; j += 256) later |= b.seqs[j] == e.seq;
+    if (__syncthreads_or(later) || s.page < 0) return;
+    uint8_t* scale = (values ? c.vs : c.ks) + int64_t(s.page) * c.kv_heads + head;
+    const int was = s.from > 0 ? *scale : 0;
+
+    const bool held = items <= 256 * kAppendItems;
+    uint32_t most = 0;
+    float f[kAppendItems][16];
+#pragma unroll
+    for (int j = 0; j < kAppendItems; j++)
+        if (tid + 256 * j < items) {
+            raw[j].values<T>(rot != nullptr, f[j]);
+            most = max(most, kv_most(f[j]));
+        }
+    for (int it = tid + 256 * kAppendItems; it < items; it += 256) {
+        const int t = it / groups;
+        KvPairs r;
+        float y[16];
+        r.load(x + int64_t(t) * stride, it % groups * 8, D, rot ? rot + int64_t(t) * D : nullptr);
+        r.values<T>(rot != nullptr, y);
+        most = max(most, kv_most(y));
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) most = max(most, uint32_t(__shfl_xor(int(most), o)));
     if ((tid & 63) == 0) red[tid >> 6] = most;
-    uint8_t* scale = (values ? c.vs : c.ks) + int64_t(s.page) * c.kv_heads + head;
-    const int was = s.from > 0 ? *scale : 0;
     __syncthreads();
     most = max(max(red[0], red[1]), max(red[2], red[3]));
     const int now = max(kv_byte(most), was);
     if (tid == 0) *scale = uint8_t(now);
     const bool move = s.from > 0 && was < now && now != 255;  // the page's older codes change their step
     const float down = __uint_as_float(unsigned(max(127 + was - now, 0)) << 23);
-    const float inv = now == 255 ? 0.f : kv_inverse(now);
+    const float inv = kv_inverse(now);
 
     int8_t* codes = (values ? c.v : c.k) + (int64_t(s.page) * c.kv_heads + head) * page_tokens * D;
     const int pitch = D + 4;
-    for (int it = tid; it < items; it += 256) {
+    auto put = [&](int it, const float (&y)[16]) __attribute__((always_inline)) {
         const int t = it / groups, d0 = it % groups * 8;
-        float f[16];
-        kv_pairs<T>(x + int64_t(t) * stride, d0, D, rot ? rot + int64_t(t) * D : nullptr, f, f + 8);
         uint32_t w[4] = {0u, 0u, 0u, 0u};
         if (now != 255) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) w[i >> 2] |= kv_code(f[i], inv) << (8 * (i & 3));
+            for (int i = 0; i < 16; i++) w[i >> 2] |= kv_code(y[i], inv) << (8 * (i & 3));
         }
         if (values) {
             uint32_t* p = reinterpret_cast<uint32_t*>(turn + t * pitch + d0);
@@ -222,6 +278,19 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvView c, KvBatch b, con
             int8_t* row = codes + (s.from + t) * D + d0;
             *reinterpret_cast<uint2*>(row) = make_uint2(w[0], w[1]);
             *reinterpret_cast<uint2*>(row + D / 2) = make_uint2(w[2], w[3]);
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < kAppendItems; j++)
+        if (tid + 256 * j < items) put(tid + 256 * j, f[j]);
+    if (!held) {
+        for (int it = tid + 256 * kAppendItems; it < items; it += 256) {
+            const int t = it / groups;
+            KvPairs r;
+            float y[16];
+            r.load(x + int64_t(t) * stride, it % groups * 8, D, rot ? rot + int64_t(t) * D : nullptr);
+            r.values<T>(rot != nullptr, y);
+            put(it, y);
         }
     }
     if (!values) {
@@ -236,37 +305,46 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvView c, KvBatch b, con
         return;
     }
     __syncthreads();
-    // 16 places of a dimension: older codes, then new ones, then what was there
+    // 16 places of 4 dimensions: older codes, then new ones, then what was there
     const int first = move ? 0 : s.from >> 4, blocks = ((s.until + 15) >> 4) - first;
-    for (int it = tid; it < blocks * D; it += 256) {
-        const int d = it / blocks, t0 = (first + it % blocks) * 16;
-        uint4* p = reinterpret_cast<uint4*>(codes + int64_t(d) * page_tokens + t0);
-        uint4 o = *p;
-        uint32_t* w = reinterpret_cast<uint32_t*>(&o);
-        if (move && t0 < s.from) {
+    for (int it = tid; it < blocks * (D / 4); it += 256) {
+        const int d4 = it / blocks, t0 = (first + it - d4 * blocks) * 16;
+        uint32_t n[4][4];  // [dimension][4 places]
 #pragma unroll
-            for (int j = 0; j < 4; j++) w[j] = kv_rescale4(w[j], down);
-            // places at and behind `until` keep their bytes
-            if (t0 + 16 > s.until) {
-                const uint4 was4 = *p;
-                const uint32_t* ow = reinterpret_cast<const uint32_t*>(&was4);
+        for (int q = 0; q < 4; q++) {
+            uint32_t r[4], col[4];
 #pragma unroll
-                for (int j = 0; j < 16; j++)
-                    if (t0 + j >= s.until) w[j >> 2] = (w[j >> 2] & ~(0xffu << (8 * (j & 3)))) | (ow[j >> 2] & (0xffu << (8 * (j & 3))));
+            for (int i = 0; i < 4; i++) {
+                const int t = t0 + 4 * q + i;
+                r[i] = t >= s.from && t < s.until ? *reinterpret_cast<const uint32_t*>(turn + (t - s.from) * pitch + 4 * d4) : 0u;
             }
-        }
+            kv_turn4(r[0], r[1], r[2], r[3], col);
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const int t = t0 + j - s.from;
-            if (t >= 0 && t0 + j < s.until)
-                w[j >> 2] = (w[j >> 2] & ~(0xffu << (8 * (j & 3)))) | (uint32_t(turn[t * pitch + d]) << (8 * (j & 3)));
+            for (int i = 0; i < 4; i++) n[i][q] = col[i];
         }
-        *p = o;
+        uint4* p = reinterpret_cast<uint4*>(codes + int64_t(4 * d4) * page_tokens + t0);
+        const bool whole = t0 >= s.from && t0 + 16 <= s.until;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint4* at = reinterpret_cast<uint4*>(reinterpret_cast<int8_t*>(p) + i * page_tokens);
+            if (!whole) {
+                const uint4 o = *at;
+                const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const uint32_t fresh = kv_places(t0 + 4 * q, s.from, s.until), old = kv_places(t0 + 4 * q, 0, s.from);
+                    uint32_t keep = w[q];
+                    if (move) keep = (keep & ~old) | (kv_rescale4(keep, down) & old);
+                    n[i][q] = (n[i][q] & fresh) | (keep & ~fresh);
+                }
+            }
+            *at = make_uint4(n[i][0], n[i][1], n[i][2], n[i][3]);
+        }
     }
 }
 
 // Grid (page units, kv_heads, keys | values), 256 threads: the rows of one page
-// and head; values turn through LDS.
+// and head; values turn in LDS, by 4 x 4 bytes.
 template <typename T>
 __global__ __launch_bounds__(256) void kv_read_kernel(typename T::storage* __restrict__ k,
                                                       typename T::storage* __restrict__ v, KvView c, KvBatch b, int D) {
@@ -287,14 +365,23 @@ __global__ __launch_bounds__(256) void kv_read_kernel(typename T::storage* __res
     const float scale = here ? e8m0_to_f32((values ? c.vs : c.ks)[at]) : 0.f;
     if (values && here) {
         const int first = s.from >> 4, blocks = ((s.until + 15) >> 4) - first;
-        for (int it = tid; it < blocks * D; it += 256) {
-            const int d = it / blocks, t0 = (first + it % blocks) * 16;
-            const uint4 o = *reinterpret_cast<const uint4*>(codes + int64_t(d) * page_tokens + t0);
-            const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+        for (int it = tid; it < blocks * (D / 4); it += 256) {
+            const int d4 = it / blocks, t0 = (first + it - d4 * blocks) * 16;
+            const int8_t* p = codes + int64_t(4 * d4) * page_tokens + t0;
+            uint4 o[4];
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const int t = t0 + j - s.from;
-                if (t >= 0 && t0 + j < s.until) turn[t * pitch + d] = uint8_t(w[j >> 2] >> (8 * (j & 3)));
+            for (int i = 0; i < 4; i++) o[i] = *reinterpret_cast<const uint4*>(p + i * page_tokens);
+            const uint32_t w[4][4] = {{o[0].x, o[0].y, o[0].z, o[0].w}, {o[1].x, o[1].y, o[1].z, o[1].w},
+                                      {o[2].x, o[2].y, o[2].z, o[2].w}, {o[3].x, o[3].y, o[3].z, o[3].w}};
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                uint32_t row[4];
+                kv_turn4(w[0][q], w[1][q], w[2][q], w[3][q], row);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int t = t0 + 4 * q + i;
+                    if (t >= s.from && t < s.until) *reinterpret_cast<uint32_t*>(turn + (t - s.from) * pitch + 4 * d4) = row[i];
+                }
             }
         }
         __syncthreads();
@@ -528,14 +615,14 @@ __global__ __launch_bounds__(kPlanThreads) void kv_compact_plan_kernel(KvPages c
     if (tid == 0) s.count[0] = live - stay;
 }
 
-// Copies the pages of the move list, all layers, 16 KiB a step; then (map not
+// Copies the pages of the move list, all layers, 32 KiB a step; then (map not
 // null) the tables' entries follow their pages.
 __global__ __launch_bounds__(256) void kv_move_kernel(KvPages c, int8_t* k, int8_t* v, uint8_t* ks, uint8_t* vs,
                                                       int layers, int kv_heads, int64_t page_bytes,
                                                       const int32_t* __restrict__ moves,
                                                       const int32_t* __restrict__ count,
                                                       const int32_t* __restrict__ map) {
-    constexpr int kStep = 16384;
+    constexpr int kVecs = 8, kStep = kVecs * 256 * 16;
     const int steps = int((page_bytes + kStep - 1) / kStep), tid = threadIdx.x;
     const int64_t units = int64_t(*count) * layers * 2 * steps;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
@@ -547,13 +634,15 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvPages c, int8_t* k, int8
         const uint4* src = reinterpret_cast<const uint4*>(codes + from * page_bytes + int64_t(step) * kStep);
         uint4* dst = reinterpret_cast<uint4*>(codes + to * page_bytes + int64_t(step) * kStep);
         const int vecs = int(min(int64_t(kStep), page_bytes - int64_t(step) * kStep) / 16);
-        uint4 t[4];
+        uint4 t[kVecs];
+        if (vecs == kStep / 16) {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (tid + 256 * i < vecs) t[i] = src[tid + 256 * i];
+            for (int i = 0; i < kVecs; i++) t[i] = load_stream16(src + tid + 256 * i);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (tid + 256 * i < vecs) dst[tid + 256 * i] = t[i];
+            for (int i = 0; i < kVecs; i++) store_stream16(dst + tid + 256 * i, t[i]);
+        } else {
+            for (int i = tid; i < vecs; i += 256) dst[i] = src[i];
+        }
         if (step == 0) {
             uint8_t* scales = half ? vs : ks;
             for (int h = tid; h < kv_heads; h += 256) scales[to * kv_heads + h] = scales[from * kv_heads + h];
@@ -674,7 +763,11 @@ bool kv_list_ok(const char* who, const int32_t* a, const int32_t* b, int64_t n) 
 }
 
 void launch_moves(const eq_kv_cache* c, const KvPlanScratch& s, const int32_t* map, hipStream_t st) {
-    kv_move_kernel<<<dim3(1024), dim3(256), 0, st>>>(pages_of(c), c->k_codes, c->v_codes, c->k_scales, c->v_scales,
+    // (no more workgroups than a small cache has work for: a launch that moves nothing is a launch)
+    const int64_t page = int64_t(c->kv_heads) * c->page_tokens * c->head_dim;
+    const int64_t steps = c->pages * c->layers * 2 * ((page + 32767) / 32768), entries = c->sequences * c->width / 1024 + 1;
+    const int64_t most = steps > entries ? steps : entries, grid = most < 4096 ? most : 4096;
+    kv_move_kernel<<<dim3(unsigned(grid)), dim3(256), 0, st>>>(pages_of(c), c->k_codes, c->v_codes, c->k_scales, c->v_scales,
                                                      int(c->layers), c->kv_heads,
                                                      int64_t(c->kv_heads) * c->page_tokens * c->head_dim, s.moves,
                                                      s.count, map);

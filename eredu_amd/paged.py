@@ -59,12 +59,6 @@ def _ids(t: torch.Tensor, what: str, index: int) -> torch.Tensor:
 # Whether the current stream is being captured (a method of torch.cuda without its wrapper).
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
-# Scratch of an eager call up to this size comes from the library's workspace of
-# the stream, which saves a call its allocation (about 3 us); more comes from torch and
-# goes back to it.
-_OWN_SCRATCH = 64 << 20
-
-
 class PagedKVCache:
     """``n_pages`` pages of ``page_size`` tokens (16, 32, 64 or 128) for
     ``n_layers`` layers of ``n_kv_heads`` heads of ``head_dim`` (64, 128 or 256),
@@ -175,12 +169,12 @@ class PagedKVCache:
         return rope.data_ptr(), rope.shape[0]
 
     def _scratch(self, need: int) -> Tuple[Optional[int], int, Optional[torch.Tensor]]:
-        """Scratch of a call: the library's workspace of the stream (None), or, under
-        capture and where it is large, torch's memory, in stream order and a captured
-        graph's own, so that graphs share nothing."""
+        """Scratch of a call from torch: in stream order, and under capture a graph's
+        own, so that graphs share nothing.  (Eager calls that need little take the
+        library's workspace of their stream, which saves them the allocation.)"""
         if need < 0:
             check(1)
-        if need <= _OWN_SCRATCH and not _capturing():
+        if need == 0:
             return None, 0, None
         t = torch.empty((need,), dtype=torch.uint8, device=self.device)
         return t.data_ptr(), need, t
@@ -215,16 +209,16 @@ class PagedKVCache:
         seqs, n, cu = self._batch(seqs, cu, rows)
         rp, rn = self._rope(rope)
         if out is None:
-            out = torch.empty((rows, heads, D), dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q) if q.is_contiguous() else torch.empty((rows, heads, D), dtype=q.dtype, device=self.device)
         elif out.dtype != q.dtype or out.numel() != q.numel() or not out.is_contiguous() or out.get_device() != self._index:
             raise EreduError(f"out must be a contiguous {q.dtype} tensor of {q.numel()} values on {self.device}")
         L, st = _native.lib(), self._here()
-        wp = wn = ws = None
-        if rows * heads > 8192 or _capturing():  # (fewer rows take a few MB of the library's workspace)
+        wp, wn, ws = None, 0, None
+        if rows * heads > 8192 or _capturing():  # (what fewer rows need is a few MB)
             wp, wn, ws = self._scratch(L.eq_kv_attention_scratch(self._ref, heads, n, rows, cu is not None))
         check(L.eq_kv_attention(out.data_ptr(), q.data_ptr(), q.stride(0), heads, self._ref, layer, seqs.data_ptr(), n,
                                 None if cu is None else cu.data_ptr(), rows, self._scale if scale is None else scale,
-                                causal, window, rp, rn, _DTYPE_CODE[q.dtype], wp, wn or 0, st))
+                                causal, window, rp, rn, _DTYPE_CODE[q.dtype], wp, wn, st))
         return out
 
     def read(self, layer: int, seqs: torch.Tensor, tokens: Union[int, torch.Tensor], total: Optional[int] = None,
@@ -255,7 +249,7 @@ class PagedKVCache:
         cu = tokens if isinstance(tokens, torch.Tensor) else None
         seqs, n, cu = self._batch(seqs, cu, 0)
         L, st = _native.lib(), self._here()
-        wp, wn, ws = self._scratch(L.eq_kv_pages_scratch(self._ref, n))
+        wp, wn, ws = self._scratch(L.eq_kv_pages_scratch(self._ref, n) if _capturing() else 0)
         check(L.eq_kv_extend(self._ref, seqs.data_ptr(), n, None if cu is None else cu.data_ptr(),
                              0 if cu is not None else tokens, wp, wn, st))
 
@@ -266,7 +260,7 @@ class PagedKVCache:
         if src.numel() != dst.numel():
             raise EreduError(f"src and dst must be of one length, got {src.numel()} and {dst.numel()}")
         L, st = _native.lib(), self._here()
-        wp, wn, ws = self._scratch(L.eq_kv_pages_scratch(self._ref, src.numel()))
+        wp, wn, ws = self._scratch(L.eq_kv_pages_scratch(self._ref, src.numel()) if _capturing() else 0)
         check(L.eq_kv_fork(self._ref, src.data_ptr(), dst.data_ptr(), src.numel(), wp, wn, st))
 
     def free(self, seqs: torch.Tensor) -> None:
@@ -277,7 +271,7 @@ class PagedKVCache:
     def compact(self) -> None:
         """Moves the pages in use to the lowest indices (C ABI: eq_kv_compact)."""
         L, st = _native.lib(), self._here()
-        wp, wn, ws = self._scratch(L.eq_kv_pages_scratch(self._ref, 0))
+        wp, wn, ws = self._scratch(L.eq_kv_pages_scratch(self._ref, 0) if _capturing() else 0)
         check(L.eq_kv_compact(self._ref, wp, wn, st))
 
     def free_pages(self) -> int:
