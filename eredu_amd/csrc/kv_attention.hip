@@ -1014,7 +1014,6 @@ Plan plan_attention(const eq_kv_cache* c, int n_heads, int64_t n, int64_t total,
     };
     const int64_t most = blocks(kStreamRows) * c->kv_heads;  // units of a stream (over 2^31 tiles are not listed)
     p.rows = rows <= 48 && most < INT32_MAX / cap ? kStreamRows : (rows <= 64 || c->head_dim > 128 ? 64 : 128);
-    if (const char* e=getenv("KVR")) if (p.rows==128) p.rows=atoi(e);
     p.tiles = blocks(p.rows);
     const int64_t units = p.tiles * c->kv_heads;
     if (p.rows == kStreamRows) {
