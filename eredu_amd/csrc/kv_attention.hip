@@ -1006,7 +1006,7 @@ struct Plan {
     size_t part_bytes, lse_bytes;
 };
 Plan plan_attention(const eq_kv_cache* c, int n_heads, int64_t n, int64_t total, bool ragged) {
-    Plan p;
+    Plan p = {};
     const int64_t group = n_heads / c->kv_heads, rows = n ? total * group / n : 0;  // of a sequence and KV head, on average
     const int64_t cap = (c->width * c->page_tokens + 63) / 64;
     auto blocks = [&](int bm) {
@@ -1015,9 +1015,8 @@ Plan plan_attention(const eq_kv_cache* c, int n_heads, int64_t n, int64_t total,
     const int64_t most = blocks(kStreamRows) * c->kv_heads;  // units of a stream (over 2^31 tiles are not listed)
     p.rows = rows <= 48 && most < INT32_MAX / cap ? kStreamRows : (rows <= 64 || c->head_dim > 128 ? 64 : 128);
     p.tiles = blocks(p.rows);
-    const int64_t units = p.tiles * c->kv_heads;
     if (p.rows == kStreamRows) {
-        const int64_t runs = (units * cap + 3) / 4;  // at least a tile for each of 4 waves
+        const int64_t runs = (most * cap + 3) / 4;  // at least a tile for each of 4 waves
         p.splits = 1;
         p.groups = int(runs < 2 * device_cu_count() ? runs : 2 * device_cu_count());
         // 256 parts take 16 waves 2.7 us instead of 4 waves 6 us, 17 parts 4.7 instead of 3.9
@@ -1026,7 +1025,11 @@ Plan plan_attention(const eq_kv_cache* c, int n_heads, int64_t n, int64_t total,
         p.lse_bytes = (size_t(p.groups) * 8 * kStreamRows * 4 + 255) & ~size_t(255);
         return p;
     }
-    int64_t splits = units ? (2 * device_cu_count() + units - 1) / units : 1;
+    // two workgroups fit a CU: as many splits as come nearest to filling that once (300 queries over
+    // 8000 tokens, 80 blocks: 560 workgroups 95 us, 480 79 us)
+    // (of a ragged batch, whose blocks are bounded by one a sequence too many, those of even sequences)
+    const int64_t likely = n * ((rows + p.rows - 1) / p.rows) * c->kv_heads;
+    int64_t splits = likely ? (2 * device_cu_count() + likely / 2) / likely : 1;
     if (splits > (cap + 3) / 4) splits = (cap + 3) / 4;
     if (splits > 1024) splits = 1024;
     p.splits = splits < 1 ? 1 : int(splits);
@@ -1078,8 +1081,9 @@ extern "C" int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n
         return 1;
     }
     const Plan plan = plan_attention(cache, n_heads, n, total, cu != nullptr);
-    const int64_t blocks = plan.tiles * cache->kv_heads * plan.splits;
-    if (blocks >= (1 << 24) || total >= (1 << 24)) {  // grids of under 2^32 threads a side
+    // (grids of under 2^32 threads a side; a stream's own is small)
+    const int64_t blocks = plan.rows == kStreamRows ? 0 : plan.tiles * cache->kv_heads * plan.splits;
+    if (blocks >= (1 << 24) || total >= (1 << 24)) {
         set_error("eq_kv_attention: too many rows");
         return 1;
     }

@@ -33,6 +33,7 @@ import torch
 
 from . import _native
 from ._native import check
+from .paged import PagedKVCache, rope_table
 from .quantization import _stream
 
 HEAD_DIM = 128
@@ -228,12 +229,19 @@ class LlamaDecoder:
     projection's launch instead when K is not a whole number of the decode
     kernel's code blocks): 6 launches per layer instead of 9.  The hidden
     state then alternates between two buffers (every workgroup of a launch
-    reads the old one)."""
+    reads the old one).
+
+    ``kv_cache`` (with ``sequence``, its row): decode into that paged 8-bit cache
+    (eredu_amd.paged) instead of dense bf16 caches of ``max_seq`` positions, from
+    whatever the sequence holds already -- a prompt's tokens, or a prefix that
+    other sequences share.  The cache keeps the position, so steps are
+    ``step_device()``; each grows the sequence by a token, and one captured graph of
+    it decodes across page borders."""
 
     def __init__(self, layers: Sequence[DecoderLayer], embed: torch.Tensor, final_norm: torch.Tensor,
                  lm_head: QLinear, *, n_heads: int, n_kv_heads: int, eps: float, freqs: np.ndarray, max_seq: int,
                  k_caches: Optional[List[torch.Tensor]] = None, v_caches: Optional[List[torch.Tensor]] = None,
-                 fused: Optional[bool] = None):
+                 fused: Optional[bool] = None, kv_cache: Optional[PagedKVCache] = None, sequence: int = 0):
         dev = embed.device
         self.layers = list(layers)
         self.embed, self.final_norm, self.lm_head = embed, final_norm, lm_head
@@ -247,11 +255,23 @@ class LlamaDecoder:
         H, bf = self.hidden, torch.bfloat16
         if n_heads * HEAD_DIM != L0.q.N or n_kv_heads * HEAD_DIM != L0.k.N or L0.q.K != H:
             raise _native.EreduError("projection shapes do not match the head geometry")
-        cache_shape = (n_kv_heads, max_seq, HEAD_DIM)
-        self.k_caches = k_caches if k_caches is not None else [torch.zeros(cache_shape, dtype=bf, device=dev)
-                                                                for _ in self.layers]
-        self.v_caches = v_caches if v_caches is not None else [torch.zeros(cache_shape, dtype=bf, device=dev)
-                                                                for _ in self.layers]
+        self.kv_cache, self.k_caches, self.v_caches = kv_cache, [], []
+        if kv_cache is None:
+            cache_shape = (n_kv_heads, max_seq, HEAD_DIM)
+            self.k_caches = k_caches if k_caches is not None else [torch.zeros(cache_shape, dtype=bf, device=dev)
+                                                                    for _ in self.layers]
+            self.v_caches = v_caches if v_caches is not None else [torch.zeros(cache_shape, dtype=bf, device=dev)
+                                                                    for _ in self.layers]
+        else:
+            if k_caches is not None or v_caches is not None:
+                raise _native.EreduError("a paged cache takes the place of k_caches and v_caches")
+            if (kv_cache.n_layers, kv_cache.n_kv_heads, kv_cache.head_dim) != (len(self.layers), n_kv_heads, HEAD_DIM) or \
+                    kv_cache.device != dev:
+                raise _native.EreduError("the paged cache's layers, heads, head width or device are not the model's")
+            if not 0 <= sequence < kv_cache.max_seqs:
+                raise _native.EreduError(f"sequence {sequence} outside the cache's {kv_cache.max_seqs}")
+            self._seq = torch.tensor([sequence], dtype=torch.int32, device=dev)
+            self._rope = rope_table(freqs, kv_cache.max_pages_per_seq * kv_cache.page_size, dev)
         e = lambda n: torch.empty((n,), dtype=bf, device=dev)
         self.x, self.h = e(H), e(H)
         self.q, self.k, self.v = e(L0.q.N), e(L0.k.N), e(L0.v.N)
@@ -337,9 +357,11 @@ class LlamaDecoder:
         # embedding; per layer 2 norms, 4 projection launches, attention (2
         # kernels), silu_mul; final norm, LM head, argmax, and the position
         # advance of step_device (fused: the norms and silu_mul ride in the
-        # projections' launches)
-        per_layer = 6 if self.fused else 9
-        tail = (2 if self.fused else 3) + (1 if device_position else 0)
+        # projections' launches).  A paged cache: an append more per layer, and
+        # its extension (2 kernels) instead of the advance.
+        paged = self.kv_cache is not None
+        per_layer = (6 if self.fused else 9) + (1 if paged else 0)
+        tail = (2 if self.fused else 3) + (2 if paged else 1 if device_position else 0)
         return 1 + len(self.layers) * per_layer + tail
 
     def _pro(self, probs, count: int, lin: QLinear, pro, st: int) -> None:
@@ -350,7 +372,11 @@ class LlamaDecoder:
     def _attend(self, li: int, pos: Optional[int], st: int) -> None:
         """Layer li's attention at ``pos``, or at the device position when None."""
         n, L = _native, _native.lib()
-        if pos is None:
+        if self.kv_cache is not None:
+            heads = lambda t: t.view(1, -1, HEAD_DIM)
+            self.kv_cache.append(li, heads(self.k), heads(self.v), self._seq, rope=self._rope)
+            self.kv_cache.attention(li, heads(self.q), self._seq, scale=self.scale, rope=self._rope, out=heads(self.att))
+        elif pos is None:
             check(L.eq_rope_attention_decode_at(
                 self.att.data_ptr(), self.q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(),
                 self.k_caches[li].data_ptr(), self.v_caches[li].data_ptr(), self.freqs.data_ptr(),
@@ -365,6 +391,8 @@ class LlamaDecoder:
     def set_position(self, pos: int) -> None:
         """Writes the device position that ``step_device`` decodes next (a copy
         on the current stream; not inside a capture)."""
+        if self.kv_cache is not None:
+            raise _native.EreduError("a paged cache keeps the position itself")
         if not 0 <= pos < self.max_seq:
             raise _native.EreduError(f"position {pos} outside the cache of {self.max_seq}")
         self.position.fill_(int(pos))
@@ -372,13 +400,18 @@ class LlamaDecoder:
     def step_device(self) -> None:
         """One step at the device position, then position += 1 (one launch).  A
         position that reaches max_seq makes attention write no cache row and
-        return zeros; the caller stops before that, as it would with step()."""
+        return zeros; the caller stops before that, as it would with step().
+        With a paged cache its sequence grows by the token first; when pages run out the
+        new token is not kept, and ``kv_cache.check()`` says so."""
         st = _stream()
+        if self.kv_cache is not None:
+            self.kv_cache.extend(self._seq, 1)
         if self.fused:
             self._step_fused(None, st)
         else:
             self._step_unfused(None, st)
-        check(_native.lib().eq_advance_position(self.position.data_ptr(), st))
+        if self.kv_cache is None:
+            check(_native.lib().eq_advance_position(self.position.data_ptr(), st))
 
     def _step_fused(self, pos: Optional[int], st: int) -> None:
         n, L = _native, _native.lib()
@@ -403,6 +436,8 @@ class LlamaDecoder:
         check(L.eq_argmax(self.token.data_ptr(), self.logits.data_ptr(), 1, self.lm_head.N, bf, st))
 
     def step(self, pos: int) -> None:
+        if self.kv_cache is not None:
+            raise _native.EreduError("a paged cache keeps the position: use step_device()")
         if not 0 <= pos < self.max_seq:
             raise _native.EreduError(f"position {pos} outside the cache of {self.max_seq}")
         st = _stream()
@@ -446,7 +481,7 @@ class LlamaDecoder:
         total = sum(lin_bytes(getattr(Lr, p)) for Lr in self.layers
                     for p in ("q", "k", "v", "o", "gate", "up", "down"))
         total += lin_bytes(self.lm_head)
-        kv = 2 * self.n_kv_heads * HEAD_DIM * 2  # one row of K and of V
+        kv = 2 * self.n_kv_heads * HEAD_DIM * (2 if self.kv_cache is None else 1)  # one row of K and of V
         total += len(self.layers) * (kv * (pos + 1) + kv)  # rows 0..pos read, row pos written
         total += len(self.layers) * 2 * self.hidden * 2 + self.hidden * 2  # norm weights
         total += self.hidden * 2  # embedding row
