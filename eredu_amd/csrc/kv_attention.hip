@@ -12,11 +12,10 @@ namespace {
 //
 //   S^T = K . q^T on the int8 matrix cores.  K is the codes as they lie in the cache; q
 //   is, per row, an integer of 16 bits of its largest magnitude, split into two
-//   signed digits q = 256 hi + lo: the products are exact in 32 bits
-//   (256 * 127 * 32512 < 2^31) and the digits' sums join by a shift before the
-//   second product, S = sum lo c + 256 sum hi c.  No key is converted.
+//   signed digits q = 256 hi + lo: the products are exact
+//   and the digits' sums join in f32, S = sum lo c + 256 sum hi c.  No key is converted.
 //   softmax: a row's score is S * f + const with f = scale * log2 e * (row's step) *
-//   (page's step), one fma and one exp2 from the integer.
+//   (page's step), one fma and one exp2.
 //   O^T += V^T . P^T in f16.  S^T comes out of the matrix cores with a lane
 //   holding one query row and 4 tokens of each of 4 products; the 16 tokens of
 //   a product are chosen as {16 a + 4 t + b}, so that lane group g holds the tokens
@@ -76,6 +75,34 @@ __device__ __forceinline__ void kv_query_load(const uint16_t* x, const float* ro
     }
 }
 
+// A row's integers: multiples of its largest magnitude (given by its bits) / 32512,
+// as two signed digits q = 256 hi + lo; f: what a product of them with a page's codes is
+// worth in exponents, before the page's scale (s2 = scale * log2 e).
+struct Digits {
+    float f, inv;
+    int e;
+    bool fine;
+    __device__ __forceinline__ Digits(uint32_t most, float s2) {
+        fine = most > 0u && most < 0x7f800000u;
+        const float one = fine ? __uint_as_float(most) : 1.f;
+        e = __builtin_amdgcn_frexp_expf(one);
+        const float mant = __builtin_amdgcn_frexp_mantf(one);
+        inv = 32512.f / mant;
+        f = fine ? __builtin_amdgcn_ldexpf(mant * (s2 / 32512.f), e) : (most ? __uint_as_float(0x7fc00000u) : 0.f);
+    }
+    __device__ __forceinline__ void word(const float* v, i32x4& hi, i32x4& lo, int w) const {
+        uint32_t h = 0, l = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int x = int(rintf(__builtin_amdgcn_ldexpf(v[i], -e) * inv));
+            const int top = (x + 128) >> 8;
+            h |= uint32_t(top & 0xff) << (8 * i);
+            l |= uint32_t((x - 256 * top) & 0xff) << (8 * i);
+        }
+        hi[w] = fine ? int(h) : 0, lo[w] = fine ? int(l) : 0;
+    }
+};
+
 // The row turned (where it has angles), as digits of its largest magnitude;
 // s2 = scale * log2 e.  sees: whether there is a row that sees anything.
 template <typename T, int D>
@@ -121,33 +148,24 @@ __device__ __forceinline__ void kv_query(const RawQuery<D>& q, bool sees, bool t
         for (int i = 0; i < 16; i++) most = max(most, __float_as_uint(v[ks][i]) & 0x7fffffffu);
     most = max(most, uint32_t(__shfl_xor(int(most), 16)));
     most = max(most, uint32_t(__shfl_xor(int(most), 32)));
-    const bool fine = most > 0u && most < 0x7f800000u;
-    const float one = fine ? __uint_as_float(most) : 1.f;
-    const int e = __builtin_amdgcn_frexp_expf(one);
-    const float mant = __builtin_amdgcn_frexp_mantf(one), inv = 32512.f / mant;
-    f = fine ? __builtin_amdgcn_ldexpf(mant * (s2 / 32512.f), e) : (most ? __uint_as_float(0x7fc00000u) : 0.f);
+    const Digits dg(most, s2);
+    f = dg.f;
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++) {
+    for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            uint32_t h = 0, l = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int x = int(rintf(__builtin_amdgcn_ldexpf(v[ks][4 * w + i], -e) * inv));
-                const int top = (x + 128) >> 8;
-                h |= uint32_t(top & 0xff) << (8 * i);
-                l |= uint32_t((x - 256 * top) & 0xff) << (8 * i);
-            }
-            hi[ks][w] = fine ? int(h) : 0, lo[ks][w] = fine ? int(l) : 0;
-        }
-    }
+        for (int w = 0; w < 4; w++) dg.word(v[ks] + 4 * w, hi[ks], lo[ks], w);
 }
 
-// The integer scores of 64 tokens: s[r][t][i] is row r's with token 4 t + i of
-// this lane group's 16; k(t, ks) gives the operands.
+// The scores of 64 tokens, plus kMagic: s[r][t][i] is row r's with token 4 t + i
+// of this lane group's 16; k(t, ks) gives the operands.  The products of a digit
+// stay below 2^22 (256 * 127 * 128), so sums that begin with the bits of 1.5 * 2^23
+// are that float plus the sum, and no score is converted (v_cvt_f32_i32 takes as long as two
+// or three fmas: 83 ns for 16 in a loop, where 16 fmas take 39).
+constexpr float kMagic = 12582912.f;
 template <int D, int NR, typename KF>
-__device__ __forceinline__ void kv_scores(const Rows<D, NR>& R, KF k, i32x4 (&s)[NR][4]) {
+__device__ __forceinline__ void kv_scores(const Rows<D, NR>& R, KF k, f32x4 (&s)[NR][4]) {
     constexpr int KS = D / 64;
+    constexpr int M = 0x4b400000;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
         i32x4 a[KS];
@@ -155,12 +173,13 @@ __device__ __forceinline__ void kv_scores(const Rows<D, NR>& R, KF k, i32x4 (&s)
         for (int ks = 0; ks < KS; ks++) a[ks] = k(t, ks);
 #pragma unroll
         for (int r = 0; r < NR; r++) {
-            i32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
+            i32x4 hi = {M, M, M, M}, lo = {M, M, M, M};
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[ks], R.hi[r][ks], hi, 0, 0, 0);
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[ks], R.lo[r][ks], lo, 0, 0, 0);
-            s[r][t] = (hi << 8) + lo;
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[r][t][i] = fmaf(__int_as_float(hi[i]) - kMagic, 256.f, __int_as_float(lo[i]));
         }
     }
 }
@@ -172,7 +191,7 @@ __device__ __forceinline__ void kv_scores(const Rows<D, NR>& R, KF k, i32x4 (&s)
 // this tile's included.  edge (the same for the wave): some row does not see some of the
 // tokens; their scores are set below all others for the maximum, their exponents to -inf.
 template <int D, int NR>
-__device__ __forceinline__ void kv_softmax(Rows<D, NR>& R, i32x4 (&s)[NR][4], int kb, bool nan, int j0, bool dead, bool edge,
+__device__ __forceinline__ void kv_softmax(Rows<D, NR>& R, f32x4 (&s)[NR][4], int kb, bool nan, int j0, bool dead, bool edge,
                                            int base, h16x8 (&p)[NR][2]) {
     constexpr int DT = D / 16;
     const float kf = nan ? __uint_as_float(0x7fc00000u) : e8m0_to_f32(uint32_t(kb));
@@ -188,16 +207,16 @@ __device__ __forceinline__ void kv_softmax(Rows<D, NR>& R, i32x4 (&s)[NR][4], in
             seen[r] = max(min(R.until[r] - j0, 16) - first[r], 0);
 #pragma unroll
             for (int n = 0; n < 16; n++)
-                if (unsigned(n - first[r]) >= unsigned(seen[r])) s[r][n >> 2][n & 3] = INT32_MIN;
+                if (unsigned(n - first[r]) >= unsigned(seen[r])) s[r][n >> 2][n & 3] = -1e30f;
         }
     }
 #pragma unroll
     for (int r = 0; r < NR; r++) {
         f[r] = R.f[r] * kf;
-        int mx = s[r][0][0];
+        float mx = s[r][0][0];
 #pragma unroll
-        for (int n = 1; n < 16; n++) mx = max(mx, s[r][n >> 2][n & 3]);
-        top[r] = seen[r] > 0 ? float(mx) * f[r] : -INFINITY;
+        for (int n = 1; n < 16; n++) mx = fmaxf(mx, s[r][n >> 2][n & 3]);
+        top[r] = seen[r] > 0 ? (mx - kMagic) * f[r] : -INFINITY;
         need |= top[r] > R.m[r] + kMaxSlack;
     }
     if (__any(need)) {
@@ -214,19 +233,18 @@ __device__ __forceinline__ void kv_softmax(Rows<D, NR>& R, i32x4 (&s)[NR][4], in
             for (int dt = 0; dt < DT; dt++) R.o[r][dt] *= al * down;
         }
     }
-    f32x4 x[NR][4];
 #pragma unroll
     for (int r = 0; r < NR; r++) {
-        const float shift = kProbBias - R.m[r];
+        const float shift = fmaf(-kMagic, f[r], kProbBias - R.m[r]);
 #pragma unroll
-        for (int n = 0; n < 16; n++) x[r][n >> 2][n & 3] = fmaf(float(s[r][n >> 2][n & 3]), f[r], shift);
+        for (int n = 0; n < 16; n++) s[r][n >> 2][n & 3] = fmaf(s[r][n >> 2][n & 3], f[r], shift);
     }
     if (edge) {
 #pragma unroll
         for (int r = 0; r < NR; r++)
 #pragma unroll
             for (int n = 0; n < 16; n++)
-                if (unsigned(n - first[r]) >= unsigned(seen[r])) x[r][n >> 2][n & 3] = -INFINITY;
+                if (unsigned(n - first[r]) >= unsigned(seen[r])) s[r][n >> 2][n & 3] = -INFINITY;
     }
 #pragma unroll
     for (int r = 0; r < NR; r++) {
@@ -235,10 +253,10 @@ __device__ __forceinline__ void kv_softmax(Rows<D, NR>& R, i32x4 (&s)[NR][4], in
         for (int t = 0; t < 4; t++) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                x[r][t][i] = __builtin_amdgcn_exp2f(x[r][t][i]);
-                sum += x[r][t][i];
+                s[r][t][i] = __builtin_amdgcn_exp2f(s[r][t][i]);
+                sum += s[r][t][i];
             }
-            const h16x4 h = __builtin_convertvector(x[r][t], h16x4);
+            const h16x4 h = __builtin_convertvector(s[r][t], h16x4);
 #pragma unroll
             for (int i = 0; i < 4; i++) p[r][t >> 1][(t & 1) * 4 + i] = h[i];
         }
@@ -621,7 +639,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_stream_kernel(const 
         kv_fetch_values<D>(A, P, tile, idg, t);
         for (; tile < end; tile++) {
             const bool more = tile + 1 < end;
-            i32x4 s[NR][4];
+            f32x4 s[NR][4];
             kv_scores<D, NR>(R, [&](int i, int ks) __attribute__((always_inline)) { return t.k[i][ks]; }, s);
             int kbn = 0, vbn = 0, idn = -1;
             if (more) {
@@ -801,42 +819,41 @@ __device__ __forceinline__ int kv_key_swap(int token) {
 }
 __device__ __forceinline__ int kv_value_swap(int d) { return (d & 1) | (d >> 1 & 2) | (d << 1 & 4); }
 
-// A wave's share of a tile's keys, pieces (j * 4 + wave) * 64 + lane of it: from a page
-// (a scalar: a wave's 1024 / D tokens lie in one block of 16) and an offset in it that is
-// the same for every tile.
+// A tile's keys and values are 4 D pieces each; piece p = j * threads + thread of
+// the keys is in a page (a scalar: a wave's 1024 / D tokens lie in one block of 16) at an
+// offset that is the same for every tile.
 template <int D>
-__device__ __forceinline__ int kv_key_offset(int j, int T) {
+__device__ __forceinline__ int kv_key_offset(int p, int T) {
     constexpr int KP = D / 16;  // 16-byte pieces of a key
-    const int p = (j * 4 + int(threadIdx.x >> 6)) * 64 + (threadIdx.x & 63), token = p / KP;
-    return (token & (T - 1)) * D + 16 * (p % KP);
+    return (p / KP & (T - 1)) * D + 16 * (p % KP);
 }
 template <int D>
-__device__ __forceinline__ int kv_key_place(int j) {
+__device__ __forceinline__ int kv_key_place(int p) {
     constexpr int KP = D / 16;
-    const int p = (j * 4 + int(threadIdx.x >> 6)) * 64 + (threadIdx.x & 63), token = p / KP;
-    return token * KP + ((p % KP) ^ kv_key_swap<D>(token));
+    return p / KP * KP + ((p % KP) ^ kv_key_swap<D>(p / KP));
 }
-// Where piece (j * 4 + wave) * 64 of a tile's keys lies, in page `id` of those of this lane's group.
+// The page of a wave's pieces, the first of them piece p; id: of this lane's group.
 template <int D>
-__device__ __forceinline__ const int8_t* kv_key_page(const AttnCall& A, const Place& P, int tile, int idg, int j) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), T = 1 << A.c.log2_page;
-    const int id = __builtin_amdgcn_readlane(idg, (j * 4 + wave) * 64 / D * 16);  // of token block (j * 4 + wave) * 64 / D
+__device__ __forceinline__ const int8_t* kv_key_page(const AttnCall& A, const Place& P, int tile, int idg, int p) {
+    const int T = 1 << A.c.log2_page, id = __builtin_amdgcn_readlane(idg, p / D * 16);  // of token block p / D
     return A.c.k + ((int64_t(max(id, 0)) * A.c.kv_heads + P.kvh) * T + (tile * 64 & (T - 1))) * D;
 }
 
-template <typename T, int D, int NR>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_block_kernel(const AttnCall A) {
-    constexpr int BM = 64 * NR;
+// NW waves of 16 * NR rows; WPS of them to a SIMD.
+template <typename T, int D, int NR, int NW, int WPS>
+__global__ __launch_bounds__(64 * NW, WPS) void kv_block_kernel(const AttnCall A) {
+    constexpr int BM = 16 * NR * NW, THREADS = 64 * NW, PT = 4 * D / THREADS;
+    static_assert(PT * THREADS == 4 * D, "whole pieces a thread");
     __shared__ i32x4 k0[4 * D], k1[4 * D];
     __shared__ __attribute__((aligned(16))) h16x8 v0[8 * D], v1[8 * D];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
     Place P;
     if (!kv_place<BM>(A, P)) return;
     const int rows = min(BM, P.e.count * int(A.group) - P.first);
     const TileRange all = kv_tiles(A, P.e, unsigned(P.first) / A.group, unsigned(P.first + rows - 1) / A.group);
     const int share = kv_share(A, all), begin = all.begin + P.split * share, end = min(all.end, begin + share);
     if (A.part && begin >= end) {
-        if (int(threadIdx.x) < rows) kv_store_lse(A, P, P.first + threadIdx.x, -INFINITY);
+        if (tid < rows) kv_store_lse(A, P, P.first + tid, -INFINITY);
         return;
     }
     // this wave's rows, the tiles that any of them sees and those that all see whole
@@ -855,11 +872,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_block_kernel(const A
         clear_from = (kv_from(A, P.e, i1) + 63) >> 6, clear_until = max(kv_until(A, P.e, i0), 0) >> 6;
     }
     const int page_tokens = 1 << A.c.log2_page;
-    int ofs[D / 64];
+    int ofs[PT];
 #pragma unroll
-    for (int j = 0; j < D / 64; j++) ofs[j] = kv_key_offset<D>(j, page_tokens);
-    // of the values, this thread's pieces are the 16 tokens 16 gv .. of dimensions tid / 4 + 64 j
-    const int gv = lane & 3, dv = threadIdx.x >> 2;
+    for (int j = 0; j < PT; j++) ofs[j] = kv_key_offset<D>(j * THREADS + tid, page_tokens);
+    // of the values, piece p is the 16 tokens 16 (p % 4) .. of dimension p / 4
+    const int gv = lane & 3, dv = tid >> 2;
     // (table entries and scale bytes are looked at a step after they are requested, so that nothing
     // waits for them; begin < end: there is a sequence)
     auto table = [&](int tile, int block) __attribute__((always_inline)) {
@@ -868,7 +885,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_block_kernel(const A
     if (begin < end) {
         int tile = begin, base = 0, base_next = 0;
         int eg = table(tile, g), ev = table(tile, gv), idn, idv, kb, vb, kbn, vbn, vbv;
-        i32x4 raw[D / 64], rawk[D / 64];
+        i32x4 raw[PT], rawk[PT];
         // requests tile `t` (table entries eg, ev): its scales, values and keys
         auto request = [&](int t) __attribute__((always_inline)) {
             idn = kv_page_of(A.c, eg), idv = kv_page_of(A.c, ev);
@@ -878,20 +895,20 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_block_kernel(const A
             kbn = A.c.ks[at], vbn = A.c.vs[at], vbv = A.c.vs[av];
             const int8_t* src = A.c.v + (av * D + dv) * page_tokens + ((t * 64 + 16 * gv) & (page_tokens - 1));
 #pragma unroll
-            for (int j = 0; j < D / 64; j++) raw[j] = *reinterpret_cast<const i32x4*>(src + 64 * j * page_tokens);
+            for (int j = 0; j < PT; j++) raw[j] = *reinterpret_cast<const i32x4*>(src + THREADS / 4 * j * page_tokens);
 #pragma unroll
-            for (int j = 0; j < D / 64; j++)
-                rawk[j] = *reinterpret_cast<const i32x4*>(kv_key_page<D>(A, P, t, idn, j) + unsigned(ofs[j]));
+            for (int j = 0; j < PT; j++)
+                rawk[j] = *reinterpret_cast<const i32x4*>(kv_key_page<D>(A, P, t, idn, j * THREADS + 64 * wave) + unsigned(ofs[j]));
         };
         // its values as f16
         auto convert = [&](i32x4* kbuf, h16x8* vbuf) __attribute__((always_inline)) {
             base_next = max(base, kv_group_max(idn < 0 || vbn == 255 ? 0 : vbn));
 #pragma unroll
-            for (int j = 0; j < D / 64; j++) kbuf[kv_key_place<D>(j)] = rawk[j];
+            for (int j = 0; j < PT; j++) kbuf[kv_key_place<D>(j * THREADS + tid)] = rawk[j];
             const Convert to(idv < 0 || vbv == 255 ? 0 : vbv, base_next);
 #pragma unroll
-            for (int j = 0; j < D / 64; j++) {
-                const int d = dv + 64 * j;
+            for (int j = 0; j < PT; j++) {
+                const int d = dv + THREADS / 4 * j;
                 vbuf[8 * d + (gv ^ kv_value_swap(d))] = to(uint32_t(raw[j][0]), uint32_t(raw[j][1]));
                 vbuf[8 * d + ((4 + gv) ^ kv_value_swap(d))] = to(uint32_t(raw[j][2]), uint32_t(raw[j][3]));
             }
@@ -904,7 +921,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_block_kernel(const A
             kb = kbn, vb = vbn, base = base_next;
             if (more) request(tile + 1);
             if (tile >= see_from && tile < see_until) {
-                i32x4 s[NR][4];
+                f32x4 s[NR][4];
                 kv_scores<D, NR>(R, [&](int t, int ks) __attribute__((always_inline)) {
                     const int token = 4 * (lane & 12) + 4 * t + (lane & 3);
                     return kc[token * (D / 16) + ((4 * ks + g) ^ kv_key_swap<D>(token))];
@@ -1013,7 +1030,7 @@ Plan plan_attention(const eq_kv_cache* c, int n_heads, int64_t n, int64_t total,
         return ragged ? total * group / bm + n : n * ((total / (n ? n : 1) * group + bm - 1) / bm);
     };
     const int64_t most = blocks(kStreamRows) * c->kv_heads;  // units of a stream (over 2^31 tiles are not listed)
-    p.rows = rows <= 48 && most < INT32_MAX / cap ? kStreamRows : (rows <= 64 || c->head_dim > 128 ? 64 : 128);
+    p.rows = rows <= 48 && most < INT32_MAX / cap ? kStreamRows : (rows <= 64 ? 64 : 128);
     p.tiles = blocks(p.rows);
     if (p.rows == kStreamRows) {
         const int64_t runs = (most * cap + 3) / 4;  // at least a tile for each of 4 waves
@@ -1025,11 +1042,11 @@ Plan plan_attention(const eq_kv_cache* c, int n_heads, int64_t n, int64_t total,
         p.lse_bytes = (size_t(p.groups) * 8 * kStreamRows * 4 + 255) & ~size_t(255);
         return p;
     }
-    // two workgroups fit a CU: as many splits as come nearest to filling that once (300 queries over
-    // 8000 tokens, 80 blocks: 560 workgroups 95 us, 480 79 us)
+    // two workgroups fit a CU, at 256 dimensions one: as many splits as come nearest to filling that once
+    // (300 queries over 8000 tokens, 80 blocks: 560 workgroups 95 us, 480 79 us)
     // (of a ragged batch, whose blocks are bounded by one a sequence too many, those of even sequences)
     const int64_t likely = n * ((rows + p.rows - 1) / p.rows) * c->kv_heads;
-    int64_t splits = likely ? (2 * device_cu_count() + likely / 2) / likely : 1;
+    int64_t splits = likely ? ((c->head_dim <= 128 ? 2 : 1) * device_cu_count() + likely / 2) / likely : 1;
     if (splits > (cap + 3) / 4) splits = (cap + 3) / 4;
     if (splits > 1024) splits = 1024;
     p.splits = splits < 1 ? 1 : int(splits);
@@ -1130,8 +1147,12 @@ extern "C" int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n
             else kv_stream_join_kernel<T, DIM, 4><<<rows, dim3(256), 0, st>>>(A);
             return;
         }
-        if (plan.rows == 64) kv_block_kernel<T, DIM, 1><<<grid, dim3(256), 0, st>>>(A);
-        else if constexpr (DIM <= 128) kv_block_kernel<T, DIM, 2><<<grid, dim3(256), 0, st>>>(A);
+        // 128 rows are 4 waves of 32 up to 128 dimensions (2048 queries over 32768 tokens of 128: 1.19 ms;
+        // 8 of 16, whose registers spill at four to a SIMD, 1.33), 8 of 16 at 256, where 4 waves of 32 do not
+        // fit and 64 rows to a workgroup read every key twice as often (0.59 ms against 1.05)
+        if (plan.rows == 64) kv_block_kernel<T, DIM, 1, 4, DIM == 64 ? 4 : DIM == 128 ? 3 : 1><<<grid, dim3(256), 0, st>>>(A);
+        else if constexpr (DIM <= 128) kv_block_kernel<T, DIM, 2, 4, 2><<<grid, dim3(256), 0, st>>>(A);
+        else kv_block_kernel<T, DIM, 1, 8, 2><<<grid, dim3(512), 0, st>>>(A);
         if (plan.splits > 16) kv_join_kernel<T, DIM, 4><<<dim3(unsigned(total), unsigned(n_heads)), dim3(256), 0, st>>>(A);
         else if (plan.splits > 1) kv_join_kernel<T, DIM, 1><<<dim3(unsigned(total), unsigned((n_heads + 3) / 4)), dim3(256), 0, st>>>(A);
     };
