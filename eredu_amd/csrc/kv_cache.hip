@@ -201,10 +201,10 @@ __device__ __forceinline__ uint32_t kv_places(int t, int from, int until) {
 // bytes, to be written along the tokens, 16 of a dimension at once.
 constexpr int kAppendItems = 2;
 
-template <typename T>
+template <typename T, int D>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvView c, KvBatch b, const uint16_t* __restrict__ k,
                                                         const uint16_t* __restrict__ v, int64_t k_stride,
-                                                        int64_t v_stride, const float* __restrict__ rope, int D) {
+                                                        int64_t v_stride, const float* __restrict__ rope) {
     extern __shared__ __attribute__((aligned(16))) uint8_t turn[];  // values: [token][D + 4]
     __shared__ uint32_t red[4];
     const int tid = threadIdx.x, head = blockIdx.y, log2_page = c.log2_page, page_tokens = 1 << log2_page;
@@ -214,7 +214,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvView c, KvBatch b, con
     const KvEntry e = kv_entry(c, b, entry);
     if (e.seq < 0) return;
     const KvSpan s = kv_span(c, e, place);
-    const int groups = D / 16, items = max(s.until - s.from, 0) * groups;
+    constexpr int groups = D / 16, pitch = D + 4;
+    const int items = max(s.until - s.from, 0) * groups;
     const uint16_t* x = (values ? v + int64_t(s.row) * v_stride : k + int64_t(s.row) * k_stride) + int64_t(head) * D;
     const int64_t stride = values ? v_stride : k_stride;
     // (the rows are read whether or not the page is there: they are rows of this call; the angles only
@@ -261,7 +262,6 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvView c, KvBatch b, con
     const float inv = kv_inverse(now);
 
     int8_t* codes = (values ? c.v : c.k) + (int64_t(s.page) * c.kv_heads + head) * page_tokens * D;
-    const int pitch = D + 4;
     auto put = [&](int it, const float (&y)[16]) __attribute__((always_inline)) {
         const int t = it / groups, d0 = it % groups * 8;
         uint32_t w[4] = {0u, 0u, 0u, 0u};
@@ -345,9 +345,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvView c, KvBatch b, con
 
 // Grid (page units, kv_heads, keys | values), 256 threads: the rows of one page
 // and head; values turn in LDS, by 4 x 4 bytes.
-template <typename T>
+template <typename T, int D>
 __global__ __launch_bounds__(256) void kv_read_kernel(typename T::storage* __restrict__ k,
-                                                      typename T::storage* __restrict__ v, KvView c, KvBatch b, int D) {
+                                                      typename T::storage* __restrict__ v, KvView c, KvBatch b) {
     extern __shared__ __attribute__((aligned(16))) uint8_t turn[];  // values: [token][D + 4]
     const int tid = threadIdx.x, head = blockIdx.y, log2_page = c.log2_page, page_tokens = 1 << log2_page;
     const bool values = blockIdx.z != 0;
@@ -358,7 +358,8 @@ __global__ __launch_bounds__(256) void kv_read_kernel(typename T::storage* __res
     if (s.from >= s.until) return;
     typename T::storage* out = (values ? v : k) + (int64_t(s.row) * c.kv_heads + head) * D;
     const int64_t stride = int64_t(c.kv_heads) * D;
-    const int groups = D / 8, items = (s.until - s.from) * groups, pitch = D + 4;
+    constexpr int groups = D / 8, pitch = D + 4;
+    const int items = (s.until - s.from) * groups;
     const bool here = s.page >= 0;
     const int64_t at = (int64_t(here ? s.page : 0) * c.kv_heads + head);
     const int8_t* codes = (values ? c.v : c.k) + at * page_tokens * D;
@@ -386,20 +387,33 @@ __global__ __launch_bounds__(256) void kv_read_kernel(typename T::storage* __res
         }
         __syncthreads();
     }
-    for (int it = tid; it < items; it += 256) {
-        const int t = it / groups, d0 = it % groups * 8;
-        uint32_t w[2] = {0u, 0u};
-        if (here) {
-            const uint32_t* p = values ? reinterpret_cast<const uint32_t*>(turn + t * pitch + d0)
-                                       : reinterpret_cast<const uint32_t*>(codes + (s.from + t) * D + d0);
-            w[0] = p[0], w[1] = p[1];
+    constexpr int kAtOnce = 4;  // pieces of 8 codes a thread requests before it writes one
+    for (int base = tid; base < items; base += kAtOnce * 256) {
+        uint2 w[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; u++) {
+            const int it = base + 256 * u, t = it / groups, d0 = it % groups * 8;
+            w[u] = make_uint2(0u, 0u);
+            if (!here || it >= items) continue;
+            if (values) {
+                const uint32_t* p = reinterpret_cast<const uint32_t*>(turn + t * pitch + d0);
+                w[u] = make_uint2(p[0], p[1]);
+            } else {
+                w[u] = *reinterpret_cast<const uint2*>(codes + (s.from + t) * D + d0);
+            }
         }
-        alignas(16) typename T::storage o[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) o[i] = to_storage<T>(here ? float(int8_t(w[i >> 2] >> (8 * (i & 3)))) * scale : 0.f);
-        uint4* to = reinterpret_cast<uint4*>(out + t * stride + d0);
+        for (int u = 0; u < kAtOnce; u++) {
+            const int it = base + 256 * u, t = it / groups, d0 = it % groups * 8;
+            if (it >= items) continue;
+            alignas(16) typename T::storage o[8];
 #pragma unroll
-        for (int i = 0; i < int(sizeof(o) / 16); i++) to[i] = reinterpret_cast<const uint4*>(o)[i];
+            for (int i = 0; i < 8; i++)
+                o[i] = to_storage<T>(here ? float(int8_t((i < 4 ? w[u].x : w[u].y) >> (8 * (i & 3)))) * scale : 0.f);
+            uint4* to = reinterpret_cast<uint4*>(out + t * stride + d0);
+#pragma unroll
+            for (int i = 0; i < int(sizeof(o) / 16); i++) to[i] = reinterpret_cast<const uint4*>(o)[i];
+        }
     }
 }
 
@@ -814,10 +828,16 @@ extern "C" int eq_kv_append(const eq_kv_cache* cache, int64_t layer, const void*
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     auto go = [&](auto kern) {
         kern<<<grid, dim3(256), lds, st>>>(c, b, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
-                                           k_stride, v_stride, rope, D);
+                                           k_stride, v_stride, rope);
     };
-    if (dtype == EQ_DTYPE_BF16) go(kv_append_kernel<BF16T>);
-    else go(kv_append_kernel<F16T>);
+    auto of = [&](auto t) {
+        typedef decltype(t) T;
+        if (D == 64) go(kv_append_kernel<T, 64>);
+        else if (D == 128) go(kv_append_kernel<T, 128>);
+        else go(kv_append_kernel<T, 256>);
+    };
+    if (dtype == EQ_DTYPE_BF16) of(BF16T{});
+    else of(F16T{});
     return check_launch(who);
 }
 
@@ -847,8 +867,13 @@ extern "C" int eq_kv_read(void* k, void* v, const eq_kv_cache* cache, int64_t la
     const dim3 grid(unsigned(units), unsigned(cache->kv_heads), 2);
     with_dtype(dtype, [&](auto t) {
         typedef decltype(t) T;
-        kv_read_kernel<T><<<grid, dim3(256), lds, reinterpret_cast<hipStream_t>(stream)>>>(
-            static_cast<typename T::storage*>(k), static_cast<typename T::storage*>(v), c, b, D);
+        auto go = [&](auto kern) {
+            kern<<<grid, dim3(256), lds, reinterpret_cast<hipStream_t>(stream)>>>(
+                static_cast<typename T::storage*>(k), static_cast<typename T::storage*>(v), c, b);
+        };
+        if (D == 64) go(kv_read_kernel<T, 64>);
+        else if (D == 128) go(kv_read_kernel<T, 128>);
+        else go(kv_read_kernel<T, 256>);
     });
     return check_launch(who);
 }
