@@ -68,7 +68,8 @@ def read(c=None, k=4096, v=4096, layer=0, seqs=4096, n=2, cu=None, total=2, dt=2
 BAD_CACHES = [(dict(k_codes=None), "null"), (dict(missing=None), "null"), (dict(page_tokens=48), "page_tokens"),
               (dict(page_tokens=8), "page_tokens"), (dict(page_tokens=256), "page_tokens"), (dict(head_dim=96), "head_dim"),
               (dict(kv_heads=0), "kv_heads"), (dict(pages=0), "positive"), (dict(width=0), "positive"),
-              (dict(width=1 << 40), "2^30"), (dict(pages=1 << 40), "positive"), (dict(v_codes=4104), "16-byte")]
+              (dict(width=1 << 40), "2^30"), (dict(width=1 << 20, sequences=1 << 11), "2^31"),
+              (dict(pages=1 << 40), "positive"), (dict(v_codes=4104), "16-byte")]
 
 
 @pytest.mark.parametrize("bad,word", BAD_CACHES)
