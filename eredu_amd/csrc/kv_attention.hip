@@ -821,18 +821,20 @@ __device__ __forceinline__ void kv_out4(const AttnCall& A, int64_t at, int t, fl
     *reinterpret_cast<uint2*>(A.out + at * D + 4 * t) = make_uint2(w[0] | uint32_t(w[1]) << 16, w[2] | uint32_t(w[3]) << 16);
 }
 
-// The units that lie in several runs of kv_stream_kernel: a workgroup for each row
-// (of the rows that entries cover) and query head, of 4 waves, or of 16 where there are
-// few (at most 64 entries, which TileList keeps within a wave): then a unit has many parts.
+// The units that lie in several runs of kv_stream_kernel: for each row (of the rows
+// that entries cover) and query head a wave, or a workgroup of 4, or of 16 (at most 64
+// entries, which TileList keeps within a wave): the fewer rows, the more parts a unit has.
 template <typename T, int D, int W>
-__global__ __launch_bounds__(64 * W) void kv_stream_join_kernel(const AttnCall A) {
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv_stream_join_kernel(const AttnCall A) {
     __shared__ Joiner<D, W> J;
     __shared__ TileListLds lds;
-    const int t = threadIdx.x, h = blockIdx.y, u = blockIdx.x;
+    const int t = W == 1 ? threadIdx.x & 63 : threadIdx.x, u = blockIdx.x;
+    const int h = W == 1 ? __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + (threadIdx.x >> 6)) : blockIdx.y;
     int entry, i;
     if (!kv_locate(A.b, u, [](int n) { return n; }, entry, i)) return;
     TileList list(A, lds);
     const int run = kv_run(A, list.all), base = list.tiles_before(A, entry);
+    if (W == 1 && h >= A.heads) return;
     const KvEntry e = list.entry(A, entry);
     const Units U = kv_units(A, e);
     const int row = i * A.group + unsigned(h) % A.group;
@@ -1091,7 +1093,7 @@ struct Plan {
     int64_t tiles;
     int splits;  // of a block's tokens
     int groups;  // workgroups of a stream
-    bool wide_join;
+    int join_waves;  // of a stream's rows: 16, 4 or 1
     size_t part_bytes, lse_bytes;
 };
 Plan plan_attention(const eq_kv_cache* c, int n_heads, int64_t n, int64_t total, bool ragged) {
@@ -1102,23 +1104,34 @@ Plan plan_attention(const eq_kv_cache* c, int n_heads, int64_t n, int64_t total,
         return ragged ? total * group / bm + n : n * ((total / (n ? n : 1) * group + bm - 1) / bm);
     };
     const int64_t most = blocks(kStreamRows) * c->kv_heads;  // units of a stream (over 2^31 tiles are not listed)
-    p.rows = rows <= 48 && most < INT32_MAX / cap ? kStreamRows : (rows <= 64 ? 64 : 128);
+    // blocks, and (of a ragged batch, whose blocks are bounded by one a sequence too many) those of even sequences
+    auto likely = [&](int bm) { return n * ((rows + bm - 1) / bm) * c->kv_heads; };
+    p.rows = 128;
+    if (rows <= 48 && most < INT32_MAX / cap) p.rows = kStreamRows;
+    else if (rows <= 64) p.rows = 64;
+    // 64 rows use a tile for half as many products (2048 rows over 4000 tokens of 128 dimensions: 114 us,
+    // 98 with 128), but fill the CUs with fewer (2 prompts of 128 tokens, 16 heads of 128 dimensions: 9.7 us, 15.2
+    // with 128; 512 rows over 8000 tokens lose by it, 61.6 and 57.6) and waste fewer (150 rows in 192: 44 us, in
+    // 256 57); at 256 dimensions, where they need the LDS of 128, they lose always (37 us, 29)
+    else if (c->head_dim <= 128 && (2 * likely(128) <= device_cu_count() || 7 * likely(64) < 12 * likely(128))) p.rows = 64;
     p.tiles = blocks(p.rows);
     if (p.rows == kStreamRows) {
         const int64_t runs = (most * cap + 3) / 4;  // at least a tile for each of 4 waves
         p.splits = 1;
         p.groups = int(runs < 2 * device_cu_count() ? runs : 2 * device_cu_count());
-        // 256 parts take 16 waves 2.7 us instead of 4 waves 6 us, 17 parts 4.7 instead of 3.9
-        p.wide_join = n <= 64 && total * n_heads <= 2 * device_cu_count() && cap > 64;
+        // few rows have many parts: 256 parts take 16 waves 2.7 us instead of 4 waves 6 us, 17 parts 4.7 instead
+        // of 3.9.  Many have few: 7200 rows take a wave each 6.3 us instead of 18.5 with 4 waves, 640 rows 7.2 instead of 5.4
+        const int64_t joins = total * n_heads;
+        p.join_waves = n <= 64 && joins <= 2 * device_cu_count() && cap > 64 ? 16 : (joins <= 4 * device_cu_count() ? 4 : 1);
         p.part_bytes = size_t(p.groups) * 8 * kStreamRows * c->head_dim * 4;
         p.lse_bytes = (size_t(p.groups) * 8 * kStreamRows * 4 + 255) & ~size_t(255);
         return p;
     }
-    // two workgroups fit a CU, at 256 dimensions one: as many splits as come nearest to filling that once
-    // (300 queries over 8000 tokens, 80 blocks: 560 workgroups 95 us, 480 79 us)
-    // (of a ragged batch, whose blocks are bounded by one a sequence too many, those of even sequences)
-    const int64_t likely = n * ((rows + p.rows - 1) / p.rows) * c->kv_heads;
-    int64_t splits = likely ? ((c->head_dim <= 128 ? 2 : 1) * device_cu_count() + likely / 2) / likely : 1;
+    // as many splits as come nearest to filling the CUs once (300 queries over 8000 tokens, 80 blocks: 560
+    // workgroups 95 us, 480 79 us); of 128 rows two workgroups fit a CU, of 64 three or, at 64 dimensions, four, at 256 one
+    const int fit = c->head_dim > 128 ? 1 : p.rows == 128 ? 2 : c->head_dim == 128 ? 3 : 4;
+    const int64_t units = likely(p.rows);
+    int64_t splits = units ? (fit * device_cu_count() + units / 2) / units : 1;
     if (splits > (cap + 3) / 4) splits = (cap + 3) / 4;
     if (splits > 1024) splits = 1024;
     p.splits = splits < 1 ? 1 : int(splits);
@@ -1215,8 +1228,9 @@ extern "C" int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n
         if (plan.rows == kStreamRows) {
             kv_stream_kernel<T, DIM><<<dim3(unsigned(plan.groups)), dim3(256), 0, st>>>(A);
             const dim3 rows{unsigned(total), unsigned(n_heads)};
-            if (plan.wide_join) kv_stream_join_kernel<T, DIM, 16><<<rows, dim3(1024), 0, st>>>(A);
-            else kv_stream_join_kernel<T, DIM, 4><<<rows, dim3(256), 0, st>>>(A);
+            if (plan.join_waves == 16) kv_stream_join_kernel<T, DIM, 16><<<rows, dim3(1024), 0, st>>>(A);
+            else if (plan.join_waves == 4) kv_stream_join_kernel<T, DIM, 4><<<rows, dim3(256), 0, st>>>(A);
+            else kv_stream_join_kernel<T, DIM, 1><<<dim3(unsigned(total), unsigned((n_heads + 3) / 4)), dim3(256), 0, st>>>(A);
             return;
         }
         // 128 rows are 4 waves of 32 up to 128 dimensions (2048 queries over 32768 tokens of 128: 1.19 ms;
