@@ -323,7 +323,7 @@ struct AttnCall {
     KvBatch b;
     const float* rope;
     float s2;      // scale * log2 e
-    int heads, tiles, splits, window;  // window 0: none
+    int heads, rows, tiles, splits, window;  // rows: of a workgroup; window 0: none
     unsigned group;
     bool causal;
     int groups;    // kv_stream_kernel's workgroups
@@ -349,9 +349,16 @@ __device__ __forceinline__ TileRange kv_tiles(const AttnCall& A, const KvEntry& 
     t.end = max((max(kv_until(A, e, i1), 0) + 63) >> 6, t.begin);
     return t;
 }
-// Tiles of a split: at least one for each of a workgroup's waves.
+// Tiles of a split of a block's, at least 4.
 __device__ __forceinline__ int kv_share(const AttnCall& A, const TileRange& t) {
     return max(4, (t.end - t.begin + A.splits - 1) / A.splits);
+}
+// Whether a block's first split does all of it and writes it out.  2 or 3 splits
+// are those of many rows, whose parts cost more than up to 16 tiles take longer in one: 4 prompts of 512
+// tokens, 16 heads of 64 dimensions, take 27 us so, 35 with all blocks split.  (Without a mask all blocks of a
+// sequence see the same, and looking costs the join 2 us.)
+__device__ __forceinline__ bool kv_whole(const AttnCall& A, const TileRange& t) {
+    return A.splits == 1 || (A.causal && t.end - t.begin <= (A.splits <= 3 ? 16 : 4));
 }
 
 // Over the wave.
@@ -915,8 +922,10 @@ __global__ __launch_bounds__(64 * NW, WPS) void kv_block_kernel(const AttnCall A
     if (!kv_place<BM>(A, P)) return;
     const int rows = min(BM, P.e.count * int(A.group) - P.first);
     const TileRange all = kv_tiles(A, P.e, unsigned(P.first) / A.group, unsigned(P.first + rows - 1) / A.group);
-    const int share = kv_share(A, all), begin = all.begin + P.split * share, end = min(all.end, begin + share);
-    if (A.part && begin >= end) {
+    const bool part = !kv_whole(A, all);
+    if (!part && P.split > 0) return;
+    const int share = kv_share(A, all), begin = all.begin + P.split * share, end = part ? min(all.end, begin + share) : all.end;
+    if (part && begin >= end) {
         if (tid < rows) kv_store_lse(A, P, P.first + tid, -INFINITY);
         return;
     }
@@ -1014,17 +1023,17 @@ __global__ __launch_bounds__(64 * NW, WPS) void kv_block_kernel(const AttnCall A
         l += __shfl_xor(l, 32);
         const int row = 16 * r + (lane & 15);
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (A.part && g == 0 && row < mine) kv_store_lse(A, P, first + row, l == 0.f ? -INFINITY : R.m[r] + __builtin_amdgcn_logf(l));
+        if (part && g == 0 && row < mine) kv_store_lse(A, P, first + row, l == 0.f ? -INFINITY : R.m[r] + __builtin_amdgcn_logf(l));
 #pragma unroll
         for (int dt = 0; dt < D / 16; dt++) {
             f32x4 o;
 #pragma unroll
             for (int j = 0; j < 4; j++) o[j] = __builtin_amdgcn_ldexpf(R.o[r][dt][j] * inv, R.base - 132);
-            if (!A.part) *reinterpret_cast<uint2*>(turn + row * PITCH + 16 * dt + 4 * g) = kv_pack4<T>(o);
+            if (!part) *reinterpret_cast<uint2*>(turn + row * PITCH + 16 * dt + 4 * g) = kv_pack4<T>(o);
             else if (row < mine) kv_store_part4<D>(A, P, first + row, 16 * dt + 4 * g, o);
         }
     }
-    if (A.part) return;
+    if (part) return;
     __syncthreads();
     // whole rows at once (32 prompts of 128 tokens: 38.6 us with 8-byte stores from the registers, 37.7 so)
     constexpr int LANES = D / 8, AT = 64 / LANES;
@@ -1046,15 +1055,18 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttnCall A) {
     const int t = W == 1 ? threadIdx.x & 63 : threadIdx.x;
     // (grid: rows by heads, or by 4 heads)
     const int h = W == 1 ? blockIdx.y * 4 + (threadIdx.x >> 6) : blockIdx.y;
-    int64_t row = blockIdx.x;
     if (h >= A.heads) return;
-    if (A.b.cu) {  // which row of the call that is
-        int entry, i, start, count;
-        if (!kv_locate(A.b, int(row), [](int n) { return n; }, entry, i)) return;
-        kv_rows(A.b, entry, start, count);
-        row = start + i;
+    int entry, i;
+    if (!kv_locate(A.b, blockIdx.x, [](int n) { return n; }, entry, i)) return;
+    int start, count;
+    kv_rows(A.b, entry, start, count);
+    if (A.causal) {
+        const KvEntry e = kv_entry(A.c, A.b, entry);
+        const unsigned first = (unsigned(i) * A.group + unsigned(h) % A.group) / A.rows * A.rows;
+        const unsigned last = min(first + A.rows, unsigned(count) * A.group) - 1;
+        if (kv_whole(A, kv_tiles(A, e, first / A.group, last / A.group))) return;  // written out
     }
-    const int64_t at = row * A.heads + h;
+    const int64_t at = int64_t(start + i) * A.heads + h;
     const float* lse = A.lse + at * A.splits;
     const f32x4* part = reinterpret_cast<const f32x4*>(A.part + at * A.splits * D) + t % LANES;
     const int set = t / LANES;
@@ -1062,14 +1074,14 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttnCall A) {
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < A.splits; s0 += 4 * SETS) {
         f32x4 x[4];
-        float e[4];
+        float f[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int s = s0 + j * SETS + set;
-            e[j] = s < A.splits ? lse[s] : -INFINITY;
+            f[j] = s < A.splits ? lse[s] : -INFINITY;
             x[j] = s < A.splits ? part[int64_t(s) * LANES] : f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        kv_merge4(e, x, m, sum, o);
+        kv_merge4(f, x, m, sum, o);
     }
     if (J.join(t, m, sum, o)) kv_out4<T, D>(A, at, t, sum, o);
 }
@@ -1216,6 +1228,7 @@ extern "C" int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n
     A.s2 = scale * 1.44269504088896340736f;
     A.heads = n_heads;
     A.group = n_heads / cache->kv_heads;
+    A.rows = plan.rows;
     A.tiles = int(plan.tiles);
     A.splits = plan.splits;
     A.groups = plan.groups;
