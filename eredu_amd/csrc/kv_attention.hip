@@ -846,7 +846,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv_stream_join_kernel(c
     const Units U = kv_units(A, e);
     const int row = i * A.group + unsigned(h) % A.group;
     const int S = base + (row / kStreamRows * A.c.kv_heads + int(unsigned(h) / A.group)) * U.tiles;
-    const int w0 = unsigned(S) / unsigned(run), w1 = unsigned(S + U.tiles - 1) / unsigned(run);
+    // (offsets that cover rows many times over may list more tiles than an int counts: no slot behind the last)
+    const unsigned slots = 4 * A.groups;
+    const int w0 = min(unsigned(S) / unsigned(run), slots - 1), w1 = min(unsigned(S + U.tiles - 1) / unsigned(run), slots - 1);
     if (w0 == w1) return;  // written out
     constexpr int LANES = D / 4, SETS = 64 * W / LANES;
     const int set = t / LANES;
