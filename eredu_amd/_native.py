@@ -90,6 +90,7 @@ KV_SIGNATURES["eq_kv_attention_scratch"] = ([_kv, _i32, _i64, _i64, _b], _i64)
 KV_SIGNATURES["eq_kv_read"] = ([_vp, _vp, _kv, _i64, _vp, _i64, _vp, _i64, _i32, _vp], _i32)
 KV_SIGNATURES["eq_kv_extend"] = ([_kv, _vp, _i64, _vp, _i64, _vp, _i64, _vp], _i32)
 KV_SIGNATURES["eq_kv_fork"] = ([_kv, _vp, _vp, _i64, _vp, _i64, _vp], _i32)
+KV_SIGNATURES["eq_kv_shrink"] = ([_kv, _vp, _i64, _vp, _i64, _vp], _i32)
 KV_SIGNATURES["eq_kv_free"] = ([_kv, _vp, _i64, _vp], _i32)
 KV_SIGNATURES["eq_kv_compact"] = ([_kv, _vp, _i64, _vp], _i32)
 KV_SIGNATURES["eq_kv_pages_scratch"] = ([_kv, _i64], _i64)

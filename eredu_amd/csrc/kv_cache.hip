@@ -780,6 +780,25 @@ __global__ __launch_bounds__(256) void kv_fork_give_kernel(KvPages c, const int3
     if (threadIdx.x == 0) c.lengths[to] = row[c.width];
 }
 
+// One workgroup per entry: the length, and the pages behind the tokens that stay.
+__global__ __launch_bounds__(256) void kv_shrink_kernel(KvPages c, const int32_t* __restrict__ seqs,
+                                                        const int32_t* __restrict__ counts, int count, int n) {
+    const int i = blockIdx.x, seq = seqs[i], tid = threadIdx.x, T = 1 << c.log2_page;
+    bool later = false;
+    for (int j = i + 1 + tid; j < n; j += 256) later |= seqs[j] == seq;
+    const bool is = unsigned(seq) < unsigned(c.sequences);
+    const int length = is ? kv_clamp(c.lengths[seq], 0, kKvMaxLength) : 0;
+    if (__syncthreads_or(later) || !is) return;  // (and every thread has the length)
+    const int rest = length - kv_clamp(counts ? counts[i] : count, 0, length);
+    int32_t* row = c.tables + int64_t(seq) * c.width;
+    for (int w = ((rest + T - 1) >> c.log2_page) + tid; w < c.width; w += 256) {
+        const int id = row[w];
+        if (unsigned(id) < unsigned(c.pages)) atomicSub(c.refs + id, 1);
+        row[w] = -1;
+    }
+    if (tid == 0) c.lengths[seq] = rest;
+}
+
 // One workgroup per sequence; the exchange lets one of several entries that
 // name a sequence give up each page.
 __global__ __launch_bounds__(256) void kv_free_kernel(KvPages c, const int32_t* __restrict__ seqs) {
@@ -998,6 +1017,21 @@ extern "C" int eq_kv_fork(const eq_kv_cache* cache, const int32_t* src, const in
     const KvPages c = pages_of(cache);
     kv_fork_take_kernel<<<dim3(unsigned(n)), dim3(256), 0, st>>>(c, src, dst, int(n), rows);
     kv_fork_give_kernel<<<dim3(unsigned(n)), dim3(256), 0, st>>>(c, dst, rows);
+    return check_launch(who);
+}
+
+extern "C" int eq_kv_shrink(const eq_kv_cache* cache, const int32_t* seqs, int64_t n, const int32_t* counts, int64_t count,
+                            eq_stream_t stream) {
+    clear_error();
+    const char* who = "eq_kv_shrink";
+    if (!kv_cache_ok(who, cache) || !kv_list_ok(who, seqs, seqs, n)) return 1;
+    if (!counts && (count < 0 || count > kKvMaxLength)) {
+        set_error("eq_kv_shrink: count must be in [0, 2^30]");
+        return 1;
+    }
+    if (n == 0) return 0;
+    kv_shrink_kernel<<<dim3(unsigned(n)), dim3(256), 0, reinterpret_cast<hipStream_t>(stream)>>>(pages_of(cache), seqs, counts,
+                                                                                                 int(count), int(n));
     return check_launch(who);
 }
 

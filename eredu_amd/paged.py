@@ -18,7 +18,7 @@ their sequences.  Tables, lengths and reference counts live on the device and
 are read when the kernels run: nothing here waits for the GPU but ``check`` and
 ``free_pages``, and a captured graph decodes across page borders.
 
-Calls that write a cache (extend, append, fork, free, compact) have to be
+Calls that write a cache (extend, append, fork, shrink, free, compact) have to be
 ordered with every other call on it, as with any tensor that is written in
 place.
 """
@@ -262,6 +262,18 @@ class PagedKVCache:
         L, st = _native.lib(), self._here()
         wp, wn, ws = self._scratch(L.eq_kv_pages_scratch(self._ref, src.numel()) if _capturing() else 0)
         check(L.eq_kv_fork(self._ref, src.data_ptr(), dst.data_ptr(), src.numel(), wp, wn, st))
+
+    def shrink(self, seqs: torch.Tensor, tokens: Union[int, torch.Tensor]) -> None:
+        """Takes the sequences' last ``tokens`` back (of all the same number, or int32
+        [n] on the device, at most what each has) with the pages behind the rest: the
+        drafts of a step that were refused (C ABI: eq_kv_shrink)."""
+        seqs = _ids(seqs, "seqs", self._index)
+        counts = _ids(tokens, "tokens", self._index) if isinstance(tokens, torch.Tensor) else None
+        if counts is not None and counts.numel() != seqs.numel():
+            raise EreduError(f"tokens must hold {seqs.numel()} numbers for as many sequences, got {counts.numel()}")
+        check(_native.lib().eq_kv_shrink(self._ref, seqs.data_ptr(), seqs.numel(),
+                                         None if counts is None else counts.data_ptr(),
+                                         0 if counts is not None else tokens, self._here()))
 
     def free(self, seqs: torch.Tensor) -> None:
         """Empties the sequences and gives up their pages (C ABI: eq_kv_free)."""

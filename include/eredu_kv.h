@@ -40,9 +40,9 @@ extern "C" {
  * [0, pages) is a missing page (its tokens are not written, not attended to and
  * read as zeros), a sequence outside [0, sequences) has no tokens, cu is
  * clamped to [0, total] and a decreasing pair is an empty entry.  Where a
- * sequence is named twice, eq_kv_append and eq_kv_extend go by the last entry
- * that names it and eq_kv_fork by the last pair with that destination.
- * Calls that write a cache (append, extend, fork, free, compact) are to be
+ * sequence is named twice, eq_kv_append, eq_kv_extend and eq_kv_shrink go by the
+ * last entry that names it and eq_kv_fork by the last pair with that destination.
+ * Calls that write a cache (append, extend, fork, shrink, free, compact) are to be
  * ordered with every other call on it, by stream order or events.
  *
  * scratch: scratch_bytes of device memory (256-byte aligned) that the call may
@@ -92,7 +92,8 @@ int eq_kv_append(const eq_kv_cache* cache, int64_t layer, const void* k, const v
  * for q.  Rows that no entry covers are left as they are in out.  Scores,
  * softmax sums and outputs are held in f32; q in 16 bits of each row's
  * largest magnitude, probabilities in f16, values exactly where their page's
- * scale is at least 2^-29 of the sequence's largest. */
+ * scale is at least 2^-29 of the sequence's largest.  scale * max|q| * max|k|
+ * of a row and a page has to be below 2^124 (a score may be NaN beyond). */
 int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n_heads, const eq_kv_cache* cache, int64_t layer,
                     const int32_t* seqs, int64_t n, const int32_t* cu, int64_t total, float scale, bool causal,
                     int64_t window, const float* rope, int64_t rope_positions, int dtype, void* scratch,
@@ -122,6 +123,15 @@ int eq_kv_extend(const eq_kv_cache* cache, const int32_t* seqs, int64_t n, const
  * that beams can be permuted.  Pairs with an id out of range do nothing. */
 int eq_kv_fork(const eq_kv_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* scratch,
                int64_t scratch_bytes, eq_stream_t stream);
+
+/* Takes the last counts[i] tokens (device int32 [n]; NULL: `count`) of sequence
+ * seqs[i] back, at most all it has, and gives up the pages behind the rest:
+ * the drafts of a step that were refused.  A sequence that is named twice
+ * goes by the last entry.  The page that the rest ends in keeps its scale bytes, so one
+ * that a value which is not finite made NaN stays so.  (A length that is lowered by
+ * other means keeps its pages, and eq_kv_extend would lose them.) */
+int eq_kv_shrink(const eq_kv_cache* cache, const int32_t* seqs, int64_t n, const int32_t* counts, int64_t count,
+                 eq_stream_t stream);
 
 /* Empties the sequences: length 0, table entries -1, one reference less for each of their pages. */
 int eq_kv_free(const eq_kv_cache* cache, const int32_t* seqs, int64_t n, eq_stream_t stream);

@@ -88,6 +88,17 @@ class Paged:
                 self.refs[p] -= 1
             self.tables[d], self.lengths[d] = row, n
 
+    def shrink(self, seqs, counts):
+        last = {s: i for i, s in enumerate(seqs)}
+        for i, (s, n) in enumerate(zip(seqs, counts)):
+            if last[s] != i or not 0 <= s < len(self.lengths):
+                continue
+            self.lengths[s] -= min(max(n, 0), self.lengths[s])
+            behind = self.tables[s, -(-self.lengths[s] // self.T):]
+            for p in behind[behind >= 0]:
+                self.refs[p] -= 1
+            behind[...] = -1
+
     def free(self, seqs):
         for s in seqs:
             if 0 <= s < len(self.lengths):

@@ -81,6 +81,7 @@ def test_every_entry_point_refuses_a_bad_cache(bad, word):
     r = ctypes.byref(c)
     refused(L.eq_kv_extend(r, 4096, 1, None, 1, None, 0, None), word)
     refused(L.eq_kv_fork(r, 4096, 4096, 1, None, 0, None), word)
+    refused(L.eq_kv_shrink(r, 4096, 1, None, 1, None), word)
     refused(L.eq_kv_free(r, 4096, 1, None), word)
     refused(L.eq_kv_compact(r, None, 0, None), word)
     refused(L.eq_kv_pages_scratch(r, 1), word)
@@ -125,6 +126,9 @@ def test_pages():
     refused(L.eq_kv_fork(r, 4096, None, 1, None, 0, None), "null")
     refused(L.eq_kv_fork(r, 4096, 4096, 1 << 21, None, 0, None), "n <=")
     refused(L.eq_kv_fork(r, 4096, 4096, 1, 4096, 4, None), "scratch")
+    refused(L.eq_kv_shrink(r, None, 1, None, 1, None), "null")
+    refused(L.eq_kv_shrink(r, 4096, 1, None, -1, None), "count")
+    refused(L.eq_kv_shrink(r, 4096, 1 << 21, None, 1, None), "n <=")
     refused(L.eq_kv_free(r, None, 1, None), "null")
     refused(L.eq_kv_compact(r, 4096, 4, None), "scratch")
     refused(L.eq_kv_pages_scratch(r, -1), "n <=")
@@ -138,6 +142,7 @@ def test_empty_calls_launch_nothing():
     assert L.eq_kv_extend(r, None, 0, None, 1, None, 0, None) == 0
     assert L.eq_kv_extend(r, 4096, 3, None, 0, None, 0, None) == 0
     assert L.eq_kv_fork(r, None, None, 0, None, 0, None) == 0
+    assert L.eq_kv_shrink(r, None, 0, None, 1, None) == 0
     assert L.eq_kv_free(r, None, 0, None) == 0
 
 
