@@ -19,6 +19,7 @@ namespace eq {
 
 constexpr int kKvMaxPage = 128;
 constexpr int kKvMaxLength = 1 << 30;  // of a sequence, and of width * page
+constexpr int kKvMaxEntries = 1 << 16;  // of a call (every workgroup goes through them)
 
 struct KvView {
     int8_t* k;          // this layer's pages

@@ -30,7 +30,7 @@ extern "C" {
  * that the kernels read when they run, so a captured graph decodes across
  * page borders.
  *
- * A call covers n sequences, named by seqs (device int32), with `total` rows of
+ * A call covers n sequences (up to 2^16), named by seqs (device int32), with `total` rows of
  * tokens: entry i has rows cu[i] .. cu[i + 1] - 1 (cu: n + 1 device int32), or
  * total / n rows where cu is NULL; they are the LAST ones of its lengths[seq]
  * tokens.  So a step is: eq_kv_extend once, then eq_kv_append and

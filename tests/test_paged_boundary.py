@@ -90,7 +90,7 @@ def test_every_entry_point_refuses_a_bad_cache(bad, word):
 
 @pytest.mark.parametrize("call", [append, attend, read])
 @pytest.mark.parametrize("bad,word", [(dict(layer=2), "layer"), (dict(layer=-1), "layer"), (dict(n=-1), "n <="),
-                                      (dict(n=(1 << 20) + 1, total=0), "n <="), (dict(seqs=None), "null"),
+                                      (dict(n=(1 << 16) + 1, total=0), "n <="), (dict(seqs=None), "null"),
                                       (dict(total=3), "divide"), (dict(total=-2), "total"), (dict(total=1 << 31), "total"),
                                       (dict(n=0, total=1), "total"), (dict(dt=9), "")])
 def test_batches(call, bad, word):
