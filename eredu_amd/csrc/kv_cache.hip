@@ -529,14 +529,14 @@ __device__ __forceinline__ int kv_open_page(const KvPages& c, int seq, int lengt
     return unsigned(id) < unsigned(c.pages) ? id : -1;
 }
 
-// Gives an entry its pages, free ones from rank `at` on (list: by rank).
-__device__ __forceinline__ void kv_grow(const KvPages& c, const KvPlanScratch& s, int seq, int length, int count, bool copy, int at,
+// Gives an entry its pages, free ones from rank `at` on (list: by rank); from: the page it copies first, or -1.
+__device__ __forceinline__ void kv_grow(const KvPages& c, const KvPlanScratch& s, int seq, int length, int count, int from, int at,
                                         int free_pages, const int32_t* list, int* copies, int* lack) {
     const int T = 1 << c.log2_page;
     int32_t* row = c.tables + int64_t(seq) * c.width;
     int none = 0;
-    if (copy) {
-        const int from = row[length >> c.log2_page], to = at < free_pages ? list[at] : -1;
+    if (from >= 0) {
+        const int to = at < free_pages ? list[at] : -1;
         at++;
         if (to >= 0) {
             const int m = atomicAdd(copies, 1);
@@ -612,7 +612,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_extend_plan_kernel(KvPages c,
     for (int i = tid; i < b.n; i += kPlanThreads) {
         int seq, length, count;
         if (!kv_grows(c, b, s, i, seq, length, count)) continue;
-        kv_grow(c, s, seq, length, count, s.offset[i] >> 30, s.offset[i] & ((1 << 30) - 1), free_pages, s.list, &copies, &lack);
+        kv_grow(c, s, seq, length, count, s.offset[i] >> 30 ? kv_open_page(c, seq, length) : -1, s.offset[i] & ((1 << 30) - 1), free_pages, s.list, &copies, &lack);
     }
     __syncthreads();
     if (tid == 0) {
@@ -672,8 +672,8 @@ __global__ __launch_bounds__(kPlanThreads) void kv_extend_few_kernel(KvPages c, 
     else kv_list_free(c, bits, before, all, s.list);
     __syncthreads();
     if (grows) {
-        if (near) kv_grow(c, s, seq, length, count, copy, at, free_pages, list, &copies, &lack);
-        else kv_grow(c, s, seq, length, count, copy, at, free_pages, s.list, &copies, &lack);
+        if (near) kv_grow(c, s, seq, length, count, copy ? open : -1, at, free_pages, list, &copies, &lack);
+        else kv_grow(c, s, seq, length, count, copy ? open : -1, at, free_pages, s.list, &copies, &lack);
     }
     __syncthreads();
     if (tid == 0) {
