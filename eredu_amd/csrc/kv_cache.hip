@@ -197,21 +197,21 @@ __device__ __forceinline__ uint32_t kv_places(int t, int from, int until) {
     return m;
 }
 
-// Grid (page units, kv_heads, keys | values), 256 threads: one page of one
+// Grid (page units, kv_heads, keys | values), NT threads: one page of one
 // head.  The page's new rows are read for their largest magnitude and, where
 // that is one round of 2 pieces a thread (64 tokens of 128 dimensions), stay in registers for
 // their codes; else they are read again, from L2.  Values turn in LDS, by 4 x 4
 // bytes, to be written along the tokens, 16 of a dimension at once.
 // 6 waves a SIMD: 80 registers instead of 117 cover more of the loads' trips, 10000
-// tokens 20.1 -> 18.0 us, in pages of 16 38 -> 29.
+// tokens 20.1 -> 18.0 us.
 constexpr int kAppendItems = 2;
 
-template <typename T, int D>
-__global__ __launch_bounds__(256, 6) void kv_append_kernel(KvView c, KvBatch b, const uint16_t* __restrict__ k,
+template <typename T, int D, int NT>
+__global__ __launch_bounds__(NT, 6) void kv_append_kernel(KvView c, KvBatch b, const uint16_t* __restrict__ k,
                                                         const uint16_t* __restrict__ v, int64_t k_stride,
                                                         int64_t v_stride, const float* __restrict__ rope) {
     extern __shared__ __attribute__((aligned(16))) uint8_t turn[];  // values: [token][D + 4]
-    __shared__ uint32_t red[4];
+    __shared__ uint32_t red[NT / 64];
     const int tid = threadIdx.x, head = blockIdx.y, log2_page = c.log2_page, page_tokens = 1 << log2_page;
     const bool values = blockIdx.z != 0;
     int entry, place;
@@ -229,25 +229,25 @@ __global__ __launch_bounds__(256, 6) void kv_append_kernel(KvView c, KvBatch b, 
     KvPairs raw[kAppendItems];
 #pragma unroll
     for (int j = 0; j < kAppendItems; j++) {
-        const int it = tid + 256 * j, t = it / groups;
+        const int it = tid + NT * j, t = it / groups;
         if (it < items) raw[j].load(x + int64_t(t) * stride, it % groups * 8, D, rot ? rot + int64_t(t) * D : nullptr);
     }
     bool later = false;  // another entry names this sequence
-    for (int j = entry + 1 + tid; j < b.n; j += 256) later |= b.seqs[j] == e.seq;
+    for (int j = entry + 1 + tid; j < b.n; j += NT) later |= b.seqs[j] == e.seq;
     if (__syncthreads_or(later) || s.page < 0) return;
     uint8_t* scale = (values ? c.vs : c.ks) + int64_t(s.page) * c.kv_heads + head;
     const int was = s.from > 0 ? *scale : 0;
 
-    const bool held = items <= 256 * kAppendItems;
+    const bool held = items <= NT * kAppendItems;
     uint32_t most = 0;
     float f[kAppendItems][16];
 #pragma unroll
     for (int j = 0; j < kAppendItems; j++)
-        if (tid + 256 * j < items) {
+        if (tid + NT * j < items) {
             raw[j].values<T>(rot != nullptr, f[j]);
             most = max(most, kv_most(f[j]));
         }
-    for (int it = tid + 256 * kAppendItems; it < items; it += 256) {
+    for (int it = tid + NT * kAppendItems; it < items; it += NT) {
         const int t = it / groups;
         KvPairs r;
         float y[16];
@@ -259,7 +259,8 @@ __global__ __launch_bounds__(256, 6) void kv_append_kernel(KvView c, KvBatch b, 
     for (int o = 32; o > 0; o >>= 1) most = max(most, uint32_t(__shfl_xor(int(most), o)));
     if ((tid & 63) == 0) red[tid >> 6] = most;
     __syncthreads();
-    most = max(max(red[0], red[1]), max(red[2], red[3]));
+#pragma unroll
+    for (int w = 0; w < NT / 64; w++) most = max(most, red[w]);
     const int now = max(kv_byte(most), was);
     if (tid == 0) *scale = uint8_t(now);
     const bool move = s.from > 0 && was < now && now != 255;  // the page's older codes change their step
@@ -287,9 +288,9 @@ __global__ __launch_bounds__(256, 6) void kv_append_kernel(KvView c, KvBatch b, 
     };
 #pragma unroll
     for (int j = 0; j < kAppendItems; j++)
-        if (tid + 256 * j < items) put(tid + 256 * j, f[j]);
+        if (tid + NT * j < items) put(tid + NT * j, f[j]);
     if (!held) {
-        for (int it = tid + 256 * kAppendItems; it < items; it += 256) {
+        for (int it = tid + NT * kAppendItems; it < items; it += NT) {
             const int t = it / groups;
             KvPairs r;
             float y[16];
@@ -301,7 +302,7 @@ __global__ __launch_bounds__(256, 6) void kv_append_kernel(KvView c, KvBatch b, 
     if (!values) {
         if (move) {
             uint4* p = reinterpret_cast<uint4*>(codes);
-            for (int i = tid; i < s.from * D / 16; i += 256) {
+            for (int i = tid; i < s.from * D / 16; i += NT) {
                 const uint4 o = p[i];
                 p[i] = make_uint4(kv_rescale4(o.x, down), kv_rescale4(o.y, down), kv_rescale4(o.z, down),
                                   kv_rescale4(o.w, down));
@@ -312,7 +313,7 @@ __global__ __launch_bounds__(256, 6) void kv_append_kernel(KvView c, KvBatch b, 
     __syncthreads();
     // 16 places of 4 dimensions: older codes, then new ones, then what was there
     const int first = move ? 0 : s.from >> 4, blocks = ((s.until + 15) >> 4) - first;
-    for (int it = tid; it < blocks * (D / 4); it += 256) {
+    for (int it = tid; it < blocks * (D / 4); it += NT) {
         const int d4 = it / blocks, t0 = (first + it - d4 * blocks) * 16;
         uint32_t n[4][4];  // [dimension][4 places]
 #pragma unroll
@@ -348,10 +349,10 @@ __global__ __launch_bounds__(256, 6) void kv_append_kernel(KvView c, KvBatch b, 
     }
 }
 
-// Grid (page units, kv_heads, keys | values), 256 threads: the rows of one page
+// Grid (page units, kv_heads, keys | values), NT threads: the rows of one page
 // and head; values turn in LDS, by 4 x 4 bytes.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void kv_read_kernel(typename T::storage* __restrict__ k,
+template <typename T, int D, int NT>
+__global__ __launch_bounds__(NT) void kv_read_kernel(typename T::storage* __restrict__ k,
                                                       typename T::storage* __restrict__ v, KvView c, KvBatch b) {
     extern __shared__ __attribute__((aligned(16))) uint8_t turn[];  // values: [token][D + 4]
     const int tid = threadIdx.x, head = blockIdx.y, log2_page = c.log2_page, page_tokens = 1 << log2_page;
@@ -371,7 +372,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(typename T::storage* __res
     const float scale = here ? e8m0_to_f32((values ? c.vs : c.ks)[at]) : 0.f;
     if (values && here) {
         const int first = s.from >> 4, blocks = ((s.until + 15) >> 4) - first;
-        for (int it = tid; it < blocks * (D / 4); it += 256) {
+        for (int it = tid; it < blocks * (D / 4); it += NT) {
             const int d4 = it / blocks, t0 = (first + it - d4 * blocks) * 16;
             const int8_t* p = codes + int64_t(4 * d4) * page_tokens + t0;
             uint4 o[4];
@@ -393,11 +394,11 @@ __global__ __launch_bounds__(256) void kv_read_kernel(typename T::storage* __res
         __syncthreads();
     }
     constexpr int kAtOnce = 4;  // pieces of 8 codes a thread requests before it writes one
-    for (int base = tid; base < items; base += kAtOnce * 256) {
+    for (int base = tid; base < items; base += kAtOnce * NT) {
         uint2 w[kAtOnce];
 #pragma unroll
         for (int u = 0; u < kAtOnce; u++) {
-            const int it = base + 256 * u, t = it / groups, d0 = it % groups * 8;
+            const int it = base + NT * u, t = it / groups, d0 = it % groups * 8;
             w[u] = make_uint2(0u, 0u);
             if (!here || it >= items) continue;
             if (values) {
@@ -409,7 +410,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(typename T::storage* __res
         }
 #pragma unroll
         for (int u = 0; u < kAtOnce; u++) {
-            const int it = base + 256 * u, t = it / groups, d0 = it % groups * 8;
+            const int it = base + NT * u, t = it / groups, d0 = it % groups * 8;
             if (it >= items) continue;
             alignas(16) typename T::storage o[8];
 #pragma unroll
@@ -879,6 +880,27 @@ bool kv_list_ok(const char* who, const int32_t* a, const int32_t* b, int64_t n) 
     return true;
 }
 
+// Head dimension and threads of a workgroup that has one page of one head: as many
+// as a page has 16-byte pieces (10000 tokens in pages of 16, 128 dimensions: append 20 us with 128 threads, 29 with
+// 256, read 16 and 21; in pages of 64 with 128 threads read 15, with 256 14).
+template <typename F>
+void with_page(const eq_kv_cache* c, F f) {
+    const int pieces = c->page_tokens * c->head_dim / 16;
+    auto threads = [&](auto d) {  // (the smallest page, of 16 tokens, has as many pieces as the head has dimensions)
+        constexpr int D = decltype(d)::value;
+        if constexpr (D <= 64) {
+            if (pieces <= 64) return f(d, std::integral_constant<int, 64>{});
+        }
+        if constexpr (D <= 128) {
+            if (pieces <= 128) return f(d, std::integral_constant<int, 128>{});
+        }
+        f(d, std::integral_constant<int, 256>{});
+    };
+    if (c->head_dim == 64) threads(std::integral_constant<int, 64>{});
+    else if (c->head_dim == 128) threads(std::integral_constant<int, 128>{});
+    else threads(std::integral_constant<int, 256>{});
+}
+
 // Of at most `moves` pages.
 void launch_moves(const eq_kv_cache* c, const KvPlanScratch& s, int64_t moves, const int32_t* map, hipStream_t st) {
     // (no more workgroups than a small cache has work for: a launch that moves nothing is a launch)
@@ -930,15 +952,12 @@ extern "C" int eq_kv_append(const eq_kv_cache* cache, int64_t layer, const void*
     const size_t lds = size_t(cache->page_tokens) * (D + 4);
     const dim3 grid(unsigned(units), unsigned(cache->kv_heads), 2);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    auto go = [&](auto kern) {
-        kern<<<grid, dim3(256), lds, st>>>(c, b, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
-                                           k_stride, v_stride, rope);
-    };
     auto of = [&](auto t) {
         typedef decltype(t) T;
-        if (D == 64) go(kv_append_kernel<T, 64>);
-        else if (D == 128) go(kv_append_kernel<T, 128>);
-        else go(kv_append_kernel<T, 256>);
+        with_page(cache, [&](auto d, auto nt) {
+            kv_append_kernel<T, decltype(d)::value, decltype(nt)::value><<<grid, dim3(decltype(nt)::value), lds, st>>>(
+                c, b, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), k_stride, v_stride, rope);
+        });
     };
     if (dtype == EQ_DTYPE_BF16) of(BF16T{});
     else of(F16T{});
@@ -971,13 +990,11 @@ extern "C" int eq_kv_read(void* k, void* v, const eq_kv_cache* cache, int64_t la
     const dim3 grid(unsigned(units), unsigned(cache->kv_heads), 2);
     with_dtype(dtype, [&](auto t) {
         typedef decltype(t) T;
-        auto go = [&](auto kern) {
-            kern<<<grid, dim3(256), lds, reinterpret_cast<hipStream_t>(stream)>>>(
-                static_cast<typename T::storage*>(k), static_cast<typename T::storage*>(v), c, b);
-        };
-        if (D == 64) go(kv_read_kernel<T, 64>);
-        else if (D == 128) go(kv_read_kernel<T, 128>);
-        else go(kv_read_kernel<T, 256>);
+        with_page(cache, [&](auto d, auto nt) {
+            kv_read_kernel<T, decltype(d)::value, decltype(nt)::value>
+                <<<grid, dim3(decltype(nt)::value), lds, reinterpret_cast<hipStream_t>(stream)>>>(
+                    static_cast<typename T::storage*>(k), static_cast<typename T::storage*>(v), c, b);
+        });
     });
     return check_launch(who);
 }
