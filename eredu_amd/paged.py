@@ -67,8 +67,8 @@ class PagedKVCache:
     Keys and values are int8 codes with a power-of-two scale for each page and
     head (E8M0 bytes): half the bytes of a bf16 cache, a value off by less than one
     step, at most max|x| / 63.5 over its page and head.  A page takes
-    2 * n_layers * n_kv_heads * (page_size * head_dim + 1) bytes.  Long contexts are
-    read fastest in pages of 64, a tile of the kernels' (128: about 15 % slower)."""
+    2 * n_layers * n_kv_heads * (page_size * head_dim + 1) bytes.  Long contexts
+    are read about 15 % slower from pages of 128 than from smaller ones."""
 
     def __init__(self, n_layers: int, n_pages: int, n_kv_heads: int, head_dim: int, max_seqs: int,
                  max_pages_per_seq: int, page_size: int = 64, device=None):
