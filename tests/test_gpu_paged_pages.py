@@ -70,3 +70,19 @@ def test_many_pages(cuda, pages):
     b.ref.compact()
     b.same_tables()
     assert (held > 0).sum() > (b.ref.refs > 0).sum()
+
+
+@pytest.mark.parametrize("n,width", [(1, 1), (3, 341), (16, 256), (16, 257), (256, 16), (257, 15), (100, 41)])
+def test_forks(cuda, n, width):
+    """Permutations, repeats, pairs that name nothing and copies of oneself, on both sides of
+    what one workgroup takes (256 pairs, 4096 table entries)."""
+    print(f"[case] forks n={n} width={width}", flush=True)
+    b = Both(T=16, D=64, heads=1, pages=700, seqs=n + 3, width=width, seed=n + width)
+    start = [int(s) for s in b.rng.permutation(n + 3)[:40]]
+    grow(b, start, [int(x) for x in b.rng.integers(0, min(16 * width, 200), len(start))])
+    for _ in range(4):
+        src = [int(s) for s in b.rng.integers(-1, n + 4, n)]
+        dst = [int(s) for s in b.rng.permutation(n + 3)[:n]] if _ % 2 else [int(s) for s in b.rng.integers(-1, n + 4, n)]
+        b.dev.fork(ints(src), ints(dst))
+        b.ref.fork(src, dst)
+        b.same_tables()
