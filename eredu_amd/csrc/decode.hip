@@ -707,7 +707,8 @@ extern "C" int eq_rope_attention_decode(void* out, const void* q, const void* k_
                            n_heads, n_kv_heads, head_dim, dtype))
         return 1;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    float* ws = static_cast<float*>(ws_acquire(nullptr, attention_states_bytes(n_heads), st));
+    WsHold hold;
+    float* ws = static_cast<float*>(ws_acquire(hold, nullptr, attention_states_bytes(n_heads), st));
     if (!ws) {
         set_error("eq_rope_attention_decode: no workspace (its stream's workspace cannot grow while capturing: "
                   "make one call with this head count on the stream before capturing)");
@@ -738,7 +739,8 @@ extern "C" int eq_rope_attention_decode_at(void* out, const void* q, const void*
         return 1;
     }
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    float* ws = static_cast<float*>(ws_acquire(nullptr, attention_states_bytes(n_heads), st));
+    WsHold hold;
+    float* ws = static_cast<float*>(ws_acquire(hold, nullptr, attention_states_bytes(n_heads), st));
     if (!ws) {
         set_error(std::string(who) + ": no workspace (its stream's workspace cannot grow while capturing: make one "
                   "call with this head count on the stream before capturing)");

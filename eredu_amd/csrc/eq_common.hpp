@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <cstring>
+#include <mutex>
 #include <string>
 #include <type_traits>
 
@@ -483,10 +484,22 @@ struct WsSource {
 // are zero between launches.
 constexpr int kWsCounters = 16384;
 
+// Keeps a stream's library workspace with one host thread while a call makes
+// the launches that hand results over through it: two threads may call on one
+// stream, and a launch of another call between a call's first and its last
+// would overwrite what the last one reads.  Declared before ws_acquire, which
+// takes the lock (of a caller's fixed region none), and left after the last
+// such launch.  A thread may take the same stream's again.
+class WsHold {
+    friend void* ws_acquire(WsHold&, const WsSource*, size_t, hipStream_t);
+    std::unique_lock<std::recursive_mutex> lock_;
+};
+
 // At least `bytes` of device scratch, 256-byte aligned, or null when none can
 // be provided (fixed region too small, or the library buffer would have to
-// grow while `st` is capturing).  Launches that use it are ordered on `st`.
-void* ws_acquire(const WsSource* src, size_t bytes, hipStream_t st);
+// grow while `st` is capturing).  Launches that use it are ordered on `st`,
+// and those of one call follow one another there as long as `hold` lives.
+void* ws_acquire(WsHold& hold, const WsSource* src, size_t bytes, hipStream_t st);
 
 // The kWsCounters arrival counters of `src` (null: the library's, one
 // zero-filled buffer per device and stream, used for nothing else), or null

@@ -1591,8 +1591,9 @@ bool launch_native_prefill(int ggml_type, bool big, const Geometry& geo, uint16_
     // behind the triple: the 2/3/5/6-bit path's byte codes and split-K partials
     const size_t rest = size_t(nc) * size_t(K) + size_t(4) * size_t(M) * size_t(nc) * 4u + 512;
     size_t want = triple + rest;
-    char* base = static_cast<char*>(ws_acquire(nullptr, want, st));
-    if (!base) base = static_cast<char*>(ws_acquire(nullptr, want = triple, st));
+    WsHold hold;
+    char* base = static_cast<char*>(ws_acquire(hold, nullptr, want, st));
+    if (!base) base = static_cast<char*>(ws_acquire(hold, nullptr, want = triple, st));
     if (!base) return false;
     uint32_t* w = reinterpret_cast<uint32_t*>(base);
     uint16_t* s = reinterpret_cast<uint16_t*>(base + wsz);
@@ -1910,7 +1911,8 @@ extern "C" int eq_gguf_embedding(void* out, const uint8_t* raw, int64_t raw_len,
     }
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const int64_t row_bytes = cols / geo.values * geo.bytes;
-    uint8_t* picked = static_cast<uint8_t*>(ws_acquire(nullptr, size_t(n_tokens) * size_t(row_bytes), st));
+    WsHold hold;
+    uint8_t* picked = static_cast<uint8_t*>(ws_acquire(hold, nullptr, size_t(n_tokens) * size_t(row_bytes), st));
     if (!picked) {
         set_error("could not obtain " + std::to_string(n_tokens * row_bytes) +
                   " bytes of workspace for the picked rows (first call on a stream under graph capture?)");
@@ -2146,7 +2148,8 @@ extern "C" int eq_gguf_grouped_linear(void* y, const void* x, const uint8_t* raw
         const size_t psz = up(size_t(experts * N) * size_t(K / geo.gs) * 2);
         const size_t triple = wsz + 2 * psz;
         const size_t rest = up(qmm_grouped_list_bytes(routes, experts));
-        char* base = static_cast<char*>(ws_acquire(nullptr, triple + rest, st));
+        WsHold hold;
+        char* base = static_cast<char*>(ws_acquire(hold, nullptr, triple + rest, st));
         if (!base) {
             set_error("could not obtain workspace for the re-packed expert bank");
             return 1;

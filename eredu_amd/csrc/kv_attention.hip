@@ -1211,6 +1211,7 @@ extern "C" int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n
         return 1;
     }
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    WsHold hold;
     AttnCall A;
     A.part = A.lse = nullptr;
     if (plan.part_bytes) {
@@ -1219,7 +1220,7 @@ extern "C" int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n
             set_error("eq_kv_attention: needs " + std::to_string(need) + " bytes of 256-byte aligned scratch");
             return 1;
         }
-        char* ws = static_cast<char*>(scratch ? scratch : ws_acquire(nullptr, need, st));
+        char* ws = static_cast<char*>(scratch ? scratch : ws_acquire(hold, nullptr, need, st));
         if (!ws) {
             set_error("eq_kv_attention: no workspace (its stream's workspace cannot grow while capturing: pass "
                       "scratch, or make one such call on the stream before capturing)");

@@ -891,7 +891,7 @@ size_t pages_scratch_bytes(const eq_kv_cache* c, int64_t n) {
     return plan > fork ? plan : fork;
 }
 
-char* scratch_for(const char* who, void* scratch, int64_t scratch_bytes, size_t need, hipStream_t st) {
+char* scratch_for(WsHold& hold, const char* who, void* scratch, int64_t scratch_bytes, size_t need, hipStream_t st) {
     if (scratch) {
         if (scratch_bytes < 0 || size_t(scratch_bytes) < need || !aligned(scratch, 256)) {
             set_error(std::string(who) + ": needs " + std::to_string(need) + " bytes of 256-byte aligned scratch");
@@ -899,7 +899,7 @@ char* scratch_for(const char* who, void* scratch, int64_t scratch_bytes, size_t 
         }
         return static_cast<char*>(scratch);
     }
-    void* p = ws_acquire(nullptr, need, st);
+    void* p = ws_acquire(hold, nullptr, need, st);
     if (!p)
         set_error(std::string(who) + ": no workspace (its stream's workspace cannot grow while capturing: pass "
                   "scratch, or make one such call on the stream before capturing)");
@@ -1058,7 +1058,8 @@ extern "C" int eq_kv_extend(const eq_kv_cache* cache, const int32_t* seqs, int64
     }
     if (n == 0 || (!cu && count == 0)) return 0;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    char* base = scratch_for(who, scratch, scratch_bytes, pages_scratch_bytes(cache, n), st);
+    WsHold hold;
+    char* base = scratch_for(hold, who, scratch, scratch_bytes, pages_scratch_bytes(cache, n), st);
     if (!base) return 1;
     KvPlanScratch s;
     plan_scratch(cache, n, base, &s);
@@ -1076,7 +1077,8 @@ extern "C" int eq_kv_fork(const eq_kv_cache* cache, const int32_t* src, const in
     if (!kv_cache_ok(who, cache) || !kv_list_ok(who, src, dst, n)) return 1;
     if (n == 0) return 0;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    char* base = scratch_for(who, scratch, scratch_bytes, pages_scratch_bytes(cache, n), st);
+    WsHold hold;
+    char* base = scratch_for(hold, who, scratch, scratch_bytes, pages_scratch_bytes(cache, n), st);
     if (!base) return 1;
     int32_t* rows = reinterpret_cast<int32_t*>(base);
     const KvPages c = pages_of(cache);
@@ -1118,7 +1120,8 @@ extern "C" int eq_kv_compact(const eq_kv_cache* cache, void* scratch, int64_t sc
     const char* who = "eq_kv_compact";
     if (!kv_cache_ok(who, cache)) return 1;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    char* base = scratch_for(who, scratch, scratch_bytes, pages_scratch_bytes(cache, 0), st);
+    WsHold hold;
+    char* base = scratch_for(hold, who, scratch, scratch_bytes, pages_scratch_bytes(cache, 0), st);
     if (!base) return 1;
     KvPlanScratch s;
     plan_scratch(cache, 0, base, &s);

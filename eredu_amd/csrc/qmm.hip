@@ -62,6 +62,7 @@ static bool qmm_run(int tm, int tn, const QmmTypes& t, const QmmArgs& a, int wor
 // One launch (plus the split reduction): every buffer below 2^31 bytes.
 static bool launch_qmm_piece(const QmmTypes& t, uint16_t* y, int ldy, const uint16_t* x, const uint32_t* w, const void* s,
                              const void* b, int M, int N, int K, bool may_split, const WsSource* src, hipStream_t st) {
+    WsHold hold;
     QmmArgs a{};
     a.y = y, a.x = x, a.w = w, a.s = static_cast<const uint16_t*>(s), a.b = static_cast<const uint16_t*>(b);
     a.M = M, a.N = N, a.K = K, a.ldy = ldy;
@@ -86,7 +87,7 @@ static bool launch_qmm_piece(const QmmTypes& t, uint16_t* y, int ldy, const uint
             }
         }
         if (splits > 1) {
-            a.ws = static_cast<float*>(ws_acquire(src, size_t(splits) * per_split, st));
+            a.ws = static_cast<float*>(ws_acquire(hold, src, size_t(splits) * per_split, st));
             if (!a.ws && !src) {
                 // The library workspace cannot grow (the stream is capturing,
                 // or the allocation failed).  Running unsplit would be a
@@ -250,7 +251,8 @@ static bool launch_qmm_grouped_t(const QmmTypes& t, uint16_t* y, const uint16_t*
     if (int64_t(N) * K * t.bits / 8 >= (int64_t(1) << 31) || int64_t(batch) * K * 2 >= (int64_t(1) << 31)) return false;
     const bool direct = x_batches * int64_t(K) * 2 < (int64_t(1) << 31);
     const size_t xg_bytes = direct ? 0 : (size_t(batch) * size_t(K) * 2u + 255u) & ~size_t(255);
-    void* ws = ws_acquire(src, xg_bytes + size_t(cap + 1) * sizeof(int4), st);
+    WsHold hold;
+    void* ws = ws_acquire(hold, src, xg_bytes + size_t(cap + 1) * sizeof(int4), st);
     if (!ws) return false;
     uint16_t* xg = reinterpret_cast<uint16_t*>(ws);
     int4* list = reinterpret_cast<int4*>(reinterpret_cast<char*>(ws) + xg_bytes);
@@ -337,7 +339,8 @@ static bool launch_qmm_odd_t(const QmmTypes& t, uint16_t* y, const uint16_t* x, 
     const int splits = qmm_plan(M, int(nc), K, gs, 8, true, qmm_cu_count()).splits;
     const size_t part_bytes = splits > 1 ? size_t(splits) * size_t(M) * size_t(nc) * 4u : 0;
     size_t want = code_bytes + part_bytes;
-    char* base = static_cast<char*>(ws_acquire(src, want, st));
+    WsHold hold;
+    char* base = static_cast<char*>(ws_acquire(hold, src, want, st));
     if (!base && !src) {
         // the library workspace cannot grow (capture): fail rather than run
         // another plan than the same call made eagerly
@@ -347,7 +350,7 @@ static bool launch_qmm_odd_t(const QmmTypes& t, uint16_t* y, const uint16_t* x, 
         note_refusal();
         return true;
     }
-    if (!base) base = static_cast<char*>(ws_acquire(src, want = code_bytes, st));
+    if (!base) base = static_cast<char*>(ws_acquire(hold, src, want = code_bytes, st));
     if (!base) return false;
     const size_t cap = src ? src->cap : want;
     WsSource rest{base + code_bytes, cap > code_bytes ? cap - code_bytes : 0, nullptr};

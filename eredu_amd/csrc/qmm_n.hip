@@ -674,13 +674,14 @@ bool launch_qmm_n_m1(int bits, int scale_dtype, uint16_t* y, const uint16_t* x, 
     if (!mfma && R > kQmmN1Stage / ng) R = kQmmN1Stage / ng;
     const int splits = (K + R - 1) / R;
     if (int64_t(ctiles) * splits > INT32_MAX) return false;
+    WsHold hold;
     QmmN1Args a{};
     a.y = y, a.x = x, a.w = w, a.s = s, a.b = b, a.g = g;
     a.N = N, a.K = K, a.gs = gs, a.R = R, a.splits = splits, a.ctiles = ctiles;
     a.batch_total = batch;
     int64_t per_launch = kMaxBatchesPerLaunch;
     if (splits > 1) {
-        a.ws = static_cast<float*>(ws_acquire(src, size_t(splits) * size_t(batch) * size_t(N) * 4u, st));
+        a.ws = static_cast<float*>(ws_acquire(hold, src, size_t(splits) * size_t(batch) * size_t(N) * 4u, st));
         if (!a.ws) return false;
         a.counters = ws_counters(src, st);
         // one counter per (batch in the launch, column tile), in the lower half of the counter block
@@ -742,6 +743,7 @@ bool launch_qmm_n_small(int bits, int scale_dtype, uint16_t* y, const uint16_t* 
         tiles = int64_t((Nw + tl - 1) / tl) * batch;
         pick_splits(tiles, K, kp, 4, 1024, splits, kchunk);
     }
+    WsHold hold;
     float* ws = nullptr;
     if (splits > 1 && src && size_t(splits) * size_t(mn) * 4u > src->cap) {
         // a fixed scratch region holds fewer splits: re-plan for what fits
@@ -755,7 +757,7 @@ bool launch_qmm_n_small(int bits, int scale_dtype, uint16_t* y, const uint16_t* 
         }
     }
     if (splits > 1) {
-        ws = static_cast<float*>(ws_acquire(src, size_t(splits) * size_t(mn) * 4u, st));
+        ws = static_cast<float*>(ws_acquire(hold, src, size_t(splits) * size_t(mn) * 4u, st));
         if (!ws) {
             splits = 1;
             kchunk = K;

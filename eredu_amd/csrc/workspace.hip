@@ -4,8 +4,9 @@
 //
 // Two sources:
 //  * the library-owned workspace, one buffer per (device, stream).  Calls on
-//    one stream are ordered, so they may share its buffer; calls on two
-//    streams never share one.  Buffers only grow, and a buffer is never
+//    one stream are ordered, so they may share its buffer (from several host
+//    threads too: a call holds it from its first launch to its last, WsHold);
+//    calls on two streams never share one.  Buffers only grow, and a buffer is never
 //    freed while the process runs: a HIP graph captured earlier keeps the
 //    address it recorded, so the retired buffer must stay valid for its
 //    replays.  Growth is geometric (at least twice the old size), so the
@@ -34,9 +35,10 @@ namespace {
 struct OwnedBuffer {
     void* ptr = nullptr;
     size_t cap = 0;
+    std::recursive_mutex mu;  // of ptr and cap, and of the launches that use them (WsHold)
 };
 
-std::mutex g_ws_mu;
+std::mutex g_ws_mu;  // of the maps and the list, taken for no longer than they are looked into
 std::map<std::pair<int, hipStream_t>, OwnedBuffer>& owned_buffers() {
     static auto* m = new std::map<std::pair<int, hipStream_t>, OwnedBuffer>();  // lives until exit
     return *m;
@@ -64,13 +66,18 @@ int device_cu_count() {
     return v;
 }
 
-void* ws_acquire(const WsSource* src, size_t bytes, hipStream_t st) {
+void* ws_acquire(WsHold& hold, const WsSource* src, size_t bytes, hipStream_t st) {
     if (bytes == 0) bytes = 256;
     if (src) return bytes <= src->cap ? src->ptr : nullptr;
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return nullptr;
-    std::lock_guard<std::mutex> lock(g_ws_mu);
-    OwnedBuffer& buf = owned_buffers()[std::make_pair(dev, st)];
+    OwnedBuffer* found;
+    {
+        std::lock_guard<std::mutex> lock(g_ws_mu);
+        found = &owned_buffers()[std::make_pair(dev, st)];  // (a map's entries stay where they are)
+    }
+    OwnedBuffer& buf = *found;
+    hold.lock_ = std::unique_lock<std::recursive_mutex>(buf.mu);
     if (buf.cap >= bytes) return buf.ptr;
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(st, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone) return nullptr;
@@ -83,7 +90,10 @@ void* ws_acquire(const WsSource* src, size_t bytes, hipStream_t st) {
         (void)hipGetLastError();  // a failed allocation is reported by the caller, not by the next launch check
         return nullptr;
     }
-    if (buf.ptr) retired_buffers().push_back(buf.ptr);
+    if (buf.ptr) {
+        std::lock_guard<std::mutex> lock(g_ws_mu);
+        retired_buffers().push_back(buf.ptr);
+    }
     buf.ptr = p;
     buf.cap = want;
     return p;

@@ -49,7 +49,8 @@ extern "C" {
  * use until it has run, at least what the query beside the call returns; NULL:
  * the library's workspace of `stream`, which cannot grow while `stream` is
  * capturing and which graphs captured on one stream share, so such graphs must
- * not run at the same time.
+ * not run at the same time.  (Calls of several host threads on one stream may
+ * share it: a call keeps its launches together.)
  */
 typedef struct eq_kv_cache {
     int8_t* k_codes;    /* [layers, pages, kv_heads, page_tokens, head_dim], 16-byte aligned */
