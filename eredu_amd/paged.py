@@ -144,7 +144,9 @@ class PagedKVCache:
         if t.dim() != 3 or t.shape[2] != D:
             raise EreduError(f"{what} must be [rows, heads, {D}], got {tuple(t.shape)}")
         if t.is_contiguous() and t.data_ptr() % 16 == 0:
-            return t
+            # (a single row is contiguous at any stride: heads that were turned to the front of one token)
+            row = t.shape[1] * D
+            return t if t.stride(0) == row or t.shape[0] != 1 else t.as_strided(t.shape, (row, D, 1))
         if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != D) or t.stride(0) % 8 or \
                 t.stride(0) < t.shape[1] * D or t.data_ptr() % 16:
             t = t.clone(memory_format=torch.contiguous_format)
