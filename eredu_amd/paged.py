@@ -131,16 +131,16 @@ class PagedKVCache:
         return _stream()
 
     def _rows(self, t: torch.Tensor, what: str) -> torch.Tensor:
-        """[rows, heads, dim] (or [rows, heads * dim]) with heads and dimensions
-        contiguous; rows may lie at any stride of a multiple of 8, as parts of a
-        fused projection do."""
+        """[rows, heads, dim] or [rows, heads * dim] as the kernels read it: heads and
+        dimensions contiguous, rows at any stride of a multiple of 8, as parts of a
+        fused projection are.  Any other layout is copied."""
         if t.get_device() != self._index:
             raise EreduError(f"{what} must live on {self.device}")
         if t.dtype not in _HALVES:
             raise EreduError(f"{what} must be bfloat16 or float16, got {t.dtype}")
         D = self.head_dim
-        if t.dim() == 2 and t.shape[1] % D == 0 and t.stride(1) == 1:
-            t = t.unflatten(1, (-1, D))
+        if t.dim() == 2 and t.shape[1] % D == 0:
+            t = t.unflatten(1, (t.shape[1] // D, D))
         if t.dim() != 3 or t.shape[2] != D:
             raise EreduError(f"{what} must be [rows, heads, {D}], got {tuple(t.shape)}")
         if t.is_contiguous() and t.data_ptr() % 16 == 0:

@@ -70,3 +70,12 @@ def test_refusals():
             rows(bad)
     with pytest.raises(EreduError, match="bfloat16"):
         rows(torch.zeros(2, HEADS, D))
+
+
+@pytest.mark.parametrize("make", [lambda: filled(HEADS * D, 3).t(), lambda: filled(HEADS * D, 1).t(),
+                                  lambda: filled(3, 2 * HEADS * D)[:, ::2], lambda: filled(D, 3).t(),
+                                  lambda: filled(1, 1).expand(3, HEADS * D)])
+def test_flat_rows_with_their_values_apart(make):
+    t = make()
+    got = rows(t)
+    assert got.is_contiguous() and got.stride(0) == t.shape[1] and torch.equal(got, t.reshape(t.shape[0], -1, D))
