@@ -1095,12 +1095,13 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttnCall A) {
     if (J.join(t, m, sum, o)) kv_out4<T, D>(A, at, t, sum, o);
 }
 
-bool attention_sizes_ok(const char* who, const eq_kv_cache* c, int n_heads, int64_t n, int64_t total) {
+// (n and total are looked at before: kv_rows_ok)
+bool attention_sizes_ok(const char* who, const eq_kv_cache* c, int n_heads, int64_t total) {
     if (n_heads <= 0 || n_heads > 65535 || n_heads % c->kv_heads != 0) {
         set_error(std::string(who) + ": n_heads must be a multiple of kv_heads, at most 65535");
         return false;
     }
-    if (n < 0 || n > kKvMaxEntries || total < 0 || total > INT32_MAX / 2 || total * n_heads > INT32_MAX) {
+    if (total * n_heads > INT32_MAX) {
         set_error(std::string(who) + ": need 0 <= n <= 2^16 sequences and 0 <= total * n_heads < 2^31");
         return false;
     }
@@ -1162,6 +1163,17 @@ Plan plan_attention(const eq_kv_cache* c, int n_heads, int64_t n, int64_t total,
     return p;
 }
 
+// Workgroups of a plan's block kernel, and threads of one.
+int64_t plan_blocks(const eq_kv_cache* c, const Plan& p) { return p.rows == kStreamRows ? 0 : p.tiles * c->kv_heads * p.splits; }
+int plan_threads(const eq_kv_cache* c, const Plan& p) { return p.rows == 128 && c->head_dim > 128 ? 512 : 256; }
+
+// Grids of under 2^32 threads a side, of the blocks and of the joins (a row's heads lie in y); a stream's own is small.
+bool plan_ok(const char* who, const eq_kv_cache* c, const Plan& p, int64_t total) {
+    if (total < (1 << 24) && plan_blocks(c, p) * plan_threads(c, p) < int64_t(1) << 32) return true;
+    set_error(std::string(who) + ": too many rows");
+    return false;
+}
+
 }  // namespace
 }  // namespace eq
 
@@ -1170,8 +1182,9 @@ using namespace eq;
 extern "C" int64_t eq_kv_attention_scratch(const eq_kv_cache* cache, int n_heads, int64_t n, int64_t total, bool ragged) {
     clear_error();
     const char* who = "eq_kv_attention_scratch";
-    if (!kv_cache_ok(who, cache) || !attention_sizes_ok(who, cache, n_heads, n, total)) return -1;
+    if (!kv_cache_ok(who, cache) || !kv_rows_ok(who, n, total, !ragged) || !attention_sizes_ok(who, cache, n_heads, total)) return -1;
     const Plan p = plan_attention(cache, n_heads, n, total, ragged);
+    if (!plan_ok(who, cache, p, total)) return -1;
     return int64_t(p.part_bytes + p.lse_bytes);
 }
 
@@ -1182,7 +1195,7 @@ extern "C" int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n
     clear_error();
     const char* who = "eq_kv_attention";
     if (!kv_cache_ok(who, cache) || !kv_batch_ok(who, cache, layer, seqs, n, cu, total) ||
-        !attention_sizes_ok(who, cache, n_heads, n, total) || !kv_rope_ok(who, cache, rope, rope_positions))
+        !attention_sizes_ok(who, cache, n_heads, total) || !kv_rope_ok(who, cache, rope, rope_positions))
         return 1;
     if (dtype != EQ_DTYPE_BF16 && dtype != EQ_DTYPE_F16) {
         set_error("eq_kv_attention: q and out must be bfloat16 or float16");
@@ -1204,12 +1217,7 @@ extern "C" int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n
         return 1;
     }
     const Plan plan = plan_attention(cache, n_heads, n, total, cu != nullptr);
-    // (grids of under 2^32 threads a side; a stream's own is small)
-    const int64_t blocks = plan.rows == kStreamRows ? 0 : plan.tiles * cache->kv_heads * plan.splits;
-    if (blocks >= (1 << 24) || total >= (1 << 24)) {
-        set_error("eq_kv_attention: too many rows");
-        return 1;
-    }
+    if (!plan_ok(who, cache, plan, total)) return 1;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     WsHold hold;
     AttnCall A;
@@ -1244,7 +1252,7 @@ extern "C" int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n
     A.groups = plan.groups;
     A.window = int(window < kKvMaxLength ? window : kKvMaxLength);
     A.causal = causal;
-    const dim3 grid{unsigned(blocks)};
+    const dim3 grid{unsigned(plan_blocks(cache, plan))};
     auto go = [&](auto t, auto d) {
         typedef decltype(t) T;
         constexpr int DIM = decltype(d)::value;

@@ -33,6 +33,18 @@ bool kv_cache_ok(const char* name, const eq_kv_cache* c) {
     return true;
 }
 
+bool kv_rows_ok(const char* name, int64_t n, int64_t total, bool even) {
+    if (n < 0 || total < 0 || n > kKvMaxEntries || total > INT32_MAX / 2 || (n == 0 && total != 0)) {
+        set_error(std::string(name) + ": need 0 <= n <= 2^16 sequences and 0 <= total < 2^30 rows");
+        return false;
+    }
+    if (n > 0 && even && total % n != 0) {
+        set_error(std::string(name) + ": without offsets the rows must divide evenly among the sequences");
+        return false;
+    }
+    return true;
+}
+
 bool kv_batch_ok(const char* name, const eq_kv_cache* c, int64_t layer, const int32_t* seqs, int64_t n,
                  const int32_t* cu, int64_t total) {
     const std::string who(name);
@@ -40,16 +52,9 @@ bool kv_batch_ok(const char* name, const eq_kv_cache* c, int64_t layer, const in
         set_error(who + ": layer " + std::to_string(layer) + " outside [0, " + std::to_string(c->layers) + ")");
         return false;
     }
-    if (n < 0 || total < 0 || n > kKvMaxEntries || total > INT32_MAX / 2 || (n == 0 && total != 0)) {
-        set_error(who + ": need 0 <= n <= 2^16 sequences and 0 <= total < 2^30 rows");
-        return false;
-    }
+    if (!kv_rows_ok(name, n, total, !cu)) return false;
     if (n > 0 && !seqs) {
         set_error(who + ": null pointer argument");
-        return false;
-    }
-    if (n > 0 && !cu && total % n != 0) {
-        set_error(who + ": without offsets the rows must divide evenly among the sequences");
         return false;
     }
     return true;

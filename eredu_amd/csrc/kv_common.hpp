@@ -132,6 +132,7 @@ __device__ __forceinline__ void kv_load8(const uint16_t* p, float* f) {
 
 // Host side: argument checks of every entry point, and the views they make.
 bool kv_cache_ok(const char* who, const eq_kv_cache* c);
+bool kv_rows_ok(const char* who, int64_t n, int64_t total, bool even);  // even: no offsets
 bool kv_batch_ok(const char* who, const eq_kv_cache* c, int64_t layer, const int32_t* seqs, int64_t n,
                  const int32_t* cu, int64_t total);
 bool kv_rope_ok(const char* who, const eq_kv_cache* c, const float* rope, int64_t positions);
