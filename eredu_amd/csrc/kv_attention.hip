@@ -671,6 +671,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_stream_kernel(const 
         return kv_units(A, P.e);
     };
     Units U = enter();
+    // (offsets that cover rows many times over may list more tiles than an int counts: then no entry need
+    // have this one, and the first, which find gives, need not have a row)
+    if (unsigned(pos - base) >= unsigned(U.all)) return;
     while (true) {
         const int local = pos - base, unit = unsigned(local) / unsigned(U.tiles), tile0 = local - unit * U.tiles;
         const int tiles = min(U.tiles - tile0, stop - pos);

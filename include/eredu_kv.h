@@ -39,7 +39,8 @@ extern "C" {
  * Nothing on the device is trusted as an index: a table entry outside
  * [0, pages) is a missing page (its tokens are not written, not attended to and
  * read as zeros), a sequence outside [0, sequences) has no tokens, cu is
- * clamped to [0, total] and a decreasing pair is an empty entry.  Where a
+ * clamped to [0, total] and a decreasing pair is an empty entry (where entries
+ * then cover a row more than once, its results are not defined).  Where a
  * sequence is named twice, eq_kv_append, eq_kv_extend and eq_kv_shrink go by the
  * last entry that names it and eq_kv_fork by the last pair with that destination.
  * Calls that write a cache (append, extend, fork, shrink, free, compact) are to be
