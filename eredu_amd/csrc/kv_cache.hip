@@ -535,9 +535,14 @@ __device__ __forceinline__ int kv_open_page(const KvPages& c, int seq, int lengt
     return unsigned(id) < unsigned(c.pages) ? id : -1;
 }
 
+// Adds to the cache's count, which stays where an int ends (2^16 entries may each lack 2^26 pages).
+__device__ __forceinline__ void kv_count_missing(const KvPages& c, uint64_t lack) {
+    if (lack) *c.missing = int32_t(min(uint64_t(max(*c.missing, 0)) + lack, uint64_t(INT32_MAX)));
+}
+
 // Gives an entry its pages, free ones from rank `at` on (list: by rank); from: the page it copies first, or -1.
 __device__ __forceinline__ void kv_grow(const KvPages& c, const KvPlanScratch& s, int seq, int length, int count, int from, int at,
-                                        int free_pages, const int32_t* list, int* copies, int* lack) {
+                                        int free_pages, const int32_t* list, int* copies, uint64_t* lack) {
     const int T = 1 << c.log2_page;
     int32_t* row = c.tables + int64_t(seq) * c.width;
     int none = 0;
@@ -564,14 +569,15 @@ __device__ __forceinline__ void kv_grow(const KvPages& c, const KvPlanScratch& s
     }
     none += need - max(have, min(need, c.width));
     c.lengths[seq] = length + count;
-    if (none) atomicAdd(lack, none);
+    if (none) atomicAdd(reinterpret_cast<unsigned long long*>(lack), (unsigned long long)none);
 }
 
 __global__ __launch_bounds__(kPlanThreads) void kv_extend_plan_kernel(KvPages c, KvBatch b, KvPlanScratch s) {
     __shared__ int red[kPlanThreads / 64];
-    __shared__ int lack, copies;
+    __shared__ uint64_t lack;
+    __shared__ int copies;
     const int tid = threadIdx.x, T = 1 << c.log2_page;
-    if (tid == 0) lack = copies = 0;
+    if (tid == 0) lack = 0, copies = 0;
     int32_t* writers = s.map;
     // of the entries that name a sequence the last counts
     for (int i = tid; i < b.n; i += kPlanThreads) {
@@ -623,7 +629,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_extend_plan_kernel(KvPages c,
     __syncthreads();
     if (tid == 0) {
         s.count[0] = copies;
-        if (lack) atomicAdd(c.missing, lack);
+        kv_count_missing(c, lack);
     }
 }
 
@@ -635,11 +641,12 @@ constexpr int kFewEntries = 256, kFewPages = 64 * kPlanThreads, kFewTaken = 4096
 
 __global__ __launch_bounds__(kPlanThreads) void kv_extend_few_kernel(KvPages c, KvBatch b, KvPlanScratch s) {
     __shared__ int red[kPlanThreads / 64];
-    __shared__ int lack, copies;
+    __shared__ uint64_t lack;
+    __shared__ int copies;
     __shared__ uint64_t bits[kFewPages / 64];
     __shared__ int32_t before[kFewPages / 64], seqs[kFewEntries], opens[kFewEntries], list[kFewTaken];
     const int tid = threadIdx.x, T = 1 << c.log2_page;
-    if (tid == 0) lack = copies = 0;
+    if (tid == 0) lack = 0, copies = 0;
     int seq = -1, length = 0, count = 0, open = -1, refs = 0;
     if (tid < b.n) {
         int start;
@@ -684,7 +691,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_extend_few_kernel(KvPages c, 
     __syncthreads();
     if (tid == 0) {
         s.count[0] = copies;
-        if (lack) atomicAdd(c.missing, lack);
+        kv_count_missing(c, lack);
     }
 }
 

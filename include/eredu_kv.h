@@ -61,7 +61,7 @@ typedef struct eq_kv_cache {
     int32_t* tables;    /* [sequences, width] */
     int32_t* lengths;   /* [sequences] */
     int32_t* refs;      /* [pages] */
-    int32_t* missing;   /* [1]: pages that eq_kv_extend had none for, since it was last cleared */
+    int32_t* missing;   /* [1]: pages that eq_kv_extend had none for, since it was last cleared (at most 2^31 - 1) */
     int64_t layers, pages, sequences, width; /* width * page_tokens <= 2^30, sequences * width < 2^31 */
     int kv_heads, page_tokens, head_dim; /* page_tokens 16, 32, 64 or 128; head_dim 64, 128 or 256 */
 } eq_kv_cache;
