@@ -11,9 +11,10 @@ namespace {
 // token and one of the query heads that share the KV head):
 //
 //   S^T = K . q^T on the int8 matrix cores.  K is the codes as they lie in the cache; q
-//   is, per row, an integer of 16 bits of its largest magnitude, split into two
-//   signed digits q = 256 hi + lo: the products are exact
-//   and the digits' sums join in f32, S = sum lo c + 256 sum hi c.  No key is converted.
+//   is, per row, an integer of 24 bits of its largest magnitude, split into three
+//   signed digits q = 256 hi + mid + low / 256: the products are exact
+//   and the digits' sums join in f32.  No key is converted.  Two digits, 16 bits, are as good as
+//   three but where a row's products with a page are large (Fine): there alone the third is multiplied.
 //   softmax: a row's score is S * f + const with f = scale * log2 e * (row's step) *
 //   (page's step), one fma and one exp2.
 //   O^T += V^T . P^T in f16.  S^T comes out of the matrix cores with a lane
@@ -39,10 +40,44 @@ typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 
+// Over the wave.
+template <typename F>
+__device__ __forceinline__ int kv_wave(int v, F f) {
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false));
+    return f(f(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             f(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+
+// When two digits, 16 bits of a row's largest magnitude, will do.  A query is off by at most half of their unit u, a
+// score with a page's codes c by 0.29 u |c| in the mean, where |c| is 25 to 35 sqrt(D) for normal values
+// (73 sqrt(D) for codes spread evenly over a byte).  Where u in exponents, f * (page step), is at most 2^-15 /
+// sqrt(D), a probability is so off by 2e-4 for the usual codes, as much as an output that is rounded to
+// f16 (2.1e-4 in the mean, at most 4.9e-4); bf16 rounds 8 times as coarsely and gets 4 times the limit.  Normal queries and
+// keys whose scores spread by 1.5 stay under half of it.  With two digits everywhere, one channel of the
+// queries 30, 100 and 300 times the others (and the keys' as much smaller) made f16 outputs 1.8, 4.4 and 13 times as far
+// off as rounding alone; so it is 1.4 times, as without such a channel.  Where the third digit is needed it costs as
+// much again as the matrix cores take for one: 2048 queries over 32768 tokens 1.64 ms instead of 1.19, a token
+// after 131071 87 us instead of 69, seven prompts 155 instead of 113.
+template <typename T, int D>
+struct Fine {
+    static constexpr int exponent = std::is_same<T, F16T>::value ? -15 : -13;
+    // the limit as frexp has it
+    static constexpr int e = D == 64 ? exponent - 2 : exponent - 3;
+    static constexpr float mant = D == 128 ? 0.70710678f : 0.5f;
+    // The smallest scale byte of a page with which a row of factor f > 0 is over it.
+    static __device__ __forceinline__ int from(float f) {
+        return 127 + e - __builtin_amdgcn_frexp_expf(f) + (mant >= __builtin_amdgcn_frexp_mantf(f) ? 1 : 0);
+    }
+};
+
 template <int D, int NR>
 struct Rows {
     static constexpr int KS = D / 64, DT = D / 16;
-    i32x4 hi[NR][KS], lo[NR][KS];  // the queries' digits: row lane % 16, dimensions 64 ks + 16 g ..
+    i32x4 hi[NR][KS], mid[NR][KS];  // the queries' digits: row lane % 16, dimensions 64 ks + 16 g ..
+    int fine;                       // pages with a key scale byte from here on take the third digit too (the same for the wave)
     float f[NR];                   // what turns their integer scores into exponents (NaN: a query that is not finite)
     int from[NR], until[NR];       // the tokens that they see
     f32x4 o[NR][DT];               // O^T: row lane % 16, dimensions 16 dt + 4 g ..
@@ -76,39 +111,23 @@ __device__ __forceinline__ void kv_query_load(const uint16_t* x, const float* ro
     }
 }
 
-// A row's integers: multiples of its largest magnitude (given by its bits) / 32512,
-// as two signed digits q = 256 hi + lo; f: what a product of them with a page's codes is
-// worth in exponents, before the page's scale (s2 = scale * log2 e).
-struct Digits {
-    float f, inv;
-    int e;
-    bool fine;
-    __device__ __forceinline__ Digits(uint32_t most, float s2) {
-        fine = most > 0u && most < 0x7f800000u;
-        const float one = fine ? __uint_as_float(most) : 1.f;
-        e = __builtin_amdgcn_frexp_expf(one);
-        const float mant = __builtin_amdgcn_frexp_mantf(one);
-        inv = 32512.f / mant;
-        f = fine ? __builtin_amdgcn_ldexpf(mant * (s2 / 32512.f), e) : (most ? __uint_as_float(0x7fc00000u) : 0.f);
-    }
-    // Four values.  The fma rounds q to the lowest bits of kMagic + q; q's lowest byte is lo as it is, and
-    // hi the next one of q + 128.
-    __device__ __forceinline__ void word(const float* v, int& hi, int& lo) const {
-        uint32_t x[4];
+// Four values of a row as three signed digits of whole numbers, inv times the values: the lower bytes of q + 128 +
+// 256 * 128 are their digits plus 128, the third the highest digit.
+__device__ __forceinline__ void kv_digits(const float* v, float inv, int& hi, int& mid, int& low) {
+    uint32_t x[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = __float_as_uint(fmaf(__builtin_amdgcn_ldexpf(v[i], -e), inv, kMagic));
-        const uint32_t l = __builtin_amdgcn_perm(__builtin_amdgcn_perm(x[3], x[2], 0x0c0c0400u), __builtin_amdgcn_perm(x[1], x[0], 0x0c0c0400u), 0x05040100u);
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[i] += 128;
-        const uint32_t h = __builtin_amdgcn_perm(__builtin_amdgcn_perm(x[3], x[2], 0x0c0c0501u), __builtin_amdgcn_perm(x[1], x[0], 0x0c0c0501u), 0x05040100u);
-        hi = fine ? int(h) : 0, lo = fine ? int(l) : 0;
-    }
-};
+    for (int i = 0; i < 4; i++) x[i] = uint32_t(int(rintf(v[i] * inv))) + 0x8080u;
+    const uint32_t a = __builtin_amdgcn_perm(x[1], x[0], 0x05040100u), b = __builtin_amdgcn_perm(x[3], x[2], 0x05040100u);
+    hi = int(__builtin_amdgcn_perm(__builtin_amdgcn_perm(x[3], x[2], 0x0c0c0602u), __builtin_amdgcn_perm(x[1], x[0], 0x0c0c0602u), 0x05040100u));
+    mid = int(__builtin_amdgcn_perm(b, a, 0x07050301u) ^ 0x80808080u);
+    low = int(__builtin_amdgcn_perm(b, a, 0x06040200u) ^ 0x80808080u);
+}
 
-// The row turned (where it has angles), as digits of its largest magnitude;
-// s2 = scale * log2 e.  sees: whether there is a row that sees anything.
-template <typename T, int D>
-__device__ __forceinline__ void kv_query(const RawQuery<D>& q, bool sees, bool turn, float s2, i32x4* hi, i32x4* lo, float& f) {
+// The row turned (where it has angles), as multiples of its largest magnitude / (256 * 32512); f: what a product of
+// the middle digit's unit with a page's codes is worth in exponents, before the page's scale (s2 = scale *
+// log2 e; NaN where the row is not finite, and its digits are any).  sees: whether there is a row that sees anything.  keep(ks, digits) gets the lowest ones.
+template <typename T, int D, typename KF>
+__device__ __forceinline__ void kv_query(const RawQuery<D>& q, bool sees, bool turn, float s2, i32x4* hi, i32x4* mid, float& f, KF keep) {
     constexpr int KS = D / 64;
     float v[KS][16];
     uint32_t most = 0;
@@ -150,20 +169,41 @@ __device__ __forceinline__ void kv_query(const RawQuery<D>& q, bool sees, bool t
         for (int i = 0; i < 16; i++) most = max(most, __float_as_uint(v[ks][i]) & 0x7fffffffu);
     most = max(most, uint32_t(__shfl_xor(int(most), 16)));
     most = max(most, uint32_t(__shfl_xor(int(most), 32)));
-    const Digits dg(sees ? most : 0u, s2);  // (a row that sees nothing is zero)
-    f = dg.f;
+    if (!sees) most = 0u;  // (a row that sees nothing is zero)
+    const bool fine = most > 0u && most < 0x7f800000u;
+    float top = __uint_as_float(most), down = 1.f;
+    if (__any(fine && top < 0x1p-100f)) {  // (256 * 32512 / top may be no f32)
+        const float up = fine && top < 0x1p-100f ? 0x1p64f : 1.f;
+        down = 1.f / up, top *= up;
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++)
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[ks][i] *= up;
+    }
+    const float inv = fine ? 256.f * 32512.f / top : 0.f;
+    f = fine ? top * (s2 / 32512.f) * down : (most ? __uint_as_float(0x7fc00000u) : 0.f);
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+        i32x4 low;
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            int h, l;
-            dg.word(v[ks] + 4 * w, h, l);
-            hi[ks][w] = h, lo[ks][w] = l;
+            int h, m, l;
+            kv_digits(v[ks] + 4 * w, inv, h, m, l);
+            hi[ks][w] = h, mid[ks][w] = m, low[w] = l;
         }
+        keep(ks, low);
+    }
 }
 
-// The scores of 64 tokens, plus kMagic: s[r][t][i] is row r's with token 4 t + i
-// of this lane group's 16; k(t, ks) gives the operands.  The products of a digit
+// The lane, made anew where it is asked for (an address that is seldom used would else keep a register).
+__device__ __forceinline__ int kv_lane() {
+    int l;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=&v"(l));
+    return l;
+}
+
+// The scores of 64 tokens: s[r][t][i] is row r's with token 4 t + i
+// of this lane group's 16, plus kMagic; k(t, ks) gives the operands.  The products of a digit
 // stay below 2^22 (256 * 127 * 128), so sums that begin with the bits of 1.5 * 2^23
 // are that float plus the sum, and no score is converted (v_cvt_f32_i32 takes as long as two
 // or three fmas: 83 ns for 16 in a loop, where 16 fmas take 39).
@@ -178,42 +218,74 @@ __device__ __forceinline__ void kv_scores(const Rows<D, NR>& R, KF k, f32x4 (&s)
         for (int ks = 0; ks < KS; ks++) a[ks] = k(t, ks);
 #pragma unroll
         for (int r = 0; r < NR; r++) {
-            i32x4 hi = {M, M, M, M}, lo = {M, M, M, M};
+            i32x4 hi = {M, M, M, M}, mid = {M, M, M, M};
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[ks], R.hi[r][ks], hi, 0, 0, 0);
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[ks], R.lo[r][ks], lo, 0, 0, 0);
+            for (int ks = 0; ks < KS; ks++) mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[ks], R.mid[r][ks], mid, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < 4; i++) s[r][t][i] = fmaf(__int_as_float(hi[i]) - kMagic, 256.f, __int_as_float(lo[i]));
+            for (int i = 0; i < 4; i++) s[r][t][i] = fmaf(__int_as_float(hi[i]) - kMagic, 256.f, __int_as_float(mid[i]));
         }
     }
 }
 
+// The same scores with the third digit, without kMagic.  (A sum next to kMagic is a whole number, one far from it
+// rounded as f32 rounds it: neither loses what is added here.)
+template <int D, int NR, typename KF, typename LF>
+__device__ __forceinline__ void kv_scores_fine(KF k, LF low, f32x4 (&s)[NR][4]) {
+    constexpr int M = 0x4b400000;
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        i32x4 l[NR];
+#pragma unroll
+        for (int r = 0; r < NR; r++) l[r] = i32x4{M, M, M, M};
+#pragma unroll
+        for (int ks = 0; ks < D / 64; ks++) {
+            const i32x4 a = k(t, ks);
+#pragma unroll
+            for (int r = 0; r < NR; r++) l[r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, low(r, ks), l[r], 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < NR; r++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[r][t][i] = fmaf(__int_as_float(l[r][i]) - kMagic, 1.f / 256, s[r][t][i] - kMagic);
+        __builtin_amdgcn_sched_barrier(0);  // (seldom done: no registers for more than one product at a time)
+    }
+}
+
 // The softmax of those scores: the probabilities p, their sums, and the
-// states so far brought to the tile's maximum (if that moves) and base.  kb is
-// this lane group's key scale byte, nan: it or the value's is 255; j0 its first
+// states so far brought to the tile's maximum (if that moves) and base.  kf is
+// this lane group's page step (NaN: the key's scale byte or the value's is 255), j0 its first
 // token; dead: its page is missing; base: the largest value scale byte so far,
-// this tile's included.  edge (the same for the wave): some row does not see some of the
+// this tile's included.  fine (the same for the wave): the tile takes the third digit, k(t, ks) and low(r, ks) give
+// its operands.  (It shares the masks' branch: with one more on the way from the products to the exponents cross
+// attention took 37.6 us instead of 31.4.)  edge (the same for the wave): some row does not see some of the
 // tokens; their scores are set below all others for the maximum, their exponents to -inf.
-template <int D, int NR>
-__device__ __forceinline__ void kv_softmax(Rows<D, NR>& R, f32x4 (&s)[NR][4], int kb, bool nan, int j0, bool dead, bool edge,
-                                           int base, h16x8 (&p)[NR][2]) {
+template <int D, int NR, typename KF, typename LF>
+__device__ __forceinline__ void kv_softmax(Rows<D, NR>& R, f32x4 (&s)[NR][4], bool fine, KF k, LF low, float kf, int j0, bool dead,
+                                           bool edge, int base, h16x8 (&p)[NR][2]) {
     constexpr int DT = D / 16;
-    const float kf = nan ? __uint_as_float(0x7fc00000u) : e8m0_to_f32(uint32_t(kb));
     float f[NR], top[NR];
     int first[NR], seen[NR];
     bool need = base > R.base;
+    float zero = kMagic;  // what stands for 0 in the scores
 #pragma unroll
     for (int r = 0; r < NR; r++) first[r] = 0, seen[r] = 16;
-    if (edge) {
-#pragma unroll
-        for (int r = 0; r < NR; r++) {
-            first[r] = dead ? 16 : max(R.from[r] - j0, 0);
-            seen[r] = max(min(R.until[r] - j0, 16) - first[r], 0);
-#pragma unroll
-            for (int n = 0; n < 16; n++)
-                if (unsigned(n - first[r]) >= unsigned(seen[r])) s[r][n >> 2][n & 3] = -1e30f;
+    if (edge | fine) {
+        if (fine) {
+            kv_scores_fine<D, NR>(k, low, s);
+            zero = 0.f;
         }
+        if (edge) {
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                first[r] = dead ? 16 : max(R.from[r] - j0, 0);
+                seen[r] = max(min(R.until[r] - j0, 16) - first[r], 0);
+#pragma unroll
+                for (int n = 0; n < 16; n++)
+                    if (unsigned(n - first[r]) >= unsigned(seen[r])) s[r][n >> 2][n & 3] = -1e30f;
+        }
+    }
     }
 #pragma unroll
     for (int r = 0; r < NR; r++) {
@@ -221,7 +293,7 @@ __device__ __forceinline__ void kv_softmax(Rows<D, NR>& R, f32x4 (&s)[NR][4], in
         float mx = s[r][0][0];
 #pragma unroll
         for (int n = 1; n < 16; n++) mx = fmaxf(mx, s[r][n >> 2][n & 3]);
-        top[r] = seen[r] > 0 ? (mx - kMagic) * f[r] : -INFINITY;
+        top[r] = seen[r] > 0 ? (mx - zero) * f[r] : -INFINITY;
         need |= top[r] > R.m[r] + kMaxSlack;
     }
     if (__any(need)) {
@@ -240,7 +312,7 @@ __device__ __forceinline__ void kv_softmax(Rows<D, NR>& R, f32x4 (&s)[NR][4], in
     }
 #pragma unroll
     for (int r = 0; r < NR; r++) {
-        const float shift = fmaf(-kMagic, f[r], kProbBias - R.m[r]);
+        const float shift = fmaf(-zero, f[r], kProbBias - R.m[r]);
 #pragma unroll
         for (int n = 0; n < 16; n++) s[r][n >> 2][n & 3] = fmaf(s[r][n >> 2][n & 3], f[r], shift);
     }
@@ -361,17 +433,6 @@ __device__ __forceinline__ bool kv_whole(const AttnCall& A, const TileRange& t) 
     return A.splits == 1 || (A.causal && t.end - t.begin <= (A.splits <= 3 ? 16 : 4));
 }
 
-// Over the wave.
-template <typename F>
-__device__ __forceinline__ int kv_wave(int v, F f) {
-    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
-    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
-    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
-    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false));
-    return f(f(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
-             f(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
-}
-
 // Where a launch's workgroup works: the KV head varies fastest, so that one
 // head's codes stay in one XCD's L2 where there are 8 of them.
 struct Place {
@@ -462,10 +523,17 @@ __device__ __forceinline__ void kv_nothing(Rows<D, NR>& R) {  // no tokens yet
     }
     R.base = 0;
 }
-template <typename T, int D, int NR>
-__device__ __forceinline__ void kv_begin(const AttnCall& A, Rows<D, NR>& R, const RowLoads<D, NR>& W) {
+// (keep(r, ks, digits) gets the rows' lowest digits)
+template <typename T, int D, int NR, typename KF>
+__device__ __forceinline__ void kv_begin(const AttnCall& A, Rows<D, NR>& R, const RowLoads<D, NR>& W, KF keep) {
+    int fine = 256;
 #pragma unroll
-    for (int r = 0; r < NR; r++) kv_query<T, D>(W.q[r], W.sees[r], A.rope != nullptr, A.s2, R.hi[r], R.lo[r], R.f[r]);
+    for (int r = 0; r < NR; r++) {
+        kv_query<T, D>(W.q[r], W.sees[r], A.rope != nullptr, A.s2, R.hi[r], R.mid[r], R.f[r],
+                       [&](int ks, const i32x4& low) __attribute__((always_inline)) { keep(r, ks, low); });
+        if (R.f[r] > 0.f) fine = min(fine, Fine<T, D>::from(R.f[r]));
+    }
+    R.fine = kv_wave(fine, [](int a, int b) { return min(a, b); });
     kv_nothing<D, NR>(R);
 }
 
@@ -636,9 +704,13 @@ struct Tile {
 };
 
 template <int D>
+__device__ __forceinline__ const int8_t* kv_keys(const AttnCall& A, const Place& P, int tile, int id, int lane) {
+    const int g = lane >> 4, a = (lane & 15) >> 2, T = 1 << A.c.log2_page;
+    return A.c.k + ((int64_t(max(id, 0)) * A.c.kv_heads + P.kvh) * T + ((tile * 64 + 16 * a) & (T - 1)) + (lane & 3)) * D + 16 * g;
+}
+template <int D>
 __device__ __forceinline__ void kv_fetch_keys(const AttnCall& A, const Place& P, int tile, int id, Tile<D>& t) {
-    const int lane = threadIdx.x & 63, g = lane >> 4, a = (lane & 15) >> 2, T = 1 << A.c.log2_page;
-    const int8_t* k = A.c.k + ((int64_t(max(id, 0)) * A.c.kv_heads + P.kvh) * T + ((tile * 64 + 16 * a) & (T - 1)) + (lane & 3)) * D + 16 * g;
+    const int8_t* k = kv_keys<D>(A, P, tile, id, threadIdx.x & 63);
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -654,8 +726,10 @@ __device__ __forceinline__ void kv_fetch_values(const AttnCall& A, const Place& 
 
 template <typename T, int D>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_stream_kernel(const AttnCall A) {
-    constexpr int NR = 1, BM = kStreamRows;
+    constexpr int NR = 1, BM = kStreamRows, KS = D / 64;
     __shared__ TileListLds lds;
+    __shared__ i32x4 digits[4 * KS * 64];  // each lane's own lowest ones
+    i32x4* const low = digits + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * KS * 64;
     const int lane = threadIdx.x & 63, g = lane >> 4, a = (lane & 15) >> 2;
     TileList list(A, lds);
     const int run = kv_run(A, list.all), wid = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -702,29 +776,36 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_stream_kernel(const 
         __builtin_amdgcn_sched_barrier(0);
         // (a unit without tiles, of rows that see nothing, reads some page and uses none of it)
         Tile<D> t;
-        int idg = kv_page_of(A.c, eg);
-        kv_fetch_keys<D>(A, P, tile, kv_page_of(A.c, ea), t);
+        int idg = kv_page_of(A.c, eg), ida = kv_page_of(A.c, ea);
+        kv_fetch_keys<D>(A, P, tile, ida, t);
         scales(idg, kb, vb);
         ea = table(tile + 1, a), eg = table(tile + 1, g);
         __builtin_amdgcn_sched_barrier(0);
-        kv_begin<T, D, NR>(A, R, W);  // (while the first keys are under way)
+        kv_begin<T, D, NR>(A, R, W, [&](int, int ks, const i32x4& x) __attribute__((always_inline)) {
+            low[64 * ks + lane] = x;
+        });  // (while the first keys are under way)
         __builtin_amdgcn_sched_barrier(0);
         kv_fetch_values<D>(A, P, tile, idg, t);
         for (; tile < end; tile++) {
             const bool more = tile + 1 < end;
+            const bool fine = kv_group_max(kb) >= R.fine;
+            const float kf = kb == 255 || vb == 255 ? __uint_as_float(0x7fc00000u) : e8m0_to_f32(uint32_t(kb));
             f32x4 s[NR][4];
             kv_scores<D, NR>(R, [&](int i, int ks) __attribute__((always_inline)) { return t.k[i][ks]; }, s);
-            int kbn = 0, vbn = 0, idn = -1;
+            int kbn = 0, vbn = 0, idn = -1, idk = ida;
             if (more) {
-                idn = kv_page_of(A.c, eg);
-                kv_fetch_keys<D>(A, P, tile + 1, kv_page_of(A.c, ea), t);
+                idn = kv_page_of(A.c, eg), ida = kv_page_of(A.c, ea);
+                kv_fetch_keys<D>(A, P, tile + 1, ida, t);
                 scales(idn, kbn, vbn);
                 ea = table(tile + 2, a), eg = table(tile + 2, g);
             }
             const bool dead = idg < 0;
             const int ev = vb == 255 || dead ? 0 : vb, top = max(R.base, kv_group_max(ev));
             h16x8 p[NR][2];
-            kv_softmax<D, NR>(R, s, kb, kb == 255 || vb == 255, tile * 64 + 16 * g, dead,
+            // (the third digit reads the tile's keys again: their registers have the next one's)
+            kv_softmax<D, NR>(R, s, fine, [&](int i, int ks) __attribute__((always_inline)) {
+                return *reinterpret_cast<const i32x4*>(kv_keys<D>(A, P, tile, idk, kv_lane()) + 4 * i * D + 64 * ks);
+            }, [&](int, int ks) __attribute__((always_inline)) { return low[64 * ks + kv_lane()]; }, kf, tile * 64 + 16 * g, dead,
                               tile < clear_from || tile >= clear_until || __any(dead), top, p);
             const Convert to(ev, top);
             kv_values<D, NR>(R, p, [&](int dt, int u) __attribute__((always_inline)) {
@@ -927,6 +1008,13 @@ __global__ __launch_bounds__(64 * NW, WPS) void kv_block_kernel(const AttnCall A
     constexpr int PITCH = D + 8;  // of an output row in LDS: 16 rows' 8 bytes are in different banks
     __shared__ i32x4 lds[24 * D];
     static_assert(BM * PITCH * 2 <= 24 * D * 16, "the output fits where the tiles were");
+    // the queries' lowest digits, each lane's own: as many in LDS as leave a CU its workgroups, as registers
+    // are short (all, but for 64 rows of 128 dimensions half of them: held in registers they all spill)
+    constexpr int KS = D / 64;
+    constexpr int SPARE = (160 * 1024 / (4 * WPS / NW) - 24 * D * 16) / (THREADS * 16), IN_LDS = SPARE < NR * KS ? SPARE : NR * KS;
+    __shared__ i32x4 digits[NW * IN_LDS * 64];
+    i32x4* const low_lds = digits + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * IN_LDS * 64;
+    i32x4 low_regs[NR * KS - IN_LDS + 1];
     i32x4 *const k0 = lds, *const k1 = lds + 4 * D;
     h16x8 *const v0 = reinterpret_cast<h16x8*>(lds + 8 * D), *const v1 = v0 + 8 * D;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
@@ -996,7 +1084,10 @@ __global__ __launch_bounds__(64 * NW, WPS) void kv_block_kernel(const AttnCall A
             }
         };
         request(tile);
-        kv_begin<T, D, NR>(A, R, W);  // (while the first tile is on its way)
+        kv_begin<T, D, NR>(A, R, W, [&](int r, int ks, const i32x4& x) __attribute__((always_inline)) {
+            if (r * KS + ks < IN_LDS) low_lds[(r * KS + ks) * 64 + lane] = x;
+            else low_regs[r * KS + ks - IN_LDS] = x;
+        });  // (while the first tile is on its way)
         convert(k0, v0);
         auto step = [&](const i32x4* kc, const h16x8* vc, i32x4* kn, h16x8* vn) __attribute__((always_inline)) {
             __syncthreads();  // this tile is there, and the other buffers are read
@@ -1004,13 +1095,18 @@ __global__ __launch_bounds__(64 * NW, WPS) void kv_block_kernel(const AttnCall A
             kb = kbn, vb = vbn, base = base_next;
             if (more) request(tile + 1);
             if (tile >= see_from && tile < see_until) {
+                const bool fine = kv_group_max(kb) >= R.fine;
+                const float kf = kb == 255 || vb == 255 ? __uint_as_float(0x7fc00000u) : e8m0_to_f32(uint32_t(kb));
                 f32x4 s[NR][4];
-                kv_scores<D, NR>(R, [&](int t, int ks) __attribute__((always_inline)) {
+                auto keys = [&](int t, int ks) __attribute__((always_inline)) {
                     const int token = 4 * (lane & 12) + 4 * t + (lane & 3);
                     return kc[token * (D / 16) + ((4 * ks + g) ^ kv_key_swap<D>(token))];
-                }, s);
+                };
+                kv_scores<D, NR>(R, keys, s);
                 h16x8 p[NR][2];
-                kv_softmax<D, NR>(R, s, kb, kb == 255 || vb == 255, tile * 64 + 16 * g, dead,
+                kv_softmax<D, NR>(R, s, fine, keys, [&](int r, int ks) __attribute__((always_inline)) {
+                    return r * KS + ks < IN_LDS ? low_lds[(r * KS + ks) * 64 + kv_lane()] : low_regs[r * KS + ks - IN_LDS];
+                }, kf, tile * 64 + 16 * g, dead,
                                   tile < clear_from || tile >= clear_until || __any(dead), base, p);
                 kv_values<D, NR>(R, p, [&](int dt, int u) __attribute__((always_inline)) {
                     const int d = 16 * dt + (lane & 15);

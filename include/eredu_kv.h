@@ -92,8 +92,9 @@ int eq_kv_append(const eq_kv_cache* cache, int64_t layer, const void* k, const v
  * gives zeros.  q and out bf16 or f16 (the same), q's rows at stride q_stride as
  * in eq_kv_append, out [total, n_heads, head_dim] contiguous; rope as there,
  * for q.  Rows that no entry covers are left as they are in out.  Scores,
- * softmax sums and outputs are held in f32; q in 16 bits of each row's
- * largest magnitude, probabilities in f16, values exactly where their page's
+ * softmax sums and outputs are held in f32; q in 24 bits of each row's
+ * largest magnitude, in 16 where that moves its scores with a page's keys by no more than
+ * rounding moves the output (all but scores that spread by tens), probabilities in f16, values exactly where their page's
  * scale is at least 2^-29 of the sequence's largest.  scale * max|q| * max|k|
  * of a row and a page has to be below 2^124 (a score may be NaN beyond). */
 int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n_heads, const eq_kv_cache* cache, int64_t layer,
