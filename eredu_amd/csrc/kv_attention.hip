@@ -28,10 +28,10 @@ namespace {
 //   met (`base`): 1 + (c + 128) / 1024 -> c * 2^(5 + b - base), exact down
 //   to 2^-29 of the largest page.
 //
-// The running maximum moves only when a score exceeds it by 2^8 (and base when
-// a page's scale exceeds it): then, rarely, maxima are exchanged between the lane groups
-// and O and l rescaled.  Probabilities are held as f16 of 2^6 exp2(score - m):
-// at most 2^14, down to 2^-20 with all their bits.
+// Probabilities are held as f16 of exp2(score + b), b = 6 less the maximum that was
+// met: at most 2^14, down to 2^-20 with all their bits.  b moves only when a score would pass
+// that (and base when a page's scale exceeds it): then, rarely, maxima are exchanged between the lane
+// groups and O and l rescaled.
 constexpr float kProbBias = 6.f, kMaxSlack = 8.f;
 constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: floats next to it are whole numbers
 
@@ -81,7 +81,7 @@ struct Rows {
     float f[NR];                   // what turns their integer scores into exponents (NaN: a query that is not finite)
     int from[NR], until[NR];       // the tokens that they see
     f32x4 o[NR][DT];               // O^T: row lane % 16, dimensions 16 dt + 4 g ..
-    float m[NR], l[NR];            // l: this lane group's part
+    float b[NR], l[NR];            // b: inf before the first token; l: this lane group's part
     int base;                      // scale byte that o is relative to
 };
 
@@ -229,10 +229,11 @@ __device__ __forceinline__ void kv_scores(const Rows<D, NR>& R, KF k, f32x4 (&s)
     }
 }
 
-// The same scores with the third digit, without kMagic.  (A sum next to kMagic is a whole number, one far from it
+// The same scores with the third digit, as exponents by kf, this lane group's page step: rounded once, so that
+// scores of any size stay below their maximum.  (A sum next to kMagic is a whole number, one far from it
 // rounded as f32 rounds it: neither loses what is added here.)
 template <int D, int NR, typename KF, typename LF>
-__device__ __forceinline__ void kv_scores_fine(KF k, LF low, f32x4 (&s)[NR][4]) {
+__device__ __forceinline__ void kv_scores_fine(const Rows<D, NR>& R, KF k, float kf, LF low, f32x4 (&s)[NR][4]) {
     constexpr int M = 0x4b400000;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
@@ -248,8 +249,18 @@ __device__ __forceinline__ void kv_scores_fine(KF k, LF low, f32x4 (&s)[NR][4]) 
 #pragma unroll
         for (int r = 0; r < NR; r++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) s[r][t][i] = fmaf(__int_as_float(l[r][i]) - kMagic, 1.f / 256, s[r][t][i] - kMagic);
+            for (int i = 0; i < 4; i++) s[r][t][i] = fmaf(__int_as_float(l[r][i]) - kMagic, 1.f / 256, s[r][t][i] - kMagic) * (R.f[r] * kf);
         __builtin_amdgcn_sched_barrier(0);  // (seldom done: no registers for more than one product at a time)
+    }
+}
+
+template <int NR>
+__device__ __forceinline__ void kv_tops(const f32x4 (&s)[NR][4], float (&top)[NR]) {
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        top[r] = s[r][0][0];
+#pragma unroll
+        for (int n = 1; n < 16; n++) top[r] = fmaxf(top[r], s[r][n >> 2][n & 3]);
     }
 }
 
@@ -260,21 +271,23 @@ __device__ __forceinline__ void kv_scores_fine(KF k, LF low, f32x4 (&s)[NR][4]) 
 // this tile's included.  fine (the same for the wave): the tile takes the third digit, k(t, ks) and low(r, ks) give
 // its operands.  (It shares the masks' branch: with one more on the way from the products to the exponents cross
 // attention took 37.6 us instead of 31.4.)  edge (the same for the wave): some row does not see some of the
-// tokens; their scores are set below all others for the maximum, their exponents to -inf.
+// tokens; these are left out of the maximum, and their exponents are -inf.
 template <int D, int NR, typename KF, typename LF>
 __device__ __forceinline__ void kv_softmax(Rows<D, NR>& R, f32x4 (&s)[NR][4], bool fine, KF k, LF low, float kf, int j0, bool dead,
                                            bool edge, int base, h16x8 (&p)[NR][2]) {
     constexpr int DT = D / 16;
-    float f[NR], top[NR];
+    float f[NR], top[NR], shift[NR];
     int first[NR], seen[NR];
     bool need = base > R.base;
     float zero = kMagic;  // what stands for 0 in the scores
 #pragma unroll
-    for (int r = 0; r < NR; r++) first[r] = 0, seen[r] = 16;
+    for (int r = 0; r < NR; r++) first[r] = 0, seen[r] = 16, f[r] = R.f[r] * kf;
     if (edge | fine) {
         if (fine) {
-            kv_scores_fine<D, NR>(k, low, s);
+            kv_scores_fine<D, NR>(R, k, kf, low, s);
             zero = 0.f;
+#pragma unroll
+            for (int r = 0; r < NR; r++) f[r] = 1.f;
         }
         if (edge) {
 #pragma unroll
@@ -283,39 +296,36 @@ __device__ __forceinline__ void kv_softmax(Rows<D, NR>& R, f32x4 (&s)[NR][4], bo
                 seen[r] = max(min(R.until[r] - j0, 16) - first[r], 0);
 #pragma unroll
                 for (int n = 0; n < 16; n++)
-                    if (unsigned(n - first[r]) >= unsigned(seen[r])) s[r][n >> 2][n & 3] = -1e30f;
+                    if (unsigned(n - first[r]) >= unsigned(seen[r])) s[r][n >> 2][n & 3] = -INFINITY;
         }
     }
     }
+    kv_tops<NR>(s, top);
 #pragma unroll
     for (int r = 0; r < NR; r++) {
-        f[r] = R.f[r] * kf;
-        float mx = s[r][0][0];
-#pragma unroll
-        for (int n = 1; n < 16; n++) mx = fmaxf(mx, s[r][n >> 2][n & 3]);
-        top[r] = seen[r] > 0 ? (mx - zero) * f[r] : -INFINITY;
-        need |= top[r] > R.m[r] + kMaxSlack;
+        shift[r] = fmaf(-zero, f[r], R.b[r]);
+        need |= seen[r] > 0 && fmaf(top[r], f[r], shift[r]) > kProbBias + kMaxSlack;
     }
     if (__any(need)) {
         const float down = __builtin_amdgcn_ldexpf(1.f, R.base - base);
         R.base = base;
 #pragma unroll
         for (int r = 0; r < NR; r++) {
-            float mn = fmaxf(top[r], __shfl_xor(top[r], 16));
-            mn = fmaxf(R.m[r], fmaxf(mn, __shfl_xor(mn, 32)));
-            const float al = mn == R.m[r] ? 1.f : __builtin_amdgcn_exp2f(R.m[r] - mn);
-            R.m[r] = mn;
+            float mn = seen[r] > 0 ? (top[r] - zero) * f[r] : -INFINITY;
+            mn = fmaxf(mn, __shfl_xor(mn, 16));
+            mn = fmaxf(mn, __shfl_xor(mn, 32));
+            const float b = fminf(R.b[r], kProbBias - mn), al = b == R.b[r] ? 1.f : __builtin_amdgcn_exp2f(b - R.b[r]);
+            R.b[r] = b;
+            shift[r] = fmaf(-zero, f[r], b);
             R.l[r] *= al;
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) R.o[r][dt] *= al * down;
         }
     }
 #pragma unroll
-    for (int r = 0; r < NR; r++) {
-        const float shift = fmaf(-zero, f[r], kProbBias - R.m[r]);
+    for (int r = 0; r < NR; r++)
 #pragma unroll
-        for (int n = 0; n < 16; n++) s[r][n >> 2][n & 3] = fmaf(s[r][n >> 2][n & 3], f[r], shift);
-    }
+        for (int n = 0; n < 16; n++) s[r][n >> 2][n & 3] = fmaf(s[r][n >> 2][n & 3], f[r], shift[r]);
     if (edge) {
 #pragma unroll
         for (int r = 0; r < NR; r++)
@@ -516,7 +526,7 @@ template <int D, int NR>
 __device__ __forceinline__ void kv_nothing(Rows<D, NR>& R) {  // no tokens yet
 #pragma unroll
     for (int r = 0; r < NR; r++) {
-        R.m[r] = -INFINITY;
+        R.b[r] = INFINITY;
         R.l[r] = 0.f;
 #pragma unroll
         for (int dt = 0; dt < D / 16; dt++) R.o[r][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -822,7 +832,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_stream_kernel(const 
         l += __shfl_xor(l, 32);
         if (row < rows) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            if (part && g == 0) A.lse[slot * BM + row] = l == 0.f ? -INFINITY : R.m[0] + __builtin_amdgcn_logf(l);
+            if (part && g == 0) A.lse[slot * BM + row] = l == 0.f ? -INFINITY : __builtin_amdgcn_logf(l) - R.b[0];
 #pragma unroll
             for (int dt = 0; dt < D / 16; dt++) {
                 f32x4 o;
@@ -1131,7 +1141,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void kv_block_kernel(const AttnCall A
         l += __shfl_xor(l, 32);
         const int row = 16 * r + (lane & 15);
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (part && g == 0 && row < mine) kv_store_lse(A, P, first + row, l == 0.f ? -INFINITY : R.m[r] + __builtin_amdgcn_logf(l));
+        if (part && g == 0 && row < mine) kv_store_lse(A, P, first + row, l == 0.f ? -INFINITY : __builtin_amdgcn_logf(l) - R.b[r]);
 #pragma unroll
         for (int dt = 0; dt < D / 16; dt++) {
             f32x4 o;
