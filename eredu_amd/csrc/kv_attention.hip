@@ -409,6 +409,7 @@ struct AttnCall {
     unsigned group;
     bool causal;
     int groups;    // kv_stream_kernel's workgroups
+    int slot_rows;  // rows of its slots: as many as a unit may have
     float* part;   // kv_block_kernel: [row][head][split][D], normalised; null: one split.  kv_stream_kernel: [slot][row][D]
     float* lse;    // [row][head][split], or [slot][row]
 };
@@ -832,13 +833,13 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_stream_kernel(const 
         l += __shfl_xor(l, 32);
         if (row < rows) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            if (part && g == 0) A.lse[slot * BM + row] = l == 0.f ? -INFINITY : __builtin_amdgcn_logf(l) - R.b[0];
+            if (part && g == 0) A.lse[slot * A.slot_rows + row] = l == 0.f ? -INFINITY : __builtin_amdgcn_logf(l) - R.b[0];
 #pragma unroll
             for (int dt = 0; dt < D / 16; dt++) {
                 f32x4 o;
 #pragma unroll
                 for (int j = 0; j < 4; j++) o[j] = __builtin_amdgcn_ldexpf(R.o[0][dt][j] * inv, R.base - 132);
-                if (part) *reinterpret_cast<f32x4*>(A.part + (int64_t(slot) * BM + row) * D + 16 * dt + 4 * g) = o;
+                if (part) *reinterpret_cast<f32x4*>(A.part + (int64_t(slot) * A.slot_rows + row) * D + 16 * dt + 4 * g) = o;
                 else kv_store4<T, D>(A, P, P.first + row, 16 * dt + 4 * g, o);
             }
         }
@@ -959,7 +960,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv_stream_join_kernel(c
         for (int j = 0; j < 4; j++) {
             const int w = b + j * SETS + set;
             const bool is = w <= w1;
-            const int64_t slot = int64_t(2 * (is ? w : w0) + (w == w0 && S != w0 * run ? 1 : 0)) * kStreamRows + row % kStreamRows;
+            const int64_t slot = int64_t(2 * (is ? w : w0) + (w == w0 && S != w0 * run ? 1 : 0)) * A.slot_rows + row % kStreamRows;
             f[j] = is ? A.lse[slot] : -INFINITY;
             x[j] = is ? reinterpret_cast<const f32x4*>(A.part + slot * D)[t % LANES] : f32x4{0.f, 0.f, 0.f, 0.f};
         }
@@ -1224,6 +1225,7 @@ struct Plan {
     int64_t tiles;
     int splits;  // of a block's tokens
     int groups;  // workgroups of a stream
+    int slot_rows;  // of a stream's slots
     int join_waves;  // of a stream's rows: 16, 4 or 1
     size_t part_bytes, lse_bytes;
 };
@@ -1254,8 +1256,11 @@ Plan plan_attention(const eq_kv_cache* c, int n_heads, int64_t n, int64_t total,
         // of 3.9.  Many have few: 7200 rows take a wave each 6.3 us instead of 18.5 with 4 waves, 640 rows 7.2 instead of 5.4
         const int64_t joins = total * n_heads;
         p.join_waves = n <= 64 && joins <= 2 * device_cu_count() && cap > 64 ? 16 : (joins <= 4 * device_cu_count() ? 4 : 1);
-        p.part_bytes = size_t(p.groups) * 8 * kStreamRows * c->head_dim * 4;
-        p.lse_bytes = (size_t(p.groups) * 8 * kStreamRows * 4 + 255) & ~size_t(255);
+        // (a decode step of 4 heads a group fills a quarter of 16 rows: 8.4 MB at 128 dimensions instead of 33.8)
+        const int64_t unit = (ragged || !n ? total : total / n) * group;
+        p.slot_rows = int(unit < kStreamRows ? unit : kStreamRows);
+        p.part_bytes = size_t(p.groups) * 8 * p.slot_rows * c->head_dim * 4;
+        p.lse_bytes = (size_t(p.groups) * 8 * p.slot_rows * 4 + 255) & ~size_t(255);
         return p;
     }
     // as many splits as come nearest to filling the CUs once (300 queries over 8000 tokens, 80 blocks: 560
@@ -1359,6 +1364,7 @@ extern "C" int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n
     A.tiles = int(plan.tiles);
     A.splits = plan.splits;
     A.groups = plan.groups;
+    A.slot_rows = plan.slot_rows;
     A.window = int(window < kKvMaxLength ? window : kKvMaxLength);
     A.causal = causal;
     const dim3 grid{unsigned(plan_blocks(cache, plan))};

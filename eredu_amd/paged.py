@@ -173,8 +173,9 @@ class PagedKVCache:
 
     def _scratch(self, need: int) -> Tuple[Optional[int], int, Optional[torch.Tensor]]:
         """Scratch of a call from torch: in stream order, and under capture a graph's
-        own, so that graphs share nothing.  (Eager calls that need little take the
-        library's workspace of their stream, which saves them the allocation.)"""
+        own, so that graphs share nothing.  (Other eager calls take the library's
+        workspace of their stream, which saves them the allocation, and which keeps the
+        most that such a call needed as long as the process runs.)"""
         if need < 0:
             check(1)
         if need == 0:
@@ -217,7 +218,7 @@ class PagedKVCache:
             raise EreduError(f"out must be a contiguous {q.dtype} tensor of {q.numel()} values on {self.device}")
         L, st = _native.lib(), self._here()
         wp, wn, ws = None, 0, None
-        if rows * heads > 8192 or _capturing():  # (what fewer rows need is a few MB)
+        if rows * heads > 8192 or _capturing():  # (fewer rows need at most 64 MiB, decode steps of 4 heads a group 8)
             wp, wn, ws = self._scratch(L.eq_kv_attention_scratch(self._ref, heads, n, rows, cu is not None))
         check(L.eq_kv_attention(out.data_ptr(), q.data_ptr(), q.stride(0), heads, self._ref, layer, seqs.data_ptr(), n,
                                 None if cu is None else cu.data_ptr(), rows, self._scale if scale is None else scale,

@@ -49,3 +49,26 @@ def test_other_refusals(bad, words):
     a.update(bad)
     refused(attend(**a), *words)
     refused(scratch(cache(), a["heads"], a["n"], a["total"]), *words)
+
+
+@pytest.mark.parametrize("D,heads,kv,n,each", [(128, 32, 8, 1, 1), (256, 32, 8, 4, 1), (128, 32, 8, 48, 1), (64, 16, 16, 16, 5),
+                                               (128, 8, 8, 3, 1), (128, 32, 8, 2, 4), (256, 16, 1, 1, 1), (128, 32, 8, 2, 12)])
+def test_a_decode_step_takes_scratch_for_the_rows_it_has(D, heads, kv, n, each):
+    """Two slots for each of 2048 waves (of 256 CUs, as where there is no GPU to ask), of the rows that a sequence and
+    KV head have, up to 16."""
+    c = cache(head_dim=D, kv_heads=kv, width=512)
+    rows = min(16, each * heads // kv)
+    assert 0 < scratch(c, heads, n, n * each) <= 2 * 2048 * rows * (D + 1) * 4 + 256
+    assert scratch(c, heads, n, n * each, True) <= 2 * 2048 * min(16, n * each * heads // kv) * (D + 1) * 4 + 256
+
+
+def test_scratch_of_calls_of_few_rows():
+    """What eager calls of up to 8192 rows and heads keep in their stream's workspace."""
+    most = 0
+    for D in (64, 128, 256):
+        for heads, kv in ((1, 1), (8, 2), (32, 8), (32, 32), (64, 1)):
+            for n in (1, 2, 7, 48, 512):
+                for each in (1, 2, 5, 13, 33, 64, 128, 300, 8192):
+                    if n * each * heads <= 8192:
+                        most = max(most, *(scratch(cache(head_dim=D, kv_heads=kv, width=2048), heads, n, n * each, r) for r in (False, True)))
+    assert 32 << 20 < most <= 65 << 20
