@@ -118,18 +118,6 @@ template <typename T> __device__ __forceinline__ float kv_to_f32(uint32_t bits);
 template <> __device__ __forceinline__ float kv_to_f32<BF16T>(uint32_t b) { return bf16_bits_to_f32(b); }
 template <> __device__ __forceinline__ float kv_to_f32<F16T>(uint32_t b) { return f16_bits_to_f32(b); }
 
-// 8 consecutive 16-bit values (16-byte aligned) as f32.
-template <typename T>
-__device__ __forceinline__ void kv_load8(const uint16_t* p, float* f) {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        f[2 * i] = kv_to_f32<T>(w[i] & 0xffffu);
-        f[2 * i + 1] = kv_to_f32<T>(w[i] >> 16);
-    }
-}
-
 // Host side: argument checks of every entry point, and the views they make.
 bool kv_cache_ok(const char* who, const eq_kv_cache* c);
 bool kv_rows_ok(const char* who, int64_t n, int64_t total, bool even);  // even: no offsets
