@@ -589,8 +589,8 @@ __device__ __forceinline__ void kv_store_lse(const AttnCall& A, const Place& P, 
 // these go to two slots of the wave, to be joined by kv_stream_join_kernel.
 // Memory bounds it where contexts are long (one row over 131071 tokens, 8 KV heads of 128
 // dimensions: 268 MB in 54 us with pages of 64, 5.0 TB/s, 63 us with pages of 128, whose tiles are
-// not contiguous; 48 sequences of 17 .. 8191: 121 MB in 31.5 us), the trips to
-// lengths, table, scales and first tile, about 5 us, where they are short (1025 tokens: 7.8 us).
+// not contiguous; 48 sequences of 17 .. 8191: 121 MB in 31.7 us), the trips to
+// lengths, table, scales and first tile, about 5 us, where they are short (1025 tokens: 8.0 us).
 
 constexpr int kStreamRows = 16;
 
@@ -975,10 +975,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv_stream_join_kernel(c
 // tokens.  A tile's keys and values go through registers, where the values become f16
 // once for the workgroup (a wave converting them for itself had 3/8 of its vector
 // instructions for that), to LDS, one tile ahead, and each wave takes its operands from there.
-// (Keys loaded straight to LDS took the same time, and could not be held back.)  What bounds it is a
+// (Keys loaded straight to LDS took the same time, and could not be held back.)  What bounds it most is a
 // SIMD's vector and matrix instructions, which hardly overlap: 2048 rows over 32768 tokens, 32 heads on 8
-// of 128 dimensions, 1.18 ms, 906 TFLOP/s, the matrix cores busy 37 % and the vector unit 62 % of the
-// cycles; a block's life before its first tile and after its last is about 9 us.  16-byte pieces of a row are swapped by
+// of 128 dimensions, 1.18 ms, 900 TFLOP/s, the matrix cores busy 36 % of the cycles and the vector unit, but for
+// their instructions' issue, 52 %; a block's life before its first tile and after its last is about 9 us.  16-byte pieces of a row are swapped by
 // an exclusive or with bits of the row, so that the lanes that a read or a write takes
 // together (16 of them, of two lane groups) lie in different banks: a key's (row =
 // token 16 a + 4 t + b, read for all a and b at once) by bits of a and b, a value's
@@ -1219,7 +1219,9 @@ bool attention_sizes_ok(const char* who, const eq_kv_cache* c, int n_heads, int6
 }
 
 // Which kernel, how many rows a workgroup, how many splits: from the call's
-// sizes alone (lengths are on the device; the table's width bounds them).
+// sizes alone (lengths and offsets are on the device; the table's width bounds them), so of a ragged batch by
+// its rows on average: a prompt of 2000 rows beside one row after 65536 tokens takes 1.71 ms in one call, whose
+// row is one workgroup's a KV head, 71 and 33 us in two.
 struct Plan {
     int rows;    // of a workgroup: 16 (stream), 64 or 128 (block)
     int64_t tiles;
@@ -1381,7 +1383,7 @@ extern "C" int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n
         }
         // 128 rows are 4 waves of 32 up to 128 dimensions (2048 queries over 32768 tokens of 128: 1.19 ms;
         // 8 of 16, whose registers spill at four to a SIMD, 1.33), 8 of 16 at 256, where 4 waves of 32 do not
-        // fit and 64 rows to a workgroup read every key twice as often (0.59 ms against 1.05)
+        // fit and 64 rows to a workgroup read every key twice as often (0.60 ms against 1.05)
         if (plan.rows == 64) kv_block_kernel<T, DIM, 1, 4, DIM == 64 ? 4 : DIM == 128 ? 3 : 1><<<grid, dim3(256), 0, st>>>(A);
         else if constexpr (DIM <= 128) kv_block_kernel<T, DIM, 2, 4, 2><<<grid, dim3(256), 0, st>>>(A);
         else kv_block_kernel<T, DIM, 1, 8, 2><<<grid, dim3(512), 0, st>>>(A);

@@ -4,8 +4,8 @@
 //
 // All of these move bytes: append reads 2 bytes and writes 1 a value (10000 tokens of 8 heads
 // of 128 dimensions 18 us, 3.4 TB/s), read the reverse (14 us, 4.4 TB/s), extend and
-// compact read and write whole pages (335 MB in 50 us); fork, shrink and free are trips to the tables, 2
-// to 6 us.
+// compact read and write whole pages (335 MB in 50 us); fork, shrink and free are trips to the tables: a fork
+// to 15 sequences of 31 pages 3.7 us, 16 sequences shrunk 2.5, 15 freed 1.6 to 4.
 #include "kv_common.hpp"
 
 namespace eq {

@@ -207,7 +207,9 @@ class PagedKVCache:
         sequences: causal with an optional sliding ``window``, or, not causal, over all
         tokens of the sequence (cross attention).  scale: 1 / sqrt(head_dim) if None.
         Rows that see no token give zeros; rows that no entry of cu covers are left as
-        they are in ``out`` (C ABI: eq_kv_attention)."""
+        they are in ``out``.  The work is laid out by the entries' rows on average: long
+        prompts and single tokens after long contexts are faster in calls of their own
+        (C ABI: eq_kv_attention)."""
         q = self._rows(q, "q")
         rows, heads, D = q.shape
         seqs, n, cu = self._batch(seqs, cu, rows)

@@ -77,8 +77,9 @@ typedef struct eq_kv_cache {
  * max|x| <= 127 * 2^(b - 127) over its new tokens; one that held tokens keeps
  * its b or takes that larger one, and its codes are rounded to the new step (ties
  * to even, as all codes).  Steps are powers of two, so a value is off by less
- * than one step of its page's scale, however often that grew.  A new value that
- * is not finite: b = 255.  Codes behind a page's last token keep what they
+ * than one step of its page's scale, however often that grew.  (One of at least
+ * 63.5 * 2^122, bf16's two largest, is rounded to 2^128, which f32 has as infinity.)
+ * A new value that is not finite: b = 255.  Codes behind a page's last token keep what they
  * were.  The pages written must belong to one sequence (eq_kv_extend sees to it). */
 int eq_kv_append(const eq_kv_cache* cache, int64_t layer, const void* k, const void* v, int64_t k_stride,
                  int64_t v_stride, const int32_t* seqs, int64_t n, const int32_t* cu, int64_t total,
@@ -96,7 +97,9 @@ int eq_kv_append(const eq_kv_cache* cache, int64_t layer, const void* k, const v
  * largest magnitude, in 16 where that moves its scores with a page's keys by no more than
  * rounding moves the output (all but scores that spread by tens), probabilities in f16, values exactly where their page's
  * scale is at least 2^-29 of the sequence's largest.  scale * max|q| * max|k|
- * of a row and a page has to be below 2^124 (a score may be NaN beyond). */
+ * of a row and a page has to be below 2^124 (a score may be NaN beyond).
+ * How the work is laid out follows from the entries' rows on average: give
+ * long prompts and single tokens after long contexts calls of their own. */
 int eq_kv_attention(void* out, const void* q, int64_t q_stride, int n_heads, const eq_kv_cache* cache, int64_t layer,
                     const int32_t* seqs, int64_t n, const int32_t* cu, int64_t total, float scale, bool causal,
                     int64_t window, const float* rope, int64_t rope_positions, int dtype, void* scratch,
