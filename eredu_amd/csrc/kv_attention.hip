@@ -77,7 +77,7 @@ template <int D, int NR>
 struct Rows {
     static constexpr int KS = D / 64, DT = D / 16;
     i32x4 hi[NR][KS], mid[NR][KS];  // the queries' digits: row lane % 16, dimensions 64 ks + 16 g ..
-    int fine;                       // pages with a key scale byte from here on take the third digit too (the same for the wave)
+    int fine;                      // key scale bytes from here on take the third digit too (the same for the wave)
     float f[NR];                   // what turns their integer scores into exponents (NaN: a query that is not finite)
     int from[NR], until[NR];       // the tokens that they see
     f32x4 o[NR][DT];               // O^T: row lane % 16, dimensions 16 dt + 4 g ..
@@ -125,7 +125,8 @@ __device__ __forceinline__ void kv_digits(const float* v, float inv, int& hi, in
 
 // The row turned (where it has angles), as multiples of its largest magnitude / (256 * 32512); f: what a product of
 // the middle digit's unit with a page's codes is worth in exponents, before the page's scale (s2 = scale *
-// log2 e; NaN where the row is not finite, and its digits are any).  sees: whether there is a row that sees anything.  keep(ks, digits) gets the lowest ones.
+// log2 e; NaN where the row is not finite, and its digits are any).  sees: whether there is a row that sees
+// anything.  keep(ks, digits) gets the lowest ones.
 template <typename T, int D, typename KF>
 __device__ __forceinline__ void kv_query(const RawQuery<D>& q, bool sees, bool turn, float s2, i32x4* hi, i32x4* mid, float& f, KF keep) {
     constexpr int KS = D / 64;
@@ -297,8 +298,8 @@ __device__ __forceinline__ void kv_softmax(Rows<D, NR>& R, f32x4 (&s)[NR][4], bo
 #pragma unroll
                 for (int n = 0; n < 16; n++)
                     if (unsigned(n - first[r]) >= unsigned(seen[r])) s[r][n >> 2][n & 3] = -INFINITY;
+            }
         }
-    }
     }
     kv_tops<NR>(s, top);
 #pragma unroll
