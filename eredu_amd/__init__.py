@@ -20,7 +20,11 @@ host-side mirror of the reference's operator API:
 * :mod:`eredu_amd.decode` -- the Llama decode step around the projections.
 * :mod:`eredu_amd.paged` -- ``PagedKVCache``: the paged 8-bit key/value cache of
   many sequences, its attention and its pages.
+* :mod:`eredu_amd.fp8` -- linears in 8-bit floating point with block scales: products
+  of one weight or of routed experts, and the norm, gated activation and
+  quantizers that give their operands.
 """
+from . import fp8
 from ._native import EreduError
 from .paged import PagedKVCache, rope_table
 from .quantization import (
@@ -51,6 +55,7 @@ __all__ = [
     "QuantizedLinear",
     "dequantize",
     "dequantize_with_mode",
+    "fp8",
     "gather_qmm",
     "gather_qmm_with_mode",
     "quantized_matmul",

@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in ``include/eredu_hip.h`` and ``include/eredu_kv.h``.
+"""ctypes binding of the C ABI in ``include/eredu_hip.h``, ``include/eredu_kv.h`` and ``include/eredu_fp8.h``.
 
 The shared library is built in-tree by ``eredu_amd.build``.  There is no
 fallback: if the library is missing, loading fails with an error that says so.
@@ -95,6 +95,20 @@ KV_SIGNATURES["eq_kv_free"] = ([_kv, _vp, _i64, _vp], _i32)
 KV_SIGNATURES["eq_kv_compact"] = ([_kv, _vp, _i64, _vp], _i32)
 KV_SIGNATURES["eq_kv_pages_scratch"] = ([_kv, _i64], _i64)
 
+# the entry points of include/eredu_fp8.h
+EQ_DTYPE_F8E4M3 = 4
+FP8_SIGNATURES = {
+    "eq_fp8_quantize": ([_vp, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp], _i32),
+    "eq_fp8_quantize_weight": ([_vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp], _i32),
+    "eq_fp8_rms_norm": ([_vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, ctypes.c_float, _i32, _vp], _i32),
+    "eq_fp8_silu_mul": ([_vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp], _i32),
+    "eq_fp8_matmul": ([_vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _i64, _vp], _i32),
+    "eq_fp8_matmul_scratch": ([_i64, _i64, _i64, _i32, _i32], _i64),
+    "eq_fp8_grouped_matmul": ([_vp, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _i32,
+                               _vp, _i64, _vp], _i32),
+    "eq_fp8_grouped_matmul_scratch": ([_i64, _i64, _i64, _i64, _i64, _i32, _i32], _i64),
+}
+
 _lib = None
 _lock = threading.Lock()
 
@@ -118,7 +132,7 @@ def lib() -> ctypes.CDLL:
                     f"HIP kernel library not found at {path}; build it with `python -m eredu_amd.build`"
                 )
             L = ctypes.CDLL(path)
-            for name, (args, res) in {**SIGNATURES, **KV_SIGNATURES}.items():
+            for name, (args, res) in {**SIGNATURES, **KV_SIGNATURES, **FP8_SIGNATURES}.items():
                 fn = getattr(L, name)
                 fn.argtypes = args
                 fn.restype = res

@@ -2,8 +2,8 @@
 
 ``python -m eredu_amd.build`` (or ``__graft_entry__.build()``) compiles every
 ``eredu_amd/csrc/*.hip`` with hipcc for gfx950 and links one shared library
-whose exported symbols are the C ABI of ``include/eredu_hip.h`` and
-``include/eredu_kv.h``.
+whose exported symbols are the C ABI of ``include/eredu_hip.h``,
+``include/eredu_kv.h`` and ``include/eredu_fp8.h``.
 """
 from __future__ import annotations
 
@@ -98,7 +98,7 @@ def build_host_sanitized() -> str:
     (``sanitizer_runtime()``) and ``EREDU_AMD_LIB`` pointing at it."""
     os.makedirs(SAN_DIR, exist_ok=True)
     srcs = sources()
-    newest = max(os.path.getmtime(f) for f in srcs + [os.path.join(ROOT, "include", h) for h in ("eredu_hip.h", "eredu_kv.h")] +
+    newest = max(os.path.getmtime(f) for f in srcs + [os.path.join(ROOT, "include", h) for h in ("eredu_hip.h", "eredu_kv.h", "eredu_fp8.h")] +
                  [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hpp")])
     if os.path.exists(SAN_LIB) and os.path.getmtime(SAN_LIB) > newest:
         return SAN_LIB

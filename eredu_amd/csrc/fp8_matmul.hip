@@ -1,0 +1,551 @@
+// Products of rows in e4m3 codes with e4m3 weights, both with block scales:
+//
+//   y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in block b} cx[m, k] cw[n, k]
+//
+// A block of 128 columns is one v_mfma_f32_16x16x128_f8f6f4 (twice the rate of
+// the 16x16x32 fp8 instruction).  Its sums start at zero and are added to the
+// f32 accumulators with the scale: four FMAs a lane beside 32 cycles of matrix
+// core, so half of the vector unit's time.  The weights are the A operand,
+// whose rows are the result's: a lane has results of one activation row, so
+// the scale is one register, sx sw, for all of its weight rows.  Which of the
+// block's columns a lane's 32 bytes hold is the same for both operands, so it
+// can be any of them.
+//
+// The e4m3 instructions (16x16x32 as well) line the products of 8 neighbouring
+// columns up to the largest's exponent and keep 13 bits below it, cut off
+// towards zero, before they are summed in f32 (measured with single products).
+// That is 2^-13 of a product where the result's own rounding is 2^-9 or 2^-12 of
+// the sum, so results of 16 bits take them.  f32 results take the codes as
+// bf16, which holds them exactly, through v_mfma_f32_16x16x32_bf16: twice the cycles, and
+// sums that are off by f32's rounding alone (of 128 products 7e-8 where the e4m3 ones are off by 5e-5).
+#include <algorithm>
+
+#include "fp8_common.hpp"
+
+namespace eq {
+namespace {
+
+constexpr int kMostExperts = 4095;  // (two counters each in 64 KiB of LDS with room to spare)
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) const float lds_f32;
+
+struct Fp8Args {
+    void* y;
+    const uint8_t* x;
+    const float* xs;
+    int64_t x_stride, xs_stride;
+    const uint8_t* w;
+    const float* ws;
+    int M, N, K, KB;  // KB: blocks of K
+    int mtiles, ntiles;
+    // Grouped: tiles[i] = {expert, first, rows} of row tile i, the rows being
+    // routes order[first ..]; tiles[mtiles].x: how many there are.  Expert -1: rows of zeros.
+    const int4* tiles;
+    const int32_t* order;
+    const int32_t* rows;
+    int64_t x_rows;
+};
+
+__device__ __forceinline__ f32x4 mfma128(u32x4 a0, u32x4 a1, u32x4 b0, u32x4 b1) {
+    const i32x8 a = __builtin_bit_cast(i32x8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+    const i32x8 b = __builtin_bit_cast(i32x8, __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7));
+    // formats 0, 0: e4m3; scales 0: the form without scales
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f32x4{}, 0, 0, 0, 0, 0, 0);
+}
+
+// Eight codes as bf16.
+__device__ __forceinline__ bf16x8 codes_bf16(uint32_t lo, uint32_t hi) {
+    const u32x4 v = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true))};
+    return __builtin_bit_cast(bf16x8, v);
+}
+
+// A lane's 32 codes of a row and block, as the matrix instruction takes them.
+template <bool EXACT>
+struct Operand;
+template <>
+struct Operand<false> {
+    u32x4 c[2];
+    __device__ __forceinline__ void take(u32x4 a, u32x4 b) { c[0] = a, c[1] = b; }
+};
+template <>
+struct Operand<true> {
+    bf16x8 c[4];
+    __device__ __forceinline__ void take(u32x4 a, u32x4 b) {
+        c[0] = codes_bf16(a[0], a[1]), c[1] = codes_bf16(a[2], a[3]);
+        c[2] = codes_bf16(b[0], b[1]), c[3] = codes_bf16(b[2], b[3]);
+    }
+};
+__device__ __forceinline__ f32x4 block_sums(const Operand<false>& a, const Operand<false>& b) {
+    return mfma128(a.c[0], a.c[1], b.c[0], b.c[1]);
+}
+__device__ __forceinline__ f32x4 block_sums(const Operand<true>& a, const Operand<true>& b) {
+    f32x4 d{};
+#pragma unroll
+    for (int i = 0; i < 4; i++) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.c[i], b.c[i], d, 0, 0, 0);
+    return d;
+}
+
+// VALS consecutive results of a row, n of them inside it; whole: 16-byte stores will do.
+template <typename YT, int VALS>
+__device__ __forceinline__ void store_run(typename YT::storage* p, const float* v, int n, bool whole) {
+    constexpr int VEC = 16 / int(sizeof(typename YT::storage));
+#pragma unroll
+    for (int i = 0; i < VALS; i += VEC) {
+        if (whole) {
+            if (i < n) {
+                if constexpr (VEC == 8) store8<YT>(p + i, v + i);
+                else *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                if (i + e < n) store_out<YT>(p, i + e, v[i + e]);
+        }
+    }
+}
+
+// WN x WM waves of NT x MT tiles of 16 x 16: 16 NT WN weight rows by 16 MT WM
+// activation rows a workgroup.  Both operands go straight from memory to LDS,
+// two blocks of K deep.
+//
+// Row i of a wave's A tile t is its weight row 4 NT (i / 4) + 4 t + i % 4, so that
+// a lane ends with 4 NT consecutive results of its activation row.  A row's 128
+// bytes of a block lie in LDS in slots of 16, chunk c in slot c ^ key: 16 lanes read
+// 16 rows at one chunk, LDS has 64 banks of 4 bytes (two rows), so the
+// rows of one parity have to differ in their key: (row / 2) % 8 for the
+// activations, (row / 2) % 2 + 2 (row / (4 NT) % 4) for the weights' rows above.
+template <typename YT, int WN, int WM, int NT, int MT>
+__global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_tile_kernel(
+    const Fp8Args args) {
+    constexpr int WAVES = WN * WM, TN = 16 * NT * WN, TM = 16 * MT * WM;
+    constexpr int LA = TN / 8 / WAVES, LB = TM / 8 / WAVES;  // loads of 1 KiB (8 rows) a wave
+    static_assert(LA * 8 * WAVES == TN && LB * 8 * WAVES == TM && TN % 128 == 0, "whole loads");
+    constexpr int SROWS = TM < 64 ? 64 : TM, BUF = (TN + TM) * 128 + SROWS * 4;
+    static_assert(64 * WAVES >= SROWS, "a scale load a wave");
+    constexpr bool EXACT = std::is_same<YT, F32T>::value;
+    // (separate arrays, so that the compiler knows that a read of one does not wait for loads into the other)
+    __shared__ __attribute__((aligned(16))) char buf0[BUF], buf1[BUF];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+    const int wn = wave % WN, wm = wave / WN, l16 = lane & 15, quad = lane >> 4;
+    const int N = args.N, K = args.K, KB = args.KB;
+
+    // The workgroups of one XCD (id % 8) take a run of tiles.
+    const int used = args.tiles ? args.tiles[args.mtiles].x : args.mtiles;
+    const int64_t total = int64_t(used) * args.ntiles, run = (total + 7) >> 3;
+    const int64_t tile = (blockIdx.x & 7) * run + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= run || tile >= total) return;  // (the whole workgroup)
+    const int tm = int(tile / args.ntiles), tn = int(tile % args.ntiles), n0 = tn * TN;
+    int m0 = tm * TM, mrows = min(TM, args.M - m0), first = 0, expert = 0;
+    const uint8_t* xp = args.x + m0 * args.x_stride;
+    const float* xsp = args.xs + m0;
+    uint32_t x_bytes = uint32_t(mrows - 1) * uint32_t(args.x_stride) + uint32_t(K);
+    if (args.tiles) {
+        const int4 t = args.tiles[tm];
+        expert = t.x, first = t.y, mrows = t.z;
+        m0 = 0;
+        xp = args.x;
+        xsp = args.xs;
+        x_bytes = uint32_t((args.x_rows - 1) * args.x_stride + K);
+    }
+    typename YT::storage* const y = static_cast<typename YT::storage*>(args.y);
+    const bool whole = N % (16 / int(sizeof(typename YT::storage))) == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
+    // the results' row of this tile's row i < mrows
+    auto out_row = [&](int i) __attribute__((always_inline)) { return int64_t(args.tiles ? args.order[first + i] : m0 + i); };
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) acc[t][j] = f32x4{};
+
+    if (expert >= 0) {
+        const int nrows = min(TN, N - n0);
+        const __amdgpu_buffer_rsrc_t xr = raw_rsrc(xp, x_bytes);
+        const __amdgpu_buffer_rsrc_t wr =
+            raw_rsrc(args.w + (int64_t(expert) * N + n0) * K, uint32_t(nrows) * uint32_t(K));
+        const int nblocks = (N + 127) / 128, nb = min((n0 + 16 * NT * wn) / 128, nblocks - 1);
+        const float* const wsp = args.ws + (int64_t(expert) * nblocks + nb) * KB;
+
+        // Lane l of load i of a wave: row 8 (L wave + i) + l / 8 of the tile, the chunk that belongs in slot l % 8.
+        uint32_t a_off[LA], b_off[LB], s_off;
+        auto a_chunk = [&](int i) __attribute__((always_inline)) {
+            const int row = 8 * (LA * wave + i) + (lane >> 3);
+            return (lane & 7) ^ (((row >> 1) & 1) | ((row / (4 * NT)) & 3) << 1);
+        };
+        auto b_chunk = [&](int i) __attribute__((always_inline)) {
+            const int row = 8 * (LB * wave + i) + (lane >> 3);
+            return (lane & 7) ^ ((row >> 1) & 7);
+        };
+        // the x row of tile row i, -1 past the tile's end
+        auto x_row = [&](int i) __attribute__((always_inline)) {
+            if (i >= mrows) return -1;
+            if (!args.tiles) return i;
+            const int r = args.order[first + i], s = args.rows ? args.rows[r] : r;
+            return uint32_t(s) < uint64_t(args.x_rows) ? s : -1;
+        };
+#pragma unroll
+        for (int i = 0; i < LA; i++) {
+            const int row = 8 * (LA * wave + i) + (lane >> 3);
+            a_off[i] = row < nrows ? uint32_t(row) * uint32_t(K) + 16u * a_chunk(i) : kOutOfRange;
+        }
+#pragma unroll
+        for (int i = 0; i < LB; i++) {
+            const int r = x_row(8 * (LB * wave + i) + (lane >> 3));
+            b_off[i] = r >= 0 ? uint32_t(r) * uint32_t(args.x_stride) + 16u * b_chunk(i) : kOutOfRange;
+        }
+        const int s_wave = wave % (SROWS / 64);
+        {
+            const int r = x_row(64 * s_wave + lane);
+            s_off = r >= 0 ? uint32_t(r) * 4u : kOutOfRange;
+        }
+        const uint32_t s_bytes = uint32_t(args.tiles ? args.x_rows : mrows) * 4u;
+
+        auto load = [&](char* to, int kb) __attribute__((always_inline)) {
+            lds_char* const buf = (lds_char*)to;
+            const uint32_t k = uint32_t(kb) * 128u;
+            const bool tail = K - int(k) < 128;  // (only the last block: chunks past K are zeros)
+            const int left = K - int(k);
+#pragma unroll
+            for (int i = 0; i < LA; i++) {
+                uint32_t off = a_off[i];
+                if (tail) off = 16 * a_chunk(i) < left ? off : kOutOfRange;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    wr, (__attribute__((address_space(3))) void*)(buf + (LA * wave + i) * 1024), 16, off, k, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < LB; i++) {
+                uint32_t off = b_off[i];
+                if (tail) off = 16 * b_chunk(i) < left ? off : kOutOfRange;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    xr, (__attribute__((address_space(3))) void*)(buf + TN * 128 + (LB * wave + i) * 1024), 16, off, k, 0, 0);
+            }
+            const __amdgpu_buffer_rsrc_t sr = raw_rsrc(xsp + kb * args.xs_stride, s_bytes);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                sr, (__attribute__((address_space(3))) void*)(buf + (TN + TM) * 128 + s_wave * 256), 4, s_off, 0, 0, 0);
+        };
+
+        // A: weight row of tile t is a_row + 4 t; B: activation row 16 (MT wm + j) + l16.  Chunks quad and quad + 4.
+        const int a_row = 16 * NT * wn + 4 * NT * (l16 >> 2) + (l16 & 3);
+        const uint32_t a_at = uint32_t(a_row * 128 + ((quad ^ (((l16 >> 1) & 1) | ((l16 >> 2) << 1))) << 4));
+        const uint32_t b_at = uint32_t(TN * 128 + (16 * MT * wm + l16) * 128 + ((quad ^ ((l16 >> 1) & 7)) << 4));
+        const uint32_t s_at = uint32_t((TN + TM) * 128 + (16 * MT * wm + l16) * 4);
+        auto compute = [&](char* from, float sw) __attribute__((always_inline)) {
+            lds_char* const buf = (lds_char*)from;
+            Operand<EXACT> a[NT], b;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+                a[t].take(*(lds_u32x4*)(buf + a_at + t * 512), *(lds_u32x4*)(buf + (a_at ^ 64u) + t * 512));
+#pragma unroll
+            for (int j = 0; j < MT; j++) {
+                const float s = *(lds_f32*)(buf + s_at + j * 64) * sw;
+                b.take(*(lds_u32x4*)(buf + b_at + j * 2048), *(lds_u32x4*)(buf + (b_at ^ 64u) + j * 2048));
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const f32x4 p = block_sums(a[t], b);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[t][j][r] = fmaf(s, p[r], acc[t][j][r]);
+                }
+            }
+        };
+        // Every load of this wave has landed and its reads are done; then all waves'.
+        auto turn = [&]() __attribute__((always_inline)) {
+            __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+            asm volatile("s_barrier" ::: "memory");
+        };
+
+        load(buf0, 0);
+        float sw = wsp[0];
+        for (int kb = 0; kb < KB; kb += 2) {
+            turn();
+            if (kb + 1 < KB) load(buf1, kb + 1);
+            const float sw1 = wsp[min(kb + 1, KB - 1)];
+            compute(buf0, sw);
+            if (kb + 1 >= KB) break;
+            turn();
+            if (kb + 2 < KB) load(buf0, kb + 2);
+            sw = wsp[min(kb + 2, KB - 1)];
+            compute(buf1, sw1);
+        }
+    }
+
+    const int n = n0 + 16 * NT * wn + 4 * NT * quad;
+#pragma unroll
+    for (int j = 0; j < MT; j++) {
+        const int i = 16 * (MT * wm + j) + l16;
+        if (i < mrows && n < N) {
+            float v[4 * NT];
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) v[4 * t + r] = acc[t][j][r];
+            store_run<YT, 4 * NT>(y + out_row(i) * N + n, v, N - n, whole);
+        }
+    }
+}
+
+// The routes of each expert side by side, and the row tiles that they make
+// (fp8_tile_kernel's `tiles` and `order`): counted, summed up and placed by one
+// workgroup.  Routes without an expert or a row come last, as expert -1.  Their places
+// within an expert are not in order, which no result depends on.
+__global__ __launch_bounds__(1024) void fp8_routes_kernel(int4* __restrict__ tiles, int32_t* __restrict__ order,
+                                                          const int32_t* __restrict__ ids,
+                                                          const int32_t* __restrict__ rows, int routes, int experts,
+                                                          int64_t x_rows, int tile_rows, int mtiles) {
+    extern __shared__ int shared[];
+    int* const count = shared;               // [experts + 1]
+    int* const place = shared + experts + 1;  // [experts + 1]
+    __shared__ int sums[2][16], base[2];
+    auto bucket = [&](int r) {
+        const int e = ids[r], s = rows ? rows[r] : r;
+        return uint32_t(e) < uint32_t(experts) && s >= 0 && s < x_rows ? e : experts;
+    };
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int e = threadIdx.x; e <= experts; e += 1024) count[e] = 0;
+    if (threadIdx.x < 2) base[threadIdx.x] = 0;
+    __syncthreads();
+    for (int r = threadIdx.x; r < routes; r += 1024) atomicAdd(&count[bucket(r)], 1);
+    __syncthreads();
+    // running sums of routes and tiles over the experts, 1024 of them a step
+    for (int e0 = 0; e0 <= experts; e0 += 1024) {
+        const int e = e0 + threadIdx.x, c = e <= experts ? count[e] : 0, t = (c + tile_rows - 1) / tile_rows;
+        int cs = c, ts = t;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int cu = __shfl_up(cs, o), tu = __shfl_up(ts, o);
+            if (lane >= o) cs += cu, ts += tu;
+        }
+        if (lane == 63) sums[0][wave] = cs, sums[1][wave] = ts;
+        __syncthreads();
+        int cb = base[0], tb = base[1];
+        for (int i = 0; i < wave; i++) cb += sums[0][i], tb += sums[1][i];
+        __syncthreads();
+        if (threadIdx.x == 1023) base[0] = cb + cs, base[1] = tb + ts;
+        if (e <= experts) {
+            place[e] = cb + cs - c;
+            for (int i = 0; i < t; i++)
+                if (tb + ts - t + i < mtiles)  // (always: mtiles is what the routes can make)
+                    tiles[tb + ts - t + i] =
+                        make_int4(e < experts ? e : -1, cb + cs - c + i * tile_rows, min(tile_rows, c - i * tile_rows), 0);
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) tiles[mtiles] = make_int4(base[1], 0, 0, 0);
+    for (int r = threadIdx.x; r < routes; r += 1024) order[atomicAdd(&place[bucket(r)], 1)] = r;
+}
+
+template <typename YT>
+void launch_tiles(const Fp8Args& a, hipStream_t st) {
+    const int64_t total = (int64_t(a.mtiles) * a.ntiles + 7) / 8 * 8;
+    fp8_tile_kernel<YT, 2, 2, 4, 4><<<dim3(unsigned(total)), dim3(256), 0, st>>>(a);
+}
+
+constexpr int kTileRows = 128, kTileCols = 128;
+
+size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+
+// How a product is done, from its sizes and types alone (the scratch queries
+// and the calls go by the same), and its scratch: lists of routes, the codes and scales of x.
+struct Plan {
+    int64_t mtiles, ntiles;
+    size_t tiles = 0, order = 0, codes = 0, scales = 0;
+    size_t bytes() const { return tiles + order + codes + scales; }
+};
+
+bool sizes_ok(const char* who, int64_t rows, int64_t n, int64_t k) {
+    if (!fp8_cols_ok(who, "k", k)) return false;
+    if (rows < 0 || n < 0 || rows >= (int64_t(1) << 30) || n >= (int64_t(1) << 30)) {
+        set_error(std::string(who) + ": rows and n must be in [0, 2^30)");
+        return false;
+    }
+    if (rows * fp8_blocks(k) >= kFp8MaxGroups) {
+        set_error(std::string(who) + ": rows * ceil(k / 128) must be below 2^26");
+        return false;
+    }
+    return true;
+}
+
+bool dtypes_ok(const char* who, int x_dtype, int y_dtype) {
+    if (x_dtype != EQ_DTYPE_F8E4M3 && !valid_dtype(x_dtype)) {
+        set_error(std::string(who) + ": x must be e4m3 codes, f32, f16 or bf16");
+        return false;
+    }
+    if (!valid_dtype(y_dtype)) {
+        set_error(std::string(who) + ": y must be f32, f16 or bf16");
+        return false;
+    }
+    return true;
+}
+
+bool grid_ok(const char* who, const Plan& p) {
+    if (p.mtiles * p.ntiles < (int64_t(1) << 23)) return true;  // (fewer than 2^32 threads)
+    set_error(std::string(who) + ": 2^23 tiles of 128 x 128 or more");
+    return false;
+}
+
+bool plan_product(const char* who, Plan& p, int64_t m, int64_t n, int64_t k, int x_dtype, int y_dtype) {
+    if (!sizes_ok(who, m, n, k) || !dtypes_ok(who, x_dtype, y_dtype)) return false;
+    p.mtiles = (m + kTileRows - 1) / kTileRows;
+    p.ntiles = (n + kTileCols - 1) / kTileCols;
+    if (x_dtype != EQ_DTYPE_F8E4M3) {
+        p.codes = round256(size_t(m) * size_t(k));
+        p.scales = round256(size_t(m) * size_t(fp8_blocks(k)) * 4u);
+    }
+    return grid_ok(who, p);
+}
+
+bool plan_routes(const char* who, Plan& p, int64_t x_rows, int64_t experts, int64_t routes, int64_t n, int64_t k,
+                 int x_dtype, int y_dtype) {
+    if (!sizes_ok(who, routes, n, k) || !sizes_ok(who, x_rows, n, k) || !dtypes_ok(who, x_dtype, y_dtype)) return false;
+    if (experts < 1 || experts > kMostExperts) {
+        set_error(std::string(who) + ": experts must be in [1, " + std::to_string(kMostExperts) + "]");
+        return false;
+    }
+    // (a part tile for each expert that has one, and for the routes without)
+    p.mtiles = std::min(routes, routes / kTileRows + experts + 1);
+    p.ntiles = (n + kTileCols - 1) / kTileCols;
+    p.tiles = round256(size_t(p.mtiles + 1) * sizeof(int4));
+    p.order = round256(size_t(routes) * 4u);
+    if (x_dtype != EQ_DTYPE_F8E4M3) {
+        p.codes = round256(size_t(x_rows) * size_t(k));
+        p.scales = round256(size_t(x_rows) * size_t(fp8_blocks(k)) * 4u);
+    }
+    return grid_ok(who, p);
+}
+
+bool operands_ok(const char* who, const void* y, const void* x, int64_t x_stride, const float* x_scales,
+                 int64_t scale_stride, const void* w, const float* w_scales, int64_t x_rows, int64_t k, int x_dtype,
+                 int y_dtype) {
+    const bool coded = x_dtype == EQ_DTYPE_F8E4M3;
+    if (!y || !w_scales || (coded && !x_scales)) {
+        set_error(std::string(who) + ": null pointer argument");
+        return false;
+    }
+    if (!coded && x_scales) {
+        set_error(std::string(who) + ": x_scales belong to codes");
+        return false;
+    }
+    if (!aligned(y, y_dtype == EQ_DTYPE_F32 ? 4 : 2) || !aligned(w_scales, 4) || (coded && !aligned(x_scales, 4))) {
+        set_error(std::string(who) + ": y and scales must be aligned to their values");
+        return false;
+    }
+    return fp8_rows_ok(who, "x", x, x_stride, k, coded ? 1 : x_dtype == EQ_DTYPE_F32 ? 4 : 2) &&
+           fp8_rows_ok(who, "w", w, k, k, 1) && (!coded || fp8_scales_ok(who, scale_stride, x_rows, k));
+}
+
+// The caller's scratch or the stream's workspace; null: the error is set.
+char* scratch_of(WsHold& hold, const char* who, void* scratch, int64_t scratch_bytes, size_t need, hipStream_t st) {
+    if (scratch) {
+        if (scratch_bytes >= 0 && size_t(scratch_bytes) >= need && aligned(scratch, 256)) return static_cast<char*>(scratch);
+        set_error(std::string(who) + ": needs " + std::to_string(need) + " bytes of 256-byte aligned scratch");
+        return nullptr;
+    }
+    char* p = static_cast<char*>(ws_acquire(hold, nullptr, need, st));
+    if (!p)
+        set_error(std::string(who) + ": no workspace (its stream's workspace cannot grow while capturing: pass scratch, "
+                  "or make one such call on the stream before capturing)");
+    return p;
+}
+
+// x of a call, quantized into scratch first where it is not in codes.
+void take_x(Fp8Args& a, char* scratch, const Plan& p, const void* x, int64_t x_stride, const float* x_scales,
+            int64_t scale_stride, int64_t rows, int64_t k, int x_dtype, hipStream_t st) {
+    if (x_dtype == EQ_DTYPE_F8E4M3) {
+        a.x = static_cast<const uint8_t*>(x), a.xs = x_scales, a.x_stride = x_stride, a.xs_stride = scale_stride;
+        return;
+    }
+    float* scales = reinterpret_cast<float*>(scratch + p.codes);
+    launch_fp8_quantize(scratch, scales, rows, x, x_stride, rows, k, x_dtype, st);
+    a.x = reinterpret_cast<const uint8_t*>(scratch), a.xs = scales, a.x_stride = k, a.xs_stride = rows;
+}
+
+}  // namespace
+}  // namespace eq
+
+using namespace eq;
+
+extern "C" int64_t eq_fp8_matmul_scratch(int64_t m, int64_t n, int64_t k, int x_dtype, int y_dtype) {
+    clear_error();
+    Plan p;
+    return plan_product("eq_fp8_matmul", p, m, n, k, x_dtype, y_dtype) ? int64_t(p.bytes()) : -1;
+}
+
+extern "C" int eq_fp8_matmul(void* y, const void* x, int64_t x_stride, const float* x_scales, int64_t scale_stride,
+                             const void* w, const float* w_scales, int64_t m, int64_t n, int64_t k, int x_dtype,
+                             int y_dtype, void* scratch, int64_t scratch_bytes, eq_stream_t stream) {
+    clear_error();
+    const char* who = "eq_fp8_matmul";
+    Plan p;
+    if (!plan_product(who, p, m, n, k, x_dtype, y_dtype)) return 1;
+    if (m == 0 || n == 0) return 0;
+    if (!operands_ok(who, y, x, x_stride, x_scales, scale_stride, w, w_scales, m, k, x_dtype, y_dtype)) return 1;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    WsHold hold;
+    char* base = nullptr;
+    if (p.bytes() && !(base = scratch_of(hold, who, scratch, scratch_bytes, p.bytes(), st))) return 1;
+    Fp8Args a{};
+    a.y = y;
+    a.w = static_cast<const uint8_t*>(w);
+    a.ws = w_scales;
+    a.M = int(m), a.N = int(n), a.K = int(k), a.KB = int(fp8_blocks(k));
+    a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles);
+    take_x(a, base, p, x, x_stride, x_scales, scale_stride, m, k, x_dtype, st);
+    with_dtype(y_dtype, [&](auto t) { launch_tiles<decltype(t)>(a, st); });
+    return check_launch(who);
+}
+
+extern "C" int64_t eq_fp8_grouped_matmul_scratch(int64_t x_rows, int64_t experts, int64_t routes, int64_t n, int64_t k,
+                                                 int x_dtype, int y_dtype) {
+    clear_error();
+    Plan p;
+    return plan_routes("eq_fp8_grouped_matmul", p, x_rows, experts, routes, n, k, x_dtype, y_dtype) ? int64_t(p.bytes()) : -1;
+}
+
+extern "C" int eq_fp8_grouped_matmul(void* y, const void* x, int64_t x_stride, const float* x_scales,
+                                     int64_t scale_stride, int64_t x_rows, const void* w, const float* w_scales,
+                                     int64_t experts, const int32_t* ids, const int32_t* rows, int64_t routes,
+                                     int64_t n, int64_t k, int x_dtype, int y_dtype, void* scratch,
+                                     int64_t scratch_bytes, eq_stream_t stream) {
+    clear_error();
+    const char* who = "eq_fp8_grouped_matmul";
+    Plan p;
+    if (!plan_routes(who, p, x_rows, experts, routes, n, k, x_dtype, y_dtype)) return 1;
+    if (routes == 0 || n == 0) return 0;
+    if (x_rows < 1 || (!rows && x_rows != routes)) {
+        set_error(std::string(who) + ": x must have a row, without `rows` one for each route");
+        return 1;
+    }
+    if (!ids || !aligned(ids, 4) || !aligned(rows, 4)) {
+        set_error(std::string(who) + ": ids must be given, ids and rows aligned");
+        return 1;
+    }
+    if (!operands_ok(who, y, x, x_stride, x_scales, scale_stride, w, w_scales, x_rows, k, x_dtype, y_dtype)) return 1;
+    if (x_rows * (x_dtype == EQ_DTYPE_F8E4M3 ? x_stride : k) >= int64_t(kOutOfRange)) {
+        set_error(std::string(who) + ": the codes of x must be fewer than 3 * 2^30 bytes");
+        return 1;
+    }
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    WsHold hold;
+    char* base = scratch_of(hold, who, scratch, scratch_bytes, p.bytes(), st);
+    if (!base) return 1;
+    Fp8Args a{};
+    a.y = y;
+    a.w = static_cast<const uint8_t*>(w);
+    a.ws = w_scales;
+    a.M = int(routes), a.N = int(n), a.K = int(k), a.KB = int(fp8_blocks(k));
+    a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles);
+    a.rows = rows, a.x_rows = x_rows;
+    a.tiles = reinterpret_cast<const int4*>(base);
+    a.order = reinterpret_cast<const int32_t*>(base + p.tiles);
+    take_x(a, base + p.tiles + p.order, p, x, x_stride, x_scales, scale_stride, x_rows, k, x_dtype, st);
+    fp8_routes_kernel<<<dim3(1), dim3(1024), size_t(2 * (experts + 1)) * 4u, st>>>(
+        reinterpret_cast<int4*>(base), reinterpret_cast<int32_t*>(base + p.tiles), ids, rows, int(routes), int(experts),
+        x_rows, kTileRows, a.mtiles);
+    with_dtype(y_dtype, [&](auto t) { launch_tiles<decltype(t)>(a, st); });
+    return check_launch(who);
+}

@@ -1,0 +1,272 @@
+"""Linears in 8-bit floating point with block scales, on the HIP kernels
+(``include/eredu_fp8.h``: eq_fp8_*).
+
+Stands beside the affine and MXFP4 matmuls of :mod:`eredu_amd.quantization`, in
+the place of the reference's block-FP8 projections
+(eredu/src/backend/mlx/nn/fp8.rs).  A value is an e4m3 code times a float32
+scale: weights [N, K] have a scale for each block of 128 x 128, activations one
+for each 128 columns of a row, so both operands of a product go to the matrix
+cores as they are.  An MLP over rows of 16-bit activations:
+
+    h = fp8.rms_norm(hidden, norm, eps, residual)        # Fp8Rows
+    both = fp8.matmul(h, gate_up, gate_up_scales, torch.bfloat16)
+    a = fp8.silu_mul(both[:, :F], both[:, F:])           # Fp8Rows
+    out = fp8.matmul(a, down, down_scales, torch.bfloat16)
+
+A group of 128 values v gets the scale max|v| / 448 (at least 2^-126) and codes
+448 v / max|v|, rounded once to the nearest, ties to even; a group that holds a value
+that is not finite gets the scale NaN and codes 0.  Row lengths are multiples of 16.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Tuple, Union
+
+import torch
+
+from . import _native
+from ._native import EreduError, check
+from .quantization import _DTYPE_CODE, _get_device, _stream
+
+BLOCK = 128  # columns of a scale, and rows of a weight's
+CODE_DTYPE = torch.float8_e4m3fn
+
+# Whether the current stream is being captured (a method of torch.cuda without its wrapper).
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
+class Fp8Rows(NamedTuple):
+    """Rows in codes: ``codes`` [..., K] float8_e4m3fn and ``scales`` [...,
+    ceil(K / 128)] float32, value = code * scale of its 128 columns.  The scales
+    of a block lie side by side for all rows (the last axis has the larger stride)."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        wide = self.scales.repeat_interleave(BLOCK, -1)[..., :self.codes.shape[-1]]
+        return (self.codes.float() * wide).to(dtype)
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _here(*tensors: Optional[torch.Tensor]) -> int:
+    """The current stream, once every tensor lives on the current device."""
+    index = _get_device() if _get_device is not None else torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise EreduError(f"all arrays must live on the current device, cuda:{index}: got one on {t.device}")
+    return _stream()
+
+
+def _float_code(t: torch.Tensor, what: str) -> int:
+    code = _DTYPE_CODE.get(t.dtype)
+    if code is None:
+        raise EreduError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
+    """t [..., K] as rows [M, K] whose values are contiguous, at any stride of a
+    multiple of 16 bytes, as slices of a fused projection are.  Any other layout is copied."""
+    if t.dim() == 0:
+        raise EreduError(f"{what} must have at least one dimension")
+    K = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(-1, K) if K else t.reshape(t.numel(), 0)
+    if t.is_contiguous():
+        # (a single row is contiguous at any stride)
+        t = t if t.stride(0) == K or t.shape[0] != 1 else t.as_strided(t.shape, (K, 1))
+    elif t.stride(1) != 1 or t.stride(0) < K or t.stride(0) >= 1 << 23 or t.stride(0) * t.element_size() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _new_rows(shape, K: int, device) -> Tuple[torch.Tensor, torch.Tensor, int]:
+    """Codes [rows, K] and scales [rows, blocks], the scales of a block side by side."""
+    rows = 1
+    for d in shape[:-1]:
+        rows *= d
+    codes = torch.empty(shape, dtype=CODE_DTYPE, device=device)
+    return codes, torch.empty_strided((rows, _blocks(K)), (1, max(rows, 1)), dtype=torch.float32, device=device), rows
+
+
+def _out(codes: torch.Tensor, scales: torch.Tensor) -> Fp8Rows:
+    return Fp8Rows(codes, scales if codes.dim() == 2 else scales.unflatten(0, codes.shape[:-1]) if codes.dim() > 2 else scales[0])
+
+
+def quantize(x: torch.Tensor) -> Fp8Rows:
+    """Codes and scales of x [..., K] (C ABI: eq_fp8_quantize)."""
+    code = _float_code(x, "x")
+    st = _here(x)
+    x2 = _rows(x, "x")
+    K = x2.shape[1]
+    codes, scales, rows = _new_rows(x.shape, K, x.device)
+    check(_native.lib().eq_fp8_quantize(codes.data_ptr(), scales.data_ptr(), max(rows, 1), x2.data_ptr(), x2.stride(0), rows, K,
+                                        code, st))
+    return _out(codes, scales)
+
+
+def quantize_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes float8_e4m3fn, scales float32) of weights w [..., N, K]: a scale
+    for each block of 128 x 128 (C ABI: eq_fp8_quantize_weight)."""
+    code = _float_code(w, "w")
+    if w.dim() < 2:
+        raise EreduError("w must be [..., N, K]")
+    st = _here(w)
+    w = w.contiguous()
+    if w.data_ptr() % 16:
+        w = w.clone()
+    N, K = w.shape[-2:]
+    count = 1
+    for d in w.shape[:-2]:
+        count *= d
+    codes = torch.empty(w.shape, dtype=CODE_DTYPE, device=w.device)
+    scales = torch.empty((*w.shape[:-2], _blocks(N), _blocks(K)), dtype=torch.float32, device=w.device)
+    check(_native.lib().eq_fp8_quantize_weight(codes.data_ptr(), scales.data_ptr(), w.data_ptr(), count, N, K, code, st))
+    return codes, scales
+
+
+def rms_norm(hidden: torch.Tensor, weight: torch.Tensor, eps: float, residual: Optional[torch.Tensor] = None) -> Fp8Rows:
+    """``hidden += residual`` (in place, when given), then RMSNorm(hidden) *
+    weight in codes (C ABI: eq_fp8_rms_norm): ``decode.rms_norm`` for what a
+    projection in codes reads next, of any of the three float types."""
+    code = _float_code(hidden, "hidden")
+    K = hidden.shape[-1]
+    if tuple(weight.shape) != (K,) or weight.dtype != hidden.dtype or not weight.is_contiguous():
+        raise EreduError(f"weight must be a contiguous {hidden.dtype} tensor [{K}]")
+    if not hidden.is_contiguous():
+        raise EreduError("hidden must be contiguous")
+    if residual is not None:
+        if residual.shape != hidden.shape or residual.dtype != hidden.dtype:
+            raise EreduError("residual must match hidden in shape and dtype")
+        residual = residual.contiguous()
+    st = _here(hidden, weight, residual)
+    codes, scales, rows = _new_rows(hidden.shape, K, hidden.device)
+    check(_native.lib().eq_fp8_rms_norm(codes.data_ptr(), scales.data_ptr(), max(rows, 1), hidden.data_ptr(),
+                                        None if residual is None else residual.data_ptr(), weight.data_ptr(), rows, K,
+                                        eps, code, st))
+    return _out(codes, scales)
+
+
+def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> Fp8Rows:
+    """silu(gate) * up in codes, gate and up [..., F] (slices of one projection
+    will do); nothing is rounded before the codes (C ABI: eq_fp8_silu_mul)."""
+    code = _float_code(gate, "gate")
+    if gate.shape != up.shape or gate.dtype != up.dtype:
+        raise EreduError("gate and up must match in shape and dtype")
+    st = _here(gate, up)
+    g, u = _rows(gate, "gate"), _rows(up, "up")
+    K = g.shape[1]
+    codes, scales, rows = _new_rows(gate.shape, K, gate.device)
+    check(_native.lib().eq_fp8_silu_mul(codes.data_ptr(), scales.data_ptr(), max(rows, 1), g.data_ptr(), g.stride(0),
+                                        u.data_ptr(), u.stride(0), rows, K, code, st))
+    return _out(codes, scales)
+
+
+def _x_of(x: Union[Fp8Rows, torch.Tensor], K: int):
+    """(rows, scales or None, scale stride, dtype code, shape) of a product's left operand."""
+    if isinstance(x, torch.Tensor):
+        if x.dtype is CODE_DTYPE:
+            raise EreduError("rows in codes come with their scales: pass Fp8Rows(codes, scales)")
+        code, scales, stride, shape = _float_code(x, "x"), None, 0, x.shape
+        rows = _rows(x, "x")
+    else:
+        codes, scales = x
+        if codes.dtype is not CODE_DTYPE or scales.dtype is not torch.float32:
+            raise EreduError(f"codes must be float8_e4m3fn and scales float32, got {codes.dtype} and {scales.dtype}")
+        code, shape = _native.EQ_DTYPE_F8E4M3, codes.shape
+        rows = _rows(codes, "x")
+        blocks = _blocks(rows.shape[1])
+        if tuple(scales.shape) != (*shape[:-1], blocks):
+            raise EreduError(f"scales has shape {tuple(scales.shape)}, expected {(*shape[:-1], blocks)}")
+        if scales.dim() != 2:
+            scales = scales.reshape(-1, blocks)
+        M = rows.shape[0]
+        if (scales.stride(0) != 1 and M > 1) or (scales.stride(1) < M and blocks > 1):
+            scales = scales.t().contiguous().t()
+        stride = scales.stride(1) if blocks > 1 else max(M, 1)
+    if rows.shape[1] != K:
+        raise EreduError(f"x has rows of {rows.shape[1]} values, the weight of {K}")
+    return rows, scales, stride, code, shape
+
+
+def _weight(w: torch.Tensor, w_scales: torch.Tensor, dims: int) -> Tuple[int, int]:
+    if w.dim() != dims or w.dtype is not CODE_DTYPE or not w.is_contiguous():
+        raise EreduError(f"w must be a contiguous float8_e4m3fn tensor {'[N, K]' if dims == 2 else '[experts, N, K]'}")
+    N, K = w.shape[-2:]
+    expect = (*w.shape[:-2], _blocks(N), _blocks(K))
+    if tuple(w_scales.shape) != expect or w_scales.dtype is not torch.float32 or not w_scales.is_contiguous():
+        raise EreduError(f"w_scales must be a contiguous float32 tensor {expect}, got {w_scales.dtype} {tuple(w_scales.shape)}")
+    return N, K
+
+
+def _out_dtype(x, dtype: Optional[torch.dtype]) -> torch.dtype:
+    if dtype is None:
+        if not isinstance(x, torch.Tensor):
+            raise EreduError("rows in codes have no dtype of their own: say which the result has")
+        return x.dtype
+    if dtype not in _DTYPE_CODE:
+        raise EreduError(f"the result's dtype must be float32, float16 or bfloat16, got {dtype}")
+    return dtype
+
+
+def _scratch(need: int, device) -> Tuple[Optional[int], int, Optional[torch.Tensor]]:
+    """Scratch of a call from torch: a graph's own, so that graphs share nothing.
+    (Eager calls take the library's workspace of their stream.)"""
+    if need < 0:
+        check(1)
+    if need == 0:
+        return None, 0, None
+    t = torch.empty((need,), dtype=torch.uint8, device=device)
+    return t.data_ptr(), need, t
+
+
+def matmul(x: Union[Fp8Rows, torch.Tensor], w: torch.Tensor, w_scales: torch.Tensor,
+           dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x . w^T of x [..., K] and w [N, K] in codes with w_scales [ceil(N / 128),
+    ceil(K / 128)]: [..., N] in ``dtype`` (x's own where it is None).  x is
+    ``Fp8Rows``, or float rows that the call quantizes first, as ``quantize``
+    does (C ABI: eq_fp8_matmul)."""
+    N, K = _weight(w, w_scales, 2)
+    rows, scales, stride, code, shape = _x_of(x, K)
+    dtype = _out_dtype(x, dtype)
+    st = _here(rows, scales, w, w_scales)
+    M, lib, out = rows.shape[0], _native.lib(), _DTYPE_CODE[dtype]
+    y = torch.empty((M, N), dtype=dtype, device=rows.device)
+    sp, sn, hold = _scratch(lib.eq_fp8_matmul_scratch(M, N, K, code, out), rows.device) if _capturing() else (None, 0, None)
+    check(lib.eq_fp8_matmul(y.data_ptr(), rows.data_ptr(), rows.stride(0), None if scales is None else scales.data_ptr(),
+                            stride, w.data_ptr(), w_scales.data_ptr(), M, N, K, code, out, sp, sn, st))
+    return y if len(shape) == 2 else y.view(*shape[:-1], N)
+
+
+def grouped_matmul(x: Union[Fp8Rows, torch.Tensor], w: torch.Tensor, w_scales: torch.Tensor, ids: torch.Tensor,
+                   rows: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """Routed experts: y [routes, N], y[r] = x[rows[r]] . w[ids[r]]^T, with
+    x [T, K] as in ``matmul``, a bank w [experts, N, K], w_scales [experts,
+    ceil(N / 128), ceil(K / 128)], and ids and rows int32 [routes] on the device, in
+    any order (rows None: x has a row for each route).  A route whose expert or
+    row is out of range, as padded ones may have, gives zeros (C ABI:
+    eq_fp8_grouped_matmul)."""
+    N, K = _weight(w, w_scales, 3)
+    xr, scales, stride, code, shape = _x_of(x, K)
+    if len(shape) != 2:
+        raise EreduError(f"x must be [rows, {K}]")
+    dtype = _out_dtype(x, dtype)
+    st = _here(xr, scales, w, w_scales, ids, rows)
+    for t, what in ((ids, "ids"), (rows, "rows")):
+        if t is not None and (t.dtype is not torch.int32 or t.dim() != 1 or t.shape != ids.shape):
+            raise EreduError(f"{what} must be a one-dimensional int32 tensor, rows as long as ids")
+    ids = ids.contiguous()
+    rows = None if rows is None else rows.contiguous()
+    R, T, E = ids.shape[0], xr.shape[0], w.shape[0]
+    lib, out = _native.lib(), _DTYPE_CODE[dtype]
+    y = torch.empty((R, N), dtype=dtype, device=xr.device)
+    sp, sn, hold = (_scratch(lib.eq_fp8_grouped_matmul_scratch(T, E, R, N, K, code, out), xr.device) if _capturing()
+                    else (None, 0, None))
+    check(lib.eq_fp8_grouped_matmul(y.data_ptr(), xr.data_ptr(), xr.stride(0),
+                                    None if scales is None else scales.data_ptr(), stride, T, w.data_ptr(),
+                                    w_scales.data_ptr(), E, ids.data_ptr(), None if rows is None else rows.data_ptr(), R, N,
+                                    K, code, out, sp, sn, st))
+    return y
