@@ -20,96 +20,16 @@
 // sums that are off by f32's rounding alone (of 128 products 7e-8 where the e4m3 ones are off by 5e-5).
 #include <algorithm>
 
-#include "fp8_common.hpp"
+#include "fp8_product.hpp"
 
 namespace eq {
 namespace {
 
 constexpr int kMostExperts = 4095;  // (two counters each in 64 KiB of LDS with room to spare)
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
 typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) const float lds_f32;
-
-struct Fp8Args {
-    void* y;
-    const uint8_t* x;
-    const float* xs;
-    int64_t x_stride, xs_stride;
-    const uint8_t* w;
-    const float* ws;
-    int M, N, K, KB;  // KB: blocks of K
-    int mtiles, ntiles;
-    // Grouped: tiles[i] = {expert, first, rows} of row tile i, the rows being
-    // routes order[first ..]; tiles[mtiles].x: how many there are.  Expert -1: rows of zeros.
-    const int4* tiles;
-    const int32_t* order;
-    const int32_t* rows;
-    int64_t x_rows;
-};
-
-__device__ __forceinline__ f32x4 mfma128(u32x4 a0, u32x4 a1, u32x4 b0, u32x4 b1) {
-    const i32x8 a = __builtin_bit_cast(i32x8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
-    const i32x8 b = __builtin_bit_cast(i32x8, __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7));
-    // formats 0, 0: e4m3; scales 0: the form without scales
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f32x4{}, 0, 0, 0, 0, 0, 0);
-}
-
-// Eight codes as bf16.
-__device__ __forceinline__ bf16x8 codes_bf16(uint32_t lo, uint32_t hi) {
-    const u32x4 v = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false)),
-                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true)),
-                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false)),
-                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true))};
-    return __builtin_bit_cast(bf16x8, v);
-}
-
-// A lane's 32 codes of a row and block, as the matrix instruction takes them.
-template <bool EXACT>
-struct Operand;
-template <>
-struct Operand<false> {
-    u32x4 c[2];
-    __device__ __forceinline__ void take(u32x4 a, u32x4 b) { c[0] = a, c[1] = b; }
-};
-template <>
-struct Operand<true> {
-    bf16x8 c[4];
-    __device__ __forceinline__ void take(u32x4 a, u32x4 b) {
-        c[0] = codes_bf16(a[0], a[1]), c[1] = codes_bf16(a[2], a[3]);
-        c[2] = codes_bf16(b[0], b[1]), c[3] = codes_bf16(b[2], b[3]);
-    }
-};
-__device__ __forceinline__ f32x4 block_sums(const Operand<false>& a, const Operand<false>& b) {
-    return mfma128(a.c[0], a.c[1], b.c[0], b.c[1]);
-}
-__device__ __forceinline__ f32x4 block_sums(const Operand<true>& a, const Operand<true>& b) {
-    f32x4 d{};
-#pragma unroll
-    for (int i = 0; i < 4; i++) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.c[i], b.c[i], d, 0, 0, 0);
-    return d;
-}
-
-// VALS consecutive results of a row, n of them inside it; whole: 16-byte stores will do.
-template <typename YT, int VALS>
-__device__ __forceinline__ void store_run(typename YT::storage* p, const float* v, int n, bool whole) {
-    constexpr int VEC = 16 / int(sizeof(typename YT::storage));
-#pragma unroll
-    for (int i = 0; i < VALS; i += VEC) {
-        if (whole) {
-            if (i < n) {
-                if constexpr (VEC == 8) store8<YT>(p + i, v + i);
-                else *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; e++)
-                if (i + e < n) store_out<YT>(p, i + e, v[i + e]);
-        }
-    }
-}
 
 // WN x WM waves of NT x MT tiles of 16 x 16: 16 NT WN weight rows by 16 MT WM
 // activation rows a workgroup.  Both operands go straight from memory to LDS,
@@ -352,6 +272,7 @@ size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 // How a product is done, from its sizes and types alone (the scratch queries
 // and the calls go by the same), and its scratch: lists of routes, the codes and scales of x.
 struct Plan {
+    bool few = false;  // fp8_few.hip's kernel, on x as it is where that takes it
     int64_t mtiles, ntiles;
     size_t tiles = 0, order = 0, codes = 0, scales = 0;
     size_t bytes() const { return tiles + order + codes + scales; }
@@ -384,7 +305,7 @@ bool dtypes_ok(const char* who, int x_dtype, int y_dtype) {
 
 bool grid_ok(const char* who, const Plan& p) {
     if (p.mtiles * p.ntiles < (int64_t(1) << 23)) return true;  // (fewer than 2^32 threads)
-    set_error(std::string(who) + ": 2^23 tiles of 128 x 128 or more");
+    set_error(std::string(who) + ": 2^23 tiles of the result or more");
     return false;
 }
 
@@ -392,7 +313,9 @@ bool plan_product(const char* who, Plan& p, int64_t m, int64_t n, int64_t k, int
     if (!sizes_ok(who, m, n, k) || !dtypes_ok(who, x_dtype, y_dtype)) return false;
     p.mtiles = (m + kTileRows - 1) / kTileRows;
     p.ntiles = (n + kTileCols - 1) / kTileCols;
-    if (x_dtype != EQ_DTYPE_F8E4M3) {
+    p.few = m <= 16;
+    if (p.few) p.mtiles = 1, p.ntiles = (n + 15) / 16;
+    if (x_dtype != EQ_DTYPE_F8E4M3 && !(p.few && fp8_few_takes(m, k, x_dtype))) {
         p.codes = round256(size_t(m) * size_t(k));
         p.scales = round256(size_t(m) * size_t(fp8_blocks(k)) * 4u);
     }
@@ -406,15 +329,21 @@ bool plan_routes(const char* who, Plan& p, int64_t x_rows, int64_t experts, int6
         set_error(std::string(who) + ": experts must be in [1, " + std::to_string(kMostExperts) + "]");
         return false;
     }
+    p.few = routes <= 64;
+    const bool plain = x_dtype == EQ_DTYPE_F8E4M3 || (p.few && fp8_few_takes(1, k, x_dtype));
+    if (!plain) {
+        p.codes = round256(size_t(x_rows) * size_t(k));
+        p.scales = round256(size_t(x_rows) * size_t(fp8_blocks(k)) * 4u);
+    }
+    if (p.few) {
+        p.mtiles = routes, p.ntiles = (n + 15) / 16;
+        return grid_ok(who, p);
+    }
     // (a part tile for each expert that has one, and for the routes without)
     p.mtiles = std::min(routes, routes / kTileRows + experts + 1);
     p.ntiles = (n + kTileCols - 1) / kTileCols;
     p.tiles = round256(size_t(p.mtiles + 1) * sizeof(int4));
     p.order = round256(size_t(routes) * 4u);
-    if (x_dtype != EQ_DTYPE_F8E4M3) {
-        p.codes = round256(size_t(x_rows) * size_t(k));
-        p.scales = round256(size_t(x_rows) * size_t(fp8_blocks(k)) * 4u);
-    }
     return grid_ok(who, p);
 }
 
@@ -452,16 +381,17 @@ char* scratch_of(WsHold& hold, const char* who, void* scratch, int64_t scratch_b
     return p;
 }
 
-// x of a call, quantized into scratch first where it is not in codes.
-void take_x(Fp8Args& a, char* scratch, const Plan& p, const void* x, int64_t x_stride, const float* x_scales,
-            int64_t scale_stride, int64_t rows, int64_t k, int x_dtype, hipStream_t st) {
-    if (x_dtype == EQ_DTYPE_F8E4M3) {
+// x of a call: as it is, or quantized into scratch first where the plan says so; what its type is then.
+int take_x(Fp8Args& a, char* scratch, const Plan& p, const void* x, int64_t x_stride, const float* x_scales,
+           int64_t scale_stride, int64_t rows, int64_t k, int x_dtype, hipStream_t st) {
+    if (!p.codes) {
         a.x = static_cast<const uint8_t*>(x), a.xs = x_scales, a.x_stride = x_stride, a.xs_stride = scale_stride;
-        return;
+        return x_dtype;
     }
     float* scales = reinterpret_cast<float*>(scratch + p.codes);
     launch_fp8_quantize(scratch, scales, rows, x, x_stride, rows, k, x_dtype, st);
     a.x = reinterpret_cast<const uint8_t*>(scratch), a.xs = scales, a.x_stride = k, a.xs_stride = rows;
+    return EQ_DTYPE_F8E4M3;
 }
 
 }  // namespace
@@ -494,7 +424,11 @@ extern "C" int eq_fp8_matmul(void* y, const void* x, int64_t x_stride, const flo
     a.ws = w_scales;
     a.M = int(m), a.N = int(n), a.K = int(k), a.KB = int(fp8_blocks(k));
     a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles);
-    take_x(a, base, p, x, x_stride, x_scales, scale_stride, m, k, x_dtype, st);
+    x_dtype = take_x(a, base, p, x, x_stride, x_scales, scale_stride, m, k, x_dtype, st);
+    if (p.few) {
+        launch_fp8_few(a, Fp8Few{x, x_dtype, nullptr, 1}, y_dtype, st);
+        return check_launch(who);
+    }
     with_dtype(y_dtype, [&](auto t) { launch_tiles<decltype(t)>(a, st); });
     return check_launch(who);
 }
@@ -531,8 +465,8 @@ extern "C" int eq_fp8_grouped_matmul(void* y, const void* x, int64_t x_stride, c
     }
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     WsHold hold;
-    char* base = scratch_of(hold, who, scratch, scratch_bytes, p.bytes(), st);
-    if (!base) return 1;
+    char* base = nullptr;
+    if (p.bytes() && !(base = scratch_of(hold, who, scratch, scratch_bytes, p.bytes(), st))) return 1;
     Fp8Args a{};
     a.y = y;
     a.w = static_cast<const uint8_t*>(w);
@@ -540,9 +474,13 @@ extern "C" int eq_fp8_grouped_matmul(void* y, const void* x, int64_t x_stride, c
     a.M = int(routes), a.N = int(n), a.K = int(k), a.KB = int(fp8_blocks(k));
     a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles);
     a.rows = rows, a.x_rows = x_rows;
+    x_dtype = take_x(a, base + p.tiles + p.order, p, x, x_stride, x_scales, scale_stride, x_rows, k, x_dtype, st);
+    if (p.few) {
+        launch_fp8_few(a, Fp8Few{x, x_dtype, ids, int(experts)}, y_dtype, st);
+        return check_launch(who);
+    }
     a.tiles = reinterpret_cast<const int4*>(base);
     a.order = reinterpret_cast<const int32_t*>(base + p.tiles);
-    take_x(a, base + p.tiles + p.order, p, x, x_stride, x_scales, scale_stride, x_rows, k, x_dtype, st);
     fp8_routes_kernel<<<dim3(1), dim3(1024), size_t(2 * (experts + 1)) * 4u, st>>>(
         reinterpret_cast<int4*>(base), reinterpret_cast<int32_t*>(base + p.tiles), ids, rows, int(routes), int(experts),
         x_rows, kTileRows, a.mtiles);

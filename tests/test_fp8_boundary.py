@@ -122,7 +122,7 @@ def test_matmul_refuses(bad, words):
     (dict(e=0), "experts"), (dict(e=4096), "experts"), (dict(ids=None), "ids"), (dict(ids=P + 2), "ids"), (dict(rows=P + 1), "ids"),
     (dict(xr=0), "x must have"), (dict(rows=None, r=5), "without `rows`"), (dict(r=-1), "2^30"), (dict(xr=-1), "2^30"),
     (dict(xr=1 << 26), "2^26"), (dict(r=1 << 26), "2^26"), (dict(xr=1 << 20, ss=1 << 20, xs=4096), "3 * 2^30"),
-    (dict(sp=P + 16, sn=1 << 30), "scratch"), (dict(sp=P, sn=16), "scratch")])
+    (dict(sp=P + 16, sn=1 << 30, r=1000), "scratch"), (dict(sp=P, sn=16, r=1000), "scratch")])
 def test_grouped_matmul_refuses(bad, words):
     refused(grouped(**bad), words)
 
