@@ -87,7 +87,10 @@ __device__ __forceinline__ void store8(typename T::storage* p, const float* v) {
     } else {
         uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = uint32_t(to_storage<T>(v[2 * i])) | uint32_t(to_storage<T>(v[2 * i + 1])) << 16;
+        for (int i = 0; i < 4; i++) {
+            if constexpr (std::is_same<T, BF16T>::value) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+            else w[i] = uint32_t(to_storage<T>(v[2 * i])) | uint32_t(to_storage<T>(v[2 * i + 1])) << 16;
+        }
         *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }

@@ -1,29 +1,41 @@
 // Products of few rows (at most 16, or one for each route) with e4m3 weights:
 // bound by reading the weights once.
 //
-// A workgroup of 8 waves has 16 weight rows; wave v takes the blocks v, v + 8,
-// .. of K, a block being one matrix instruction (fp8_matmul.hip).  A lane reads
-// two pieces of 16 bytes of its weight row straight into the operand's
-// registers, four blocks ahead of their use; the waves' sums are added through LDS in wave order.
-// Rows of values are quantized by the workgroup into LDS while its first weights are on their way.
+// A workgroup of 8 waves has 16 NT weight rows; wave v takes the blocks v, v + 8,
+// .. of K, a block being one matrix instruction a tile (fp8_matmul.hip), and the
+// waves' sums are added through LDS in wave order.  Each wave brings its blocks
+// into a ring of its own in LDS, AHEAD blocks before it needs them, and waits for
+// none of the others.  (Straight into the operand's registers a load touches half a line of
+// 16 rows, and the 64 KiB of a compute unit took 1.7 us of its address unit's time, here 0.6.)
+// Rows of values (at most 4) are quantized by the workgroup into LDS while its first weights are on their way.
 #include "fp8_product.hpp"
 
 namespace eq {
 namespace {
 
-constexpr int kFewWaves = 8, kFewAhead = 4;
-constexpr int kFewLds = 48 * 1024;  // codes of the rows, where the kernel makes them
+constexpr int kFewWaves = 8;
+constexpr int kFewLds = 48 * 1024;  // codes and scales of the rows, where the kernel makes them
+
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) const float lds_f32;
 
 struct F8T {};  // x in codes
 
-template <typename XT, typename YT>
+// ROWS8: loads of 8 rows of x (0: the kernel quantizes them).
+template <typename XT, typename YT, int NT, int ROWS8, int AHEAD>
 __global__ __launch_bounds__(64 * kFewWaves) void fp8_few_kernel(const Fp8Args args, const Fp8Few few) {
     constexpr bool CODED = std::is_same<XT, F8T>::value, EXACT = std::is_same<YT, F32T>::value;
-    extern __shared__ __attribute__((aligned(16))) char shared[];  // codes [rows][128 KB], scales [rows][KB]
-    __shared__ float sums[kFewWaves][16][17];
+    static_assert(CODED == (ROWS8 > 0), "rows in codes are loaded");
+    constexpr int A_BYTES = NT * 2048, B_BYTES = ROWS8 * 1024, SLOT = A_BYTES + B_BYTES + (CODED ? 256 : 0);
+    constexpr int LOADS = 2 * NT + ROWS8 + (CODED ? 1 : 0), RING = AHEAD + 1;
+    constexpr int SUMS = kFewWaves * NT * 16 * 17 * 4, BYTES = kFewWaves * RING * SLOT;
+    __shared__ __attribute__((aligned(16))) char ring[BYTES > SUMS ? BYTES : SUMS];  // and the sums, afterwards
+    extern __shared__ __attribute__((aligned(16))) char coded[];                      // codes [rows][128 KB], scales [rows][KB]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
     const int l16 = lane & 15, quad = lane >> 4;
-    const int N = args.N, K = args.K, KB = args.KB, n0 = blockIdx.x * 16;
+    const int N = args.N, K = args.K, KB = args.KB, n0 = blockIdx.x * 16 * NT;
     typename YT::storage* y = static_cast<typename YT::storage*>(args.y);
 
     // The rows of this workgroup: all of them, or route blockIdx.y's.
@@ -36,63 +48,54 @@ __global__ __launch_bounds__(64 * kFewWaves) void fp8_few_kernel(const Fp8Args a
         x_row = args.rows ? args.rows[r] : r;
         y += int64_t(r) * N;
         if (uint32_t(expert) >= uint32_t(few.experts) || x_row < 0 || x_row >= args.x_rows) {  // (the whole workgroup)
-            if (int(threadIdx.x) < 16 && n0 + int(threadIdx.x) < N) store_out<YT>(y, n0 + threadIdx.x, 0.f);
+            if (int(threadIdx.x) < 16 * NT && n0 + int(threadIdx.x) < N) store_out<YT>(y, n0 + threadIdx.x, 0.f);
             return;
         }
     }
     const int nblocks = (N + 127) / 128;
-    const float* const wsp = args.ws + (int64_t(expert) * nblocks + n0 / 128) * KB;
-    const int nrows = min(16, N - n0);
-    const __amdgpu_buffer_rsrc_t wr =
-        raw_rsrc(args.w + (int64_t(expert) * N + n0) * K, uint32_t(nrows) * uint32_t(K));
-    const uint32_t a_off = l16 < nrows ? uint32_t(l16) * uint32_t(K) + 16u * quad : kOutOfRange;
+    typedef __attribute__((address_space(4))) const float const_f32;
+    const_f32* const wsp = (const_f32*)(args.ws + (int64_t(expert) * nblocks + n0 / 128) * KB);
+    const int nrows = min(16 * NT, N - n0);
+    const __amdgpu_buffer_rsrc_t wr = raw_rsrc(args.w + (int64_t(expert) * N + n0) * K, uint32_t(nrows) * uint32_t(K));
     const uint8_t* const xp = CODED ? args.x + x_row * args.x_stride : nullptr;
     const float* const xsp = CODED ? args.xs + x_row : nullptr;
     const __amdgpu_buffer_rsrc_t xr = raw_rsrc(xp, CODED ? uint32_t(M - 1) * uint32_t(args.x_stride) + uint32_t(K) : 0u);
-    const uint32_t b_off = l16 < M ? uint32_t(l16) * uint32_t(args.x_stride) + 16u * quad : kOutOfRange;
-    float* const lds_scales = reinterpret_cast<float*>(shared + M * KB * 128);
 
-    struct Block {
-        u32x4 a[2], b[2];
-        float sx, sw;
-    };
-    auto load = [&](Block& s, int kb) __attribute__((always_inline)) {
+    // Load i of the weights is rows 8 i ..: lane l has row l / 8 of them and the chunk that belongs in slot l % 8,
+    // c ^ (row / 2) % 8, so that 16 rows are read at one chunk without bank conflicts.
+    const int row8 = lane >> 3;
+    uint32_t a_off[8], b_off[2];  // (the first 2 NT and ROWS8 used; bounds that depend on NT fail clang's host pass in a lambda)
+    int chunk[2];                      // of even and odd loads
+#pragma unroll
+    for (int i = 0; i < 2; i++) chunk[i] = (lane & 7) ^ ((4 * i + (row8 >> 1)) & 7);
+#pragma unroll
+    for (int i = 0; i < 2 * NT; i++)
+        a_off[i] = 8 * i + row8 < nrows ? uint32_t(8 * i + row8) * uint32_t(K) + 16u * chunk[i & 1] : kOutOfRange;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        b_off[i] = 8 * i + row8 < M ? uint32_t(8 * i + row8) * uint32_t(args.x_stride) + 16u * chunk[i] : kOutOfRange;
+    lds_char* const mine = (lds_char*)ring + wave * RING * SLOT;
+    auto load = [&](int kb, int slot) __attribute__((always_inline)) {
         const uint32_t k = uint32_t(kb) * 128u;
-        const int left = K - int(k);  // pieces past K, and blocks past the last, are zeros
+        const int left = K - int(k);  // chunks past K, and blocks past the last, are zeros
+        lds_char* const to = mine + slot * SLOT;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const bool live = 16 * (quad + 4 * h) < left;
-            s.a[h] = __builtin_amdgcn_raw_buffer_load_b128(wr, live ? a_off + 64u * h : kOutOfRange, k, 2);
-            if constexpr (CODED) s.b[h] = __builtin_amdgcn_raw_buffer_load_b128(xr, live ? b_off + 64u * h : kOutOfRange, k, 0);
+        for (int i = 0; i < 2 * NT; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void*)(to + i * 1024), 16,
+                                                     16 * chunk[i & 1] < left ? a_off[i] : kOutOfRange, k, 0, 0);
+        if constexpr (CODED) {
+#pragma unroll
+            for (int i = 0; i < ROWS8; i++)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_void*)(to + A_BYTES + i * 1024), 16,
+                                                         16 * chunk[i] < left ? b_off[i] : kOutOfRange, k, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(raw_rsrc(xsp + int64_t(min(kb, KB - 1)) * args.xs_stride, uint32_t(M) * 4u),
+                                                     (lds_void*)(to + A_BYTES + B_BYTES), 4,
+                                                     lane < M ? uint32_t(lane) * 4u : kOutOfRange, 0, 0, 0);
         }
-        const int at = min(kb, KB - 1);
-        s.sw = wsp[at];
-        if constexpr (CODED) s.sx = l16 < M ? xsp[int64_t(at) * args.xs_stride + l16] : 0.f;
     };
-    f32x4 acc{};
-    auto add = [&](Block& s, int kb) __attribute__((always_inline)) {
-        if constexpr (!CODED) {
-            s.b[0] = s.b[1] = u32x4{};
-            s.sx = 0.f;
-            if (l16 < M) {
-                const char* const row = shared + (l16 * KB + kb) * 128 + 16 * quad;
-                s.b[0] = *reinterpret_cast<const u32x4*>(row);
-                s.b[1] = *reinterpret_cast<const u32x4*>(row + 64);
-                s.sx = lds_scales[l16 * KB + kb];
-            }
-        }
-        Operand<EXACT> a, b;
-        a.take(s.a[0], s.a[1]);
-        b.take(s.b[0], s.b[1]);
-        const f32x4 p = block_sums(a, b);
-        const float scale = s.sx * s.sw;
 #pragma unroll
-        for (int r = 0; r < 4; r++) acc[r] = fmaf(scale, p[r], acc[r]);
-    };
-
-    Block s[kFewAhead];
-#pragma unroll
-    for (int i = 0; i < kFewAhead; i++) load(s[i], wave + kFewWaves * i);
+    for (int i = 0; i < AHEAD; i++) load(wave + kFewWaves * i, i);
+    lds_f32* const lds_scales = (lds_f32*)((lds_char*)coded + M * KB * 128);
     if constexpr (!CODED) {
         // 16 lanes a group of 128 values, eight each; what lies past K is a code of 0
         using S = typename XT::storage;
@@ -106,29 +109,70 @@ __global__ __launch_bounds__(64 * kFewWaves) void fp8_few_kernel(const Fp8Args a
 #pragma unroll
             for (int i = 0; i < 8; i++) most = max(most, abs_bits(v[i]));
             const Fp8Group q(max16(most));
-            *reinterpret_cast<uint2*>(shared + g * 128 + l16 * 8) = make_uint2(q.codes4(v), q.codes4(v + 4));
-            if (l16 == 0) lds_scales[g] = q.scale;
+            *reinterpret_cast<uint2*>(coded + g * 128 + l16 * 8) = make_uint2(q.codes4(v), q.codes4(v + 4));
+            if (l16 == 0) *reinterpret_cast<float*>(coded + M * KB * 128 + g * 4) = q.scale;
         }
         lds_barrier();
     }
-    for (int kb = wave; kb < KB; kb += kFewWaves * kFewAhead) {
-#pragma unroll
-        for (int i = 0; i < kFewAhead; i++) {
-            const int at = kb + kFewWaves * i;
-            if (at < KB) {
-                add(s[i], at);
-                load(s[i], at + kFewWaves * kFewAhead);
+
+    f32x4 acc[NT] = {};
+    const uint32_t at0 = uint32_t(l16 * 128 + ((quad ^ ((l16 >> 1) & 7)) << 4));  // chunks quad and quad + 4 of row l16
+    int slot = 0;
+#pragma unroll 1
+    for (int kb = wave; kb < KB; kb += kFewWaves) {
+        const float sw = wsp[kb];
+        load(kb + kFewWaves * AHEAD, slot == 0 ? AHEAD : slot - 1);
+        // this block has landed, the AHEAD after it may be on their way
+        constexpr int LATER = LOADS * AHEAD;
+        static_assert(LATER < 64, "vmcnt range");
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LATER) : "memory");
+        const lds_char* const from = mine + slot * SLOT;
+        Operand<EXACT> a, b;
+        float sx;
+        if constexpr (CODED) {
+            const lds_char* const row = from + A_BYTES;
+            const u32x4 zero{};
+            // (rows behind the loaded ones of x are zeros)
+            const bool live = ROWS8 == 2 || l16 < 8;
+            const uint32_t at = ROWS8 == 2 ? at0 : at0 & 1023u;
+            const u32x4 lo = *(lds_u32x4*)(row + at), hi = *(lds_u32x4*)(row + (at ^ 64u));
+            b.take(live ? lo : zero, live ? hi : zero);
+            sx = *(lds_f32*)(from + A_BYTES + B_BYTES + l16 * 4);
+        } else {
+            u32x4 lo{}, hi{};
+            sx = 0.f;
+            if (l16 < M) {
+                const lds_char* const row = (lds_char*)coded + (l16 * KB + kb) * 128 + 16 * quad;
+                lo = *(lds_u32x4*)row, hi = *(lds_u32x4*)(row + 64);
+                sx = lds_scales[l16 * KB + kb];
             }
+            b.take(lo, hi);
         }
+        const float scale = sx * sw;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            a.take(*(lds_u32x4*)(from + t * 2048 + at0), *(lds_u32x4*)(from + t * 2048 + (at0 ^ 64u)));
+            const f32x4 p = block_sums(a, b);
+#pragma unroll
+            for (int r = 0; r < 4; r++) acc[t][r] = fmaf(scale, p[r], acc[t][r]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read, before the slot is loaded again)
+        slot = slot == AHEAD ? 0 : slot + 1;
     }
+    // Nothing is on its way into the ring when the sums take its place.
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    float* const sums = reinterpret_cast<float*>(ring);  // [wave][tile][row of x][17]
 #pragma unroll
-    for (int r = 0; r < 4; r++) sums[wave][l16][4 * quad + r] = acc[r];
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) sums[((wave * NT + t) * 16 + l16) * 17 + 4 * quad + r] = acc[t][r];
     __syncthreads();
-    const int m = threadIdx.x >> 4, n = n0 + l16;
-    if (m < min(M, 16) && n < N) {
-        float t = sums[0][m][l16];
+    for (int i = threadIdx.x; i < M * NT * 16; i += 64 * kFewWaves) {
+        const int m = i / (NT * 16), c = i % (NT * 16), n = n0 + c;
+        if (n >= N) continue;
+        float t = 0.f;
 #pragma unroll
-        for (int i = 1; i < kFewWaves; i++) t += sums[i][m][l16];
+        for (int w = 0; w < kFewWaves; w++) t += sums[((w * NT + (c >> 4)) * 16 + m) * 17 + (c & 15)];
         store_out<YT>(y, int64_t(m) * N + n, t);
     }
 }
@@ -140,20 +184,27 @@ bool fp8_few_takes(int64_t m, int64_t k, int x_dtype) {
     return m <= 4 && m * fp8_blocks(k) * 132 <= kFewLds;
 }
 
-void launch_fp8_few(const Fp8Args& a, const Fp8Few& f, int y_dtype, hipStream_t st) {
-    const dim3 grid(unsigned((a.N + 15) / 16), f.ids ? unsigned(a.M) : 1u);
-    const bool coded = f.x_dtype == EQ_DTYPE_F8E4M3;
-    const size_t lds = coded ? 0 : size_t(f.ids ? 1 : a.M) * size_t(a.KB) * 132;
+template <int NT>
+static void launch_few(const Fp8Args& a, const Fp8Few& f, int y_dtype, hipStream_t st) {
+    const dim3 grid(unsigned((a.N + 16 * NT - 1) / (16 * NT)), f.ids ? unsigned(a.M) : 1u), block(64 * kFewWaves);
+    const int m = f.ids ? 1 : a.M;
     with_dtype(y_dtype, [&](auto yt) {
         using YT = decltype(yt);
-        if (coded) {
-            fp8_few_kernel<F8T, YT><<<grid, dim3(64 * kFewWaves), 0, st>>>(a, f);
+        if (f.x_dtype == EQ_DTYPE_F8E4M3) {
+            if (m <= 8) fp8_few_kernel<F8T, YT, NT, 1, NT == 1 ? 3 : 2><<<grid, block, 0, st>>>(a, f);
+            else fp8_few_kernel<F8T, YT, NT, 2, NT == 1 ? 3 : 2><<<grid, block, 0, st>>>(a, f);
         } else {
             with_dtype(f.x_dtype, [&](auto xt) {
-                fp8_few_kernel<decltype(xt), YT><<<grid, dim3(64 * kFewWaves), lds, st>>>(a, f);
+                fp8_few_kernel<decltype(xt), YT, NT, 0, NT == 1 ? 3 : 2>
+                    <<<grid, block, size_t(m) * size_t(a.KB) * 132, st>>>(a, f);
             });
         }
     });
+}
+
+void launch_fp8_few(const Fp8Args& a, const Fp8Few& f, int y_dtype, hipStream_t st) {
+    if (a.N > 8192) launch_few<2>(a, f, y_dtype, st);
+    else launch_few<1>(a, f, y_dtype, st);
 }
 
 }  // namespace eq

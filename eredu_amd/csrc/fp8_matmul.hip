@@ -33,7 +33,7 @@ typedef __attribute__((address_space(3))) const float lds_f32;
 
 // WN x WM waves of NT x MT tiles of 16 x 16: 16 NT WN weight rows by 16 MT WM
 // activation rows a workgroup.  Both operands go straight from memory to LDS,
-// two blocks of K deep.
+// STAGES blocks of K deep.
 //
 // Row i of a wave's A tile t is its weight row 4 NT (i / 4) + 4 t + i % 4, so that
 // a lane ends with 4 NT consecutive results of its activation row.  A row's 128
@@ -41,28 +41,44 @@ typedef __attribute__((address_space(3))) const float lds_f32;
 // 16 rows at one chunk, LDS has 64 banks of 4 bytes (two rows), so the
 // rows of one parity have to differ in their key: (row / 2) % 8 for the
 // activations, (row / 2) % 2 + 2 (row / (4 NT) % 4) for the weights' rows above.
-template <typename YT, int WN, int WM, int NT, int MT>
+template <typename YT, int WN, int WM, int NT, int MT, int STAGES>
 __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_tile_kernel(
     const Fp8Args args) {
     constexpr int WAVES = WN * WM, TN = 16 * NT * WN, TM = 16 * MT * WM;
     constexpr int LA = TN / 8 / WAVES, LB = TM / 8 / WAVES;  // loads of 1 KiB (8 rows) a wave
-    static_assert(LA * 8 * WAVES == TN && LB * 8 * WAVES == TM && TN % 128 == 0, "whole loads");
+    constexpr int LOADS = LA + LB + 1;                        // and one of scales
+    static_assert(LA * 8 * WAVES == TN && LB * 8 * WAVES == TM && LA <= 8 && LB <= 8, "whole loads");
+    static_assert(128 % (16 * NT) == 0, "a wave's weight rows have one scale");
     constexpr int SROWS = TM < 64 ? 64 : TM, BUF = (TN + TM) * 128 + SROWS * 4;
     static_assert(64 * WAVES >= SROWS, "a scale load a wave");
+    static_assert(STAGES >= 2 && STAGES <= 4, "buffers");
     constexpr bool EXACT = std::is_same<YT, F32T>::value;
-    // (separate arrays, so that the compiler knows that a read of one does not wait for loads into the other)
-    __shared__ __attribute__((aligned(16))) char buf0[BUF], buf1[BUF];
+    // (separate arrays, so that the compiler knows that a read of one does not wait for loads into another)
+    __shared__ __attribute__((aligned(16))) char buf0[BUF], buf1[BUF], buf2[STAGES > 2 ? BUF : 16],
+        buf3[STAGES > 3 ? BUF : 16];
+    auto buf = [&](int i) __attribute__((always_inline)) {
+        return i == 0 ? (lds_char*)buf0 : i == 1 ? (lds_char*)buf1 : i == 2 ? (lds_char*)buf2 : (lds_char*)buf3;
+    };
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
     const int wn = wave % WN, wm = wave / WN, l16 = lane & 15, quad = lane >> 4;
-    const int N = args.N, K = args.K, KB = args.KB;
+    const int N = args.N, K = args.K;
 
     // The workgroups of one XCD (id % 8) take a run of tiles.
     const int used = args.tiles ? args.tiles[args.mtiles].x : args.mtiles;
-    const int64_t total = int64_t(used) * args.ntiles, run = (total + 7) >> 3;
-    const int64_t tile = (blockIdx.x & 7) * run + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= run || tile >= total) return;  // (the whole workgroup)
-    const int tm = int(tile / args.ntiles), tn = int(tile % args.ntiles), n0 = tn * TN;
+    const int64_t each = int64_t(used) * args.ntiles, total = each * args.splits, run = (total + 7) >> 3;
+    const int64_t id = (blockIdx.x & 7) * run + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= run || id >= total) return;  // (the whole workgroup)
+    const int split = int(id / each);
+    const int64_t tile = id - split * each;
+    // Bands of `band` row tiles, column by column in each: the tiles that run at once are as
+    // many rows as columns, and share their operands in the XCD's L2.
+    const int band = args.band, band_at = int(tile / (int64_t(band) * args.ntiles));
+    const int in_band = int(tile - int64_t(band_at) * band * args.ntiles), band_rows = min(band, used - band_at * band);
+    const int tm = band_at * band + in_band % band_rows, tn = in_band / band_rows, n0 = tn * TN;
+    // Blocks of K: those of this split.
+    const int k_begin = split * args.per, k_end = min(args.KB, k_begin + args.per);
+
     int m0 = tm * TM, mrows = min(TM, args.M - m0), first = 0, expert = 0;
     const uint8_t* xp = args.x + m0 * args.x_stride;
     const float* xsp = args.xs + m0;
@@ -75,10 +91,6 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(2,
         xsp = args.xs;
         x_bytes = uint32_t((args.x_rows - 1) * args.x_stride + K);
     }
-    typename YT::storage* const y = static_cast<typename YT::storage*>(args.y);
-    const bool whole = N % (16 / int(sizeof(typename YT::storage))) == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
-    // the results' row of this tile's row i < mrows
-    auto out_row = [&](int i) __attribute__((always_inline)) { return int64_t(args.tiles ? args.order[first + i] : m0 + i); };
     f32x4 acc[NT][MT];
 #pragma unroll
     for (int t = 0; t < NT; t++)
@@ -91,10 +103,12 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(2,
         const __amdgpu_buffer_rsrc_t wr =
             raw_rsrc(args.w + (int64_t(expert) * N + n0) * K, uint32_t(nrows) * uint32_t(K));
         const int nblocks = (N + 127) / 128, nb = min((n0 + 16 * NT * wn) / 128, nblocks - 1);
-        const float* const wsp = args.ws + (int64_t(expert) * nblocks + nb) * KB;
+        // (scalar loads, which the count of vector loads below leaves out)
+        typedef __attribute__((address_space(4))) const float const_f32;
+        const_f32* const wsp = (const_f32*)(args.ws + (int64_t(expert) * nblocks + nb) * args.KB);
 
         // Lane l of load i of a wave: row 8 (L wave + i) + l / 8 of the tile, the chunk that belongs in slot l % 8.
-        uint32_t a_off[LA], b_off[LB], s_off;
+        uint32_t a_off[8], b_off[8], s_off;  // (the first LA and LB used)
         auto a_chunk = [&](int i) __attribute__((always_inline)) {
             const int row = 8 * (LA * wave + i) + (lane >> 3);
             return (lane & 7) ^ (((row >> 1) & 1) | ((row / (4 * NT)) & 3) << 1);
@@ -127,28 +141,29 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(2,
         }
         const uint32_t s_bytes = uint32_t(args.tiles ? args.x_rows : mrows) * 4u;
 
-        auto load = [&](char* to, int kb) __attribute__((always_inline)) {
-            lds_char* const buf = (lds_char*)to;
-            const uint32_t k = uint32_t(kb) * 128u;
-            const bool tail = K - int(k) < 128;  // (only the last block: chunks past K are zeros)
-            const int left = K - int(k);
-#pragma unroll
-            for (int i = 0; i < LA; i++) {
-                uint32_t off = a_off[i];
-                if (tail) off = 16 * a_chunk(i) < left ? off : kOutOfRange;
+        // Load q of block kb into a buffer: weights, activations, scales.
+        auto load = [&](lds_char* to, int kb, int q) __attribute__((always_inline)) {
+            if (q < LA)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                    wr, (__attribute__((address_space(3))) void*)(buf + (LA * wave + i) * 1024), 16, off, k, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < LB; i++) {
-                uint32_t off = b_off[i];
-                if (tail) off = 16 * b_chunk(i) < left ? off : kOutOfRange;
+                    wr, (__attribute__((address_space(3))) void*)(to + (LA * wave + q) * 1024), 16, a_off[q < LA ? q : 0],
+                    uint32_t(kb) * 128u, 0, 0);
+            else if (q < LA + LB)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                    xr, (__attribute__((address_space(3))) void*)(buf + TN * 128 + (LB * wave + i) * 1024), 16, off, k, 0, 0);
-            }
-            const __amdgpu_buffer_rsrc_t sr = raw_rsrc(xsp + kb * args.xs_stride, s_bytes);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                sr, (__attribute__((address_space(3))) void*)(buf + (TN + TM) * 128 + s_wave * 256), 4, s_off, 0, 0, 0);
+                    xr, (__attribute__((address_space(3))) void*)(to + TN * 128 + (LB * wave + q - LA) * 1024), 16,
+                    b_off[q >= LA && q < LA + LB ? q - LA : 0], uint32_t(kb) * 128u, 0, 0);
+            else
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    raw_rsrc(xsp + min(kb, args.KB - 1) * args.xs_stride, s_bytes),
+                    (__attribute__((address_space(3))) void*)(to + (TN + TM) * 128 + s_wave * 256), 4, s_off, 0, 0, 0);
+        };
+        // Before the loads of block kb: of the last block the chunks past K, and behind the split's all, are zeros.
+        auto limit = [&](int kb) __attribute__((always_inline)) {
+            const int left = kb < k_end ? K - kb * 128 : 0;
+            if (left >= 128) return;
+#pragma unroll
+            for (int i = 0; i < LA; i++) a_off[i] = 16 * a_chunk(i) < left ? a_off[i] : kOutOfRange;
+#pragma unroll
+            for (int i = 0; i < LB; i++) b_off[i] = 16 * b_chunk(i) < left ? b_off[i] : kOutOfRange;
         };
 
         // A: weight row of tile t is a_row + 4 t; B: activation row 16 (MT wm + j) + l16.  Chunks quad and quad + 4.
@@ -156,45 +171,85 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(2,
         const uint32_t a_at = uint32_t(a_row * 128 + ((quad ^ (((l16 >> 1) & 1) | ((l16 >> 2) << 1))) << 4));
         const uint32_t b_at = uint32_t(TN * 128 + (16 * MT * wm + l16) * 128 + ((quad ^ ((l16 >> 1) & 7)) << 4));
         const uint32_t s_at = uint32_t((TN + TM) * 128 + (16 * MT * wm + l16) * 4);
-        auto compute = [&](char* from, float sw) __attribute__((always_inline)) {
-            lds_char* const buf = (lds_char*)from;
-            Operand<EXACT> a[NT], b;
+        // Multiplies a block from one buffer while block kb is loaded into another, a load every EVERY
+        // matrix instructions.
+        auto compute = [&](lds_char* from, float sw, lds_char* to, int kb) __attribute__((always_inline)) {
+            constexpr int EVERY = NT * MT / 2 / LOADS > 1 ? NT * MT / 2 / LOADS : 1;
+            Operand<EXACT> a[NT], b[2];
+            float s[2];
+            auto read_b = [&](int j) __attribute__((always_inline)) {
+                b[j & 1].take(*(lds_u32x4*)(from + b_at + j * 2048), *(lds_u32x4*)(from + (b_at ^ 64u) + j * 2048));
+                s[j & 1] = *(lds_f32*)(from + s_at + j * 64) * sw;
+            };
+            read_b(0);
 #pragma unroll
             for (int t = 0; t < NT; t++)
-                a[t].take(*(lds_u32x4*)(buf + a_at + t * 512), *(lds_u32x4*)(buf + (a_at ^ 64u) + t * 512));
+                a[t].take(*(lds_u32x4*)(from + a_at + t * 512), *(lds_u32x4*)(from + (a_at ^ 64u) + t * 512));
+            // Tile i = NT j + t is multiplied while tile i - LAG's sums, which have arrived by then, are
+            // scaled and added (a single wave: 72 cycles a tile with LAG 2, 38 with 3, 32 of them the matrix core's).
+            constexpr int LAG = 3;
+            f32x4 p[LAG + 1];
+            float scale[LAG + 1];
 #pragma unroll
-            for (int j = 0; j < MT; j++) {
-                const float s = *(lds_f32*)(buf + s_at + j * 64) * sw;
-                b.take(*(lds_u32x4*)(buf + b_at + j * 2048), *(lds_u32x4*)(buf + (b_at ^ 64u) + j * 2048));
+            for (int i = 0; i < NT * MT + LAG; i++) {
+                if (i < NT * MT) {
+                    const int j = i / NT, t = i % NT;
+                    if (t == 0 && j + 1 < MT) read_b(j + 1);
+                    p[i % (LAG + 1)] = block_sums(a[t], b[j & 1]);
+                    scale[i % (LAG + 1)] = s[j & 1];
+                    if (i % EVERY == 0 && i / EVERY < LOADS) load(to, kb, i / EVERY);
+                    if (i == NT * MT - 1) {
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const f32x4 p = block_sums(a[t], b);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) acc[t][j][r] = fmaf(s, p[r], acc[t][j][r]);
+                        for (int q = (NT * MT - 1) / EVERY + 1; q < LOADS; q++) load(to, kb, q);
+                    }
                 }
+                if (i >= LAG) {
+                    const int j = (i - LAG) / NT, t = (i - LAG) % NT, q = (i - LAG) % (LAG + 1);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[t][j][r] = fmaf(scale[q], p[q][r], acc[t][j][r]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
+            // (the sums are done here: the compiler would else move the additions behind the
+            // next block's branches, with a register for every product)
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int j = 0; j < MT; j++) asm volatile("" : "+v"(acc[t][j]));
         };
-        // Every load of this wave has landed and its reads are done; then all waves'.
+        // The oldest block on its way has landed and this wave's reads are done; then all waves'.
         auto turn = [&]() __attribute__((always_inline)) {
-            __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+            constexpr int N = LOADS * (STAGES - 2);
+            __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4));  // vmcnt(N) lgkmcnt(0)
             asm volatile("s_barrier" ::: "memory");
         };
 
-        load(buf0, 0);
-        float sw = wsp[0];
-        for (int kb = 0; kb < KB; kb += 2) {
-            turn();
-            if (kb + 1 < KB) load(buf1, kb + 1);
-            const float sw1 = wsp[min(kb + 1, KB - 1)];
-            compute(buf0, sw);
-            if (kb + 1 >= KB) break;
-            turn();
-            if (kb + 2 < KB) load(buf0, kb + 2);
-            sw = wsp[min(kb + 2, KB - 1)];
-            compute(buf1, sw1);
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; i++) {
+            limit(k_begin + i);
+#pragma unroll
+            for (int q = 0; q < LOADS; q++) load(buf(i), k_begin + i, q);
         }
+        float sw = wsp[k_begin];
+        auto step = [&](int kb, int i) __attribute__((always_inline)) {
+            const float next = wsp[min(kb + 1, k_end - 1)];
+            turn();
+            limit(kb + STAGES - 1);
+            compute(buf(i), sw, buf((i + STAGES - 1) % STAGES), kb + STAGES - 1);
+            sw = next;
+        };
+        int kb = k_begin;
+        for (; kb + STAGES <= k_end; kb += STAGES) {
+#pragma unroll
+            for (int i = 0; i < STAGES; i++) step(kb + i, i);
+        }
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; i++)
+            if (kb + i < k_end) step(kb + i, i);
+        __builtin_amdgcn_s_waitcnt(0x0070);  // (nothing is on its way to LDS when the workgroup ends)
     }
 
+    // Results, or the split's sums.
     const int n = n0 + 16 * NT * wn + 4 * NT * quad;
 #pragma unroll
     for (int j = 0; j < MT; j++) {
@@ -205,9 +260,39 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(2,
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) v[4 * t + r] = acc[t][j][r];
-            store_run<YT, 4 * NT>(y + out_row(i) * N + n, v, N - n, whole);
+            const int64_t row = args.tiles ? args.order[first + i] : m0 + i;
+            if (args.splits > 1) {
+                float* const p = args.part + (int64_t(split) * args.M + row) * N + n;
+                store_run<F32T, 4 * NT>(p, v, N - n, N % 4 == 0);
+            } else {
+                typename YT::storage* const y = static_cast<typename YT::storage*>(args.y);
+                constexpr int VEC = 16 / int(sizeof(typename YT::storage));
+                store_run<YT, 4 * NT>(y + row * N + n, v, N - n,
+                                      N % VEC == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0);
+            }
         }
     }
+}
+
+// y = the splits' sums, in their order.
+template <typename YT>
+__global__ __launch_bounds__(256) void fp8_join_kernel(typename YT::storage* __restrict__ y,
+                                                       const float* __restrict__ part, int64_t values, int splits,
+                                                       bool whole) {
+    const int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4;
+    if (at >= values) return;
+    const int n = int(min(values - at, int64_t(4)));
+    float v[4] = {};
+    for (int s = 0; s < splits; s++) {
+        const float* p = part + s * values + at;
+        if (whole) {
+            const float4 q = *reinterpret_cast<const float4*>(p);
+            v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+        } else {
+            for (int i = 0; i < n; i++) v[i] += p[i];
+        }
+    }
+    for (int i = 0; i < n; i++) store_out<YT>(y, at + i, v[i]);
 }
 
 // The routes of each expert side by side, and the row tiles that they make
@@ -259,10 +344,14 @@ __global__ __launch_bounds__(1024) void fp8_routes_kernel(int4* __restrict__ til
     for (int r = threadIdx.x; r < routes; r += 1024) order[atomicAdd(&place[bucket(r)], 1)] = r;
 }
 
+template <typename YT, int WN, int WM, int NT, int MT, int STAGES>
+void launch_tile(const Fp8Args& a, hipStream_t st) {
+    const int64_t total = (int64_t(a.mtiles) * a.ntiles * a.splits + 7) / 8 * 8;
+    fp8_tile_kernel<YT, WN, WM, NT, MT, STAGES><<<dim3(unsigned(total)), dim3(64 * WN * WM), 0, st>>>(a);
+}
 template <typename YT>
 void launch_tiles(const Fp8Args& a, hipStream_t st) {
-    const int64_t total = (int64_t(a.mtiles) * a.ntiles + 7) / 8 * 8;
-    fp8_tile_kernel<YT, 2, 2, 4, 4><<<dim3(unsigned(total)), dim3(256), 0, st>>>(a);
+    launch_tile<YT, 2, 2, 4, 4, 2>(a, st);
 }
 
 constexpr int kTileRows = 128, kTileCols = 128;
@@ -423,7 +512,7 @@ extern "C" int eq_fp8_matmul(void* y, const void* x, int64_t x_stride, const flo
     a.w = static_cast<const uint8_t*>(w);
     a.ws = w_scales;
     a.M = int(m), a.N = int(n), a.K = int(k), a.KB = int(fp8_blocks(k));
-    a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles);
+    a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles), a.band = 8, a.splits = 1, a.per = a.KB;
     x_dtype = take_x(a, base, p, x, x_stride, x_scales, scale_stride, m, k, x_dtype, st);
     if (p.few) {
         launch_fp8_few(a, Fp8Few{x, x_dtype, nullptr, 1}, y_dtype, st);
@@ -472,7 +561,7 @@ extern "C" int eq_fp8_grouped_matmul(void* y, const void* x, int64_t x_stride, c
     a.w = static_cast<const uint8_t*>(w);
     a.ws = w_scales;
     a.M = int(routes), a.N = int(n), a.K = int(k), a.KB = int(fp8_blocks(k));
-    a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles);
+    a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles), a.band = 8, a.splits = 1, a.per = a.KB;
     a.rows = rows, a.x_rows = x_rows;
     x_dtype = take_x(a, base + p.tiles + p.order, p, x, x_stride, x_scales, scale_stride, x_rows, k, x_dtype, st);
     if (p.few) {

@@ -17,7 +17,8 @@ struct Fp8Args {
     const uint8_t* w;
     const float* ws;
     int M, N, K, KB;  // KB: blocks of K
-    int mtiles, ntiles;
+    int mtiles, ntiles, band, splits, per;  // tiles; splits of K, of `per` blocks each
+    float* part;                            // their sums [splits][M][N]
     // Grouped: tiles[i] = {expert, first, rows} of row tile i, the rows being
     // routes order[first ..]; tiles[mtiles].x: how many there are.  Expert -1: rows of zeros.
     const int4* tiles;

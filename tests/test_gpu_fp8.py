@@ -7,7 +7,7 @@ and f32 rows, whose product with 448 is rounded) lie next to a quotient that is 
 3 u (the value, its group's largest, and their quotient): |code - q| <= step(q) / 2 + 3 u |q|.
   norm: sums of squares of at most 24 values a thread, 6 steps in the wave and 16 waves,
   halved by the root; root, quotient, inverse and two products: u = (46 / 2 + 8) 2^-24
-  silu: exp to 2 steps, sum, quotient, product: u = 6 * 2^-24
+  silu: 2^t a step (two halves), its correction, the sum, the reciprocal a step, two products: u = 8 * 2^-24
   f32 rows: u = 2^-24
 
 Products, with A = sum |x| |w| over a row and a column: f32 sums of 128 products and of
@@ -203,7 +203,7 @@ def test_silu_mul(cuda, rows, cols, dtype):
     case("silu", rows, cols, dtype)
     both = values(np.random.default_rng(rows + cols), (rows, 2 * cols), dtype)
     got = fp8.silu_mul(both[:, :cols], both[:, cols:])
-    near_codes(got, *F.quotients(F.silu_mul(f64(both[:, :cols]), f64(both[:, cols:]))), 6 * 2.0 ** -24)
+    near_codes(got, *F.quotients(F.silu_mul(f64(both[:, :cols]), f64(both[:, cols:]))), 8 * 2.0 ** -24)
 
 
 def test_silu_mul_of_rare_values(cuda):
