@@ -19,6 +19,10 @@
 // bf16, which holds them exactly, through v_mfma_f32_16x16x32_bf16: twice the cycles, and
 // sums that are off by f32's rounding alone (of 128 products 7e-8 where the e4m3 ones are off by 5e-5).
 #include <algorithm>
+#ifdef EQ_TUNE
+#include <cstdlib>
+#include <cstdio>
+#endif
 
 #include "fp8_product.hpp"
 
@@ -121,8 +125,7 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(2,
         auto x_row = [&](int i) __attribute__((always_inline)) {
             if (i >= mrows) return -1;
             if (!args.tiles) return i;
-            const int r = args.order[first + i], s = args.rows ? args.rows[r] : r;
-            return uint32_t(s) < uint64_t(args.x_rows) ? s : -1;
+            return args.order[first + i].y;
         };
 #pragma unroll
         for (int i = 0; i < LA; i++) {
@@ -260,10 +263,10 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(2,
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) v[4 * t + r] = acc[t][j][r];
-            const int64_t row = args.tiles ? args.order[first + i] : m0 + i;
+            const int64_t row = args.tiles ? args.order[first + i].x : m0 + i;
             if (args.splits > 1) {
-                float* const p = args.part + (int64_t(split) * args.M + row) * N + n;
-                store_run<F32T, 4 * NT>(p, v, N - n, N % 4 == 0);
+                const int ldp = (N + 3) & ~3;  // (rows of whole float4s)
+                store_run<F32T, 4 * NT>(args.part + (int64_t(split) * args.M + row) * ldp + n, v, ldp - n, true);
             } else {
                 typename YT::storage* const y = static_cast<typename YT::storage*>(args.y);
                 constexpr int VEC = 16 / int(sizeof(typename YT::storage));
@@ -274,32 +277,41 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(2,
     }
 }
 
-// y = the splits' sums, in their order.
+// y = the splits' sums, in their order: a thread has four results of a row.
 template <typename YT>
 __global__ __launch_bounds__(256) void fp8_join_kernel(typename YT::storage* __restrict__ y,
-                                                       const float* __restrict__ part, int64_t values, int splits,
-                                                       bool whole) {
-    const int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4;
-    if (at >= values) return;
-    const int n = int(min(values - at, int64_t(4)));
+                                                       const float* __restrict__ part, int M, int N, int ldp, int splits) {
+    const int quads = ldp / 4;
+    const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    const int m = int(at / quads), n = int(at - int64_t(m) * quads) * 4;
+    if (m >= M) return;
+    const float4* p = reinterpret_cast<const float4*>(part + int64_t(m) * ldp + n);
+    const int64_t step = int64_t(M) * quads;
     float v[4] = {};
-    for (int s = 0; s < splits; s++) {
-        const float* p = part + s * values + at;
-        if (whole) {
-            const float4 q = *reinterpret_cast<const float4*>(p);
-            v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
-        } else {
-            for (int i = 0; i < n; i++) v[i] += p[i];
-        }
-    }
-    for (int i = 0; i < n; i++) store_out<YT>(y, at + i, v[i]);
+    int s = 0;
+    auto add = [&](auto count) __attribute__((always_inline)) {  // several at once: their loads do not wait for each other
+        constexpr int C = decltype(count)::value;
+        float4 q[C];
+#pragma unroll
+        for (int i = 0; i < C; i++) q[i] = p[(s + i) * step];
+#pragma unroll
+        for (int i = 0; i < C; i++) v[0] += q[i].x, v[1] += q[i].y, v[2] += q[i].z, v[3] += q[i].w;
+        s += C;
+    };
+    while (s + 4 <= splits) add(std::integral_constant<int, 4>{});
+    while (s < splits) add(std::integral_constant<int, 1>{});
+    typename YT::storage* const row = y + int64_t(m) * N;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (n + i < N) store_out<YT>(row, n + i, v[i]);
 }
 
 // The routes of each expert side by side, and the row tiles that they make
 // (fp8_tile_kernel's `tiles` and `order`): counted, summed up and placed by one
 // workgroup.  Routes without an expert or a row come last, as expert -1.  Their places
-// within an expert are not in order, which no result depends on.
-__global__ __launch_bounds__(1024) void fp8_routes_kernel(int4* __restrict__ tiles, int32_t* __restrict__ order,
+// within an expert are not in order, which no result depends on.  Neighbouring routes of
+// one expert are counted by one of them (sorted routes would else queue for one counter).
+__global__ __launch_bounds__(1024) void fp8_routes_kernel(int4* __restrict__ tiles, int2* __restrict__ order,
                                                           const int32_t* __restrict__ ids,
                                                           const int32_t* __restrict__ rows, int routes, int experts,
                                                           int64_t x_rows, int tile_rows, int mtiles) {
@@ -307,15 +319,38 @@ __global__ __launch_bounds__(1024) void fp8_routes_kernel(int4* __restrict__ til
     int* const count = shared;               // [experts + 1]
     int* const place = shared + experts + 1;  // [experts + 1]
     __shared__ int sums[2][16], base[2];
-    auto bucket = [&](int r) {
-        const int e = ids[r], s = rows ? rows[r] : r;
-        return uint32_t(e) < uint32_t(experts) && s >= 0 && s < x_rows ? e : experts;
-    };
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // route r's counter (-1: no route) and x row
+    auto bucket = [&](int r, int& row) __attribute__((always_inline)) {
+        if (r >= routes) return -1;
+        const int e = ids[r];
+        row = rows ? rows[r] : r;
+        return uint32_t(e) < uint32_t(experts) && row >= 0 && row < x_rows ? e : experts;
+    };
+    // This lane's place among the counter's: the first of a run of lanes with one counter counts them all.
+    auto take = [&](int* counters, int b) __attribute__((always_inline)) {
+        const int before = __shfl_up(b, 1);
+        const uint64_t heads = __ballot(lane == 0 || b != before);
+        const uint64_t upto = heads & (~uint64_t(0) >> (63 - lane)), behind = lane == 63 ? 0 : heads >> (lane + 1);
+        const int head = 63 - __clzll((long long)upto);
+        const int run = behind ? __ffsll((unsigned long long)behind) : 64 - lane;  // (of a head)
+        int at = 0;
+        if (head == lane && b >= 0) at = atomicAdd(&counters[b], run);
+        return __shfl(at, head) + lane - head;
+    };
+    constexpr int KEPT = 4;  // routes of a thread that are read once
+    int kept[KEPT], kept_row[KEPT];
     for (int e = threadIdx.x; e <= experts; e += 1024) count[e] = 0;
     if (threadIdx.x < 2) base[threadIdx.x] = 0;
+#pragma unroll
+    for (int i = 0; i < KEPT; i++) kept[i] = bucket(threadIdx.x + 1024 * i, kept_row[i]);
     __syncthreads();
-    for (int r = threadIdx.x; r < routes; r += 1024) atomicAdd(&count[bucket(r)], 1);
+#pragma unroll
+    for (int i = 0; i < KEPT; i++) take(count, kept[i]);
+    for (int r0 = 1024 * KEPT; r0 < routes; r0 += 1024) {  // (all lanes of a wave go together)
+        int row;
+        take(count, bucket(r0 + threadIdx.x, row));
+    }
     __syncthreads();
     // running sums of routes and tiles over the experts, 1024 of them a step
     for (int e0 = 0; e0 <= experts; e0 += 1024) {
@@ -341,7 +376,17 @@ __global__ __launch_bounds__(1024) void fp8_routes_kernel(int4* __restrict__ til
         __syncthreads();
     }
     if (threadIdx.x == 0) tiles[mtiles] = make_int4(base[1], 0, 0, 0);
-    for (int r = threadIdx.x; r < routes; r += 1024) order[atomicAdd(&place[bucket(r)], 1)] = r;
+    auto put = [&](int r, int b, int row) __attribute__((always_inline)) {
+        const int at = take(place, b);
+        if (b >= 0) order[at] = make_int2(r, b < experts ? row : -1);
+    };
+#pragma unroll
+    for (int i = 0; i < KEPT; i++) put(threadIdx.x + 1024 * i, kept[i], kept_row[i]);
+    for (int r0 = 1024 * KEPT; r0 < routes; r0 += 1024) {
+        int row = 0;
+        const int b = bucket(r0 + threadIdx.x, row);
+        put(r0 + threadIdx.x, b, row);
+    }
 }
 
 template <typename YT, int WN, int WM, int NT, int MT, int STAGES>
@@ -349,23 +394,96 @@ void launch_tile(const Fp8Args& a, hipStream_t st) {
     const int64_t total = (int64_t(a.mtiles) * a.ntiles * a.splits + 7) / 8 * 8;
     fp8_tile_kernel<YT, WN, WM, NT, MT, STAGES><<<dim3(unsigned(total)), dim3(64 * WN * WM), 0, st>>>(a);
 }
-template <typename YT>
-void launch_tiles(const Fp8Args& a, hipStream_t st) {
-    launch_tile<YT, 2, 2, 4, 4, 2>(a, st);
-}
 
-constexpr int kTileRows = 128, kTileCols = 128;
+// The tile shapes, weight rows by activation rows, and what a workgroup of each took (measured over products
+// of 32 .. 4096 rows): us before and after its blocks, us a block alone on its compute unit, and where two share one.
+struct Shape {
+    int cols, rows;
+    float fixed, one, two;  // two 0: a second one does not fit
+};
+constexpr Shape kShapes[] = {
+    {256, 256, 8.f, 1.5f, 0.f}, {128, 128, 2.f, .72f, 1.02f}, {128, 96, 2.f, .5f, 0.f}, {128, 64, 2.f, .38f, .58f}, {128, 32, 2.f, .26f, 0.f}};
+template <typename YT>
+void launch_tiles(int shape, const Fp8Args& a, hipStream_t st) {
+    switch (shape) {
+    case 0:
+        if constexpr (!std::is_same<YT, F32T>::value) launch_tile<YT, 4, 2, 4, 8, 2>(a, st);
+        break;
+    case 1: launch_tile<YT, 2, 2, 4, 4, 2>(a, st); break;
+    case 2: launch_tile<YT, 4, 1, 2, 6, 3>(a, st); break;
+    case 3: launch_tile<YT, 4, 1, 2, 4, 3>(a, st); break;
+    default: launch_tile<YT, 4, 1, 2, 2, 4>(a, st); break;
+    }
+    if (a.splits > 1) {
+        const int ldp = (a.N + 3) & ~3;
+        const int64_t quads = int64_t(a.M) * (ldp / 4);
+        fp8_join_kernel<YT><<<dim3(unsigned((quads + 255) / 256)), dim3(256), 0, st>>>(
+            static_cast<typename YT::storage*>(a.y), a.part, a.M, a.N, ldp, a.splits);
+    }
+}
 
 size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
+constexpr int kBand = 8;  // row tiles of a band
+
 // How a product is done, from its sizes and types alone (the scratch queries
-// and the calls go by the same), and its scratch: lists of routes, the codes and scales of x.
+// and the calls go by the same), and its scratch: lists of routes, the codes and scales of x, sums of splits.
 struct Plan {
     bool few = false;  // fp8_few.hip's kernel, on x as it is where that takes it
-    int64_t mtiles, ntiles;
-    size_t tiles = 0, order = 0, codes = 0, scales = 0;
-    size_t bytes() const { return tiles + order + codes + scales; }
+    int shape = 0;     // else a tile of kShapes
+    int64_t mtiles = 0, ntiles = 0, splits = 1, per = 0;
+    size_t tiles = 0, order = 0, codes = 0, scales = 0, part = 0;
+    size_t bytes() const { return tiles + order + codes + scales + part; }
 };
+
+#ifdef EQ_TUNE
+int tune(const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; }
+#endif
+
+// Us that a product takes in tiles of a shape, `mtiles` rows of them, with K in `splits` parts, joined after
+// them; what the tiles load comes from the caches at `rate` bytes a us, `bytes` of weights at 6 TB/s, which is
+// overlapped with all but a quarter.
+double tiles_us(const Shape& s, int64_t mtiles, int64_t ntiles, int64_t m, int64_t n, int64_t blocks, int64_t splits,
+                double rate, double bytes) {
+    const int64_t cus = device_cu_count(), slots = s.two > 0.f ? 2 * cus : cus, work = mtiles * ntiles * splits;
+    const double per = double((blocks + splits - 1) / splits), full = s.fixed + per * (s.two > 0.f ? s.two : s.one);
+    const int64_t rest = work % slots;
+    double us = double(work / slots) * full + (rest == 0 ? 0. : rest <= cus ? s.fixed + per * s.one : full);
+    us = std::max(us, double(work) * per * double(s.cols + s.rows) * 128. / rate);
+    if (splits > 1) us += 4. + double(splits) * double(m) * double(n) * 8. / 6e6;
+    const double read = bytes / 6e6;
+    return std::max(us, read) + .25 * std::min(us, read);
+}
+
+// The shape and the splits of K of a product of m rows, in experts or not, and its tiles.  (f32 results hold their
+// operands as bf16, which 256 x 256 have no registers for.)
+void choose_tiles(Plan& p, int64_t m, int64_t n, int64_t k, int64_t experts, int y_dtype) {
+    const int64_t blocks = fp8_blocks(k), used = experts ? std::min(experts, m) : 1;
+    const double bytes = double(used) * double(n) * double(k);
+    double best = 0.;
+    for (int i = y_dtype == EQ_DTYPE_F32 ? 1 : 0; i < int(sizeof(kShapes) / sizeof(kShapes[0])); i++) {
+        const Shape& s = kShapes[i];
+        // (how the routes are spread is not known here: more than half a tile more for each expert; 17 TB/s where
+        // neighbouring tiles share weights and activations, 11 with routes, measured)
+        const int64_t mtiles = experts ? std::max(used, m / s.rows + used * 5 / 8) + 1 : (m + s.rows - 1) / s.rows;
+        const int64_t ntiles = (n + s.cols - 1) / s.cols;
+        for (int64_t splits = 1; splits <= 16 && (splits == 1 || blocks / splits >= 4); splits++) {
+            const double us = tiles_us(s, mtiles, ntiles, m, n, blocks, splits, experts ? 11e6 : 17e6, bytes);
+            if (best > 0. && us >= best) continue;
+            best = us, p.shape = i, p.splits = splits;
+        }
+    }
+#ifdef EQ_TUNE
+    p.shape = tune("SHAPE", p.shape); p.splits = tune("SPLITS", p.splits);
+    if (tune("SHOW", 0)) fprintf(stderr, "[shape %d splits %d: %.1f us] ", p.shape, int(p.splits), best);
+#endif
+    const Shape& s = kShapes[p.shape];
+    p.mtiles = experts ? std::min(m, m / s.rows + experts + 1) : (m + s.rows - 1) / s.rows;
+    p.ntiles = (n + s.cols - 1) / s.cols;
+    p.per = (blocks + p.splits - 1) / p.splits;
+    p.splits = (blocks + p.per - 1) / p.per;
+    if (p.splits > 1) p.part = round256(size_t(p.splits) * size_t(m) * size_t((n + 3) & ~int64_t(3)) * 4u);
+}
 
 bool sizes_ok(const char* who, int64_t rows, int64_t n, int64_t k) {
     if (!fp8_cols_ok(who, "k", k)) return false;
@@ -393,17 +511,16 @@ bool dtypes_ok(const char* who, int x_dtype, int y_dtype) {
 }
 
 bool grid_ok(const char* who, const Plan& p) {
-    if (p.mtiles * p.ntiles < (int64_t(1) << 23)) return true;  // (fewer than 2^32 threads)
+    if (p.mtiles * p.ntiles * p.splits < (int64_t(1) << 23)) return true;  // (fewer than 2^32 threads)
     set_error(std::string(who) + ": 2^23 tiles of the result or more");
     return false;
 }
 
 bool plan_product(const char* who, Plan& p, int64_t m, int64_t n, int64_t k, int x_dtype, int y_dtype) {
     if (!sizes_ok(who, m, n, k) || !dtypes_ok(who, x_dtype, y_dtype)) return false;
-    p.mtiles = (m + kTileRows - 1) / kTileRows;
-    p.ntiles = (n + kTileCols - 1) / kTileCols;
     p.few = m <= 16;
     if (p.few) p.mtiles = 1, p.ntiles = (n + 15) / 16;
+    else choose_tiles(p, m, n, k, 0, y_dtype);
     if (x_dtype != EQ_DTYPE_F8E4M3 && !(p.few && fp8_few_takes(m, k, x_dtype))) {
         p.codes = round256(size_t(m) * size_t(k));
         p.scales = round256(size_t(m) * size_t(fp8_blocks(k)) * 4u);
@@ -428,11 +545,10 @@ bool plan_routes(const char* who, Plan& p, int64_t x_rows, int64_t experts, int6
         p.mtiles = routes, p.ntiles = (n + 15) / 16;
         return grid_ok(who, p);
     }
-    // (a part tile for each expert that has one, and for the routes without)
-    p.mtiles = std::min(routes, routes / kTileRows + experts + 1);
-    p.ntiles = (n + kTileCols - 1) / kTileCols;
+    // (p.mtiles: a part tile for each expert that has one, and for the routes without)
+    choose_tiles(p, routes, n, k, experts, y_dtype);
     p.tiles = round256(size_t(p.mtiles + 1) * sizeof(int4));
-    p.order = round256(size_t(routes) * 4u);
+    p.order = round256(size_t(routes) * sizeof(int2));
     return grid_ok(who, p);
 }
 
@@ -512,13 +628,14 @@ extern "C" int eq_fp8_matmul(void* y, const void* x, int64_t x_stride, const flo
     a.w = static_cast<const uint8_t*>(w);
     a.ws = w_scales;
     a.M = int(m), a.N = int(n), a.K = int(k), a.KB = int(fp8_blocks(k));
-    a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles), a.band = 8, a.splits = 1, a.per = a.KB;
+    a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles), a.band = kBand, a.splits = int(p.splits), a.per = int(p.per);
     x_dtype = take_x(a, base, p, x, x_stride, x_scales, scale_stride, m, k, x_dtype, st);
     if (p.few) {
         launch_fp8_few(a, Fp8Few{x, x_dtype, nullptr, 1}, y_dtype, st);
         return check_launch(who);
     }
-    with_dtype(y_dtype, [&](auto t) { launch_tiles<decltype(t)>(a, st); });
+    a.part = reinterpret_cast<float*>(base + p.bytes() - p.part);
+    with_dtype(y_dtype, [&](auto t) { launch_tiles<decltype(t)>(p.shape, a, st); });
     return check_launch(who);
 }
 
@@ -561,7 +678,7 @@ extern "C" int eq_fp8_grouped_matmul(void* y, const void* x, int64_t x_stride, c
     a.w = static_cast<const uint8_t*>(w);
     a.ws = w_scales;
     a.M = int(routes), a.N = int(n), a.K = int(k), a.KB = int(fp8_blocks(k));
-    a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles), a.band = 8, a.splits = 1, a.per = a.KB;
+    a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles), a.band = kBand, a.splits = int(p.splits), a.per = int(p.per);
     a.rows = rows, a.x_rows = x_rows;
     x_dtype = take_x(a, base + p.tiles + p.order, p, x, x_stride, x_scales, scale_stride, x_rows, k, x_dtype, st);
     if (p.few) {
@@ -569,10 +686,11 @@ extern "C" int eq_fp8_grouped_matmul(void* y, const void* x, int64_t x_stride, c
         return check_launch(who);
     }
     a.tiles = reinterpret_cast<const int4*>(base);
-    a.order = reinterpret_cast<const int32_t*>(base + p.tiles);
+    a.order = reinterpret_cast<const int2*>(base + p.tiles);
     fp8_routes_kernel<<<dim3(1), dim3(1024), size_t(2 * (experts + 1)) * 4u, st>>>(
-        reinterpret_cast<int4*>(base), reinterpret_cast<int32_t*>(base + p.tiles), ids, rows, int(routes), int(experts),
-        x_rows, kTileRows, a.mtiles);
-    with_dtype(y_dtype, [&](auto t) { launch_tiles<decltype(t)>(a, st); });
+        reinterpret_cast<int4*>(base), reinterpret_cast<int2*>(base + p.tiles), ids, rows, int(routes), int(experts),
+        x_rows, kShapes[p.shape].rows, a.mtiles);
+    a.part = reinterpret_cast<float*>(base + p.bytes() - p.part);
+    with_dtype(y_dtype, [&](auto t) { launch_tiles<decltype(t)>(p.shape, a, st); });
     return check_launch(who);
 }

@@ -19,10 +19,10 @@ struct Fp8Args {
     int M, N, K, KB;  // KB: blocks of K
     int mtiles, ntiles, band, splits, per;  // tiles; splits of K, of `per` blocks each
     float* part;                            // their sums [splits][M][N]
-    // Grouped: tiles[i] = {expert, first, rows} of row tile i, the rows being
-    // routes order[first ..]; tiles[mtiles].x: how many there are.  Expert -1: rows of zeros.
+    // Grouped: tiles[i] = {expert, first, rows} of row tile i, the rows being order[first ..], {route, row of x};
+    // tiles[mtiles].x: how many there are.  Expert -1: rows of zeros.
     const int4* tiles;
-    const int32_t* order;
+    const int2* order;
     const int32_t* rows;
     int64_t x_rows;
 };
