@@ -46,7 +46,7 @@ typedef __attribute__((address_space(3))) const float lds_f32;
 // rows of one parity have to differ in their key: (row / 2) % 8 for the
 // activations, (row / 2) % 2 + 2 (row / (4 NT) % 4) for the weights' rows above.
 template <typename YT, int WN, int WM, int NT, int MT, int STAGES>
-__global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_tile_kernel(
+__global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(1, 2))) void fp8_tile_kernel(
     const Fp8Args args) {
     constexpr int WAVES = WN * WM, TN = 16 * NT * WN, TM = 16 * MT * WM;
     constexpr int LA = TN / 8 / WAVES, LB = TM / 8 / WAVES;  // loads of 1 KiB (8 rows) a wave
@@ -401,19 +401,21 @@ struct Shape {
     int cols, rows;
     float fixed, one, two;  // two 0: a second one does not fit
 };
-constexpr Shape kShapes[] = {
-    {256, 256, 8.f, 1.5f, 0.f}, {128, 128, 2.f, .72f, 1.02f}, {128, 96, 2.f, .5f, 0.f}, {128, 64, 2.f, .38f, .58f}, {128, 32, 2.f, .26f, 0.f}};
+constexpr Shape kShapes[] = {{256, 256, 8.f, 1.5f, 0.f}, {256, 192, 7.f, 1.2f, 0.f}, {256, 128, 5.f, .9f, 0.f},
+                             {128, 128, 2.f, .72f, 1.02f}, {128, 96, 2.f, .5f, 0.f}, {128, 64, 2.f, .38f, .58f},
+                             {128, 32, 2.f, .26f, 0.f}};
+constexpr int kWide = 3;  // the shapes of 256 weight rows: their f32 results would need more registers than there are
 template <typename YT>
 void launch_tiles(int shape, const Fp8Args& a, hipStream_t st) {
-    switch (shape) {
-    case 0:
-        if constexpr (!std::is_same<YT, F32T>::value) launch_tile<YT, 4, 2, 4, 8, 2>(a, st);
-        break;
-    case 1: launch_tile<YT, 2, 2, 4, 4, 2>(a, st); break;
-    case 2: launch_tile<YT, 4, 1, 2, 6, 3>(a, st); break;
-    case 3: launch_tile<YT, 4, 1, 2, 4, 3>(a, st); break;
-    default: launch_tile<YT, 4, 1, 2, 2, 4>(a, st); break;
+    if constexpr (!std::is_same<YT, F32T>::value) {
+        if (shape == 0) launch_tile<YT, 4, 2, 4, 8, 2>(a, st);
+        if (shape == 1) launch_tile<YT, 4, 2, 4, 6, 2>(a, st);
+        if (shape == 2) launch_tile<YT, 4, 2, 4, 4, 3>(a, st);
     }
+    if (shape == 3) launch_tile<YT, 2, 2, 4, 4, 2>(a, st);
+    if (shape == 4) launch_tile<YT, 4, 1, 2, 6, 3>(a, st);
+    if (shape == 5) launch_tile<YT, 4, 1, 2, 4, 3>(a, st);
+    if (shape == 6) launch_tile<YT, 4, 1, 2, 2, 4>(a, st);
     if (a.splits > 1) {
         const int ldp = (a.N + 3) & ~3;
         const int64_t quads = int64_t(a.M) * (ldp / 4);
@@ -455,13 +457,12 @@ double tiles_us(const Shape& s, int64_t mtiles, int64_t ntiles, int64_t m, int64
     return std::max(us, read) + .25 * std::min(us, read);
 }
 
-// The shape and the splits of K of a product of m rows, in experts or not, and its tiles.  (f32 results hold their
-// operands as bf16, which 256 x 256 have no registers for.)
+// The shape and the splits of K of a product of m rows, in experts or not, and its tiles.
 void choose_tiles(Plan& p, int64_t m, int64_t n, int64_t k, int64_t experts, int y_dtype) {
     const int64_t blocks = fp8_blocks(k), used = experts ? std::min(experts, m) : 1;
     const double bytes = double(used) * double(n) * double(k);
     double best = 0.;
-    for (int i = y_dtype == EQ_DTYPE_F32 ? 1 : 0; i < int(sizeof(kShapes) / sizeof(kShapes[0])); i++) {
+    for (int i = y_dtype == EQ_DTYPE_F32 ? kWide : 0; i < int(sizeof(kShapes) / sizeof(kShapes[0])); i++) {
         const Shape& s = kShapes[i];
         // (how the routes are spread is not known here: more than half a tile more for each expert; 17 TB/s where
         // neighbouring tiles share weights and activations, 11 with routes, measured)

@@ -70,10 +70,13 @@ def _float_code(t: torch.Tensor, what: str) -> int:
 def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
     """t [..., K] as rows [M, K] whose values are contiguous, at any stride of a
     multiple of 16 bytes, as slices of a fused projection are.  Any other layout is copied."""
-    if t.dim() == 0:
+    d = t.dim()
+    if d == 2 and t.is_contiguous() and t.shape[0] != 1:
+        return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    if d == 0:
         raise EreduError(f"{what} must have at least one dimension")
     K = t.shape[-1]
-    if t.dim() != 2:
+    if d != 2:
         t = t.reshape(-1, K) if K else t.reshape(t.numel(), 0)
     if t.is_contiguous():
         # (a single row is contiguous at any stride)
@@ -83,17 +86,14 @@ def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _new_rows(shape, K: int, device) -> Tuple[torch.Tensor, torch.Tensor, int]:
-    """Codes [rows, K] and scales [rows, blocks], the scales of a block side by side."""
-    rows = 1
-    for d in shape[:-1]:
-        rows *= d
-    codes = torch.empty(shape, dtype=CODE_DTYPE, device=device)
-    return codes, torch.empty_strided((rows, _blocks(K)), (1, max(rows, 1)), dtype=torch.float32, device=device), rows
+def _scales_like(t: torch.Tensor, rows: int, K: int) -> torch.Tensor:
+    """Scales [rows, blocks] whose rows of a block lie side by side."""
+    return t.new_empty_strided((rows, -(-K // BLOCK)), (1, rows or 1), dtype=torch.float32)
 
 
 def _out(codes: torch.Tensor, scales: torch.Tensor) -> Fp8Rows:
-    return Fp8Rows(codes, scales if codes.dim() == 2 else scales.unflatten(0, codes.shape[:-1]) if codes.dim() > 2 else scales[0])
+    d = codes.dim()
+    return Fp8Rows(codes, scales if d == 2 else scales.unflatten(0, codes.shape[:-1]) if d > 2 else scales[0])
 
 
 def quantize(x: torch.Tensor) -> Fp8Rows:
@@ -102,8 +102,9 @@ def quantize(x: torch.Tensor) -> Fp8Rows:
     st = _here(x)
     x2 = _rows(x, "x")
     K = x2.shape[1]
-    codes, scales, rows = _new_rows(x.shape, K, x.device)
-    check(_native.lib().eq_fp8_quantize(codes.data_ptr(), scales.data_ptr(), max(rows, 1), x2.data_ptr(), x2.stride(0), rows, K,
+    rows = x2.shape[0]
+    codes, scales = x.new_empty(x.shape, dtype=CODE_DTYPE), _scales_like(x, rows, K)
+    check(_native.lib().eq_fp8_quantize(codes.data_ptr(), scales.data_ptr(), rows, x2.data_ptr(), x2.stride(0), rows, K,
                                         code, st))
     return _out(codes, scales)
 
@@ -132,21 +133,23 @@ def rms_norm(hidden: torch.Tensor, weight: torch.Tensor, eps: float, residual: O
     """``hidden += residual`` (in place, when given), then RMSNorm(hidden) *
     weight in codes (C ABI: eq_fp8_rms_norm): ``decode.rms_norm`` for what a
     projection in codes reads next, of any of the three float types."""
-    code = _float_code(hidden, "hidden")
-    K = hidden.shape[-1]
-    if tuple(weight.shape) != (K,) or weight.dtype != hidden.dtype or not weight.is_contiguous():
-        raise EreduError(f"weight must be a contiguous {hidden.dtype} tensor [{K}]")
+    code, dtype, shape = _float_code(hidden, "hidden"), hidden.dtype, hidden.shape
+    K = shape[-1]
+    if weight.dtype is not dtype or weight.shape != shape[-1:] or not weight.is_contiguous():
+        raise EreduError(f"weight must be a contiguous {dtype} tensor [{K}]")
     if not hidden.is_contiguous():
         raise EreduError("hidden must be contiguous")
+    rp = None
     if residual is not None:
-        if residual.shape != hidden.shape or residual.dtype != hidden.dtype:
+        if residual.shape != shape or residual.dtype is not dtype:
             raise EreduError("residual must match hidden in shape and dtype")
         residual = residual.contiguous()
+        rp = residual.data_ptr()
     st = _here(hidden, weight, residual)
-    codes, scales, rows = _new_rows(hidden.shape, K, hidden.device)
-    check(_native.lib().eq_fp8_rms_norm(codes.data_ptr(), scales.data_ptr(), max(rows, 1), hidden.data_ptr(),
-                                        None if residual is None else residual.data_ptr(), weight.data_ptr(), rows, K,
-                                        eps, code, st))
+    rows = shape[0] if len(shape) == 2 else hidden.numel() // K if K else 0
+    codes, scales = torch.empty_like(hidden, dtype=CODE_DTYPE), _scales_like(hidden, rows, K)
+    check(_native.lib().eq_fp8_rms_norm(codes.data_ptr(), scales.data_ptr(), rows, hidden.data_ptr(), rp, weight.data_ptr(),
+                                        rows, K, eps, code, st))
     return _out(codes, scales)
 
 
@@ -158,9 +161,9 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> Fp8Rows:
         raise EreduError("gate and up must match in shape and dtype")
     st = _here(gate, up)
     g, u = _rows(gate, "gate"), _rows(up, "up")
-    K = g.shape[1]
-    codes, scales, rows = _new_rows(gate.shape, K, gate.device)
-    check(_native.lib().eq_fp8_silu_mul(codes.data_ptr(), scales.data_ptr(), max(rows, 1), g.data_ptr(), g.stride(0),
+    rows, K = g.shape
+    codes, scales = gate.new_empty(gate.shape, dtype=CODE_DTYPE), _scales_like(gate, rows, K)
+    check(_native.lib().eq_fp8_silu_mul(codes.data_ptr(), scales.data_ptr(), rows, g.data_ptr(), g.stride(0),
                                         u.data_ptr(), u.stride(0), rows, K, code, st))
     return _out(codes, scales)
 
@@ -193,11 +196,12 @@ def _x_of(x: Union[Fp8Rows, torch.Tensor], K: int):
 
 
 def _weight(w: torch.Tensor, w_scales: torch.Tensor, dims: int) -> Tuple[int, int]:
-    if w.dim() != dims or w.dtype is not CODE_DTYPE or not w.is_contiguous():
+    shape = w.shape
+    if len(shape) != dims or w.dtype is not CODE_DTYPE or not w.is_contiguous():
         raise EreduError(f"w must be a contiguous float8_e4m3fn tensor {'[N, K]' if dims == 2 else '[experts, N, K]'}")
-    N, K = w.shape[-2:]
-    expect = (*w.shape[:-2], _blocks(N), _blocks(K))
-    if tuple(w_scales.shape) != expect or w_scales.dtype is not torch.float32 or not w_scales.is_contiguous():
+    N, K = shape[-2:]
+    expect = (*shape[:-2], -(-N // BLOCK), -(-K // BLOCK))
+    if w_scales.shape != expect or w_scales.dtype is not torch.float32 or not w_scales.is_contiguous():
         raise EreduError(f"w_scales must be a contiguous float32 tensor {expect}, got {w_scales.dtype} {tuple(w_scales.shape)}")
     return N, K
 
@@ -234,7 +238,7 @@ def matmul(x: Union[Fp8Rows, torch.Tensor], w: torch.Tensor, w_scales: torch.Ten
     dtype = _out_dtype(x, dtype)
     st = _here(rows, scales, w, w_scales)
     M, lib, out = rows.shape[0], _native.lib(), _DTYPE_CODE[dtype]
-    y = torch.empty((M, N), dtype=dtype, device=rows.device)
+    y = rows.new_empty((M, N), dtype=dtype)
     sp, sn, hold = _scratch(lib.eq_fp8_matmul_scratch(M, N, K, code, out), rows.device) if _capturing() else (None, 0, None)
     check(lib.eq_fp8_matmul(y.data_ptr(), rows.data_ptr(), rows.stride(0), None if scales is None else scales.data_ptr(),
                             stride, w.data_ptr(), w_scales.data_ptr(), M, N, K, code, out, sp, sn, st))
@@ -262,7 +266,7 @@ def grouped_matmul(x: Union[Fp8Rows, torch.Tensor], w: torch.Tensor, w_scales: t
     rows = None if rows is None else rows.contiguous()
     R, T, E = ids.shape[0], xr.shape[0], w.shape[0]
     lib, out = _native.lib(), _DTYPE_CODE[dtype]
-    y = torch.empty((R, N), dtype=dtype, device=xr.device)
+    y = xr.new_empty((R, N), dtype=dtype)
     sp, sn, hold = (_scratch(lib.eq_fp8_grouped_matmul_scratch(T, E, R, N, K, code, out), xr.device) if _capturing()
                     else (None, 0, None))
     check(lib.eq_fp8_grouped_matmul(y.data_ptr(), xr.data_ptr(), xr.stride(0),
