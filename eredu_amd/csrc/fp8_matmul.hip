@@ -53,7 +53,7 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(1,
     constexpr int LOADS = LA + LB + 1;                        // and one of scales
     static_assert(LA * 8 * WAVES == TN && LB * 8 * WAVES == TM && LA <= 8 && LB <= 8, "whole loads");
     static_assert(128 % (16 * NT) == 0, "a wave's weight rows have one scale");
-    constexpr int SROWS = TM < 64 ? 64 : TM, BUF = (TN + TM) * 128 + SROWS * 4;
+    constexpr int SROWS = (TM + 63) & ~63, BUF = (TN + TM) * 128 + SROWS * 4;
     static_assert(64 * WAVES >= SROWS, "a scale load a wave");
     static_assert(STAGES >= 2 && STAGES <= 4, "buffers");
     constexpr bool EXACT = std::is_same<YT, F32T>::value;
