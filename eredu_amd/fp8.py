@@ -25,7 +25,7 @@ import torch
 
 from . import _native
 from ._native import EreduError, check
-from .quantization import _DTYPE_CODE, _get_device, _stream
+from .quantization import _DTYPE_CODE, _get_device, _raw_stream, _stream
 
 BLOCK = 128  # columns of a scale, and rows of a weight's
 CODE_DTYPE = torch.float8_e4m3fn
@@ -57,7 +57,7 @@ def _here(*tensors: Optional[torch.Tensor]) -> int:
     for t in tensors:
         if t is not None and t.get_device() != index:
             raise EreduError(f"all arrays must live on the current device, cuda:{index}: got one on {t.device}")
-    return _stream()
+    return _raw_stream(index) if _raw_stream is not None else _stream()
 
 
 def _float_code(t: torch.Tensor, what: str) -> int:
@@ -71,9 +71,11 @@ def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
     """t [..., K] as rows [M, K] whose values are contiguous, at any stride of a
     multiple of 16 bytes, as slices of a fused projection are.  Any other layout is copied."""
     d = t.dim()
-    if d == 2 and t.is_contiguous() and t.shape[0] != 1:
-        return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
-    if d == 0:
+    if d == 2:
+        stride, one = t.stride()
+        if one == 1 and t.shape[1] <= stride < 1 << 23 and stride * t.itemsize % 16 == 0 and t.data_ptr() % 16 == 0:
+            return t
+    elif d == 0:
         raise EreduError(f"{what} must have at least one dimension")
     K = t.shape[-1]
     if d != 2:
@@ -84,6 +86,10 @@ def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
     elif t.stride(1) != 1 or t.stride(0) < K or t.stride(0) >= 1 << 23 or t.stride(0) * t.element_size() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _codes_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, dtype=CODE_DTYPE, memory_format=torch.contiguous_format)
 
 
 def _scales_like(t: torch.Tensor, rows: int, K: int) -> torch.Tensor:
@@ -103,7 +109,7 @@ def quantize(x: torch.Tensor) -> Fp8Rows:
     x2 = _rows(x, "x")
     K = x2.shape[1]
     rows = x2.shape[0]
-    codes, scales = x.new_empty(x.shape, dtype=CODE_DTYPE), _scales_like(x, rows, K)
+    codes, scales = _codes_like(x), _scales_like(x, rows, K)
     check(_native.lib().eq_fp8_quantize(codes.data_ptr(), scales.data_ptr(), rows, x2.data_ptr(), x2.stride(0), rows, K,
                                         code, st))
     return _out(codes, scales)
@@ -147,7 +153,7 @@ def rms_norm(hidden: torch.Tensor, weight: torch.Tensor, eps: float, residual: O
         rp = residual.data_ptr()
     st = _here(hidden, weight, residual)
     rows = shape[0] if len(shape) == 2 else hidden.numel() // K if K else 0
-    codes, scales = torch.empty_like(hidden, dtype=CODE_DTYPE), _scales_like(hidden, rows, K)
+    codes, scales = _codes_like(hidden), _scales_like(hidden, rows, K)
     check(_native.lib().eq_fp8_rms_norm(codes.data_ptr(), scales.data_ptr(), rows, hidden.data_ptr(), rp, weight.data_ptr(),
                                         rows, K, eps, code, st))
     return _out(codes, scales)
@@ -162,48 +168,51 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> Fp8Rows:
     st = _here(gate, up)
     g, u = _rows(gate, "gate"), _rows(up, "up")
     rows, K = g.shape
-    codes, scales = gate.new_empty(gate.shape, dtype=CODE_DTYPE), _scales_like(gate, rows, K)
+    codes, scales = _codes_like(gate), _scales_like(gate, rows, K)
     check(_native.lib().eq_fp8_silu_mul(codes.data_ptr(), scales.data_ptr(), rows, g.data_ptr(), g.stride(0),
                                         u.data_ptr(), u.stride(0), rows, K, code, st))
     return _out(codes, scales)
 
 
 def _x_of(x: Union[Fp8Rows, torch.Tensor], K: int):
-    """(rows, scales or None, scale stride, dtype code, shape) of a product's left operand."""
+    """(rows, scales or None, scale stride, dtype code) of a product's left operand."""
     if isinstance(x, torch.Tensor):
-        if x.dtype is CODE_DTYPE:
-            raise EreduError("rows in codes come with their scales: pass Fp8Rows(codes, scales)")
-        code, scales, stride, shape = _float_code(x, "x"), None, 0, x.shape
-        rows = _rows(x, "x")
+        code = _DTYPE_CODE.get(x.dtype)
+        if code is None:
+            if x.dtype is CODE_DTYPE:
+                raise EreduError("rows in codes come with their scales: pass Fp8Rows(codes, scales)")
+            raise EreduError(f"x must be float32, float16 or bfloat16, got {x.dtype}")
+        rows, scales, stride = _rows(x, "x"), None, 0
     else:
         codes, scales = x
         if codes.dtype is not CODE_DTYPE or scales.dtype is not torch.float32:
             raise EreduError(f"codes must be float8_e4m3fn and scales float32, got {codes.dtype} and {scales.dtype}")
-        code, shape = _native.EQ_DTYPE_F8E4M3, codes.shape
-        rows = _rows(codes, "x")
-        blocks = _blocks(rows.shape[1])
-        if tuple(scales.shape) != (*shape[:-1], blocks):
-            raise EreduError(f"scales has shape {tuple(scales.shape)}, expected {(*shape[:-1], blocks)}")
-        if scales.dim() != 2:
+        code, rows = _native.EQ_DTYPE_F8E4M3, _rows(codes, "x")
+        M, blocks = rows.shape[0], -(-rows.shape[1] // BLOCK)
+        expect = (*codes.shape[:-1], blocks)
+        if scales.shape != expect:
+            raise EreduError(f"scales has shape {tuple(scales.shape)}, expected {expect}")
+        if len(expect) != 2:
             scales = scales.reshape(-1, blocks)
-        M = rows.shape[0]
-        if (scales.stride(0) != 1 and M > 1) or (scales.stride(1) < M and blocks > 1):
+        if (M > 1 and scales.stride(0) != 1) or (blocks > 1 and scales.stride(1) < M):
             scales = scales.t().contiguous().t()
-        stride = scales.stride(1) if blocks > 1 else max(M, 1)
+        stride = scales.stride(1) if blocks > 1 else M
     if rows.shape[1] != K:
         raise EreduError(f"x has rows of {rows.shape[1]} values, the weight of {K}")
-    return rows, scales, stride, code, shape
+    return rows, scales, stride, code
 
 
-def _weight(w: torch.Tensor, w_scales: torch.Tensor, dims: int) -> Tuple[int, int]:
-    shape = w.shape
+def _weight(w: torch.Tensor, w_scales: torch.Tensor, dims: int):
+    """w's shape, once it and its scales are what the products take."""
+    shape, blocks = w.shape, w_scales.shape
     if len(shape) != dims or w.dtype is not CODE_DTYPE or not w.is_contiguous():
         raise EreduError(f"w must be a contiguous float8_e4m3fn tensor {'[N, K]' if dims == 2 else '[experts, N, K]'}")
-    N, K = shape[-2:]
-    expect = (*shape[:-2], -(-N // BLOCK), -(-K // BLOCK))
-    if w_scales.shape != expect or w_scales.dtype is not torch.float32 or not w_scales.is_contiguous():
-        raise EreduError(f"w_scales must be a contiguous float32 tensor {expect}, got {w_scales.dtype} {tuple(w_scales.shape)}")
-    return N, K
+    if (w_scales.dtype is not torch.float32 or len(blocks) != dims or blocks[-1] != -(-shape[-1] // BLOCK) or
+            blocks[-2] != -(-shape[-2] // BLOCK) or blocks[0] != (shape[0] if dims == 3 else blocks[0]) or
+            not w_scales.is_contiguous()):
+        expect = (*shape[:-2], -(-shape[-2] // BLOCK), -(-shape[-1] // BLOCK))
+        raise EreduError(f"w_scales must be a contiguous float32 tensor {expect}, got {w_scales.dtype} {tuple(blocks)}")
+    return shape
 
 
 def _out_dtype(x, dtype: Optional[torch.dtype]) -> torch.dtype:
@@ -234,7 +243,7 @@ def matmul(x: Union[Fp8Rows, torch.Tensor], w: torch.Tensor, w_scales: torch.Ten
     ``Fp8Rows``, or float rows that the call quantizes first, as ``quantize``
     does (C ABI: eq_fp8_matmul)."""
     N, K = _weight(w, w_scales, 2)
-    rows, scales, stride, code, shape = _x_of(x, K)
+    rows, scales, stride, code = _x_of(x, K)
     dtype = _out_dtype(x, dtype)
     st = _here(rows, scales, w, w_scales)
     M, lib, out = rows.shape[0], _native.lib(), _DTYPE_CODE[dtype]
@@ -242,7 +251,8 @@ def matmul(x: Union[Fp8Rows, torch.Tensor], w: torch.Tensor, w_scales: torch.Ten
     sp, sn, hold = _scratch(lib.eq_fp8_matmul_scratch(M, N, K, code, out), rows.device) if _capturing() else (None, 0, None)
     check(lib.eq_fp8_matmul(y.data_ptr(), rows.data_ptr(), rows.stride(0), None if scales is None else scales.data_ptr(),
                             stride, w.data_ptr(), w_scales.data_ptr(), M, N, K, code, out, sp, sn, st))
-    return y if len(shape) == 2 else y.view(*shape[:-1], N)
+    lead = (x if scales is None else x[0]).shape[:-1]
+    return y if len(lead) == 1 else y.view(*lead, N)
 
 
 def grouped_matmul(x: Union[Fp8Rows, torch.Tensor], w: torch.Tensor, w_scales: torch.Tensor, ids: torch.Tensor,
@@ -253,18 +263,20 @@ def grouped_matmul(x: Union[Fp8Rows, torch.Tensor], w: torch.Tensor, w_scales: t
     any order (rows None: x has a row for each route).  A route whose expert or
     row is out of range, as padded ones may have, gives zeros (C ABI:
     eq_fp8_grouped_matmul)."""
-    N, K = _weight(w, w_scales, 3)
-    xr, scales, stride, code, shape = _x_of(x, K)
-    if len(shape) != 2:
+    E, N, K = _weight(w, w_scales, 3)
+    if (x if isinstance(x, torch.Tensor) else x[0]).dim() != 2:
         raise EreduError(f"x must be [rows, {K}]")
+    xr, scales, stride, code = _x_of(x, K)
     dtype = _out_dtype(x, dtype)
     st = _here(xr, scales, w, w_scales, ids, rows)
-    for t, what in ((ids, "ids"), (rows, "rows")):
-        if t is not None and (t.dtype is not torch.int32 or t.dim() != 1 or t.shape != ids.shape):
-            raise EreduError(f"{what} must be a one-dimensional int32 tensor, rows as long as ids")
+    if ids.dtype is not torch.int32 or ids.dim() != 1:
+        raise EreduError("ids must be a one-dimensional int32 tensor")
+    if rows is not None:
+        if rows.dtype is not torch.int32 or rows.shape != ids.shape:
+            raise EreduError("rows must be an int32 tensor as long as ids")
+        rows = rows.contiguous()
     ids = ids.contiguous()
-    rows = None if rows is None else rows.contiguous()
-    R, T, E = ids.shape[0], xr.shape[0], w.shape[0]
+    R, T = ids.shape[0], xr.shape[0]
     lib, out = _native.lib(), _DTYPE_CODE[dtype]
     y = xr.new_empty((R, N), dtype=dtype)
     sp, sn, hold = (_scratch(lib.eq_fp8_grouped_matmul_scratch(T, E, R, N, K, code, out), xr.device) if _capturing()
