@@ -1,19 +1,23 @@
 // Products of few rows (at most 16, or one for each route) with e4m3 weights:
 // bound by reading the weights once.
 //
-// A workgroup of 8 waves has 16 NT weight rows; wave v takes the blocks v, v + 8,
-// .. of K, a block being one matrix instruction a tile (fp8_matmul.hip), and the
-// waves' sums are added through LDS in wave order.  Each wave brings its blocks
-// into a ring of its own in LDS, AHEAD blocks before it needs them, and waits for
-// none of the others.  (Straight into the operand's registers a load touches half a line of
-// 16 rows, and the 64 KiB of a compute unit took 1.7 us of its address unit's time, here 0.6.)
+// A workgroup of WAVES waves has 16 NT weight rows; wave v takes the blocks v,
+// v + WAVES, .. of K, a block being one matrix instruction a tile (fp8_matmul.hip), and
+// the waves' sums are added through LDS in wave order.  Each wave brings its
+// blocks into a ring of its own in LDS, AHEAD blocks before it needs them, and
+// waits for none of the others.  (Straight into the operand's registers a load
+// touches half a line of 16 rows, and 64 KiB took 1.7 us of a compute unit's address unit, this way 0.6.)
 // Rows of values (at most 4) are quantized by the workgroup into LDS while its first weights are on their way.
+//
+// 8 waves, 16 rows and one block ahead leave room for more workgroups on a compute unit, which is worth
+// more than a deeper ring (us in graphs; ahead 3 and 1: 16 rows of codes by 14336 x 4096 16.7, 13.0;
+// a row of values by 14336 x 4096 13.3, 11.6; by 4096 x 4096 5.5, 5.4).  Where 64 rows to a workgroup of 4 waves
+// fill the GPU, rows of codes are read a quarter as often (the first of those 11.1; 64 routes of 2048 x 768 24.9, 15.7).
 #include "fp8_product.hpp"
 
 namespace eq {
 namespace {
 
-constexpr int kFewWaves = 8;
 constexpr int kFewLds = 48 * 1024;  // codes and scales of the rows, where the kernel makes them
 
 typedef __attribute__((address_space(3))) char lds_char;
@@ -24,13 +28,13 @@ typedef __attribute__((address_space(3))) const float lds_f32;
 struct F8T {};  // x in codes
 
 // ROWS8: loads of 8 rows of x (0: the kernel quantizes them).
-template <typename XT, typename YT, int NT, int ROWS8, int AHEAD>
-__global__ __launch_bounds__(64 * kFewWaves) void fp8_few_kernel(const Fp8Args args, const Fp8Few few) {
+template <typename XT, typename YT, int WAVES, int NT, int ROWS8, int AHEAD>
+__global__ __launch_bounds__(64 * WAVES) void fp8_few_kernel(const Fp8Args args, const Fp8Few few) {
     constexpr bool CODED = std::is_same<XT, F8T>::value, EXACT = std::is_same<YT, F32T>::value;
     static_assert(CODED == (ROWS8 > 0), "rows in codes are loaded");
     constexpr int A_BYTES = NT * 2048, B_BYTES = ROWS8 * 1024, SLOT = A_BYTES + B_BYTES + (CODED ? 256 : 0);
     constexpr int LOADS = 2 * NT + ROWS8 + (CODED ? 1 : 0), RING = AHEAD + 1;
-    constexpr int SUMS = kFewWaves * NT * 16 * 17 * 4, BYTES = kFewWaves * RING * SLOT;
+    constexpr int SUMS = WAVES * NT * 16 * 17 * 4, BYTES = WAVES * RING * SLOT;
     __shared__ __attribute__((aligned(16))) char ring[BYTES > SUMS ? BYTES : SUMS];  // and the sums, afterwards
     extern __shared__ __attribute__((aligned(16))) char coded[];                      // codes [rows][128 KB], scales [rows][KB]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
@@ -94,14 +98,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void fp8_few_kernel(const Fp8Args a
         }
     };
 #pragma unroll
-    for (int i = 0; i < AHEAD; i++) load(wave + kFewWaves * i, i);
+    for (int i = 0; i < AHEAD; i++) load(wave + WAVES * i, i);
     lds_f32* const lds_scales = (lds_f32*)((lds_char*)coded + M * KB * 128);
     if constexpr (!CODED) {
         // 16 lanes a group of 128 values, eight each; what lies past K is a code of 0
         using S = typename XT::storage;
         const S* const x = static_cast<const S*>(few.x) + x_row * args.x_stride;
         const int groups = M * KB;
-        for (int g = threadIdx.x >> 4; g < groups; g += 64 * kFewWaves / 16) {
+        for (int g = threadIdx.x >> 4; g < groups; g += 64 * WAVES / 16) {
             const int m = g / KB, at = (g - m * KB) * 128 + l16 * 8;
             float v[8] = {};
             if (at < K) load8<XT>(x + m * args.x_stride + at, v);
@@ -119,9 +123,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void fp8_few_kernel(const Fp8Args a
     const uint32_t at0 = uint32_t(l16 * 128 + ((quad ^ ((l16 >> 1) & 7)) << 4));  // chunks quad and quad + 4 of row l16
     int slot = 0;
 #pragma unroll 1
-    for (int kb = wave; kb < KB; kb += kFewWaves) {
+    for (int kb = wave; kb < KB; kb += WAVES) {
         const float sw = wsp[kb];
-        load(kb + kFewWaves * AHEAD, slot == 0 ? AHEAD : slot - 1);
+        load(kb + WAVES * AHEAD, slot == 0 ? AHEAD : slot - 1);
         // this block has landed, the AHEAD after it may be on their way
         constexpr int LATER = LOADS * AHEAD;
         static_assert(LATER < 64, "vmcnt range");
@@ -167,12 +171,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void fp8_few_kernel(const Fp8Args a
 #pragma unroll
         for (int r = 0; r < 4; r++) sums[((wave * NT + t) * 16 + l16) * 17 + 4 * quad + r] = acc[t][r];
     __syncthreads();
-    for (int i = threadIdx.x; i < M * NT * 16; i += 64 * kFewWaves) {
+    for (int i = threadIdx.x; i < M * NT * 16; i += 64 * WAVES) {
         const int m = i / (NT * 16), c = i % (NT * 16), n = n0 + c;
         if (n >= N) continue;
         float t = 0.f;
 #pragma unroll
-        for (int w = 0; w < kFewWaves; w++) t += sums[((w * NT + (c >> 4)) * 16 + m) * 17 + (c & 15)];
+        for (int w = 0; w < WAVES; w++) t += sums[((w * NT + (c >> 4)) * 16 + m) * 17 + (c & 15)];
         store_out<YT>(y, int64_t(m) * N + n, t);
     }
 }
@@ -184,27 +188,23 @@ bool fp8_few_takes(int64_t m, int64_t k, int x_dtype) {
     return m <= 4 && m * fp8_blocks(k) * 132 <= kFewLds;
 }
 
-template <int NT>
-static void launch_few(const Fp8Args& a, const Fp8Few& f, int y_dtype, hipStream_t st) {
-    const dim3 grid(unsigned((a.N + 16 * NT - 1) / (16 * NT)), f.ids ? unsigned(a.M) : 1u), block(64 * kFewWaves);
+void launch_fp8_few(const Fp8Args& a, const Fp8Few& f, int y_dtype, hipStream_t st) {
     const int m = f.ids ? 1 : a.M;
+    const unsigned routes = f.ids ? unsigned(a.M) : 1u;
+    auto grid = [&](int rows) { return dim3(unsigned((a.N + rows - 1) / rows), routes); };
+    // (of values, of which each workgroup makes its codes itself, there is nothing to read less often)
+    const bool wide = f.x_dtype == EQ_DTYPE_F8E4M3 && int64_t((a.N + 63) / 64) * routes * 4 >= 3 * device_cu_count();
     with_dtype(y_dtype, [&](auto yt) {
         using YT = decltype(yt);
-        if (f.x_dtype == EQ_DTYPE_F8E4M3) {
-            if (m <= 8) fp8_few_kernel<F8T, YT, NT, 1, NT == 1 ? 3 : 2><<<grid, block, 0, st>>>(a, f);
-            else fp8_few_kernel<F8T, YT, NT, 2, NT == 1 ? 3 : 2><<<grid, block, 0, st>>>(a, f);
-        } else {
+        if (f.x_dtype != EQ_DTYPE_F8E4M3)
             with_dtype(f.x_dtype, [&](auto xt) {
-                fp8_few_kernel<decltype(xt), YT, NT, 0, NT == 1 ? 3 : 2>
-                    <<<grid, block, size_t(m) * size_t(a.KB) * 132, st>>>(a, f);
+                fp8_few_kernel<decltype(xt), YT, 8, 1, 0, 1><<<grid(16), dim3(512), size_t(m) * size_t(a.KB) * 132, st>>>(a, f);
             });
-        }
+        else if (wide && m <= 8) fp8_few_kernel<F8T, YT, 4, 4, 1, 1><<<grid(64), dim3(256), 0, st>>>(a, f);
+        else if (wide) fp8_few_kernel<F8T, YT, 4, 4, 2, 1><<<grid(64), dim3(256), 0, st>>>(a, f);
+        else if (m <= 8) fp8_few_kernel<F8T, YT, 8, 1, 1, 1><<<grid(16), dim3(512), 0, st>>>(a, f);
+        else fp8_few_kernel<F8T, YT, 8, 1, 2, 1><<<grid(16), dim3(512), 0, st>>>(a, f);
     });
-}
-
-void launch_fp8_few(const Fp8Args& a, const Fp8Few& f, int y_dtype, hipStream_t st) {
-    if (a.N > 8192) launch_few<2>(a, f, y_dtype, st);
-    else launch_few<1>(a, f, y_dtype, st);
 }
 
 }  // namespace eq

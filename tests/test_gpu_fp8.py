@@ -242,6 +242,19 @@ def test_matmul_of_16_bit_rows(cuda, m, n, k, dtype):
     near(fp8.matmul(x, w, s), *F.matmul(F.rows_of(*F.quantize(f64(x))), F.weight_of(f64(w), f64(s))), k, dtype)
 
 
+@pytest.mark.parametrize("m,n,k,given", [(1, 14336, 1040, "codes"), (8, 12290, 400, "codes"), (9, 12305, 528, "codes"),
+                                         (16, 20001, 144, "codes"), (4, 9000, 11760, "values"), (3, 40, 14336, "values"),
+                                         (2, 12300, 272, "values"), (1, 33, 46000, "values"), (5, 33, 46000, "codes")])
+def test_matmul_of_few_rows(cuda, m, n, k, given):
+    """64 weight rows to a workgroup, rows that fill what is quantized in the launch and that pass it."""
+    case("few", m, n, k, given)
+    rng = np.random.default_rng(n)
+    x = values(rng, (m, k))
+    w, s = weights(rng, n, k)
+    want = F.matmul(F.rows_of(*F.quantize(f64(x))), F.weight_of(f64(w), f64(s)))
+    near(fp8.matmul(fp8.quantize(x) if given == "codes" else x, w, s, BF), *want, k, BF)
+
+
 @pytest.mark.parametrize("m", [1, 7, 40, 200])
 def test_matmul_of_f32_rows(cuda, m):
     """The codes of f32 rows are those of quantize."""
@@ -268,6 +281,22 @@ def test_matmul_keeps_nan_to_its_row_and_column(cuda, m):
     y = fp8.matmul(fp8.quantize(values(rng, (m, 400))), w, s, BF)
     assert torch.isnan(y[:, 128:256]).all() and torch.isfinite(y[:, :128]).all() and torch.isfinite(y[:, 256:]).all()
     assert torch.isfinite(whole).all()
+
+
+@pytest.mark.parametrize("m", [1, 20, 300])
+def test_matmul_keeps_nan_codes_to_their_rows_and_columns(cuda, m):
+    """e4m3's NaN among the codes of the weight and of a row, the last column of K beside others."""
+    case("matmul nan codes", m)
+    rng = np.random.default_rng(m + 1)
+    x = fp8.quantize(values(rng, (m, 400)))
+    w, s = weights(rng, 300, 400)
+    w.view(torch.uint8)[130, 399] = 0x7f
+    x.codes.view(torch.uint8)[m - 1, 0] = 0xff
+    for dtype in (BF, SF):
+        nan = torch.isnan(fp8.matmul(x, w, s, dtype))
+        want = torch.zeros_like(nan)
+        want[:, 130], want[m - 1] = True, True
+        assert torch.equal(nan, want)
 
 
 @pytest.mark.parametrize("m,n,k", [(3, 50, 272), (40, 200, 528), (150, 129, 400)])
@@ -458,6 +487,60 @@ def test_captured(cuda, m):
             g.replay()
             torch.cuda.synchronize()
             assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]), i
+
+
+def test_a_capture_without_scratch_is_refused(cuda):
+    """Where a stream's workspace would have to grow while it is captured, the C ABI says so and records nothing."""
+    from eredu_amd import _native as n
+
+    case("capture without scratch")
+    L, rng = n.lib(), np.random.default_rng(10)
+    w, s = weights(rng, 300, 1040)
+    x = values(rng, (7000, 1040))
+    y = torch.full((7000, 300), 3.0, dtype=BF, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        y.add_(1.0)
+        status = L.eq_fp8_matmul(y.data_ptr(), x.data_ptr(), 1040, None, 0, w.data_ptr(), s.data_ptr(), 7000, 300, 1040,
+                                 n.EQ_DTYPE_BF16, n.EQ_DTYPE_BF16, None, 0, torch.cuda.current_stream().cuda_stream)
+        said = L.eq_last_error().decode()
+    assert status == 1 and "no workspace" in said
+    g.replay()
+    torch.cuda.synchronize()
+    assert (y == 4).all()
+
+
+def test_two_threads_on_one_stream(cuda):
+    """What a call hands from one of its launches to the next lies in the stream's workspace, and stays its own."""
+    import threading
+
+    case("threads")
+    rng = np.random.default_rng(11)
+    w, s = weights(rng, 640, 2048)
+    bank, bank_scales = weights(rng, 5, 256, 512)
+    jobs = []
+    for m in (90, 333):
+        x, r = values(rng, (m, 2048)), values(rng, (m, 512))
+        ids = ints(rng.integers(-1, 5, m))
+        jobs.append((x, r, ids, fp8.matmul(x, w, s), fp8.grouped_matmul(r, bank, bank_scales, ids)))
+    torch.cuda.synchronize()
+    wrong, go = [], threading.Barrier(2)
+
+    def work(x, r, ids, y, z):
+        go.wait()
+        for i in range(40):
+            if not torch.equal(fp8.matmul(x, w, s), y) or not torch.equal(fp8.grouped_matmul(r, bank, bank_scales, ids), z):
+                wrong.append(i)
+                return
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_two_streams(cuda):
