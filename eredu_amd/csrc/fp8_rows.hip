@@ -40,7 +40,8 @@ __device__ __forceinline__ void put_group(const float* v, bool live, uint2* code
     if (first) *scale = g.scale;
 }
 
-// x, or silu(gate) * up: 16 lanes a group, eight values each; group i of the launch is row i / blocks.
+// x, or silu(gate) * up: 16 lanes a group, eight values each; group i of the launch is row i / blocks.  Bound by
+// memory: silu of 4096 x 14336 59.5 us (294 MB at 4.9 TB/s, a large copy 5.1), quantizing 4096 x 4096 12.5 us.
 template <typename T, bool SILU>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(uint8_t* __restrict__ codes, float* __restrict__ scales,
                                                            int64_t scale_stride,
@@ -65,6 +66,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(uint8_t* __restrict__
               lane == 0 && row < uint32_t(rows));
 }
 
+// Bound by memory (8192 x 4096 with a residual 43.5 us, 235 MB at 5.4 TB/s), a single row of 4096 by a launch, 2.8 us.
 // One row a workgroup.  VPT > 0: a thread keeps its (at most VPT) pieces of
 // eight values in registers between the two passes; 0: any length, read again.
 template <typename T, int VPT>

@@ -134,6 +134,25 @@ def test_scratch_of_float_rows_must_be_enough():
     refused(matmul(m=1000, xd=BF16, sc=None, sp=P + 128, sn=need), "scratch")
 
 
+def test_scratch_is_for_what_a_call_hands_on():
+    """None for rows in codes where K is not split (nor for few rows of values), else codes and scales of the values, and at most
+    16 parts of the result in f32 where it is small."""
+    def q(m, n, k, xd=E4M3, yd=BF16):
+        return L.eq_fp8_matmul_scratch(m, n, k, xd, yd)
+
+    assert q(1, 4096, 4096) == q(16, 128256, 4096) == q(4096, 14336, 4096) == q(1, 4096, 14336, BF16) == q(4, 4096, 4096, F32) == 0
+    assert q(16, 14336, 4096, BF16) == 16 * 4096 + 16 * 32 * 4
+    assert 0 < q(77, 4097, 14320) <= 16 * 77 * 4100 * 4 + 256
+    for m in (17, 33, 64, 100, 300, 1000, 5000):
+        for n in (1, 64, 1000, 4096, 20000):
+            for k in (16, 2048, 14336, 60000):
+                assert 0 <= q(m, n, k) <= 16 * m * (n + 3) * 4 + 256
+                assert q(m, n, k, F16) >= m * k
+    g = L.eq_fp8_grouped_matmul_scratch
+    assert g(1, 128, 8, 768, 2048, BF16, BF16) == 0 and g(64, 128, 64, 768, 2048, E4M3, BF16) == 0
+    assert 4096 * 8 <= g(512, 128, 4096, 768, 2048, E4M3, BF16) <= 4096 * 8 + (128 + 4096 // 32 + 2) * 16 + 512
+
+
 def test_nothing_to_do_is_no_error():
     assert quantize(rows=0, codes=None, x=None, scales=None, ss=0) == 0
     assert weight(rows=0) == 0 and weight(count=0) == 0 and norm(rows=0) == 0 and silu(rows=0) == 0
