@@ -445,7 +445,6 @@ struct Plan {
     size_t bytes() const { return tiles + order + codes + scales + part; }
 };
 
-
 // Us that a product takes in tiles of a shape, `mtiles` rows of them, with K in `splits` parts, joined after
 // them; what the tiles load comes from the caches at `rate` bytes a us, `bytes` of weights at 6 TB/s, which is
 // overlapped with all but a quarter.
@@ -472,7 +471,9 @@ void choose_tiles(Plan& p, int64_t m, int64_t n, int64_t k, int64_t experts, int
         // neighbouring tiles share weights and activations, 11 with routes, measured)
         const int64_t mtiles = experts ? std::max(used, m / s.rows + used * 5 / 8) + 1 : (m + s.rows - 1) / s.rows;
         const int64_t ntiles = (n + s.cols - 1) / s.cols;
-        for (int64_t splits = 1; splits <= 16 && (splits == 1 || blocks / splits >= 4); splits++) {
+        for (int64_t splits = 1; splits <= 16; splits++) {
+            // (parts of four blocks or more, in at most 1 GiB)
+            if (splits > 1 && (blocks / splits < 4 || double(splits) * double(m) * double(n) * 4. > 0x1p30)) break;
             const double us = tiles_us(s, mtiles, ntiles, m, n, blocks, splits, experts ? 11e6 : 17e6, bytes);
             if (best > 0. && us >= best) continue;
             best = us, p.shape = i, p.splits = splits;
@@ -512,8 +513,8 @@ bool dtypes_ok(const char* who, int x_dtype, int y_dtype) {
 }
 
 bool grid_ok(const char* who, const Plan& p) {
-    if (p.mtiles * p.ntiles * p.splits < (int64_t(1) << 23)) return true;  // (fewer than 2^32 threads)
-    set_error(std::string(who) + ": 2^23 tiles of the result or more");
+    if (p.mtiles * p.ntiles * p.splits <= (int64_t(1) << 23) - 8) return true;  // (fewer than 2^32 threads)
+    set_error(std::string(who) + ": more than 2^23 - 8 tiles of the result");
     return false;
 }
 

@@ -109,7 +109,8 @@ SHARED = [
 
 
 @pytest.mark.parametrize("bad,words", SHARED + [(dict(m=-1), "2^30"), (dict(m=1 << 30), "2^30"), (dict(m=1 << 26), "2^26"),
-                                                (dict(m=1 << 25, n=1 << 20), "tiles")])
+                                                (dict(m=1 << 25, n=1 << 20), "tiles"), (dict(m=2, n=1 << 27), "tiles"),
+                                                (dict(m=1 << 21, n=1 << 20, ss=1 << 21), "tiles")])
 def test_matmul_refuses(bad, words):
     refused(matmul(**bad), words)
     sizes = dict(m=4, n=64, k=128, xd=E4M3, yd=BF16)
@@ -148,6 +149,7 @@ def test_scratch_is_for_what_a_call_hands_on():
             for k in (16, 2048, 14336, 60000):
                 assert 0 <= q(m, n, k) <= 16 * m * (n + 3) * 4 + 256
                 assert q(m, n, k, F16) >= m * k
+    assert q(1 << 10, 1 << 18, (1 << 22) - 16) == 0  # (parts of a large result would be larger than it is worth)
     g = L.eq_fp8_grouped_matmul_scratch
     assert g(1, 128, 8, 768, 2048, BF16, BF16) == 0 and g(64, 128, 64, 768, 2048, E4M3, BF16) == 0
     assert 4096 * 8 <= g(512, 128, 4096, 768, 2048, E4M3, BF16) <= 4096 * 8 + (128 + 4096 // 32 + 2) * 16 + 512
@@ -167,6 +169,7 @@ def cpu(*shape, dtype=torch.bfloat16):
 @pytest.mark.parametrize("call,words", [
     (lambda: fp8.quantize(cpu(2, 128).int()), "float32"),
     (lambda: fp8.quantize_weight(cpu(128)), "[..., N, K]"),
+    (lambda: fp8.rms_norm(cpu(2, 64)[0, 0], cpu(64), 1e-5), "one dimension"), (lambda: fp8._rows(cpu(2)[0], "x"), "one dimension"),
     (lambda: fp8.rms_norm(cpu(2, 64), cpu(65), 1e-5), "weight"),
     (lambda: fp8.rms_norm(cpu(2, 64), cpu(64, dtype=torch.float32), 1e-5), "weight"),
     (lambda: fp8.rms_norm(cpu(64, 2).t(), cpu(64), 1e-5), "contiguous"),
