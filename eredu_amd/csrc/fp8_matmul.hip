@@ -35,12 +35,15 @@ typedef __attribute__((address_space(3))) const float lds_f32;
 // activation rows a workgroup.  Both operands go straight from memory to LDS,
 // STAGES blocks of K deep.
 //
-// Row i of a wave's A tile t is its weight row 4 NT (i / 4) + 4 t + i % 4, so that
-// a lane ends with 4 NT consecutive results of its activation row.  A row's 128
-// bytes of a block lie in LDS in slots of 16, chunk c in slot c ^ key: 16 lanes read
+// A lane's four results of a tile are consecutive, and its neighbours of the three other quads have the next ones:
+// row i of a wave's A tile t is its weight row 16 t + i where results are f32, 64 consecutive bytes of a result row to
+// a store, and 32 (t / 2) + 8 (i / 4) + 4 (t % 2) + i % 4 where two tiles make the 16 bytes of a lane.  (With
+// all of a lane's results in one run a store touches each 64 bytes in quarters: f32 results of 2270 x 11264 x 512
+// 51.5 us, this way 41.6; 16-bit ones the same.)
+// A row's 128 bytes of a block lie in LDS in slots of 16, chunk c in slot c ^ key: 16 lanes read
 // 16 rows at one chunk, LDS has 64 banks of 4 bytes (two rows), so the
 // rows of one parity have to differ in their key: (row / 2) % 8 for the
-// activations, (row / 2) % 2 + 2 (row / (4 NT) % 4) for the weights' rows above
+// activations and where A's rows are consecutive, (row / 2) % 2 + 2 (row / 8 % 4) for A's rows of pairs
 // (no bank conflict is counted).
 //
 // What bounds it: of 4096 x 14336 x 4096 (236 us in tiles of 256 x 256, 2.0 PFLOP/s; a library's unscaled fp8
@@ -120,7 +123,7 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(1,
         uint32_t a_off[8], b_off[8], s_off;  // (the first LA and LB used)
         auto a_chunk = [&](int i) __attribute__((always_inline)) {
             const int row = 8 * (LA * wave + i) + (lane >> 3);
-            return (lane & 7) ^ (((row >> 1) & 1) | ((row / (4 * NT)) & 3) << 1);
+            return (lane & 7) ^ (EXACT ? (row >> 1) & 7 : ((row >> 1) & 1) | ((row >> 3) & 3) << 1);
         };
         auto b_chunk = [&](int i) __attribute__((always_inline)) {
             const int row = 8 * (LB * wave + i) + (lane >> 3);
@@ -174,9 +177,11 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(1,
             for (int i = 0; i < LB; i++) b_off[i] = 16 * b_chunk(i) < left ? b_off[i] : kOutOfRange;
         };
 
-        // A: weight row of tile t is a_row + 4 t; B: activation row 16 (MT wm + j) + l16.  Chunks quad and quad + 4.
-        const int a_row = 16 * NT * wn + 4 * NT * (l16 >> 2) + (l16 & 3);
-        const uint32_t a_at = uint32_t(a_row * 128 + ((quad ^ (((l16 >> 1) & 1) | ((l16 >> 2) << 1))) << 4));
+        // A: weight row of tile t is a_row + 16 t, or where results are pieces of eight a_row + 32 (t / 2) + 4 (t % 2);
+        // B: activation row 16 (MT wm + j) + l16.  Chunks quad and quad + 4.
+        const int a_row = 16 * NT * wn + (EXACT ? l16 : 8 * (l16 >> 2) + (l16 & 3));
+        const int a_key = EXACT ? l16 >> 1 : ((l16 >> 1) & 1) | ((l16 >> 2) << 1);
+        const uint32_t a_at = uint32_t(a_row * 128 + ((quad ^ a_key) << 4));
         const uint32_t b_at = uint32_t(TN * 128 + (16 * MT * wm + l16) * 128 + ((quad ^ ((l16 >> 1) & 7)) << 4));
         const uint32_t s_at = uint32_t((TN + TM) * 128 + (16 * MT * wm + l16) * 4);
         // Multiplies a block from one buffer while block kb is loaded into another, a load every EVERY matrix
@@ -191,8 +196,10 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(1,
             };
             read_b(0);
 #pragma unroll
-            for (int t = 0; t < NT; t++)
-                a[t].take(*(lds_u32x4*)(from + a_at + t * 512), *(lds_u32x4*)(from + (a_at ^ 64u) + t * 512));
+            for (int t = 0; t < NT; t++) {
+                const int at = 128 * (EXACT ? 16 * t : 32 * (t / 2) + 4 * (t % 2));
+                a[t].take(*(lds_u32x4*)(from + a_at + at), *(lds_u32x4*)(from + (a_at ^ 64u) + at));
+            }
             // Tile i = NT j + t is multiplied while tile i - LAG's sums, which have arrived by then, are
             // scaled and added (a single wave: 72 cycles a tile with LAG 2, 38 with 3, 32 of them the matrix core's).
             constexpr int LAG = 3;
@@ -258,26 +265,24 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(1,
     }
 
     // Results, or the split's sums.
-    const int n = n0 + 16 * NT * wn + 4 * NT * quad;
+    constexpr int PIECE = EXACT ? 4 : 8;
+    const int n = n0 + 16 * NT * wn + PIECE * quad;
 #pragma unroll
     for (int j = 0; j < MT; j++) {
         const int i = 16 * (MT * wm + j) + l16;
-        if (i < mrows && n < N) {
-            float v[4 * NT];
+        if (i >= mrows) continue;
+        const int64_t row = args.tiles ? args.order[first + i].x : m0 + i;
+        const int ldp = (N + 3) & ~3;  // (of sums: rows of whole float4s)
+        float* const part = args.part + (int64_t(split) * args.M + row) * ldp;
+        typename YT::storage* const y = static_cast<typename YT::storage*>(args.y) + row * N;
 #pragma unroll
-            for (int t = 0; t < NT; t++)
+        for (int p = 0; p < 4 * NT / PIECE; p++) {
+            float v[PIECE];
 #pragma unroll
-                for (int r = 0; r < 4; r++) v[4 * t + r] = acc[t][j][r];
-            const int64_t row = args.tiles ? args.order[first + i].x : m0 + i;
-            if (args.splits > 1) {
-                const int ldp = (N + 3) & ~3;  // (rows of whole float4s)
-                store_run<F32T, 4 * NT>(args.part + (int64_t(split) * args.M + row) * ldp + n, v, ldp - n, true);
-            } else {
-                typename YT::storage* const y = static_cast<typename YT::storage*>(args.y);
-                constexpr int VEC = 16 / int(sizeof(typename YT::storage));
-                store_run<YT, 4 * NT>(y + row * N + n, v, N - n,
-                                      N % VEC == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0);
-            }
+            for (int e = 0; e < PIECE; e++) v[e] = acc[(PIECE * p + e) / 4][j][e % 4];
+            const int at = n + 4 * PIECE * p;
+            if (args.splits > 1) store_run<F32T, PIECE>(part + at, v, ldp - at);
+            else store_run<YT, PIECE>(y + at, v, N - at);
         }
     }
 }
@@ -306,10 +311,7 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(typename YT::storage* __r
     };
     while (s + 4 <= splits) add(std::integral_constant<int, 4>{});
     while (s < splits) add(std::integral_constant<int, 1>{});
-    typename YT::storage* const row = y + int64_t(m) * N;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (n + i < N) store_out<YT>(row, n + i, v[i]);
+    store_run<YT, 4>(y + int64_t(m) * N + n, v, N - n);
 }
 
 // The routes of each expert side by side, and the row tiles that they make
