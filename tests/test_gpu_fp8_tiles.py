@@ -123,3 +123,20 @@ def test_more_routes_than_a_workgroup_keeps(cuda):
             want, size, _ = F.matmul(xd[at[r]:at[r] + 1], wd[ids[r]])
             assert np.all(np.abs(y[r] - want[0]) <= (128 + 2 + 3) * 2.0 ** -23 * size[0] + 2.0 ** -24 * np.abs(want[0]))
         assert np.all(np.abs(y[real]).max(1) > 0)
+
+
+@pytest.mark.parametrize("routes,experts", [(1023, 5), (1025, 300), (16385, 1), (65536, 6), (65537, 1100), (200003, 3)])
+def test_every_route_is_placed_once(cuda, routes, experts):
+    """Routes in one and in several parts, up to more than 64 parts of 1024: each gets its own expert's product of its own row."""
+    case("parts of routes", routes, experts)
+    rng = np.random.default_rng(routes)
+    x, (w, s) = operands(routes, 40, 16, 16, experts)
+    ids, at = rng.integers(-1, experts + 1, routes), rng.integers(-1, 41, routes)
+    y = f64(fp8.grouped_matmul(x, w, s, ints(ids), ints(at), SF))
+    xd, wd = f64(x.dequantize(torch.float64)), F.weight_of(f64(w), f64(s))
+    real = (ids >= 0) & (ids < experts) & (at >= 0) & (at < 40)
+    assert not y[~real].any()
+    e, r = ids[real], at[real]
+    want, size = np.einsum("rk,rnk->rn", xd[r], wd[e]), np.einsum("rk,rnk->rn", np.abs(xd[r]), np.abs(wd[e]))
+    # 16 exact products, summed in f32 with 2^-23 of the sizes a sum, the scales' product and two more roundings
+    assert np.all(np.abs(y[real] - want) <= (16 + 2 + 3) * 2.0 ** -23 * size + 2.0 ** -24 * np.abs(want))
