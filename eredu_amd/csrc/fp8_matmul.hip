@@ -31,6 +31,55 @@ typedef __attribute__((address_space(3))) char lds_char;
 typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) const float lds_f32;
 
+// How `tiles` tiles are dealt out to workgroups of which `slots` run at once (0: no matter): whole ones, but
+// where half of the last round's or more would have none, its tiles are taken in parts of K, `most` at
+// the most, whose sums are joined by a kernel of their own.  Of routes the device alone knows how many tiles there are.
+struct Rounds {
+    int whole, rest = 0, parts = 1;
+    __host__ __device__ Rounds(int tiles, int slots, int most) : whole(tiles) {
+        if (most < 2 || tiles % slots == 0) return;
+        const int left = tiles % slots, fit = slots / left;
+        if (fit < 2) return;
+        rest = left, whole = tiles - left, parts = fit < most ? fit : most;
+    }
+};
+
+// Where tile `tile` of `used` row tiles by args.ntiles lies: in bands of `band` row tiles, column by column in
+// each, so that the tiles that run at once are as many rows as columns and share their operands in the XCD's L2.
+struct TileAt {
+    int n0, first, mrows, expert = 0;  // first: row of x and y, or place in args.order
+    __device__ __forceinline__ TileAt(const Fp8Args& args, int used, int tile, int cols, int rows) {
+        const int band_at = tile / (args.band * args.ntiles), in_band = tile - band_at * args.band * args.ntiles;
+        const int band_rows = min(args.band, used - band_at * args.band);
+        const int tm = band_at * args.band + in_band % band_rows;
+        n0 = in_band / band_rows * cols;
+        if (args.tiles) {
+            const int4 t = args.tiles[tm];
+            expert = t.x, first = t.y, mrows = t.z;
+        } else {
+            first = tm * rows, mrows = min(rows, args.M - first);
+        }
+    }
+};
+
+// A lane's results of a row of a tile, the wave's from column `n` on, in pieces of 16 bytes of 16-bit results or f32.
+template <typename YT, int NT>
+__device__ __forceinline__ void store_rows(const Fp8Args& args, const TileAt& tile, int i, int n, int quad,
+                                           const f32x4* v) {
+    constexpr int PIECE = std::is_same<YT, F32T>::value ? 4 : 8;
+    if (i >= tile.mrows) return;
+    const int64_t row = args.tiles ? args.order[tile.first + i].x : tile.first + i;
+    typename YT::storage* const y = static_cast<typename YT::storage*>(args.y) + row * args.N;
+#pragma unroll
+    for (int p = 0; p < 4 * NT / PIECE; p++) {
+        float w[PIECE];
+#pragma unroll
+        for (int e = 0; e < PIECE; e++) w[e] = v[(PIECE * p + e) / 4][e % 4];
+        const int at = n + PIECE * (4 * p + quad);
+        store_run<YT, PIECE>(y + at, w, args.N - at);
+    }
+}
+
 // WN x WM waves of NT x MT tiles of 16 x 16: 16 NT WN weight rows by 16 MT WM
 // activation rows a workgroup.  Both operands go straight from memory to LDS,
 // STAGES blocks of K deep.
@@ -76,32 +125,27 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(1,
     const int wn = wave % WN, wm = wave / WN, l16 = lane & 15, quad = lane >> 4;
     const int N = args.N, K = args.K;
 
-    // The workgroups of one XCD (id % 8) take a run of tiles.
+    // The workgroups of one XCD (id % 8) take a run of the whole tiles, then one of the last round's parts.
     const int used = args.tiles ? args.tiles[args.mtiles].x : args.mtiles;
-    const int64_t each = int64_t(used) * args.ntiles, total = each * args.splits, run = (total + 7) >> 3;
-    const int64_t id = (blockIdx.x & 7) * run + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= run || id >= total) return;  // (the whole workgroup)
-    const int split = int(id / each);
-    const int64_t tile = id - split * each;
-    // Bands of `band` row tiles, column by column in each: the tiles that run at once are as
-    // many rows as columns, and share their operands in the XCD's L2.
-    const int band = args.band, band_at = int(tile / (int64_t(band) * args.ntiles));
-    const int in_band = int(tile - int64_t(band_at) * band * args.ntiles), band_rows = min(band, used - band_at * band);
-    const int tm = band_at * band + in_band % band_rows, tn = in_band / band_rows, n0 = tn * TN;
-    // Blocks of K: those of this split.
-    const int k_begin = split * args.per, k_end = min(args.KB, k_begin + args.per);
+    const Rounds rounds(used * args.ntiles, args.slots, args.parts);
+    const int whole = (rounds.whole + 7) & ~7;
+    const bool parted = int(blockIdx.x) >= whole;
+    const int at = parted ? blockIdx.x - whole : blockIdx.x, total = parted ? rounds.rest * rounds.parts : rounds.whole;
+    const int run = (total + 7) >> 3, id = (at & 7) * run + (at >> 3);
+    if ((at >> 3) >= run || id >= total) return;  // (the whole workgroup)
+    const int split = parted ? id / rounds.rest : 0, parts = parted ? rounds.parts : 1;
+    const TileAt tile(args, used, parted ? rounds.whole + id - split * rounds.rest : id, TN, TM);
+    const int n0 = tile.n0, mrows = tile.mrows, expert = tile.expert;
+    // Blocks of K: those of this part.
+    const int k_begin = args.KB * split / parts, k_end = args.KB * (split + 1) / parts;
 
-    int m0 = tm * TM, mrows = min(TM, args.M - m0), first = 0, expert = 0;
-    const uint8_t* xp = args.x + m0 * args.x_stride;
-    const float* xsp = args.xs + m0;
-    uint32_t x_bytes = uint32_t(mrows - 1) * uint32_t(args.x_stride) + uint32_t(K);
-    if (args.tiles) {
-        const int4 t = args.tiles[tm];
-        expert = t.x, first = t.y, mrows = t.z;
-        m0 = 0;
-        xp = args.x;
-        xsp = args.xs;
-        x_bytes = uint32_t((args.x_rows - 1) * args.x_stride + K);
+    const uint8_t* xp = args.x;
+    const float* xsp = args.xs;
+    uint32_t x_bytes = uint32_t((args.x_rows - 1) * args.x_stride + K);
+    if (!args.tiles) {
+        xp += tile.first * args.x_stride;
+        xsp += tile.first;
+        x_bytes = uint32_t(mrows - 1) * uint32_t(args.x_stride) + uint32_t(K);
     }
     f32x4 acc[NT][MT];
 #pragma unroll
@@ -133,7 +177,7 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(1,
         auto x_row = [&](int i) __attribute__((always_inline)) {
             if (i >= mrows) return -1;
             if (!args.tiles) return i;
-            return args.order[first + i].y;
+            return args.order[tile.first + i].y;
         };
 #pragma unroll
         for (int i = 0; i < LA; i++) {
@@ -264,54 +308,58 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(1,
         __builtin_amdgcn_s_waitcnt(0x0070);  // (nothing is on its way to LDS when the workgroup ends)
     }
 
-    // Results, or the split's sums.
-    constexpr int PIECE = EXACT ? 4 : 8;
-    const int n = n0 + 16 * NT * wn + PIECE * quad;
+    if (parted) {
+        f32x4* const part = reinterpret_cast<f32x4*>(args.part + int64_t(id) * (TN * TM)) + threadIdx.x;
+#pragma unroll
+        for (int j = 0; j < MT; j++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) part[(j * NT + t) * 64 * WAVES] = acc[t][j];
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < MT; j++) {
-        const int i = 16 * (MT * wm + j) + l16;
-        if (i >= mrows) continue;
-        const int64_t row = args.tiles ? args.order[first + i].x : m0 + i;
-        const int ldp = (N + 3) & ~3;  // (of sums: rows of whole float4s)
-        float* const part = args.part + (int64_t(split) * args.M + row) * ldp;
-        typename YT::storage* const y = static_cast<typename YT::storage*>(args.y) + row * N;
+        f32x4 v[NT];
 #pragma unroll
-        for (int p = 0; p < 4 * NT / PIECE; p++) {
-            float v[PIECE];
-#pragma unroll
-            for (int e = 0; e < PIECE; e++) v[e] = acc[(PIECE * p + e) / 4][j][e % 4];
-            const int at = n + 4 * PIECE * p;
-            if (args.splits > 1) store_run<F32T, PIECE>(part + at, v, ldp - at);
-            else store_run<YT, PIECE>(y + at, v, N - at);
-        }
+        for (int t = 0; t < NT; t++) v[t] = acc[t][j];
+        store_rows<YT, NT>(args, tile, 16 * (MT * wm + j) + l16, n0 + 16 * NT * wn, quad, v);
     }
 }
 
-// y = the splits' sums, in their order: a thread has four results of a row.  Bound by its chain of loads: 3.9 us
-// for 7 parts of 77 x 4097 (7.8 with one part after the other).
-template <typename YT>
-__global__ __launch_bounds__(256) void fp8_join_kernel(typename YT::storage* __restrict__ y,
-                                                       const float* __restrict__ part, int M, int N, int ldp, int splits) {
-    const int quads = ldp / 4;
-    const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
-    const int m = int(at / quads), n = int(at - int64_t(m) * quads) * 4;
-    if (m >= M) return;
-    const float4* p = reinterpret_cast<const float4*>(part + int64_t(m) * ldp + n);
-    const int64_t step = int64_t(M) * quads;
-    float v[4] = {};
+// The last round's tiles: their parts' sums, in their order.  A workgroup has a 1 / MT of a tile, a thread what
+// the tile's thread of its number had of it.  FIGJ.
+template <typename YT, int WN, int WM, int NT, int MT>
+__global__ __launch_bounds__(64 * WN * WM) void fp8_join_kernel(const Fp8Args args) {
+    constexpr int WAVES = WN * WM, TN = 16 * NT * WN, TM = 16 * MT * WM;
+    const int used = args.tiles ? args.tiles[args.mtiles].x : args.mtiles;
+    const Rounds rounds(used * args.ntiles, args.slots, args.parts);
+    const int i = blockIdx.x / MT, j = blockIdx.x - i * MT;
+    if (i >= rounds.rest || rounds.parts == 1) return;
+    const TileAt tile(args, used, rounds.whole + i, TN, TM);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave % WN, wm = wave / WN;
+    const int row = 16 * (MT * wm + j) + (lane & 15);
+    if (row >= tile.mrows) return;
+    const int64_t step = int64_t(rounds.rest) * (TN * TM / 4);
+    const f32x4* p = reinterpret_cast<const f32x4*>(args.part + int64_t(i) * (TN * TM)) + j * NT * 64 * WAVES + threadIdx.x;
+    f32x4 v[NT] = {};
     int s = 0;
     auto add = [&](auto count) __attribute__((always_inline)) {  // several at once: their loads do not wait for each other
         constexpr int C = decltype(count)::value;
-        float4 q[C];
+        f32x4 q[4][NT];
 #pragma unroll
-        for (int i = 0; i < C; i++) q[i] = p[(s + i) * step];
+        for (int c = 0; c < C; c++)
 #pragma unroll
-        for (int i = 0; i < C; i++) v[0] += q[i].x, v[1] += q[i].y, v[2] += q[i].z, v[3] += q[i].w;
+            for (int t = 0; t < NT; t++) q[c][t] = p[(s + c) * step + t * 64 * WAVES];
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) v[t][r] += q[c][t][r];
         s += C;
     };
-    while (s + 4 <= splits) add(std::integral_constant<int, 4>{});
-    while (s < splits) add(std::integral_constant<int, 1>{});
-    store_run<YT, 4>(y + int64_t(m) * N + n, v, N - n);
+    while (s + 4 <= rounds.parts) add(std::integral_constant<int, 4>{});
+    while (s < rounds.parts) add(std::integral_constant<int, 1>{});
+    store_rows<YT, NT>(args, tile, row, tile.n0 + 16 * NT * wn, lane >> 4, v);
 }
 
 // The routes of each expert side by side, and the row tiles that they make
@@ -412,19 +460,28 @@ __global__ __launch_bounds__(1024) void fp8_routes_kernel(int4* __restrict__ til
 
 template <typename YT, int WN, int WM, int NT, int MT, int STAGES>
 void launch_tile(const Fp8Args& a, hipStream_t st) {
-    const int64_t total = (int64_t(a.mtiles) * a.ntiles * a.splits + 7) / 8 * 8;
-    fp8_tile_kernel<YT, WN, WM, NT, MT, STAGES><<<dim3(unsigned(total)), dim3(64 * WN * WM), 0, st>>>(a);
+    // (of routes there are as many row tiles as a.mtiles or fewer)
+    const int tiles = a.mtiles * a.ntiles;
+    const Rounds rounds(tiles, a.slots, a.parts);
+    const bool joined = a.tiles ? a.parts > 1 : rounds.parts > 1;
+    const int total = a.tiles ? tiles + (joined ? a.slots : 0) : ((rounds.whole + 7) & ~7) + rounds.rest * rounds.parts;
+    fp8_tile_kernel<YT, WN, WM, NT, MT, STAGES><<<dim3(unsigned(total + 7) / 8 * 8), dim3(64 * WN * WM), 0, st>>>(a);
+    if (!joined) return;
+    const int rest = a.tiles ? std::min(tiles, a.slots / 2) : rounds.rest;
+    fp8_join_kernel<YT, WN, WM, NT, MT><<<dim3(unsigned(rest * MT)), dim3(64 * WN * WM), 0, st>>>(a);
 }
 
 // The tile shapes, weight rows by activation rows, and what a workgroup of each took (measured over products
-// of 32 .. 4096 rows): us before and after its blocks, us a block alone on its compute unit, and where two share one.
+// of 32 .. 4096 rows): us before and after its blocks, us a block alone on its compute unit, and where two share one; of
+// routes, whose weights are read by few workgroups each and come from memory, so many times as long where
+// two buffers have only one block on its way (1554 routes to 8 experts of 4096 x 14336, 256 x 192: 1.6 us a block).
 struct Shape {
     int cols, rows;
-    float fixed, one, two;  // two 0: a second one does not fit
+    float fixed, one, two, routed;  // two 0: a second one does not fit
 };
-constexpr Shape kShapes[] = {{256, 256, 8.f, 1.5f, 0.f}, {256, 192, 7.f, 1.2f, 0.f}, {256, 128, 5.f, .9f, 0.f},
-                             {128, 128, 2.f, .72f, 1.02f}, {128, 96, 2.f, .5f, 0.f}, {128, 64, 2.f, .38f, .58f},
-                             {128, 32, 2.f, .26f, 0.f}};
+constexpr Shape kShapes[] = {{256, 256, 8.f, 1.5f, 0.f, 1.25f}, {256, 192, 7.f, 1.2f, 0.f, 1.3f}, {256, 128, 5.f, .9f, 0.f, 1.f},
+                             {128, 128, 2.f, .72f, 1.02f, 1.f}, {128, 96, 2.f, .5f, 0.f, 1.f},
+                             {128, 64, 2.f, .38f, .58f, 1.f}, {128, 32, 2.f, .26f, 0.f, 1.f}};
 constexpr int kWide = 3;  // the shapes of 256 weight rows: their f32 results would need more registers than there are
 template <typename YT>
 void launch_tiles(int shape, const Fp8Args& a, hipStream_t st) {
@@ -437,44 +494,52 @@ void launch_tiles(int shape, const Fp8Args& a, hipStream_t st) {
     if (shape == 4) launch_tile<YT, 4, 1, 2, 6, 3>(a, st);
     if (shape == 5) launch_tile<YT, 4, 1, 2, 4, 3>(a, st);
     if (shape == 6) launch_tile<YT, 4, 1, 2, 2, 4>(a, st);
-    if (a.splits > 1) {
-        const int ldp = (a.N + 3) & ~3;
-        const int64_t quads = int64_t(a.M) * (ldp / 4);
-        fp8_join_kernel<YT><<<dim3(unsigned((quads + 255) / 256)), dim3(256), 0, st>>>(
-            static_cast<typename YT::storage*>(a.y), a.part, a.M, a.N, ldp, a.splits);
-    }
 }
 
 size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
 constexpr int kBand = 8;  // row tiles of a band
+constexpr int64_t kMostTiles = (int64_t(1) << 23) - 4096;  // (fewer than 2^32 threads, with a round of parts behind them)
 
 // How a product is done, from its sizes and types alone (the scratch queries
 // and the calls go by the same), and its scratch: lists of routes, the codes and scales of x, sums of splits.
 struct Plan {
     bool few = false;  // fp8_few.hip's kernel, on x as it is where that takes it
     int shape = 0;     // else a tile of kShapes
-    int64_t mtiles = 0, ntiles = 0, splits = 1, per = 0;
+    int64_t mtiles = 0, ntiles = 0, slots = 0, parts = 1;
     size_t tiles = 0, order = 0, codes = 0, scales = 0, part = 0;
     size_t bytes() const { return tiles + order + codes + scales + part; }
 };
 
-// Us that a product takes in tiles of a shape, `mtiles` rows of them, with K in `splits` parts, joined after
-// them; what the tiles load comes from the caches at `rate` bytes a us, `bytes` of weights at 6 TB/s, which is
-// overlapped with all but a quarter.
-double tiles_us(const Shape& s, int64_t mtiles, int64_t ntiles, int64_t m, int64_t n, int64_t blocks, int64_t splits,
-                double rate, double bytes) {
-    const int64_t cus = device_cu_count(), slots = s.two > 0.f ? 2 * cus : cus, work = mtiles * ntiles * splits;
-    const double per = double((blocks + splits - 1) / splits), full = s.fixed + per * (s.two > 0.f ? s.two : s.one);
-    const int64_t rest = work % slots;
-    double us = double(work / slots) * full + (rest == 0 ? 0. : rest <= cus ? s.fixed + per * s.one : full);
-    us = std::max(us, double(work) * per * double(s.cols + s.rows) * 128. / rate);
-    if (splits > 1) us += 4. + double(splits) * double(m) * double(n) * 8. / 6e6;
+int64_t slots_of(const Shape& s) { return int64_t(s.two > 0.f ? 2 : 1) * device_cu_count() & ~int64_t(7); }
+
+// Us that a product takes in `tiles` tiles of a shape, those of the last round in `most` parts of K or
+// fewer; what the tiles load comes from the caches at `rate` bytes a us, `bytes` of weights at 6 TB/s, which is
+// overlapped with all but a quarter.  Of routes `tiles` is a guess.
+double tiles_us(const Shape& s, int64_t tiles, int64_t blocks, int64_t most, double rate, double bytes, bool routed) {
+    const int64_t slots = slots_of(s), cus = device_cu_count();
+    auto took = [&](int64_t at_once, int64_t per) {
+        return s.fixed + double(per) * (at_once > cus ? s.two : s.one) * (routed ? s.routed : 1.f);
+    };
+    const double unit = double(s.cols) * s.rows * 8. / 6e6;  // a part's sums, written and read (their kernel and its launch: 8)
+    double us;
+    if (routed && tiles > slots) {
+        // half of the slots in the last round, or a quarter in parts
+        us = double(tiles) / double(slots) * took(slots, blocks);
+        us += most > 1 ? took(cus, blocks / std::min<int64_t>(most, 4)) + 8. + double(slots) * unit : .5 * took(slots, blocks);
+    } else {
+        const Rounds r{int(tiles), int(slots), int(most)};
+        const int64_t parts = int64_t(r.rest) * r.parts;
+        us = double(r.whole / slots) * took(slots, blocks);
+        if (r.whole % slots) us += took(r.whole % slots, blocks);
+        if (parts) us += took(parts, (blocks + r.parts - 1) / r.parts) + 8. + double(parts) * unit;
+    }
+    us = std::max(us, double(tiles * blocks) * double(s.cols + s.rows) * 128. / rate);
     const double read = bytes / 6e6;
     return std::max(us, read) + .25 * std::min(us, read);
 }
 
-// The shape and the splits of K of a product of m rows, in experts or not, and its tiles.
+// The shape of a product of m rows, in experts or not, its tiles and the parts of the last round's.
 void choose_tiles(Plan& p, int64_t m, int64_t n, int64_t k, int64_t experts, int y_dtype) {
     const int64_t blocks = fp8_blocks(k), used = experts ? std::min(experts, m) : 1;
     const double bytes = double(used) * double(n) * double(k);
@@ -484,21 +549,24 @@ void choose_tiles(Plan& p, int64_t m, int64_t n, int64_t k, int64_t experts, int
         // (how the routes are spread is not known here: more than half a tile more for each expert; 17 TB/s where
         // neighbouring tiles share weights and activations, 11 with routes, measured)
         const int64_t mtiles = experts ? std::max(used, m / s.rows + used * 5 / 8) + 1 : (m + s.rows - 1) / s.rows;
-        const int64_t ntiles = (n + s.cols - 1) / s.cols;
-        for (int64_t splits = 1; splits <= 16; splits++) {
-            // (parts of four blocks or more, in at most 1 GiB)
-            if (splits > 1 && (blocks / splits < 4 || double(splits) * double(m) * double(n) * 4. > 0x1p30)) break;
-            const double us = tiles_us(s, mtiles, ntiles, m, n, blocks, splits, experts ? 11e6 : 17e6, bytes);
+        const int64_t tiles = mtiles * ((n + s.cols - 1) / s.cols);
+        for (int64_t most = 1; most <= 16 && (most == 1 || blocks / most >= 4); most++) {  // (parts of four blocks or more)
+            const double us = tiles_us(s, std::min(tiles, kMostTiles), blocks, most, experts ? 11e6 : 17e6, bytes, experts > 0);
             if (best > 0. && us >= best) continue;
-            best = us, p.shape = i, p.splits = splits;
+            best = us, p.shape = i, p.parts = most;
         }
     }
     const Shape& s = kShapes[p.shape];
     p.mtiles = experts ? std::min(m, m / s.rows + experts + 1) : (m + s.rows - 1) / s.rows;
     p.ntiles = (n + s.cols - 1) / s.cols;
-    p.per = (blocks + p.splits - 1) / p.splits;
-    p.splits = (blocks + p.per - 1) / p.per;
-    if (p.splits > 1) p.part = round256(size_t(p.splits) * size_t(m) * size_t((n + 3) & ~int64_t(3)) * 4u);
+    p.slots = slots_of(s);
+    if (p.parts > 1) {
+        // (a round's parts are as many as its slots or fewer)
+        const int64_t tiles = std::min(p.mtiles * p.ntiles, kMostTiles);
+        const Rounds r{int(tiles), int(p.slots), int(p.parts)};
+        const int64_t units = experts ? std::min(p.slots, tiles * p.parts) : r.rest * r.parts;
+        p.part = round256(size_t(units) * size_t(s.cols * s.rows) * 4u);
+    }
 }
 
 bool sizes_ok(const char* who, int64_t rows, int64_t n, int64_t k) {
@@ -527,8 +595,8 @@ bool dtypes_ok(const char* who, int x_dtype, int y_dtype) {
 }
 
 bool grid_ok(const char* who, const Plan& p) {
-    if (p.mtiles * p.ntiles * p.splits <= (int64_t(1) << 23) - 8) return true;  // (fewer than 2^32 threads)
-    set_error(std::string(who) + ": more than 2^23 - 8 tiles of the result");
+    if (p.mtiles * p.ntiles <= kMostTiles) return true;
+    set_error(std::string(who) + ": more than 2^23 - 4096 tiles of the result");
     return false;
 }
 
@@ -644,7 +712,7 @@ extern "C" int eq_fp8_matmul(void* y, const void* x, int64_t x_stride, const flo
     a.w = static_cast<const uint8_t*>(w);
     a.ws = w_scales;
     a.M = int(m), a.N = int(n), a.K = int(k), a.KB = int(fp8_blocks(k));
-    a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles), a.band = kBand, a.splits = int(p.splits), a.per = int(p.per);
+    a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles), a.band = kBand, a.slots = int(p.slots), a.parts = int(p.parts);
     x_dtype = take_x(a, base, p, x, x_stride, x_scales, scale_stride, m, k, x_dtype, st);
     if (p.few) {
         launch_fp8_few(a, Fp8Few{x, x_dtype, nullptr, 1}, y_dtype, st);
@@ -694,7 +762,7 @@ extern "C" int eq_fp8_grouped_matmul(void* y, const void* x, int64_t x_stride, c
     a.w = static_cast<const uint8_t*>(w);
     a.ws = w_scales;
     a.M = int(routes), a.N = int(n), a.K = int(k), a.KB = int(fp8_blocks(k));
-    a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles), a.band = kBand, a.splits = int(p.splits), a.per = int(p.per);
+    a.mtiles = int(p.mtiles), a.ntiles = int(p.ntiles), a.band = kBand, a.slots = int(p.slots), a.parts = int(p.parts);
     a.rows = rows, a.x_rows = x_rows;
     x_dtype = take_x(a, base + p.tiles + p.order, p, x, x_stride, x_scales, scale_stride, x_rows, k, x_dtype, st);
     if (p.few) {

@@ -17,8 +17,9 @@ struct Fp8Args {
     const uint8_t* w;
     const float* ws;
     int M, N, K, KB;  // KB: blocks of K
-    int mtiles, ntiles, band, splits, per;  // tiles; splits of K, of `per` blocks each
-    float* part;                            // their sums [splits][M][N]
+    int mtiles, ntiles, band;  // tiles
+    int slots, parts;          // workgroups that run at once, and the most parts of K that a tile of the last round makes
+    float* part;               // the parts' sums
     // Grouped: tiles[i] = {expert, first, rows} of row tile i, the rows being order[first ..], {route, row of x};
     // tiles[mtiles].x: how many there are.  Expert -1: rows of zeros.
     const int4* tiles;

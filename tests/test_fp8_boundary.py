@@ -137,17 +137,18 @@ def test_scratch_of_float_rows_must_be_enough():
 
 def test_scratch_is_for_what_a_call_hands_on():
     """None for rows in codes where K is not split (nor for few rows of values), else codes and scales of the values, and at most
-    16 parts of the result in f32 where it is small."""
+    16 parts of the result's tiles in f32 (whole tiles, of 256 x 256 or fewer), never more than a round of them."""
     def q(m, n, k, xd=E4M3, yd=BF16):
         return L.eq_fp8_matmul_scratch(m, n, k, xd, yd)
 
     assert q(1, 4096, 4096) == q(16, 128256, 4096) == q(4096, 14336, 4096) == q(1, 4096, 14336, BF16) == q(4, 4096, 4096, F32) == 0
     assert q(16, 14336, 4096, BF16) == 16 * 4096 + 16 * 32 * 4
-    assert 0 < q(77, 4097, 14320) <= 16 * 77 * 4100 * 4 + 256
+    assert 0 < q(77, 4097, 14320) <= 16 * 128 * 4224 * 4
     for m in (17, 33, 64, 100, 300, 1000, 5000):
         for n in (1, 64, 1000, 4096, 20000):
             for k in (16, 2048, 14336, 60000):
-                assert 0 <= q(m, n, k) <= 16 * m * (n + 3) * 4 + 256
+                # (256 workgroups with a tile of 256 x 256 each: 64 MiB)
+                assert 0 <= q(m, n, k) <= min(16 * -(-m // 256) * -(-n // 256) * 256 * 256 * 4, 64 << 20)
                 assert q(m, n, k, F16) >= m * k
     assert q(1 << 10, 1 << 18, (1 << 22) - 16) == 0  # (parts of a large result would be larger than it is worth)
     g = L.eq_fp8_grouped_matmul_scratch
