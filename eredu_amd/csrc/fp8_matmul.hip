@@ -326,7 +326,8 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(1,
 }
 
 // The last round's tiles: their parts' sums, in their order.  A workgroup has a 1 / MT of a tile, a thread what
-// the tile's thread of its number had of it.  FIGJ.
+// the tile's thread of its number had of it.  Bound by its chain of loads: 4.0 us for 7 parts of 77 x 4097, 4.7 behind
+// 1554 routes of 4096.
 template <typename YT, int WN, int WM, int NT, int MT>
 __global__ __launch_bounds__(64 * WN * WM) void fp8_join_kernel(const Fp8Args args) {
     constexpr int WAVES = WN * WM, TN = 16 * NT * WN, TM = 16 * MT * WM;

@@ -53,7 +53,8 @@ def check(y, x, w, s, rng, dtype):
     (512, 14336, 4096, BF), (380, 12799, 4112, HF),        # 256 x 128
     (700, 9001, 2000, BF), (1024, 14336, 1040, SF),        # 128 x 128
     (190, 14336, 2064, BF), (80, 4097, 14320, HF), (77, 4097, 14320, SF),  # 128 x 96, the second and third with K in 7 parts
-    (250, 14000, 1040, BF), (256, 4096, 8208, BF),         # 128 x 64, the second with split K
+    (250, 14000, 1040, BF),                                # 128 x 64
+    (256, 4096, 8208, BF),
     (90, 130, 8208, BF), (97, 4097, 3088, HF), (90, 131, 8208, SF),        # 128 x 32, the first and last with split K
 ])
 def test_shapes(cuda, m, n, k, dtype):
@@ -63,13 +64,10 @@ def test_shapes(cuda, m, n, k, dtype):
 
 
 @pytest.mark.parametrize("routes,experts,n,k,dtype", [
-    (2300, 8, 4100, 2064, BF),   # 256 x 256
-    (1554, 8, 4096, 4112, BF),   # 256 x 192
-    (900, 4, 4000, 4112, HF),    # 256 x 128
-    (3000, 3, 2000, 272, BF),    # 128 x 128
+    (1554, 8, 4096, 4112, BF), (900, 4, 4000, 4112, HF),  # 256 x 128
+    (2300, 8, 4100, 2064, BF), (3000, 3, 2000, 272, BF),  # 128 x 128
     (800, 2, 3000, 4112, BF),    # 128 x 96
-    (800, 2, 1500, 4112, SF), (4096, 128, 768, 2048, BF),  # 128 x 64
-    (700, 20, 1000, 272, BF),    # 128 x 32
+    (800, 2, 1500, 4112, SF), (4096, 128, 768, 2048, BF), (700, 20, 1000, 272, BF),  # 128 x 64
 ])
 def test_shapes_of_routes(cuda, routes, experts, n, k, dtype):
     """Experts of very different numbers of routes (one has none), rows of x named twice, some routes without an expert."""
@@ -87,6 +85,31 @@ def test_shapes_of_routes(cuda, routes, experts, n, k, dtype):
         src = torch.from_numpy(at[mine]).cuda()
         check(y[torch.from_numpy(mine).cuda()], fp8.Fp8Rows(x.codes.view(torch.uint8)[src].view(fp8.CODE_DTYPE), x.scales[src]),
               w[e], s[e], rng, dtype)
+
+
+@pytest.mark.parametrize("m,n,k,dtype", [
+    (466, 9729, 11744, BF), (2478, 6758, 3984, HF),   # 256 x 256, the second of each line behind whole rounds
+    (556, 6955, 13088, HF), (2579, 6894, 10000, BF),  # 256 x 192
+    (1372, 1536, 12560, BF), (863, 9500, 9872, HF),   # 256 x 128
+    (375, 10804, 12560, BF), (2195, 3857, 4784, SF),  # 128 x 128
+    (66, 5554, 10288, HF),                            # 128 x 96
+    (826, 134, 9280, BF), (2381, 1723, 4224, HF), (2571, 1766, 5472, SF),  # 128 x 64
+    (29, 130, 4816, BF), (21, 236, 5040, SF),         # 128 x 32
+])
+def test_parts_of_the_last_round(cuda, m, n, k, dtype):
+    test_shapes(cuda, m, n, k, dtype)
+
+
+@pytest.mark.parametrize("routes,experts,n,k,dtype", [
+    (1660, 3, 7849, 1312, BF), (957, 5, 8098, 1232, HF),  # 256 x 256, 256 x 192, whole tiles
+    (322, 2, 7487, 12864, BF), (1554, 8, 4096, 14336, BF),  # 256 x 128, the second with more tiles than workgroups at once
+    (3010, 2, 391, 12160, HF), (577, 2, 2306, 14128, SF),  # 128 x 128
+    (473, 2, 676, 11408, BF), (3838, 3, 191, 7984, SF),  # 128 x 96
+    (1188, 2, 155, 7376, BF), (1075, 2, 198, 8800, SF),  # 128 x 64
+    (84, 5, 201, 5472, HF), (115, 2, 130, 5552, SF),  # 128 x 32
+])
+def test_parts_of_the_last_round_of_routes(cuda, routes, experts, n, k, dtype):
+    test_shapes_of_routes(cuda, routes, experts, n, k, dtype)
 
 
 def test_a_bank_of_over_2_31_bytes(cuda):
