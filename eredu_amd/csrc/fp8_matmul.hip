@@ -364,13 +364,14 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_join_kernel(const Fp8Args ar
 }
 
 // The routes of each expert side by side, and the row tiles that they make
-// (fp8_tile_kernel's `tiles` and `order`).  Routes without an expert or a row come last, as expert -1.  Their places
-// within an expert are not in order, which no result depends on.
-// A workgroup places `chunk` routes (a multiple of 1024).  It counts all of them, those before its own
-// apart, so that it needs nothing of another one: counting is the cheaper part, scattered stores the other.
+// (fp8_tile_kernel's `tiles` and `order`).  Routes without an expert or a row come last, as expert -1.  An expert's
+// routes stay in their order: which tile a route is in can decide in how many parts its products are summed.
+// A workgroup places `chunk` routes (a multiple of 256).  It counts all of them, those before its own
+// apart, so that it needs nothing of another one.  It places 64 after 64, whose order among themselves they find by
+// comparing the bits of their experts' numbers.
 // Neighbouring routes of one expert are counted by one of them (sorted routes would else queue for one counter).
-// A chain of loads, counting, sums and stores bounds it, a launch of 2.5 us included: 3.9 us for 100 routes, 5.5 for 4096 of 128
-// experts, 9.8 for 16384, 16.6 for 40000 (one workgroup for all: 4.0, 6.2, 17, 42).
+// A chain of loads, counting, sums and stores bounds it, a launch of 2.5 us included: 4.2 us for 100 routes, 6.0 for 4096 of 128
+// experts, 9.2 for 16384, 18 for 40000 (one workgroup for all, in any order: 4.0, 6.2, 17, 42).
 __global__ __launch_bounds__(1024) void fp8_routes_kernel(int4* __restrict__ tiles, int2* __restrict__ order,
                                                           const int32_t* __restrict__ ids,
                                                           const int32_t* __restrict__ rows, int routes, int chunk,
@@ -391,16 +392,13 @@ __global__ __launch_bounds__(1024) void fp8_routes_kernel(int4* __restrict__ til
         if (r >= routes) return -1;
         return uint32_t(e) < uint32_t(experts) && row >= 0 && row < x_rows ? e : experts;
     };
-    // This lane's place among the counter's: the first of a run of lanes with one counter counts them all.
-    auto take = [&](int* counters, int b) __attribute__((always_inline)) {
+    // The first of a run of lanes with one counter counts them all.
+    auto add = [&](int* counters, int b) __attribute__((always_inline)) {
         const int ahead = __shfl_up(b, 1);
-        const uint64_t heads = __ballot(lane == 0 || b != ahead);
-        const uint64_t upto = heads & (~uint64_t(0) >> (63 - lane)), behind = lane == 63 ? 0 : heads >> (lane + 1);
-        const int head = 63 - __clzll((long long)upto);
-        const int run = behind ? __ffsll((unsigned long long)behind) : 64 - lane;  // (of a head)
-        int at = 0;
-        if (head == lane && b >= 0) at = atomicAdd(&counters[b], run);
-        return __shfl(at, head) + lane - head;
+        const bool head = lane == 0 || b != ahead;
+        const uint64_t heads = __ballot(head), behind = lane == 63 ? 0 : heads >> (lane + 1);
+        const int run = behind ? __ffsll((unsigned long long)behind) : 64 - lane;
+        if (head && b >= 0) atomicAdd(&counters[b], run);
     };
     constexpr int STEP = 4;  // steps of 1024 routes whose loads are on their way together
     for (int e = threadIdx.x; e <= experts; e += 1024) before[e] = rest[e] = 0;
@@ -416,7 +414,7 @@ __global__ __launch_bounds__(1024) void fp8_routes_kernel(int4* __restrict__ til
 #pragma unroll
         for (int i = 0; i < STEP; i++) {
             const int r = r0 + 1024 * i;
-            if (r < routes) take(r < begin ? before : rest, bucket(r + threadIdx.x, e[i], row[i]));
+            if (r < routes) add(r + 64 * wave < begin ? before : rest, bucket(r + threadIdx.x, e[i], row[i]));
         }
     }
     __syncthreads();
@@ -450,11 +448,28 @@ __global__ __launch_bounds__(1024) void fp8_routes_kernel(int4* __restrict__ til
         __syncthreads();
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) tiles[mtiles] = make_int4(base[1], 0, 0, 0);
+    const int bits = 32 - __clz(experts);
 #pragma unroll 1
-    for (int r0 = begin; r0 < end; r0 += 1024) {
+    for (int r0 = begin; r0 < end; r0 += 256) {
         const int r = r0 + threadIdx.x;
         if (r0 > begin) fetch(r, own, own_row);
-        const int b = bucket(r, own, own_row), at = take(before, b);
+        const int b = wave < 4 ? bucket(r, own, own_row) : -1;
+        uint64_t same = __ballot(b >= 0);
+        for (int i = 0; i < bits; i++) {
+            const bool bit = b >> i & 1;
+            const uint64_t with = __ballot(bit);
+            same &= bit ? with : ~with;
+        }
+        const int rank = __popcll(same & ((uint64_t(1) << lane) - 1));
+        int at = 0;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            if (wave == w && b >= 0) {
+                at = before[b] + rank;
+                if (rank == 0) before[b] = at + __popcll(same);
+            }
+            __syncthreads();
+        }
         if (b >= 0) order[at] = make_int2(r, b < experts ? own_row : -1);
     }
 }
@@ -773,7 +788,7 @@ extern "C" int eq_fp8_grouped_matmul(void* y, const void* x, int64_t x_stride, c
     a.tiles = reinterpret_cast<const int4*>(base);
     a.order = reinterpret_cast<const int2*>(base + p.tiles);
     // (64 workgroups at the most, each of which counts all routes)
-    const int64_t chunk = (routes + 65535) / 65536 * 1024;
+    const int64_t chunk = (routes + 16383) / 16384 * 256;
     fp8_routes_kernel<<<dim3(unsigned((routes + chunk - 1) / chunk)), dim3(1024), size_t(2 * (experts + 1)) * 4u, st>>>(
         reinterpret_cast<int4*>(base), reinterpret_cast<int2*>(base + p.tiles), ids, rows, int(routes), int(chunk),
         int(experts), x_rows, kShapes[p.shape].rows, a.mtiles);

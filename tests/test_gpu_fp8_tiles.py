@@ -163,3 +163,20 @@ def test_every_route_is_placed_once(cuda, routes, experts):
     want, size = np.einsum("rk,rnk->rn", xd[r], wd[e]), np.einsum("rk,rnk->rn", np.abs(xd[r]), np.abs(wd[e]))
     # 16 exact products, summed in f32 with 2^-23 of the sizes a sum, the scales' product and two more roundings
     assert np.all(np.abs(y[real] - want) <= (16 + 2 + 3) * 2.0 ** -23 * size + 2.0 ** -24 * np.abs(want))
+
+
+def test_routes_give_the_same_bits_every_time(cuda):
+    """Unsorted routes of which some experts' last tiles are taken in parts of K: their places do not depend on who comes first."""
+    case("repeated routes")
+    x, (w, s) = operands(8, 300, 3000, 12864, 3)
+    rng = np.random.default_rng(8)
+    ids, at = ints(rng.integers(0, 3, 1100)), ints(rng.integers(0, 300, 1100))
+    want = fp8.grouped_matmul(x, w, s, ids, at, BF)
+    for _ in range(6):
+        assert torch.equal(fp8.grouped_matmul(x, w, s, ids, at, BF), want)
+    for e in range(3):
+        mine = torch.nonzero(ids == e)[:, 0]
+        xd, wd = x.dequantize(torch.float64)[at[mine].long()], wide(w[e], s[e])
+        size = xd.abs() @ wd.abs().T
+        bound = ((128 + 12864 / 128 + 3) * 2.0 ** -23 + 7 * 2.0 ** -13) * size + ROUND[BF] * (xd @ wd.T).abs() + 2.0 ** -25
+        assert ((want[mine].double() - xd @ wd.T).abs() <= bound).all()
