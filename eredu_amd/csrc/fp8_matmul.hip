@@ -31,12 +31,12 @@ typedef __attribute__((address_space(3))) char lds_char;
 typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) const float lds_f32;
 
-// How `tiles` tiles are dealt out to workgroups of which `slots` run at once (0: no matter): whole ones, but
-// where half of the last round's or more would have none, its tiles are taken in parts of K, `most` at
+// How `tiles` tiles are dealt out to workgroups of which `slots` run at once, a pass: whole ones, but
+// where half of the last pass's or more would have none, its tiles are taken in parts of K, `most` at
 // the most, whose sums are joined by a kernel of their own.  Of routes the device alone knows how many tiles there are.
-struct Rounds {
+struct Passes {
     int whole, rest = 0, parts = 1;
-    __host__ __device__ Rounds(int tiles, int slots, int most) : whole(tiles) {
+    __host__ __device__ Passes(int tiles, int slots, int most) : whole(tiles) {
         if (most < 2 || tiles % slots == 0) return;
         const int left = tiles % slots, fit = slots / left;
         if (fit < 2) return;
@@ -125,16 +125,16 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(1,
     const int wn = wave % WN, wm = wave / WN, l16 = lane & 15, quad = lane >> 4;
     const int N = args.N, K = args.K;
 
-    // The workgroups of one XCD (id % 8) take a run of the whole tiles, then one of the last round's parts.
+    // The workgroups of one XCD (id % 8) take a run of the whole tiles, then one of the last pass's parts.
     const int used = args.tiles ? args.tiles[args.mtiles].x : args.mtiles;
-    const Rounds rounds(used * args.ntiles, args.slots, args.parts);
-    const int whole = (rounds.whole + 7) & ~7;
+    const Passes passes(used * args.ntiles, args.slots, args.parts);
+    const int whole = (passes.whole + 7) & ~7;
     const bool parted = int(blockIdx.x) >= whole;
-    const int at = parted ? blockIdx.x - whole : blockIdx.x, total = parted ? rounds.rest * rounds.parts : rounds.whole;
+    const int at = parted ? blockIdx.x - whole : blockIdx.x, total = parted ? passes.rest * passes.parts : passes.whole;
     const int run = (total + 7) >> 3, id = (at & 7) * run + (at >> 3);
     if ((at >> 3) >= run || id >= total) return;  // (the whole workgroup)
-    const int split = parted ? id / rounds.rest : 0, parts = parted ? rounds.parts : 1;
-    const TileAt tile(args, used, parted ? rounds.whole + id - split * rounds.rest : id, TN, TM);
+    const int split = parted ? id / passes.rest : 0, parts = parted ? passes.parts : 1;
+    const TileAt tile(args, used, parted ? passes.whole + id - split * passes.rest : id, TN, TM);
     const int n0 = tile.n0, mrows = tile.mrows, expert = tile.expert;
     // Blocks of K: those of this part.
     const int k_begin = args.KB * split / parts, k_end = args.KB * (split + 1) / parts;
@@ -325,21 +325,21 @@ __global__ __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(1,
     }
 }
 
-// The last round's tiles: their parts' sums, in their order.  A workgroup has a 1 / MT of a tile, a thread what
+// The last pass's tiles: their parts' sums, in their order.  A workgroup has a 1 / MT of a tile, a thread what
 // the tile's thread of its number had of it.  Bound by its chain of loads: 4.0 us for 7 parts of 77 x 4097, 4.7 behind
 // 1554 routes of 4096.
 template <typename YT, int WN, int WM, int NT, int MT>
 __global__ __launch_bounds__(64 * WN * WM) void fp8_join_kernel(const Fp8Args args) {
     constexpr int WAVES = WN * WM, TN = 16 * NT * WN, TM = 16 * MT * WM;
     const int used = args.tiles ? args.tiles[args.mtiles].x : args.mtiles;
-    const Rounds rounds(used * args.ntiles, args.slots, args.parts);
+    const Passes passes(used * args.ntiles, args.slots, args.parts);
     const int i = blockIdx.x / MT, j = blockIdx.x - i * MT;
-    if (i >= rounds.rest || rounds.parts == 1) return;
-    const TileAt tile(args, used, rounds.whole + i, TN, TM);
+    if (i >= passes.rest || passes.parts == 1) return;
+    const TileAt tile(args, used, passes.whole + i, TN, TM);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave % WN, wm = wave / WN;
     const int row = 16 * (MT * wm + j) + (lane & 15);
     if (row >= tile.mrows) return;
-    const int64_t step = int64_t(rounds.rest) * (TN * TM / 4);
+    const int64_t step = int64_t(passes.rest) * (TN * TM / 4);
     const f32x4* p = reinterpret_cast<const f32x4*>(args.part + int64_t(i) * (TN * TM)) + j * NT * 64 * WAVES + threadIdx.x;
     f32x4 v[NT] = {};
     int s = 0;
@@ -358,8 +358,8 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_join_kernel(const Fp8Args ar
                 for (int r = 0; r < 4; r++) v[t][r] += q[c][t][r];
         s += C;
     };
-    while (s + 4 <= rounds.parts) add(std::integral_constant<int, 4>{});
-    while (s < rounds.parts) add(std::integral_constant<int, 1>{});
+    while (s + 4 <= passes.parts) add(std::integral_constant<int, 4>{});
+    while (s < passes.parts) add(std::integral_constant<int, 1>{});
     store_rows<YT, NT>(args, tile, row, tile.n0 + 16 * NT * wn, lane >> 4, v);
 }
 
@@ -478,12 +478,12 @@ template <typename YT, int WN, int WM, int NT, int MT, int STAGES>
 void launch_tile(const Fp8Args& a, hipStream_t st) {
     // (of routes there are as many row tiles as a.mtiles or fewer)
     const int tiles = a.mtiles * a.ntiles;
-    const Rounds rounds(tiles, a.slots, a.parts);
-    const bool joined = a.tiles ? a.parts > 1 : rounds.parts > 1;
-    const int total = a.tiles ? tiles + (joined ? a.slots : 0) : ((rounds.whole + 7) & ~7) + rounds.rest * rounds.parts;
+    const Passes passes(tiles, a.slots, a.parts);
+    const bool joined = a.tiles ? a.parts > 1 : passes.parts > 1;
+    const int total = a.tiles ? tiles + (joined ? a.slots : 0) : ((passes.whole + 7) & ~7) + passes.rest * passes.parts;
     fp8_tile_kernel<YT, WN, WM, NT, MT, STAGES><<<dim3(unsigned(total + 7) / 8 * 8), dim3(64 * WN * WM), 0, st>>>(a);
     if (!joined) return;
-    const int rest = a.tiles ? std::min(tiles, a.slots / 2) : rounds.rest;
+    const int rest = a.tiles ? std::min(tiles, a.slots / 2) : passes.rest;
     fp8_join_kernel<YT, WN, WM, NT, MT><<<dim3(unsigned(rest * MT)), dim3(64 * WN * WM), 0, st>>>(a);
 }
 
@@ -515,7 +515,7 @@ void launch_tiles(int shape, const Fp8Args& a, hipStream_t st) {
 size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
 constexpr int kBand = 8;  // row tiles of a band
-constexpr int64_t kMostTiles = (int64_t(1) << 23) - 4096;  // (fewer than 2^32 threads, with a round of parts behind them)
+constexpr int64_t kMostTiles = (int64_t(1) << 23) - 4096;  // (fewer than 2^32 threads, with a pass of parts behind them)
 
 // How a product is done, from its sizes and types alone (the scratch queries
 // and the calls go by the same), and its scratch: lists of routes, the codes and scales of x, sums of splits.
@@ -529,7 +529,7 @@ struct Plan {
 
 int64_t slots_of(const Shape& s) { return int64_t(s.two > 0.f ? 2 : 1) * device_cu_count() & ~int64_t(7); }
 
-// Us that a product takes in `tiles` tiles of a shape, those of the last round in `most` parts of K or
+// Us that a product takes in `tiles` tiles of a shape, those of the last pass in `most` parts of K or
 // fewer; what the tiles load comes from the caches at `rate` bytes a us, `bytes` of weights at 6 TB/s, which is
 // overlapped with all but a quarter.  Of routes `tiles` is a guess.
 double tiles_us(const Shape& s, int64_t tiles, int64_t blocks, int64_t most, double rate, double bytes, bool routed) {
@@ -540,11 +540,11 @@ double tiles_us(const Shape& s, int64_t tiles, int64_t blocks, int64_t most, dou
     const double unit = double(s.cols) * s.rows * 8. / 6e6;  // a part's sums, written and read (their kernel and its launch: 8)
     double us;
     if (routed && tiles > slots) {
-        // half of the slots in the last round, or a quarter in parts
+        // half of the slots in the last pass, or a quarter in parts
         us = double(tiles) / double(slots) * took(slots, blocks);
         us += most > 1 ? took(cus, blocks / std::min<int64_t>(most, 4)) + 8. + double(slots) * unit : .5 * took(slots, blocks);
     } else {
-        const Rounds r{int(tiles), int(slots), int(most)};
+        const Passes r{int(tiles), int(slots), int(most)};
         const int64_t parts = int64_t(r.rest) * r.parts;
         us = double(r.whole / slots) * took(slots, blocks);
         if (r.whole % slots) us += took(r.whole % slots, blocks);
@@ -555,7 +555,7 @@ double tiles_us(const Shape& s, int64_t tiles, int64_t blocks, int64_t most, dou
     return std::max(us, read) + .25 * std::min(us, read);
 }
 
-// The shape of a product of m rows, in experts or not, its tiles and the parts of the last round's.
+// The shape of a product of m rows, in experts or not, its tiles and the parts of the last pass's.
 void choose_tiles(Plan& p, int64_t m, int64_t n, int64_t k, int64_t experts, int y_dtype) {
     const int64_t blocks = fp8_blocks(k), used = experts ? std::min(experts, m) : 1;
     const double bytes = double(used) * double(n) * double(k);
@@ -577,9 +577,9 @@ void choose_tiles(Plan& p, int64_t m, int64_t n, int64_t k, int64_t experts, int
     p.ntiles = (n + s.cols - 1) / s.cols;
     p.slots = slots_of(s);
     if (p.parts > 1) {
-        // (a round's parts are as many as its slots or fewer)
+        // (a pass's parts are as many as its slots or fewer)
         const int64_t tiles = std::min(p.mtiles * p.ntiles, kMostTiles);
-        const Rounds r{int(tiles), int(p.slots), int(p.parts)};
+        const Passes r{int(tiles), int(p.slots), int(p.parts)};
         const int64_t units = experts ? std::min(p.slots, tiles * p.parts) : r.rest * r.parts;
         p.part = round256(size_t(units) * size_t(s.cols * s.rows) * 4u);
     }

@@ -18,7 +18,7 @@ struct Fp8Args {
     const float* ws;
     int M, N, K, KB;  // KB: blocks of K
     int mtiles, ntiles, band;  // tiles
-    int slots, parts;          // workgroups that run at once, and the most parts of K that a tile of the last round makes
+    int slots, parts;          // workgroups that run at once, and the most parts of K that a tile of the last pass makes
     float* part;               // the parts' sums
     // Grouped: tiles[i] = {expert, first, rows} of row tile i, the rows being order[first ..], {route, row of x};
     // tiles[mtiles].x: how many there are.  Expert -1: rows of zeros.

@@ -137,7 +137,7 @@ def test_scratch_of_float_rows_must_be_enough():
 
 def test_scratch_is_for_what_a_call_hands_on():
     """None for rows in codes where K is not split (nor for few rows of values), else codes and scales of the values, and at most
-    16 parts of the result's tiles in f32 (whole tiles, of 256 x 256 or fewer), never more than a round of them."""
+    16 parts of the result's tiles in f32 (whole tiles, of 256 x 256 or fewer), never more than a pass of them."""
     def q(m, n, k, xd=E4M3, yd=BF16):
         return L.eq_fp8_matmul_scratch(m, n, k, xd, yd)
 

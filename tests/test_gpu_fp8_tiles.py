@@ -88,7 +88,7 @@ def test_shapes_of_routes(cuda, routes, experts, n, k, dtype):
 
 
 @pytest.mark.parametrize("m,n,k,dtype", [
-    (466, 9729, 11744, BF), (2478, 6758, 3984, HF),   # 256 x 256, the second of each line behind whole rounds
+    (466, 9729, 11744, BF), (2478, 6758, 3984, HF),   # 256 x 256, the second of each line behind whole passes
     (556, 6955, 13088, HF), (2579, 6894, 10000, BF),  # 256 x 192
     (1372, 1536, 12560, BF), (863, 9500, 9872, HF),   # 256 x 128
     (375, 10804, 12560, BF), (2195, 3857, 4784, SF),  # 128 x 128
@@ -96,7 +96,7 @@ def test_shapes_of_routes(cuda, routes, experts, n, k, dtype):
     (826, 134, 9280, BF), (2381, 1723, 4224, HF), (2571, 1766, 5472, SF),  # 128 x 64
     (29, 130, 4816, BF), (21, 236, 5040, SF),         # 128 x 32
 ])
-def test_parts_of_the_last_round(cuda, m, n, k, dtype):
+def test_parts_of_the_last_pass(cuda, m, n, k, dtype):
     test_shapes(cuda, m, n, k, dtype)
 
 
@@ -108,7 +108,7 @@ def test_parts_of_the_last_round(cuda, m, n, k, dtype):
     (1188, 2, 155, 7376, BF), (1075, 2, 198, 8800, SF),  # 128 x 64
     (84, 5, 201, 5472, HF), (115, 2, 130, 5552, SF),  # 128 x 32
 ])
-def test_parts_of_the_last_round_of_routes(cuda, routes, experts, n, k, dtype):
+def test_parts_of_the_last_pass_of_routes(cuda, routes, experts, n, k, dtype):
     test_shapes_of_routes(cuda, routes, experts, n, k, dtype)
 
 
