@@ -20,14 +20,26 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
     return t;
 }
 
-// 1 / (1 + e^-g): 2^(-g log2 e) with the rounding of the product put back, so that it is off by steps of f32 for large
-// |g| too (by expf and a division the kernel took 76 us for 4096 x 14336 values, bound by the vector units).
+constexpr float kLog2E = 1.44269504f, kLog2ELow = 1.92596300e-8f, kLn2 = 0.693147181f;  // log2 e in two parts
+
+// 1 / (1 + e^-g): 2^(-g log2 e) with the rounding of the product put back, so that it is off by steps of f32 for gates from
+// kFarGate on (by expf and a division the kernel took 76 us for 4096 x 14336 values, bound by the vector units).
 __device__ __forceinline__ float sigmoid(float g) {
-    constexpr float L = 1.44269504f, L_LOW = 1.92596300e-8f, LN2 = 0.693147181f;  // log2 e in two parts
-    const float t = -g * L, low = fmaf(-g, L, -t) - g * L_LOW, e = __builtin_amdgcn_exp2f(t);
+    const float t = -g * kLog2E, low = fmaf(-g, kLog2E, -t) - g * kLog2ELow, e = __builtin_amdgcn_exp2f(t);
     // (2^t = 0 and infinity, and an infinite g, have nothing to put back)
-    const float exact = fabsf(t) < 126.f ? fmaf(e, low * LN2, e) : e;
+    const float exact = fabsf(t) < 126.f ? fmaf(e, low * kLn2, e) : e;
     return __builtin_amdgcn_rcpf(1.f + exact);
+}
+
+// silu(g) u of gates below kFarGate, where 1 / (1 + e^-g) nears the smallest normal f32 (behind it v_rcp_f32 gives 0) and is
+// e^g but for 2^-124 of it.  Its power of two comes last, so that a large u finds all of its bits; it is off by
+// the 2^x of one step, its correction and two products.
+constexpr float kFarGate = -86.5f;
+__device__ __forceinline__ float silu_mul_far(float g, float u) {
+    const float c = g > -INFINITY ? fmaxf(g, -300.f) : g;  // (e^-300 of any u is below every code)
+    const float t = c * kLog2E, low = fmaf(c, kLog2E, -t) + c * kLog2ELow, n = fmaxf(rintf(t), -500.f);
+    const float e = __builtin_amdgcn_exp2f(t - n);
+    return ldexpf(c * fmaf(e, low * kLn2, e) * 0x1p-9f * u, int(n) + 9);  // (300 sqrt 2 2^-9 < 1: no u overflows)
 }
 
 // Codes of 8 values of a lane whose group lies in its 16 lanes; `first` lanes write the scale.
@@ -56,10 +68,17 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(uint8_t* __restrict__
     if (live) {
         load8<T>(x + row * x_stride + at, v);
         if constexpr (SILU) {
-            float u[8];
+            float u[8], g[8], least = 0.f;
             load8<T>(up + row * up_stride + at, u);
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = v[i] * sigmoid(v[i]) * u[i];
+            for (int i = 0; i < 8; i++) {
+                g[i] = v[i], least = fminf(least, g[i]);
+                v[i] = g[i] * sigmoid(g[i]) * u[i];
+            }
+            if (__builtin_expect(least < kFarGate, 0)) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = g[i] < kFarGate ? silu_mul_far(g[i], u[i]) : v[i];
+            }
         }
     }
     put_group(v, live, reinterpret_cast<uint2*>(codes + int64_t(row) * cols + at), scales + block * scale_stride + row,
