@@ -628,12 +628,26 @@ bool plan_product(const char* who, Plan& p, int64_t m, int64_t n, int64_t k, int
     return grid_ok(who, p);
 }
 
+// (offsets into the rows of x are 32 bits, kOutOfRange is none of them)
+bool x_fits(const char* who, int64_t x_rows, int64_t stride) {
+    if (x_rows * stride < int64_t(kOutOfRange)) return true;
+    set_error(std::string(who) + ": the codes of x must be fewer than 3 * 2^30 bytes");
+    return false;
+}
+
 bool plan_routes(const char* who, Plan& p, int64_t x_rows, int64_t experts, int64_t routes, int64_t n, int64_t k,
                  int x_dtype, int y_dtype) {
     if (!sizes_ok(who, routes, n, k) || !sizes_ok(who, x_rows, n, k) || !dtypes_ok(who, x_dtype, y_dtype)) return false;
     if (experts < 1 || experts > kMostExperts) {
         set_error(std::string(who) + ": experts must be in [1, " + std::to_string(kMostExperts) + "]");
         return false;
+    }
+    if (routes > 0 && n > 0) {
+        if (x_rows < 1) {
+            set_error(std::string(who) + ": x must have a row");
+            return false;
+        }
+        if (!x_fits(who, x_rows, k)) return false;
     }
     p.few = routes <= 64;
     const bool plain = x_dtype == EQ_DTYPE_F8E4M3 || (p.few && fp8_few_takes(1, k, x_dtype));
@@ -756,8 +770,8 @@ extern "C" int eq_fp8_grouped_matmul(void* y, const void* x, int64_t x_stride, c
     Plan p;
     if (!plan_routes(who, p, x_rows, experts, routes, n, k, x_dtype, y_dtype)) return 1;
     if (routes == 0 || n == 0) return 0;
-    if (x_rows < 1 || (!rows && x_rows != routes)) {
-        set_error(std::string(who) + ": x must have a row, without `rows` one for each route");
+    if (!rows && x_rows != routes) {
+        set_error(std::string(who) + ": without `rows` x must have a row for each route");
         return 1;
     }
     if (!ids || !aligned(ids, 4) || !aligned(rows, 4)) {
@@ -765,10 +779,7 @@ extern "C" int eq_fp8_grouped_matmul(void* y, const void* x, int64_t x_stride, c
         return 1;
     }
     if (!operands_ok(who, y, x, x_stride, x_scales, scale_stride, w, w_scales, x_rows, k, x_dtype, y_dtype)) return 1;
-    if (x_rows * (x_dtype == EQ_DTYPE_F8E4M3 ? x_stride : k) >= int64_t(kOutOfRange)) {
-        set_error(std::string(who) + ": the codes of x must be fewer than 3 * 2^30 bytes");
-        return 1;
-    }
+    if (x_dtype == EQ_DTYPE_F8E4M3 && !x_fits(who, x_rows, x_stride)) return 1;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     WsHold hold;
     char* base = nullptr;

@@ -80,8 +80,8 @@ int64_t eq_fp8_matmul_scratch(int64_t m, int64_t n, int64_t k, int x_dtype, int 
 /* Routed experts: y [routes, n], y[r] = x[rows[r]] . w[ids[r]]^T with a bank of
  * `experts` (at most 4095) weights w [experts, n, k], scales one after the other
  * too; ids and rows are device int32 (rows NULL: row r, x_rows = routes), in any
- * order.  A route whose expert or row is out of range gives zeros.  x_rows *
- * x_stride of codes, or x_rows * k of values, is below 3 * 2^30.  scratch as
+ * order.  A route whose expert or row is out of range gives zeros; x has a row at
+ * least.  x_rows * x_stride of codes, or x_rows * k of values, is below 3 * 2^30.  scratch as
  * in eq_fp8_matmul. */
 int eq_fp8_grouped_matmul(void* y, const void* x, int64_t x_stride, const float* x_scales, int64_t scale_stride,
                           int64_t x_rows, const void* w, const float* w_scales, int64_t experts, const int32_t* ids,
