@@ -1,11 +1,12 @@
-"""The block-scaled e4m3 linears at the ends of their ranges, against the restatement in 64 bits
-(oracle/fp8_oracle.py) with the bounds of test_gpu_fp8."""
+"""The block-scaled e4m3 linears at the ends of their ranges, and in the tile shapes that the sizes of
+test_gpu_fp8_tiles leave out, against the restatement in 64 bits (oracle/fp8_oracle.py) with the bounds of test_gpu_fp8."""
 import numpy as np
 import pytest
 import torch
 
 from eredu_amd import fp8
 from oracle import fp8_oracle as F
+from tests import test_gpu_fp8_tiles as tiles
 from tests.test_gpu_fp8 import BF, HF, SF, case, f64
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +42,60 @@ def test_silu_mul_of_infinite_far_gates(cuda):
     got = fp8.silu_mul(g, u)
     assert np.array_equal(np.isnan(f64(got.scales))[:, 0], [True, True, False, True])
     assert not f64(got.codes).any() and float(got.scales[2, 0]) == 2.0 ** -126
+
+
+def drawn_ids(rng, routes, experts):
+    """The experts that test_shapes_of_routes draws."""
+    ids = np.minimum((experts - 1) * rng.random(routes) ** 2.5, experts - 2).astype(np.int64) + (1 if experts > 2 else 0)
+    ids[rng.random(routes) < 0.02] = -1
+    return ids
+
+
+@pytest.mark.parametrize("m,n,k,dtype", [
+    (16549, 920, 2400, BF), (278, 12801, 15952, HF),      # 128 x 128 and 128 x 96, the last pass in parts of K behind a whole one
+    (11130, 20, 15936, SF), (1694, 16, 7728, SF),         # 128 x 128 and 128 x 64 in parts
+    (8342, 132, 16, SF), (8611, 20, 16, SF),              # 128 x 96 and 128 x 64, whole
+])
+def test_more_shapes(cuda, m, n, k, dtype):
+    tiles.test_shapes(cuda, m, n, k, dtype)
+
+
+@pytest.mark.parametrize("routes,experts,n,k,dtype", [
+    (8720, 2, 473, 16048, BF), (21714, 2, 2321, 10128, BF),  # 256 x 256 in parts of K, the second behind whole passes
+    (16018, 8, 414, 12864, HF),                              # 256 x 128 in parts behind whole passes
+    (21850, 2, 271, 7904, BF), (22844, 3, 261, 7936, SF),    # the same of 128 x 128
+    (146, 2, 11557, 13184, HF), (16903, 8, 134, 14240, SF),  # the same of 128 x 96
+    (16437, 3, 129, 16, SF), (16401, 3, 16, 16, SF),         # 128 x 128 and 128 x 96, whole
+    (66, 2, 16, 16, BF), (67, 2, 16, 16, SF),                # 128 x 32, whole
+])
+def test_more_shapes_of_routes(cuda, routes, experts, n, k, dtype):
+    tiles.test_shapes_of_routes(cuda, routes, experts, n, k, dtype)
+
+
+@pytest.mark.parametrize("routes,experts", [(65, 3), (256, 300), (257, 2), (16384, 5), (16385, 4)])
+def test_routes_in_one_part_and_at_the_borders_of_parts(cuda, routes, experts):
+    """A workgroup places 256 routes, or more where 64 workgroups would not do."""
+    tiles.test_every_route_is_placed_once(cuda, routes, experts)
+
+
+def bits(t):
+    return t.view(torch.uint8) if t.dtype is fp8.CODE_DTYPE else t
+
+
+def test_calls_give_the_same_bits_every_time(cuda):
+    """Each operator, the products in each way they are done: few rows, whole tiles, tiles in parts of K."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+
+    def rows(m, k):
+        return torch.randn(m, k, generator=g, device="cuda").to(BF)
+
+    w, s = fp8.quantize_weight(rows(4097, 14320))
+    x, wide, gain = rows(300, 14320), rows(300, 2 * 2064), rows(1, 14320)[0]
+    calls = [lambda: fp8.quantize(x), lambda: fp8.quantize_weight(x), lambda: fp8.rms_norm(x.clone(), gain, 1e-5, x),
+             lambda: fp8.silu_mul(wide[:, :2064], wide[:, 2064:])]
+    calls += [lambda m=m, d=d: (fp8.matmul(x[:m], w, s, d),) for m in (1, 3, 16, 77, 300) for d in (BF, SF)]
+    for i, call in enumerate(calls):
+        case("repeated call", i)
+        want = call()
+        for _ in range(5):
+            assert all(torch.equal(bits(a), bits(b)) for a, b in zip(call(), want))
