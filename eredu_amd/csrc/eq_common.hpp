@@ -118,7 +118,7 @@ __device__ __forceinline__ int opaque_one() {
     return v;
 }
 
-// An offset past every buffer the kernels build (all are < 2^31 bytes), leaving
+// An offset past every buffer the kernels build (all end below it), leaving
 // room for the immediate offsets added to it.
 constexpr uint32_t kOutOfRange = 0xC0000000u;
 

@@ -95,10 +95,13 @@ __device__ __forceinline__ void store_rows(const Fp8Args& args, const TileAt& ti
 // activations and where A's rows are consecutive, (row / 2) % 2 + 2 (row / 8 % 4) for A's rows of pairs
 // (no bank conflict is counted).
 //
-// What bounds it: of 4096 x 14336 x 4096 (236 us in tiles of 256 x 256, 2.0 PFLOP/s; a library's unscaled fp8
-// product 217) the matrix cores are busy for 45 % of the cycles and the clock is at 1.95 GHz; the time
+// What bounds it: 4096 rows by 4096 take 60 us a pass of 256 tiles of 256 x 256 (12288 weight rows, three passes, 181 us;
+// 16384, four, 242: 2.3 PFLOP/s), 14336 of them 225 (2.1 PFLOP/s; a library's unscaled fp8 product 217): half of the fourth
+// pass is empty, and it takes 44.  In a pass the matrix cores are busy for 45 % of the cycles and the clock is at 1.95 GHz; the time
 // follows the data (277 us with codes of more varied bits) and hardly the order of the tiles, which points at power:
 // the instructions alone, from registers with the additions beside them, reach 3.6-3.9 PFLOP/s of such data, 4.7 of zeros.
+// 512 x 14336 x 4096 (224 tiles of 256 x 128, 32.7 us, 1.8 PFLOP/s): by count 51 000 cycles of LDS a compute unit (39 000 of reads,
+// at 128 bytes a cycle) beside 28 700 of matrix cores, of some 70 000.
 // 8 us of a tile's 59 are its first loads and its stores.  Tried and not kept: the next block's operands read before
 // the waves meet (the same there, small products 2 us slower), rotating the blocks' order from workgroup to
 // workgroup and fetching ahead into L2 (the same or slower).
@@ -618,6 +621,8 @@ bool grid_ok(const char* who, const Plan& p) {
 
 bool plan_product(const char* who, Plan& p, int64_t m, int64_t n, int64_t k, int x_dtype, int y_dtype) {
     if (!sizes_ok(who, m, n, k) || !dtypes_ok(who, x_dtype, y_dtype)) return false;
+    // (what the kernel of few rows has operands for; 16 and 17 rows of codes by 4096 x 4096 6.9 and 14.9 us in graphs, by
+    // 14336 x 4096 12.5 and 14.8: a tile of 128 x 32 to a workgroup leaves most of the GPU idle where n is small)
     p.few = m <= 16;
     if (p.few) p.mtiles = 1, p.ntiles = (n + 15) / 16;
     else choose_tiles(p, m, n, k, 0, y_dtype);
@@ -649,6 +654,8 @@ bool plan_routes(const char* who, Plan& p, int64_t x_rows, int64_t experts, int6
         }
         if (!x_fits(who, x_rows, k)) return false;
     }
+    // (a route to a workgroup costs no count of routes: 64 of them to some 35 of 128 experts of 768 x 2048 15.3 us; it reads an
+    // expert's weight for each of its routes, though: 64 to 8 experts of 14336 x 4096 526 us, 66, in tiles, 103)
     p.few = routes <= 64;
     const bool plain = x_dtype == EQ_DTYPE_F8E4M3 || (p.few && fp8_few_takes(1, k, x_dtype));
     if (!plain) {

@@ -71,7 +71,7 @@ __device__ __forceinline__ f32x4 block_sums(const Operand<true>& a, const Operan
 }
 
 // VALS consecutive results of a row, n of them inside it.  Pieces of 16 bytes, at whatever place the row's length puts
-// them (global stores need no alignment; 3103 x 2662 f32 of 96 columns took 52 us value by value, 20 so).
+// them (global stores need no alignment; 3103 x 2662 f32 of 96 columns took 52 us value by value, 15.5 in pieces side by side).
 template <typename YT, int VALS>
 __device__ __forceinline__ void store_run(typename YT::storage* p, const float* v, int n) {
     using S = typename YT::storage;

@@ -14,8 +14,9 @@ cores as they are.  An MLP over rows of 16-bit activations:
     out = fp8.matmul(a, down, down_scales, torch.bfloat16)
 
 A group of 128 values v gets the scale max|v| / 448 (at least 2^-126) and codes
-448 v / max|v|, rounded once to the nearest, ties to even; a group that holds a value
-that is not finite gets the scale NaN and codes 0.  Row lengths are multiples of 16.
+448 v / max|v|, rounded to the nearest, ties to even (once of 16-bit values; of float32 ones the
+quotient is off by up to 3 * 2^-24 of itself before); a group that holds a value that is not finite gets the scale NaN and
+codes 0.  Row lengths are multiples of 16; sizes have limits, which the header names.
 """
 from __future__ import annotations
 
@@ -244,7 +245,8 @@ def matmul(x: Union[Fp8Rows, torch.Tensor], w: torch.Tensor, w_scales: torch.Ten
     ceil(K / 128)]: [..., N] in ``dtype`` (x's own where it is None).  x is
     ``Fp8Rows``, or float rows that the call quantizes first, as ``quantize``
     does (C ABI: eq_fp8_matmul).  16-bit results take the matrix cores' e4m3 products,
-    which keep 13 bits below the largest of 8; float32 results exact ones at half the rate."""
+    which keep 13 bits below the largest of 8 (cut off, so off by up to 7 * 2^-13 of it where all 8 are of its size); float32
+    results exact ones at half the rate."""
     N, K = _weight(w, w_scales, 2)
     rows, scales, stride, code = _x_of(x, K)
     dtype = _out_dtype(x, dtype)

@@ -99,3 +99,22 @@ def test_calls_give_the_same_bits_every_time(cuda):
         want = call()
         for _ in range(5):
             assert all(torch.equal(bits(a), bits(b)) for a, b in zip(call(), want))
+
+
+def test_what_passes_the_range_of_f32(cuda):
+    """Rows whose sum of squares is infinite become zeros, and where a block's two scales pass f32's range together the results
+    are not finite, those of other rows being as they are."""
+    case("past f32")
+    x = torch.full((2, 256), 2.0, dtype=BF, device="cuda")
+    x[0] = 1e25
+    r = fp8.rms_norm(x, torch.ones(256, dtype=BF, device="cuda"), 1e-5)
+    assert not f64(r.codes[0]).any() and np.all(f64(r.scales[0]) == 2.0 ** -126)
+    assert np.all(f64(r.codes[1]) == 448)
+    for m in (2, 40):
+        rows = torch.full((m, 128), 1.0, dtype=SF, device="cuda")
+        rows[0] = 1e30
+        w, s = fp8.quantize_weight(torch.full((16, 128), 1e25, dtype=SF, device="cuda"))
+        for dtype in (BF, SF):
+            y = fp8.matmul(fp8.quantize(rows), w, s, dtype)
+            # 128 products of 1 and 1e25: every code is 448 and every sum exact but for the scales' and the result's roundings
+            assert not torch.isfinite(y[0]).any() and np.all(np.abs(f64(y[1:]) / 1.28e27 - 1) < 2.0 ** -8 + 2.0 ** -11)
