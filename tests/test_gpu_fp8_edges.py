@@ -118,3 +118,52 @@ def test_what_passes_the_range_of_f32(cuda):
             y = fp8.matmul(fp8.quantize(rows), w, s, dtype)
             # 128 products of 1 and 1e25: every code is 448 and every sum exact but for the scales' and the result's roundings
             assert not torch.isfinite(y[0]).any() and np.all(np.abs(f64(y[1:]) / 1.28e27 - 1) < 2.0 ** -8 + 2.0 ** -11)
+
+
+def repeated(base, times):
+    """[times * len(base), K] of the same rows again and again."""
+    return base.expand(times, *base.shape).reshape(-1, base.shape[1])
+
+
+def test_rows_past_2_32_values(cuda):
+    """Values, codes and results whose offsets pass 32 bits: rows of the same values give the same codes and results wherever they lie."""
+    case("large rows")
+    g = torch.Generator(device="cuda").manual_seed(12)
+    few, times, K = 1024, 264, 16384
+    assert few * times * K > 1 << 32 and few * times * -(-K // 128) < 1 << 26
+    base = torch.randn(few, K, generator=g, device="cuda").to(BF)
+    gain = torch.randn(K, generator=g, device="cuda").to(BF)
+    x = repeated(base, times)
+    same = lambda got, want: all(torch.equal(bits(got[0][i:i + few]), bits(want[0])) and torch.equal(got[1][i:i + few], want[1])
+                                 for i in range(0, few * times, few))
+    codes = fp8.quantize(x)
+    assert same(codes, fp8.quantize(base))
+    assert same(fp8.silu_mul(x, x), fp8.silu_mul(base, base))
+    w, s = fp8.quantize_weight(torch.randn(40, K, generator=g, device="cuda").to(BF))
+    y = fp8.matmul(codes, w, s, BF)
+    for i in (0, few * (times // 2), few * (times - 1)):  # (the last rows' tiles are in parts of K, summed in another order)
+        tiles.check(y[i:i + few], fp8.Fp8Rows(codes.codes[i:i + few], codes.scales[i:i + few]), w, s, np.random.default_rng(1), BF)
+    assert all(torch.equal(y[i:i + few], y[:few]) for i in range(0, few * (times // 2), few))
+    assert torch.equal(fp8.matmul(x, w, s), y)
+    want = base + base
+    assert same(fp8.rms_norm(x, gain, 1e-5, x.clone()), fp8.rms_norm(want.clone(), gain, 1e-5))
+    assert all(torch.equal(x[i:i + few], want) for i in range(0, few * times, few))
+
+
+def test_results_past_2_32_values(cuda):
+    """y of more than 2^32 values, of rows and of routes."""
+    case("large results")
+    g = torch.Generator(device="cuda").manual_seed(13)
+    few, times, K, N = 1024, 264, 144, 16400
+    assert few * times * N > 1 << 32
+    base = torch.randn(few, K, generator=g, device="cuda").to(BF)
+    w, s = fp8.quantize_weight(torch.randn(N, K, generator=g, device="cuda").to(BF))
+    codes = fp8.quantize(repeated(base, times))
+    y = fp8.matmul(codes, w, s, BF)
+    tiles.check(y[:few], fp8.Fp8Rows(codes.codes[:few], codes.scales[:few]), w, s, np.random.default_rng(2), BF)
+    assert all(torch.equal(y[i:i + few], y[:few]) for i in range(0, few * times, few))
+    del y
+    rows = torch.arange(few, dtype=torch.int32, device="cuda").repeat(times)
+    z = fp8.grouped_matmul(fp8.quantize(base), w[None], s[None], torch.zeros_like(rows), rows, BF)
+    assert all(torch.equal(z[i:i + few], z[:few]) for i in range(0, few * times, few))
+    tiles.check(z[:few], fp8.quantize(base), w, s, np.random.default_rng(2), BF)
